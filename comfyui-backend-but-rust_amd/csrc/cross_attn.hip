@@ -1,0 +1,118 @@
+// Cross attention to an encoder's states: 16-bit keys and values of another length, named per batch item, with a mask or a bias per key.
+#include "attn_states.hpp"
+
+namespace {
+
+using namespace states;
+
+struct CrossArgs {
+    const uint16_t *k, *v;
+    int64_t q_bs, o_bs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs;
+    int lq, lk, aligned;
+    const int32_t* k_lens;
+    const void* mask;
+    int mask_kind;          // 1: bytes, 0 = out; 2: f32, added to the logits
+    int64_t mask_bs;
+};
+
+// What a key's mask adds to its exponent (in units of log2): -inf takes the key out.  A finite bias stays finite, so that the type's
+// lowest value is what it is in the formula: a logit like any other.
+__device__ __forceinline__ float key_bias(const CrossArgs& a, const void* mask, int key) {
+    if (a.mask_kind == 1) return ((const uint8_t*)mask)[key] ? 0.f : -INFINITY;
+    const float b = ((const float*)mask)[key], x = b * kLog2e;
+    return fabsf(b) < INFINITY && fabsf(x) == INFINITY ? copysignf(3.402823466e38f, b) : x;
+}
+
+template <int DTYPE, bool BIAS> struct Dense {
+    typedef CrossArgs Args;
+    static constexpr int DT = DTYPE;
+    static constexpr bool kBias = BIAS, kNormalize = false;
+    static constexpr float kOut = 1.f;
+    struct Scales {
+        __device__ float k(int) const { return 1.f; }
+        __device__ float lv(int) const { return 0.f; }
+        __device__ float iv(int) const { return 1.f; }
+    };
+    static __device__ __forceinline__ Problem problem(const Args& a, const Common& c, int id) {
+        const int b = id / c.hk, head = id - b * c.hk;
+        Problem p;
+        p.q_at = b * a.q_bs + head * c.group * c.q_hs;
+        p.o_at = b * a.o_bs + head * c.group * c.o_hs;
+        p.tokens = a.lq;
+        p.keys = a.k_lens ? min(max(a.k_lens[b], 0), a.lk) : a.lk;
+        p.limit0 = p.keys;
+        return p;
+    }
+    template <int DP, int TK, int NT> struct Stage {
+        static constexpr int CH = TK * DP / 8 / NT, ROW = DP / 8;
+        const Args& a;
+        const uint16_t *k, *v;
+        const void* mask;
+        int tid, keys, d;
+        u32x4 kr[CH], vr[CH];
+        float out[BIAS ? CH : 1], add;
+        __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_) : a(a_), tid(tid_), keys(p.keys), d(c.d) {
+            const int b = id / c.hk, head = id - b * c.hk;
+            k = a.k + b * a.k_bs + head * a.k_hs;
+            v = a.v + b * a.v_bs + head * a.v_hs;
+            mask = a.mask_kind == 1 ? (const void*)((const uint8_t*)a.mask + b * a.mask_bs) : (const void*)((const float*)a.mask + b * a.mask_bs);
+        }
+        __device__ __forceinline__ void load(int t) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int i = tid + j * NT, r = i / ROW, ch = i % ROW, key = t * TK + r;
+                const bool there = key < keys && 8 * ch < d;
+                kr[j] = there ? load8(k + key * a.k_rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
+                vr[j] = there ? load8(v + key * a.v_rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
+                if (BIAS) out[j] = there ? key_bias(a, mask, key) : 0.f;
+            }
+            if (BIAS && tid < TK) add = t * TK + tid < keys ? key_bias(a, mask, t * TK + tid) : -INFINITY;
+        }
+        // a key that is out has probability 0, and its value must be a number for the product to leave it out
+        __device__ __forceinline__ void write(uint8_t* kb, uint8_t* vb, float* bias) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int i = tid + j * NT, r = i / ROW, ch = i % ROW;
+                *reinterpret_cast<u32x4*>(kb + k_place<DP>(r, ch)) = kr[j];
+                *reinterpret_cast<u32x4*>(vb + v_place<DP>(r, ch)) = BIAS && out[j] == -INFINITY ? u32x4{0, 0, 0, 0} : vr[j];
+            }
+            if (BIAS && tid < TK) bias[tid] = add;
+        }
+        __device__ __forceinline__ Scales scales(bool) const { return {}; }
+    };
+};
+
+}  // namespace
+
+GPU_API int64_t gpu_cross_attn_workspace(int b, int lq, int lk, int h, int hk, int head_dim) {
+    if (b <= 0 || lq <= 0 || lk <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256) return 0;
+    return make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim).bytes;
+}
+
+GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void* o, void* ws, int b, int lq, int lk, int h, int hk,
+                           int head_dim, int64_t q_bs, int64_t q_rs, int64_t q_hs, int64_t k_bs, int64_t k_rs, int64_t k_hs, int64_t v_bs,
+                           int64_t v_rs, int64_t v_hs, int64_t o_bs, int64_t o_rs, int64_t o_hs, float scale, const int32_t* k_lens,
+                           const void* mask, int mask_kind, int64_t mask_bs, void* stream) {
+    if (dtype != DT_F16 && dtype != DT_BF16) return -4;
+    if (b < 0 || lq < 0 || lk < 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256 || head_dim % 8 != 0) return -1;
+    if (mask_kind < 0 || mask_kind > 2 || (mask_kind != 0 && !mask && lk > 0) || !(fabsf(scale) < INFINITY)) return -1;
+    if (b == 0 || lq == 0) return 0;
+    if ((int64_t)lq * (h / hk) > 0x7fffff00 || (int64_t)b * hk > 0x7fffffff || !q || !o || (lk > 0 && (!k || !v))) return -1;
+    const Plan p = make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim);
+    if (p.bytes && (!ws || (uintptr_t)ws % 16 != 0)) return -1;
+    const auto sixteen = [](const void* at, int64_t s0, int64_t s1, int64_t s2) { return (uintptr_t)at % 16 == 0 && (s0 | s1 | s2) % 8 == 0; };
+    Common c{};
+    c.q = q; c.o = o; c.q_rs = q_rs; c.q_hs = q_hs; c.o_rs = o_rs; c.o_hs = o_hs;
+    c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
+    c.row_tiles = p.row_tiles; c.problems = b * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
+    c.aligned = (sixteen(q, q_bs, q_rs, q_hs) ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_bs | o_rs | o_hs) % 4 == 0 ? 2 : 0);
+    c.c = fabsf(scale) * kLog2e; c.negate = scale < 0.f; c.part = (float*)ws;
+    CrossArgs s{};
+    s.k = (const uint16_t*)k; s.v = (const uint16_t*)v;
+    s.q_bs = q_bs; s.o_bs = o_bs; s.k_bs = k_bs; s.k_rs = k_rs; s.k_hs = k_hs; s.v_bs = v_bs; s.v_rs = v_rs; s.v_hs = v_hs;
+    s.lq = lq; s.lk = lk; s.aligned = sixteen(k, k_bs, k_rs, k_hs) && sixteen(v, v_bs, v_rs, v_hs);
+    s.k_lens = k_lens; s.mask = mask; s.mask_kind = mask_kind; s.mask_bs = mask_bs;
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == DT_BF16) return mask_kind ? launch_dim<Dense<DT_BF16, true>>(p, c, s, st) : launch_dim<Dense<DT_BF16, false>>(p, c, s, st);
+    return mask_kind ? launch_dim<Dense<DT_F16, true>>(p, c, s, st) : launch_dim<Dense<DT_F16, false>>(p, c, s, st);
+}

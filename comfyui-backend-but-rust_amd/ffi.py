@@ -50,6 +50,13 @@ SIGNATURES = {
     "gpu_int8_attn_sink": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32] + [_I64] * 12 + [_F32, _F32, _P, _F32, _P],
     "gpu_int8_attn_norm_rope": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32] + [_I64] * 12 + [_F32, _P, _P, _F32, _P, _I32, _P],
     "gpu_int8_attn_key_bias": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32] + [_I64] * 12 + [_F32, _P, _P],
+    "gpu_cross_attn": [_I32, _P, _P, _P, _P, _P] + [_I32] * 6 + [_I64] * 12 + [_F32, _P, _P, _I32, _I64, _P],
+    "gpu_cross_attn_workspace": [_I32] * 6,
+    "gpu_kv8_store": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 6 + [_P],
+    "gpu_kv8_read": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 6 + [_P],
+    "gpu_kv8_attn": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 7 + [_F32, _I32, _P],
+    "gpu_kv8_attn_workspace": [_I32] * 7,
+    "gpu_kv8_copy_pages": [_P, _P, _P, _P] + [_I32] * 5 + [_P, _P, _I32, _P],
     "gpu_internal_act_probe": [_I32, _P, _P, _I32, _P],
     "gpu_internal_geglu_form": [_I32, _I32],
     "gpu_internal_cvt_pk_u8_probe": [_P, _P, _I32, _P],
@@ -83,6 +90,8 @@ def _load():
     lib.gpu_int8_attn_key_bias_workspace.argtypes = [_I32] * 5
     lib.gpu_int8_attn_key_bias_workspace.restype = _I64
     lib.gpu_w6a8_group_gemm_scratch.restype = _I64
+    lib.gpu_cross_attn_workspace.restype = _I64
+    lib.gpu_kv8_attn_workspace.restype = _I64
     lib.gpu_int8_gemm_static_limit.argtypes = []
     lib.gpu_int8_gemm_static_limit.restype = _I64
     lib.gpu_kernels_build_info.restype = C.c_char_p

@@ -2,6 +2,7 @@
 src/unet.rs:436-456, src/h3.rs:1208-1251): quantize rows, then the fused int8 GEMM.  torch supplies device memory and
 the stream; all arithmetic happens in libgpu_kernels.so.
 """
+import contextlib
 import importlib.machinery
 import importlib.util
 import os
@@ -35,6 +36,21 @@ def _stream():
     """Handle of the current stream of the current device: torch.cuda.current_stream().cuda_stream without the Stream object made
     for it, which took 2.8 us of a call's host time; this way 0.2."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+@contextlib.contextmanager
+def _on(device):
+    """The current stream of a tensor's device, which is the current device meanwhile."""
+    if device.index == torch._C._cuda_getDevice():
+        yield _stream()
+    else:
+        with torch.cuda.device(device):
+            yield _stream()
+
+
+def _no_grad(t, what):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s asks for gradients, and this call has no backward pass: detach it, or call under torch.no_grad()" % what)
 
 
 def _ptr(t):
@@ -392,4 +408,38 @@ def int8_attn(q, k, v, scale, ws=None):
     ffi.k(name, _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(ws), b, lq, lk, h, hk, D, q.stride(0), q.stride(1), q.stride(2),
           k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), o.stride(0), o.stride(1),
           o.stride(2), float(scale), _stream())
+    return o
+
+
+def cross_attn(q, k, v, scale, k_lens=None, mask=None):
+    """softmax(scale * q k^T + mask) v over an encoder's states: q [b, lq, h, d], k, v [b, lk, hk, d] (bf16 or f16, any strides with a dense last
+    axis, h a multiple of hk, d a multiple of 8 up to 256) -> [b, lq, h, d].  k_lens (int32 [b]): item i has that many keys.  mask
+    [lk] or [b, lk]: bool, False takes a key out, or float32, added to the logits, -inf takes it out.  A row without keys gives zeros."""
+    b, lq, h, d = q.shape
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[3] != d or k.shape[2] == 0 or h % k.shape[2]:
+        raise ValueError("q [b, lq, h, d] and k, v [b, lk, hk, d] do not fit: %s, %s and %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    lk, hk = k.shape[1], k.shape[2]
+    dev = q.device
+    for t, what in ((q, "q"), (k, "k"), (v, "v")):
+        if not t.is_cuda or t.device != dev or t.stride(3) != 1:
+            raise ValueError("%s must be on q's CUDA device with a dense last axis, got strides %s on %s" % (what, t.stride(), t.device))
+        if t.dtype != q.dtype or t.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("q, k and v must all be float16 or all bfloat16, got %s" % t.dtype)
+        _no_grad(t, what)
+    if k_lens is not None and (k_lens.dtype != torch.int32 or k_lens.shape != (b,) or k_lens.device != dev or not k_lens.is_contiguous()):
+        raise ValueError("k_lens must be contiguous int32 [%d] on q's device, got %s %s on %s" % (b, k_lens.dtype, tuple(k_lens.shape), k_lens.device))
+    kind, bs = 0, 0
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.float32) or mask.shape not in ((lk,), (b, lk)) or mask.device != dev or (lk > 1 and mask.stride(-1) != 1):
+            raise ValueError("mask must be bool or float32 [%d] or [%d, %d] on q's device, dense along the keys, got %s %s with strides %s"
+                             % (lk, b, lk, mask.dtype, tuple(mask.shape), mask.stride()))
+        _no_grad(mask, "mask")
+        kind, bs = 1 if mask.dtype == torch.bool else 2, mask.stride(0) if mask.dim() == 2 else 0
+    o = torch.empty((b, lq, h, d), dtype=q.dtype, device=dev)
+    with _on(dev) as s:
+        need = ffi.lib.gpu_cross_attn_workspace(b, lq, lk, h, hk, d)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        ffi.k("gpu_cross_attn", _TORCH_DT[q.dtype], _ptr(q), _ptr(k), _ptr(v), _ptr(o), _ptr(ws), b, lq, lk, h, hk, d, q.stride(0), q.stride(1),
+              q.stride(2), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), o.stride(0), o.stride(1), o.stride(2),
+              float(scale), _ptr(k_lens), _ptr(mask), kind, bs, s)
     return o

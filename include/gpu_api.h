@@ -311,6 +311,56 @@ int gpu_w6a8_group_gemm_ws(const int8_t* A, const void* Wp, const float* xs, con
                            int32_t* partials, void* scratch, int64_t M, int64_t N, int64_t K, int out_dt, void* stream);
 int64_t gpu_w6a8_group_gemm_scratch(const void* Wp, int64_t M, int64_t N, int64_t K);
 
+/* Cross attention to an encoder's states, 16-bit throughout: o = softmax(scale * q k^T + bias) v per head, where batch item i attends
+ * to the keys j < k_lens[i] that its mask leaves.  dtype DT_F16 or DT_BF16 (others -4) for q [b, lq, h, d], k, v [b, lk, hk, d] and o
+ * [b, lq, h, d]; element strides per batch item, token and head (bs, rs, hs), the last axis dense; query head j uses key-value head
+ * j / (h / hk).  head_dim a multiple of 8 up to 256.  Rows that start on 16 bytes (o: 8) take wide loads, others work too.
+ * k_lens: int32 [b] on the device or null (all lk); values outside 0..lk count as the nearer end.  mask: null (mask_kind 0), bytes [b, lk], 0 = the
+ * key is out (1), or f32 [b, lk] added to the logits, -inf = out (2); rows mask_bs elements apart (0: one row for all), 32-bit elements on 4 bytes.
+ * A key that is out counts as absent whatever k and v hold there; a row without keys gives zeros.  Scores, probabilities' sums and
+ * outputs are held in fp32, the probabilities rounded to the row type for the product with v.
+ * ws: gpu_cross_attn_workspace bytes (0: null will do), 16-byte aligned, in use until the work queued here has run.
+ * Returns -1 for sizes, a scale that is not finite, or pointers that do not fit this. */
+int64_t gpu_cross_attn_workspace(int b, int lq, int lk, int h, int hk, int head_dim);
+int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void* o, void* ws, int b, int lq, int lk, int h, int hk,
+                   int head_dim, int64_t q_bs, int64_t q_rs, int64_t q_hs, int64_t k_bs, int64_t k_rs, int64_t k_hs, int64_t v_bs,
+                   int64_t v_rs, int64_t v_hs, int64_t o_bs, int64_t o_rs, int64_t o_hs, float scale, const int32_t* k_lens,
+                   const void* mask, int mask_kind, int64_t mask_bs, void* stream);
+
+/* A paged cache of keys and values in 8 bits.
+ *   k, v              int8 [n_pages, hk, page, d], 16-byte aligned; page a power of two from 16 to 4096, d a multiple of 16 up to 256
+ *   k_scale, v_scale  f32 [n_pages, hk, page / 16]: A, the largest magnitude of the 16 tokens' values of that head; a code c stands for c * A / 127
+ *   starts int32 [n + 1], lens int32 [n], table int32 [n, table_cols], all on the device: rows starts[s] .. starts[s + 1] of the call's
+ *     row tensors are the LAST tokens of sequence s, which holds lens[s] tokens (the new ones among them, at most 2^30); its token t is slot
+ *     t % page of page table[s, t / page].  rows: rows of the row tensors, none behind it is touched; most: the most rows of one
+ *     sequence (those above it are left out).  Sequences without rows, and without tokens, are fine.  An entry of the table that is no page
+ *     (outside 0 .. n_pages - 1, or beyond table_cols) is never accessed: tokens there are not stored, read back as NaN, and make NaN
+ *     of every attention row that sees them.
+ * gpu_kv8_store writes the rows of k and v (DT_F16 or DT_BF16, element strides of tokens and heads, dense last axis) at their places.  Per block
+ *   of 16 tokens and head: A = the largest magnitude of the new rows and, where the block was begun earlier, of its A before; codes of
+ *   new rows rne(127 x / A), codes of earlier tokens rne(code * A before / A), both exact roundings.  A block of which nothing is
+ *   earlier forgets what it held.  A value that is not finite makes A, and so all of the block, NaN.  No two sequences of a call may write one block.
+ * gpu_kv8_read gives the rows back in dtype (any): code * A / 127.  Rows on 8 bytes (f32: 16), strides multiples of 4 (-1).
+ * gpu_kv8_attn: o = softmax(scale * q k^T) v for the rows of q [rows, h, d] (DT_F16 or DT_BF16); row i of a sequence's m sees the tokens
+ *   0 .. lens[s] - m + i (causal) or all lens[s].  A row that sees none gives zeros.  ws: gpu_kv8_attn_workspace bytes (0: null will do),
+ *   16-byte aligned, in use until the work queued here has run.
+ * gpu_kv8_copy_pages copies pages src[i] -> dst[i] (int32 on the device, n <= 65535) with their scales in each of `layers` caches that lie
+ *   one behind the other in every array.  Numbers that are no page are left out.  No page may be named twice in dst, or in both.
+ * All return -4 for a dtype they do not take, -1 for sizes and pointers that do not fit the above (n <= 65535 in store and read). */
+int gpu_kv8_store(int dtype, const void* k, int64_t k_rs, int64_t k_hs, const void* v, int64_t v_rs, int64_t v_hs, int8_t* ck, int8_t* cv,
+                  float* k_scale, float* v_scale, int n_pages, int page, const int32_t* starts, const int32_t* lens, const int32_t* table,
+                  int table_cols, int n, int rows, int most, int hk, int head_dim, void* stream);
+int gpu_kv8_read(int dtype, void* k, int64_t k_rs, int64_t k_hs, void* v, int64_t v_rs, int64_t v_hs, const int8_t* ck, const int8_t* cv,
+                 const float* k_scale, const float* v_scale, int n_pages, int page, const int32_t* starts, const int32_t* lens,
+                 const int32_t* table, int table_cols, int n, int rows, int most, int hk, int head_dim, void* stream);
+int64_t gpu_kv8_attn_workspace(int n, int most, int h, int hk, int head_dim, int page, int table_cols);
+int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* o, int64_t o_rs, int64_t o_hs, void* ws, const int8_t* ck,
+                 const int8_t* cv, const float* k_scale, const float* v_scale, int n_pages, int page, const int32_t* starts,
+                 const int32_t* lens, const int32_t* table, int table_cols, int n, int rows, int most, int h, int hk, int head_dim,
+                 float scale, int causal, void* stream);
+int gpu_kv8_copy_pages(int8_t* ck, int8_t* cv, float* k_scale, float* v_scale, int layers, int n_pages, int page, int hk, int head_dim,
+                       const int32_t* src, const int32_t* dst, int n, void* stream);
+
 /* Test and tuning hook: force the GEMM kernel family.  1, 2 = 128x128 and 64x64 register-staged tiles; 5 = weights straight
  * into registers, for M <= 128; 7 = four waves multiply what four others fetch, 128x64 to 128x192 tiles, K split where they are few;
  * 7000 + 100 * width + slices = 7 with tiles of 64 * width columns (width 1 to 3) and K in that many slices;

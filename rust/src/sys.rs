@@ -87,6 +87,23 @@ extern "C" {
     pub fn gpu_w6a8_group_gemm_ws(a: P, wp: P, xs: P, sw: P, bias: P, d: PM, partials: PM, scratch: PM, m: i64,
         n: i64, k: i64, out_dt: i32, stream: PM) -> i32;
     pub fn gpu_w6a8_group_gemm_scratch(wp: P, m: i64, n: i64, k: i64) -> i64;
+    pub fn gpu_cross_attn_workspace(b: i32, lq: i32, lk: i32, h: i32, hk: i32, head_dim: i32) -> i64;
+    pub fn gpu_cross_attn(dtype: i32, q: P, k: P, v: P, o: PM, ws: PM, b: i32, lq: i32, lk: i32, h: i32, hk: i32,
+        head_dim: i32, q_bs: i64, q_rs: i64, q_hs: i64, k_bs: i64, k_rs: i64, k_hs: i64, v_bs: i64, v_rs: i64,
+        v_hs: i64, o_bs: i64, o_rs: i64, o_hs: i64, scale: f32, k_lens: P, mask: P, mask_kind: i32, mask_bs: i64,
+        stream: PM) -> i32;
+    pub fn gpu_kv8_store(dtype: i32, k: P, k_rs: i64, k_hs: i64, v: P, v_rs: i64, v_hs: i64, ck: PM, cv: PM,
+        k_scale: PM, v_scale: PM, n_pages: i32, page: i32, starts: P, lens: P, table: P, table_cols: i32, n: i32,
+        rows: i32, most: i32, hk: i32, head_dim: i32, stream: PM) -> i32;
+    pub fn gpu_kv8_read(dtype: i32, k: PM, k_rs: i64, k_hs: i64, v: PM, v_rs: i64, v_hs: i64, ck: P, cv: P,
+        k_scale: P, v_scale: P, n_pages: i32, page: i32, starts: P, lens: P, table: P, table_cols: i32, n: i32,
+        rows: i32, most: i32, hk: i32, head_dim: i32, stream: PM) -> i32;
+    pub fn gpu_kv8_attn_workspace(n: i32, most: i32, h: i32, hk: i32, head_dim: i32, page: i32, table_cols: i32) -> i64;
+    pub fn gpu_kv8_attn(dtype: i32, q: P, q_rs: i64, q_hs: i64, o: PM, o_rs: i64, o_hs: i64, ws: PM, ck: P, cv: P,
+        k_scale: P, v_scale: P, n_pages: i32, page: i32, starts: P, lens: P, table: P, table_cols: i32, n: i32,
+        rows: i32, most: i32, h: i32, hk: i32, head_dim: i32, scale: f32, causal: i32, stream: PM) -> i32;
+    pub fn gpu_kv8_copy_pages(ck: PM, cv: PM, k_scale: PM, v_scale: PM, layers: i32, n_pages: i32, page: i32,
+        hk: i32, head_dim: i32, src: P, dst: P, n: i32, stream: PM) -> i32;
     pub fn gpu_int8_gemm_force_config(cfg: i32) -> i32;
     pub fn gpu_internal_int8_gemm_plan(m: i64, n: i64, k: i64, start: i32, aligned: i32, out: PM) -> i32;
     pub fn gpu_mfma_layout_probe(out: PM, stream: PM) -> i32;
