@@ -12,16 +12,19 @@
 // key_of() does.  Probabilities never cross lanes.  V is read from LDS with the transposing 16-bit read, which turns four keys times
 // 16 channels, so it is staged as it lies in memory.
 //
-// A workgroup is QW waves of 32 rows on the same keys, or KW waves on the same 32 rows and different keys, whose results meet in LDS.
-// With SPLIT several workgroups share a row's keys and leave numerators, denominators and bases in the workspace.
+// A workgroup is four waves with rows of their own on the same keys (tiles_kernel), or several on the same 32 rows and different keys,
+// whose results meet in LDS (few_kernel).  Where that leaves CUs idle, several workgroups share a row's keys and leave numerators,
+// denominators and bases in the workspace.
 #pragma once
 #include "common.hpp"
 
 #include <math.h>
+#include <stdlib.h>
 
 namespace states {
 
 typedef float f16acc __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -40,6 +43,11 @@ template <int DT> __device__ __forceinline__ f16acc mfma(u32x4 a, u32x4 b, f16ac
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 template <int DT> __device__ __forceinline__ uint32_t pack2(float a, float b) { return DT == DT_BF16 ? pack_bf16x2(a, b) : pack_f16x2(a, b); }
+// a plus the two values of a pair: the denominator adds the probabilities as they are rounded for the product with V.
+template <int DT> __device__ __forceinline__ float add2(uint32_t two, float a) {
+    if constexpr (DT == DT_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), bf16x2{(__bf16)1.f, (__bf16)1.f}, a, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two), f16x2{(_Float16)1.f, (_Float16)1.f}, a, false);
+}
 // The larger / the sum of this lane's value and lane ^ 32's.
 __device__ __forceinline__ float half_max(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
@@ -110,280 +118,398 @@ __device__ __forceinline__ int xcd_contiguous(int b, int n) {
     return xcd * base + (xcd < rem ? xcd : rem) + idx;
 }
 
-template <class Src, int DP, int QW, int KW, int TK>
-__global__ __launch_bounds__(64 * QW * KW, DP == 256 ? 1 : 2) void rows_kernel(const Common a, const typename Src::Args sa) {
-    constexpr int DT = Src::DT, NB = TK / 32, KS = DP / 16, DB = DP / 32, NBUF = QW > 1 ? 2 : 1, TILE = TK * DP * 2;
-    static_assert(QW == 1 || KW == 1, "waves share keys or rows");
-    static_assert(KW == 1 || TK >= 32, "the results of KW waves meet in the tiles' place");
-    __shared__ __align__(16) uint8_t lds[KW * NBUF * 2 * TILE];
-    __shared__ float stat[KW > 1 ? KW * 64 : 1];
-    __shared__ __align__(16) float bias[Src::kBias ? KW * NBUF * TK : 4];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
-    const int kw = KW > 1 ? wave : 0, qw = KW > 1 ? 0 : wave, tid = KW > 1 ? lane : (int)threadIdx.x;
+// The rows of a wave: which they are, their queries, and what they have so far.
+template <class Src, int DP, int RW> struct Lanes {
+    static constexpr int KS = DP / 16, DB = DP / 32, DT = Src::DT;
+    int row[RW], token[RW], head[RW], limit[RW];     // of the lane; it sees keys below `limit`
+    int all_see;                                     // every row of the wave sees the keys below
+    u32x4 qf[RW][KS];                                // in the order of the products' channels
+    float c[RW], base[RW], sum[RW];
+    f16acc acc[RW][DB];
 
+    // rows from r0 on, of `rows`
+    __device__ __forceinline__ void start(const Common& a, const Problem& pr, int r0, int rows, int lane) {
+        const int col = lane & 31, g = lane >> 5;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            row[w] = r0 + 32 * w + col;
+            const int r = row[w] < rows ? row[w] : rows - 1;
+            token[w] = r / a.group;
+            head[w] = r - token[w] * a.group;
+            limit[w] = min(pr.keys, pr.limit0 + token[w]);
+        }
+        all_see = min(pr.keys, pr.limit0 + min(rows - 1, r0) / a.group);
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            c[w] = a.c;
+            const uint16_t* qp = (const uint16_t*)a.q + pr.q_at + token[w] * a.q_rs + head[w] * a.q_hs;
+            if (a.aligned & 1) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) qf[w][s] = 16 * s + 8 * g < a.d ? load8(qp + 16 * s + 8 * g, true) : u32x4{0, 0, 0, 0};
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) qf[w][s] = 16 * s + 8 * g < a.d ? load8(qp + 16 * s + 8 * g, false) : u32x4{0, 0, 0, 0};
+            }
+        }
+        const uint32_t flip = a.negate ? 0x80008000u : 0u;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            // The 8-bit source multiplies f16: rows are scaled by a power of two there.
+            if constexpr (Src::kNormalize) {
+                float m = 0.f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(elem(qf[w][s], i, a.q_dt)));
+                m = half_max(m);
+                const int e = m > 0.f && m < INFINITY ? ilogbf(m) : 0;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    u32x4 f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[i] = pack_f16x2(ldexpf(elem(qf[w][s], 2 * i, a.q_dt), -e), ldexpf(elem(qf[w][s], 2 * i + 1, a.q_dt), -e)) ^ flip;
+                    qf[w][s] = f;
+                }
+                c[w] = ldexpf(c[w], e);
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) qf[w][s] ^= flip;
+            }
+            base[w] = -INFINITY;
+            sum[w] = 0.f;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) acc[w][i] = f16acc{};
+        }
+    }
+
+    // Scores of 32 keys; `k`: the place of the lane's first chunk in LDS, the others are an XOR away.
+    __device__ __forceinline__ void scores(f16acc (&s)[RW], const uint8_t* lds, int k) const {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const u32x4 kf = *reinterpret_cast<const u32x4*>(lds + (k ^ (32 * ks)));
+#pragma unroll
+            for (int w = 0; w < RW; ++w) s[w] = mfma<DT>(kf, qf[w][ks], ks == 0 ? f16acc{} : s[w]);
+        }
+    }
+    // The largest x = c s + bias of 32 keys, and the base moved where a row outgrew it.  kc: what a score is multiplied with, of each 16 keys.
+    // full: every row of the wave sees every key.
+    template <class Scales>
+    __device__ __forceinline__ void raise(f16acc (&s)[RW], float (&kc)[RW][2], const Scales& sc, const float* bias, int key0, bool full, int g) {
+        if (Src::kNormalize && sc.k(0) + sc.k(1) != sc.k(0) + sc.k(1))      // a block without numbers
+#pragma unroll
+            for (int w = 0; w < RW; ++w)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (sc.k(i >> 3) != sc.k(i >> 3)) s[w][i] = NAN;
+        if (!Src::kBias && !full)
+#pragma unroll
+            for (int w = 0; w < RW; ++w)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + key_of(i, g) >= limit[w]) s[w][i] = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            float top = -INFINITY;
+            if constexpr (Src::kBias) {
+                // keys that are out, or past the end, have a bias of -inf and scores that are numbers
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const f32x4 add = *reinterpret_cast<const f32x4*>(bias + key_of(i, g));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[w][i + e] = fmaf(s[w][i + e], c[w], add[e]);
+                        top = fmaxf(top, s[w][i + e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // never 0, so that -inf stays that (a product of 0 comes from scores of 0, or a scale of 0)
+                    const float k = c[w] * sc.k(h);
+                    kc[w][h] = k > 1.17549435e-38f ? k : 1.17549435e-38f;
+                    float m = s[w][8 * h];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) m = fmaxf(m, s[w][8 * h + i]);
+                    top = fmaxf(top, fmaf(m, kc[w][h], sc.lv(h)));
+                }
+            }
+            top = half_max(top);
+            if (__any(top > base[w] + kLag)) {
+                const float nb = fmaxf(base[w], top), f = base[w] == -INFINITY ? 0.f : exp2f(base[w] - nb);
+                base[w] = nb;
+                sum[w] *= f;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) acc[w][i] *= f;
+            }
+        }
+    }
+    // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.
+    template <class Scales> __device__ __forceinline__ void probs(u32x4 (&p)[RW], const f16acc (&s)[RW], const float (&kc)[RW][2], const Scales& sc, int h) {
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            const float off = sc.lv(h) - (base[w] == -INFINITY ? 0.f : base[w]);
+            const auto prob = [&](float x) { return __builtin_amdgcn_exp2f(Src::kBias ? x + off : fmaf(x, kc[w][h], off)); };
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                p[w][i / 2] = pack2<DT>(prob(s[w][8 * h + i]), prob(s[w][8 * h + i + 1]));
+                part = add2<DT>(p[w][i / 2], part);
+            }
+            sum[w] = fmaf(part, sc.iv(h), sum[w]);
+        }
+    }
+    // acc += V^T p for those 16 keys; `v`: the lane's place in the first of their rows.
+    __device__ __forceinline__ void values(const u32x4 (&p)[RW], const uint8_t* lds, int v) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+            u32x2 half[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                half[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + (v ^ (64 * i)) + 8 * j * (2 * DP))));
+            const u32x4 vf = {half[0][0], half[0][1], half[1][0], half[1][1]};
+#pragma unroll
+            for (int w = 0; w < RW; ++w) acc[w][i] = mfma<DT>(vf, p[w], acc[w][i]);
+        }
+    }
+    template <class Stage> __device__ __forceinline__ void finish(const Stage& st, int key0, int key1) {
+#pragma unroll
+        for (int w = 0; w < RW; ++w) {
+            sum[w] = half_sum(sum[w]);
+            if (Src::kBias && base[w] == -INFINITY && sum[w] != sum[w] && !st.any_key(key0, key1)) {     // q is no number, and saw nothing
+                sum[w] = 0.f;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) acc[w][i] = f16acc{};
+            }
+        }
+    }
+};
+// The lane's places in a staged tile: chunk g of row col of K; of V the four rows and 16 channels that it turns.
+template <int DP> __device__ __forceinline__ int lane_k(int lane) { return k_place<DP>(lane & 31, lane >> 5); }
+template <int DP> __device__ __forceinline__ int lane_v(int lane) {
+    return v_place<DP>(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+}
+
+// Which tiles of TK keys a workgroup takes.
+__device__ __forceinline__ void share_of(int end, int tk, int splits, int split, int& t0, int& t1) {
+    t0 = 0;
+    t1 = end > 0 ? (end + tk - 1) / tk : 0;
+    if (splits > 1) {
+        const int share = (t1 + splits - 1) / splits;
+        t0 = min(t1, split * share);
+        t1 = min(t1, t0 + share);
+    }
+}
+
+// Many rows: four waves of 32 RW rows on the same keys, 64 at a time in two buffers.  A block's scores are multiplied under the
+// exponentials of the block before, so K runs 32 keys ahead of V: tile t is keys 64 t + 32 .. of K and 64 t .. of V.
+template <class Src, int DP, int RW>
+__global__ __launch_bounds__(256, DP * RW >= 256 ? 1 : 2) void tiles_kernel(const Common a, const typename Src::Args sa) {
+    constexpr int TK = 64, TILE = TK * DP * 2, WR = 32 * RW;
+    __shared__ __align__(16) uint8_t lds[4 * TILE];
+    __shared__ __align__(16) float bias[Src::kBias ? 2 * TK : 4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int row_tile = id % a.row_tiles;
     id /= a.row_tiles;
     const int split = id % a.splits, problem = id / a.splits;
     const Problem pr = Src::problem(sa, a, problem);
-    const int rows = pr.tokens * a.group, r0 = row_tile * 32 * QW;
+    const int rows = pr.tokens * a.group, r0 = row_tile * (4 * WR);
     if (r0 >= rows) return;     // the whole workgroup: rows of a shorter sequence
-    const int row = r0 + qw * 32 + col, token = (row < rows ? row : rows - 1) / a.group, head = (row < rows ? row : rows - 1) - token * a.group;
-    const int last_token = (min(rows, r0 + 32 * QW) - 1) / a.group;
-    const int limit = min(pr.keys, pr.limit0 + token);              // this lane's row
-    const int end = min(pr.keys, pr.limit0 + last_token);           // the workgroup's last key + 1
-    const int wave_first = min(rows - 1, r0 + qw * 32) / a.group;
-    const int all_see = min(pr.keys, pr.limit0 + wave_first);       // every row of the wave sees the keys below
+    Lanes<Src, DP, RW> L;
+    L.start(a, pr, r0 + wave * WR, rows, lane);
+    int t0, t1;
+    share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + 4 * WR) - 1) / a.group), TK, a.splits, split, t0, t1);
 
-    // the wave's share of the key tiles
-    int t0 = 0, t1 = end > 0 ? (end + TK - 1) / TK : 0;
-    if (a.splits > 1) {
-        const int share = (t1 + a.splits - 1) / a.splits;
-        t0 = min(t1, split * share);
-        t1 = min(t1, t0 + share);
+    typename Src::template Stage<DP, TK, 256> st(sa, a, problem, pr, threadIdx.x);
+    // K in the first two tiles of LDS, V in the others
+    int at_k = lane_k<DP>(lane), at_v = 2 * TILE + lane_v<DP>(lane);
+    f16acc s[2][RW];
+    if (t0 < t1) {
+        st.load_k(t0 * TK - 32);        // its second half: the first block
+        st.write_k(lds + TILE);
+        st.load_k(t0 * TK + 32);
+        st.load_v(t0 * TK);
+        __syncthreads();
+        L.scores(s[0], lds, at_k + TILE + 32 * 2 * DP);
+        st.write_k(lds);
+        st.write_v(lds + 2 * TILE, bias);
+        if (t0 + 1 < t1) {
+            st.load_k(t0 * TK + TK + 32);
+            st.load_v(t0 * TK + TK);
+        }
+        __syncthreads();
     }
-    if (KW > 1) {
+    int flip = 0;
+    for (int t = t0; t < t1; ++t) {
+        const float* const tb = bias + (Src::kBias ? flip * TK : 0);
+        const bool full = (t + 1) * TK <= L.all_see;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const auto sc = st.scales(t * TK + 32 * b);
+            float kc[RW][2];
+            L.raise(s[b], kc, sc, tb + 32 * b, t * TK + 32 * b, full, g);
+            L.scores(s[1 - b], lds, at_k + 32 * b * (2 * DP));
+            u32x4 p[2][RW];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) L.probs(p[h], s[b], kc, sc, h);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) L.values(p[h], lds, at_v + (32 * b + 16 * h) * (2 * DP));
+        }
+        flip ^= 1;
+        at_k ^= TILE;
+        at_v ^= TILE;
+        st.write_k(lds + flip * TILE);
+        st.write_v(lds + (2 + flip) * TILE, bias + (Src::kBias ? flip * TK : 0));
+        if (t + 2 < t1) {
+            st.load_k((t + 2) * TK + 32);
+            st.load_v((t + 2) * TK);
+        }
+        __syncthreads();
+    }
+    L.finish(st, t0 * TK, min(t1 * TK, pr.keys));
+
+    // Channels of register j of block i: 32 i + key_of(j, g).
+    const int64_t part_at = ((int64_t)split * a.problems + problem) * a.rows_padded;
+#pragma unroll
+    for (int w = 0; w < RW; ++w) {
+        if (L.row[w] >= rows) continue;
+        if (a.splits > 1) {
+            float* const pp = a.part + (part_at + L.row[w]) * (DP + 2);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) *reinterpret_cast<f32x2*>(pp + 32 * i + key_of(j, g)) = f32x2{L.acc[w][i][j], L.acc[w][i][j + 1]};
+            if (g == 0) *reinterpret_cast<f32x2*>(pp + DP) = f32x2{L.base[w], L.sum[w]};
+            continue;
+        }
+        const float inv = L.sum[w] == 0.f ? 0.f : Src::kOut / L.sum[w];
+        uint16_t* const op = (uint16_t*)a.o + pr.o_at + L.token[w] * a.o_rs + L.head[w] * a.o_hs;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                const int at = 32 * i + key_of(j, g);
+                if (at >= a.d) continue;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = L.acc[w][i][j + e] * inv;
+                const u32x2 u = a.q_dt == DT_BF16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])} : u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+                if (a.aligned & 2) *reinterpret_cast<u32x2*>(op + at) = u;
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) op[at + e] = (uint16_t)(u[e >> 1] >> 16 * (e & 1));
+            }
+    }
+}
+
+// Few rows: KW waves on the same 32, each with keys of its own, 32 at a time through its own piece of LDS; no barrier until they meet.
+template <class Src, int DP, int KW>
+__global__ __launch_bounds__(64 * KW, DP >= 256 ? 1 : 2) void few_kernel(const Common a, const typename Src::Args sa) {
+    constexpr int TK = 32, TILE = TK * DP * 2, DB = DP / 32;
+    __shared__ __align__(16) uint8_t lds[KW * 2 * TILE];
+    __shared__ __align__(16) float bias[Src::kBias ? KW * TK : 4];
+    __shared__ float stat[KW * 64];
+    const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    int id = xcd_contiguous(blockIdx.x, gridDim.x);
+    const int row_tile = id % a.row_tiles;
+    id /= a.row_tiles;
+    const int split = id % a.splits, problem = id / a.splits;
+    const Problem pr = Src::problem(sa, a, problem);
+    const int rows = pr.tokens * a.group, r0 = row_tile * 32;
+    if (r0 >= rows) return;
+    Lanes<Src, DP, 1> L;
+    L.start(a, pr, r0, rows, lane);
+    int t0, t1;
+    share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + 32) - 1) / a.group), TK, a.splits, split, t0, t1);
+    {
         const int share = (t1 - t0 + KW - 1) / KW;
         t0 = min(t1, t0 + kw * share);
         t1 = min(t1, t0 + share);
     }
-
-    // q: the lane's row in the order of the products' channels.  The 8-bit source multiplies f16: rows are scaled by a power of two there.
-    u32x4 qf[KS];
-    float c = a.c;
-    {
-        const uint16_t* qp = (const uint16_t*)a.q + pr.q_at + token * a.q_rs + head * a.q_hs;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int at = 16 * s + 8 * g;
-            qf[s] = at < a.d ? load8(qp + at, a.aligned & 1) : u32x4{0, 0, 0, 0};
-        }
-        const uint32_t flip = a.negate ? 0x80008000u : 0u;
-        if constexpr (Src::kNormalize) {
-            float m = 0.f;
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(elem(qf[s], i, a.q_dt)));
-            m = half_max(m);
-            const int e = m > 0.f && m < INFINITY ? ilogbf(m) : 0;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                u32x4 f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = pack_f16x2(ldexpf(elem(qf[s], 2 * i, a.q_dt), -e), ldexpf(elem(qf[s], 2 * i + 1, a.q_dt), -e)) ^ flip;
-                qf[s] = f;
-            }
-            c = ldexpf(c, e);
-        } else {
-#pragma unroll
-            for (int s = 0; s < KS; ++s) qf[s] ^= flip;
-        }
-    }
-
-    f16acc acc[DB];
-#pragma unroll
-    for (int i = 0; i < DB; ++i) acc[i] = f16acc{};
-    float base = -INFINITY, sum = 0.f;
-
-    typename Src::template Stage<DP, TK, 64 * QW> st(sa, a, problem, pr, tid);
-    uint8_t* const mine = lds + kw * (NBUF * 2 * TILE);
-    float* const my_bias = bias + (Src::kBias ? kw * (NBUF * TK) : 0);
-    const auto sync = [] {
-        if (QW > 1) __syncthreads();
-        else {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-        }
+    typename Src::template Stage<DP, TK, 64> st(sa, a, problem, pr, lane);
+    uint8_t* const mine = lds + kw * (2 * TILE);
+    float* const my_bias = bias + (Src::kBias ? kw * TK : 0);
+    const auto fence = [] {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     };
-    if (t0 < t1) st.load(t0);
-    if (NBUF == 2 && t0 < t1) {
-        st.write(mine, mine + TILE, my_bias);
-        if (t0 + 1 < t1) st.load(t0 + 1);
-        sync();
+    const int at_k = lane_k<DP>(lane), at_v = TILE + lane_v<DP>(lane);
+    if (t0 < t1) {
+        st.load_k(t0 * TK);
+        st.load_v(t0 * TK);
     }
     for (int t = t0; t < t1; ++t) {
-        uint8_t* const kb = mine + (NBUF == 2 ? ((t - t0) & 1) * 2 * TILE : 0);
-        uint8_t* const vb = kb + TILE;
-        float* const tb = my_bias + (Src::kBias && NBUF == 2 ? ((t - t0) & 1) * TK : 0);
-        const auto scales = st.scales(NBUF == 2 && t + 1 < t1);
-        if (NBUF == 1) {
-            sync();
-            st.write(kb, vb, tb);
-            if (t + 1 < t1) st.load(t + 1);
-            sync();
+        const auto sc = st.scales(t * TK);
+        fence();
+        st.write_k(mine);
+        st.write_v(mine + TILE, my_bias);
+        if (t + 1 < t1) {
+            st.load_k((t + 1) * TK);
+            st.load_v((t + 1) * TK);
         }
-        f16acc s[NB];
+        fence();
+        f16acc s[1];
+        float kc[1][2];
+        L.scores(s, mine, at_k);
+        L.raise(s, kc, sc, my_bias, t * TK, (t + 1) * TK <= L.all_see, g);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) s[b] = f16acc{};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) s[b] = mfma<DT>(*reinterpret_cast<const u32x4*>(kb + k_place<DP>(32 * b + col, 2 * ks + g)), qf[ks], s[b]);
-
-        // x = c s (+ bias), and the largest of the tile
-        const int k0 = t * TK;
-        float top = -INFINITY;
-        const bool plain = !Src::kBias && k0 + TK <= all_see;
-        if (plain) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float m = s[b][8 * h];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) m = fmaxf(m, s[b][8 * h + i]);
-                    top = fmaxf(top, fmaf(m, c * scales.k(2 * b + h), scales.lv(2 * b + h)));
-                }
-        } else {
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = 32 * b + key_of(i, g);
-                    const float add = Src::kBias ? tb[key] : 0.f;
-                    const float x = fmaf(s[b][i], c * scales.k(2 * b + (i >> 3)), add);
-                    s[b][i] = k0 + key < limit && add != -INFINITY ? x : -INFINITY;
-                    top = fmaxf(top, s[b][i] + scales.lv(2 * b + (i >> 3)));
-                }
-        }
-        top = half_max(top);
-        if (__any(top > base + kLag)) {
-            const float nb = fmaxf(base, top), f = base == -INFINITY ? 0.f : exp2f(base - nb);
-            base = nb;
-            sum *= f;
-#pragma unroll
-            for (int i = 0; i < DB; ++i) acc[i] *= f;
-        }
-        const float from = base == -INFINITY ? 0.f : base;
-
-        uint32_t p[NB][8];
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float kc = plain ? c * scales.k(2 * b + h) : 1.f, off = scales.lv(2 * b + h) - from;
-                float part = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float x0 = s[b][8 * h + i], x1 = s[b][8 * h + i + 1];
-                    const float p0 = __builtin_amdgcn_exp2f(plain ? fmaf(x0, kc, off) : x0 + off), p1 = __builtin_amdgcn_exp2f(plain ? fmaf(x1, kc, off) : x1 + off);
-                    part += p0 + p1;
-                    p[b][4 * h + i / 2] = pack2<DT>(p0, p1);
-                }
-                sum = fmaf(part, scales.iv(2 * b + h), sum);
-            }
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 pf = {p[b][4 * h], p[b][4 * h + 1], p[b][4 * h + 2], p[b][4 * h + 3]};
-#pragma unroll
-                for (int i = 0; i < DB; ++i) {
-                    u32x2 half[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int r = 32 * b + 16 * h + 8 * j + 4 * g + ((lane & 15) >> 2), chunk = 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                        half[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4*)(vb + v_place<DP>(r, chunk) + 8 * (lane & 1))));
-                    }
-                    acc[i] = mfma<DT>(u32x4{half[0][0], half[0][1], half[1][0], half[1][1]}, pf, acc[i]);
-                }
-            }
-        if (NBUF == 2) {
-            if (t + 1 < t1) {
-                uint8_t* const nk = mine + ((t + 1 - t0) & 1) * 2 * TILE;
-                st.write(nk, nk + TILE, my_bias + (Src::kBias ? ((t + 1 - t0) & 1) * TK : 0));
-                if (t + 2 < t1) st.load(t + 2);
-            }
-            sync();
+        for (int h = 0; h < 2; ++h) {
+            u32x4 p[1];
+            L.probs(p, s, kc, sc, h);
+            L.values(p, mine, at_v + 16 * h * (2 * DP));
         }
     }
-    sum = half_sum(sum);
+    L.finish(st, t0 * TK, min(t1 * TK, pr.keys));
 
-    // Channels of register j of block i: 32 i + key_of(j, g).
     const int64_t part_at = ((int64_t)split * a.problems + problem) * a.rows_padded;
-    if constexpr (KW > 1) {
-        __syncthreads();
-        float* const mo = reinterpret_cast<float*>(lds) + kw * 32 * DP;
+    __syncthreads();
+    float* const mo = reinterpret_cast<float*>(lds) + kw * 32 * DP;
 #pragma unroll
-        for (int i = 0; i < DB; ++i)
+    for (int i = 0; i < DB; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) mo[(32 * i + key_of(j, g)) * 32 + col] = acc[i][j];
-        if (g == 0) {
-            stat[kw * 64 + col] = base;
-            stat[kw * 64 + 32 + col] = sum;
+        for (int j = 0; j < 16; ++j) mo[(32 * i + key_of(j, g)) * 32 + col] = L.acc[0][i][j];
+    if (g == 0) {
+        stat[kw * 64 + col] = L.base[0];
+        stat[kw * 64 + 32 + col] = L.sum[0];
+    }
+    __syncthreads();
+    // every wave adds a part of the channels: DP / KW of them for its lane's row
+    float nb = -INFINITY, w[KW];
+#pragma unroll
+    for (int k = 0; k < KW; ++k) nb = fmaxf(nb, stat[k * 64 + col]);
+    float l = 0.f;
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+        const float b = stat[k * 64 + col];
+        w[k] = b == -INFINITY ? 0.f : exp2f(b - nb);
+        l = fmaf(stat[k * 64 + 32 + col], w[k], l);
+    }
+    if (L.row[0] >= rows) return;
+    constexpr int EACH = DP / KW / 2;      // channels of a lane
+    const int d0 = kw * (DP / KW) + g * EACH;
+    const float inv = l == 0.f ? 0.f : Src::kOut / l;
+    uint16_t* const op = (uint16_t*)a.o + pr.o_at + L.token[0] * a.o_rs + L.head[0] * a.o_hs;
+    float* const pp = a.part + (part_at + L.row[0]) * (DP + 2);
+#pragma unroll
+    for (int j = 0; j < EACH; j += 4) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KW; ++k) v[e] = fmaf(reinterpret_cast<const float*>(lds)[(k * DP + d0 + j + e) * 32 + col], w[k], v[e]);
         }
-        __syncthreads();
-        // every wave adds a part of the channels: DP / KW of them for its lane's row
-        float nb = -INFINITY, w[KW];
-#pragma unroll
-        for (int k = 0; k < KW; ++k) nb = fmaxf(nb, stat[k * 64 + col]);
-        float l = 0.f;
-#pragma unroll
-        for (int k = 0; k < KW; ++k) {
-            const float b = stat[k * 64 + col];
-            w[k] = b == -INFINITY ? 0.f : exp2f(b - nb);
-            l = fmaf(stat[k * 64 + 32 + col], w[k], l);
-        }
-        if (row >= rows) return;
-        constexpr int EACH = DP / KW / 2;      // channels of a lane
-        const int d0 = kw * (DP / KW) + g * EACH;
-        const float inv = l == 0.f ? 0.f : Src::kOut / l;
-        uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + head * a.o_hs;
-        float* const pp = a.part + (part_at + row) * (DP + 2);
-#pragma unroll
-        for (int j = 0; j < EACH; j += 4) {
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = 0.f;
-#pragma unroll
-                for (int k = 0; k < KW; ++k) v[e] = fmaf(reinterpret_cast<const float*>(lds)[(k * DP + d0 + j + e) * 32 + col], w[k], v[e]);
-            }
-            if (a.splits > 1) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pp[d0 + j + e] = v[e];
-            } else if (d0 + j < a.d) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) op[d0 + j + e] = a.q_dt == DT_BF16 ? f_to_bf16(v[e] * inv) : f_to_f16(v[e] * inv);
-            }
-        }
-        if (a.splits > 1 && kw == 0 && g == 0) {
-            pp[DP] = nb;
-            pp[DP + 1] = l;
-        }
-    } else {
-        if (row >= rows) return;
         if (a.splits > 1) {
-            float* const pp = a.part + (part_at + row) * (DP + 2);
 #pragma unroll
-            for (int i = 0; i < DB; ++i)
+            for (int e = 0; e < 4; ++e) pp[d0 + j + e] = v[e];
+        } else if (d0 + j < a.d) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) pp[32 * i + key_of(j, g)] = acc[i][j];
-            if (g == 0) {
-                pp[DP] = base;
-                pp[DP + 1] = sum;
-            }
-        } else {
-            const float inv = sum == 0.f ? 0.f : Src::kOut / sum;
-            uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + head * a.o_hs;
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    const int at = 32 * i + key_of(j, g);
-                    if (at >= a.d) continue;
-                    float v[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j + e] * inv;
-                    const u32x2 u = a.q_dt == DT_BF16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])} : u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
-                    if (a.aligned & 2) *reinterpret_cast<u32x2*>(op + at) = u;
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) op[at + e] = (uint16_t)(u[e >> 1] >> 16 * (e & 1));
-                }
+            for (int e = 0; e < 4; ++e) op[d0 + j + e] = a.q_dt == DT_BF16 ? f_to_bf16(v[e] * inv) : f_to_f16(v[e] * inv);
         }
+    }
+    if (a.splits > 1 && kw == 0 && g == 0) {
+        pp[DP] = nb;
+        pp[DP + 1] = l;
     }
 }
 
@@ -421,6 +547,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
     const int dp = padded_dim(d);
     p.few = rows <= 32;
     p.rows = p.few ? 32 : 128;
+    if (!p.few && dp < 256 && getenv("RW2")) p.rows = 256;
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     const int64_t groups = p.row_tiles * problems, want = 2 * (int64_t)device_cu_count();
     const int64_t least = p.few ? 256 : 512;       // keys that are worth a workgroup
@@ -434,8 +561,10 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
 template <class Src, int DP> inline int launch(const Plan& p, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid > 0x7fffffff) return -1;
-    if (p.few) rows_kernel<Src, DP, 1, DP == 256 ? 2 : 4, 32><<<(int)grid, DP == 256 ? 128 : 256, 0, stream>>>(a, sa);
-    else rows_kernel<Src, DP, 4, 1, DP == 256 ? 32 : 64><<<(int)grid, 256, 0, stream>>>(a, sa);
+    constexpr int KW = DP == 256 ? 2 : 4;
+    if (p.few) few_kernel<Src, DP, KW><<<(int)grid, 64 * KW, 0, stream>>>(a, sa);
+    else if (p.rows == 128) tiles_kernel<Src, DP, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if constexpr (DP < 256) tiles_kernel<Src, DP, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     KCHECK();
     if (p.splits > 1) {
         join_kernel<Src, DP><<<a.problems * a.rows_padded, DP, 0, stream>>>(a, sa);

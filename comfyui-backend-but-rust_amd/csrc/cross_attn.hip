@@ -15,11 +15,15 @@ struct CrossArgs {
     int64_t mask_bs;
 };
 
-// What a key's mask adds to its exponent (in units of log2): -inf takes the key out.  A finite bias stays finite, so that the type's
-// lowest value is what it is in the formula: a logit like any other.
-__device__ __forceinline__ float key_bias(const CrossArgs& a, const void* mask, int key) {
-    if (a.mask_kind == 1) return ((const uint8_t*)mask)[key] ? 0.f : -INFINITY;
-    const float b = ((const float*)mask)[key], x = b * kLog2e;
+// What a key's mask holds, and what that adds to its exponent (in units of log2): -inf takes the key out.  A finite bias stays finite, so
+// that the type's lowest value is what it is in the formula: a logit like any other.
+__device__ __forceinline__ uint32_t mask_word(const CrossArgs& a, const void* mask, int key) {
+    return a.mask_kind == 1 ? ((const uint8_t*)mask)[key] : ((const uint32_t*)mask)[key];
+}
+__device__ __forceinline__ bool is_out(const CrossArgs& a, uint32_t w) { return w == (a.mask_kind == 1 ? 0u : 0xff800000u); }
+__device__ __forceinline__ float key_bias(const CrossArgs& a, uint32_t w) {
+    if (a.mask_kind == 1) return w ? 0.f : -INFINITY;
+    const float b = u2f(w), x = b * kLog2e;
     return fabsf(b) < INFINITY && fabsf(x) == INFINITY ? copysignf(3.402823466e38f, b) : x;
 }
 
@@ -50,35 +54,74 @@ template <int DTYPE, bool BIAS> struct Dense {
         const void* mask;
         int tid, keys, d;
         u32x4 kr[CH], vr[CH];
-        float out[BIAS ? CH : 1], add;
+        uint32_t k_mask[BIAS ? CH : 1], v_mask[BIAS ? CH : 1], row_mask;     // as they lie in memory: looked at when they have arrived
+        int row_key;
         __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_) : a(a_), tid(tid_), keys(p.keys), d(c.d) {
             const int b = id / c.hk, head = id - b * c.hk;
             k = a.k + b * a.k_bs + head * a.k_hs;
             v = a.v + b * a.v_bs + head * a.v_hs;
             mask = a.mask_kind == 1 ? (const void*)((const uint8_t*)a.mask + b * a.mask_bs) : (const void*)((const float*)a.mask + b * a.mask_bs);
         }
-        __device__ __forceinline__ void load(int t) {
+        // K rows from key0 (which may lie before the first) into registers; V rows with what their keys' masks say
+        __device__ __forceinline__ void rows(u32x4 (&x)[CH], const uint16_t* p, int64_t rs, int key0) {
+            if (a.aligned && d == DP && key0 >= 0 && key0 + TK <= keys) {     // whole rows of 16-byte pieces: a scalar base and 32-bit offsets
+                const char* const at = (const char*)(p + (int64_t)key0 * rs);
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const int i = tid + j * NT;
+                    x[j] = *reinterpret_cast<const u32x4*>(at + (uint32_t)(2 * (i / ROW * (int)rs + 8 * (i % ROW))));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const int i = tid + j * NT, key = key0 + i / ROW, ch = i % ROW;
+                    x[j] = key >= 0 && key < keys && 8 * ch < d ? load8(p + key * rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
+                }
+            }
+        }
+        __device__ __forceinline__ void load_k(int key0) {
+            rows(kr, k, a.k_rs, key0);
+            if (BIAS)
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const int key = key0 + (tid + j * NT) / ROW;
+                    k_mask[j] = key >= 0 && key < keys ? mask_word(a, mask, key) : 1u;
+                }
+        }
+        __device__ __forceinline__ void load_v(int key0) {
+            rows(vr, v, a.v_rs, key0);
+            if (BIAS) {
+#pragma unroll
+                for (int j = 0; j < CH; ++j) {
+                    const int key = key0 + (tid + j * NT) / ROW;
+                    v_mask[j] = key < keys ? mask_word(a, mask, key) : 1u;
+                }
+                row_key = key0 + tid;
+                if (tid < TK) row_mask = row_key < keys ? mask_word(a, mask, row_key) : 1u;
+            }
+        }
+        // a key that is out has probability 0, and its value must be a number for the product to leave it out, its score for the bias to
+        __device__ __forceinline__ void write_k(uint8_t* kb) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
-                const int i = tid + j * NT, r = i / ROW, ch = i % ROW, key = t * TK + r;
-                const bool there = key < keys && 8 * ch < d;
-                kr[j] = there ? load8(k + key * a.k_rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
-                vr[j] = there ? load8(v + key * a.v_rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
-                if (BIAS) out[j] = there ? key_bias(a, mask, key) : 0.f;
+                const int i = tid + j * NT;
+                *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, k_mask[j]) ? u32x4{0, 0, 0, 0} : kr[j];
             }
-            if (BIAS && tid < TK) add = t * TK + tid < keys ? key_bias(a, mask, t * TK + tid) : -INFINITY;
         }
-        // a key that is out has probability 0, and its value must be a number for the product to leave it out
-        __device__ __forceinline__ void write(uint8_t* kb, uint8_t* vb, float* bias) {
+        __device__ __forceinline__ void write_v(uint8_t* vb, float* bias) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
-                const int i = tid + j * NT, r = i / ROW, ch = i % ROW;
-                *reinterpret_cast<u32x4*>(kb + k_place<DP>(r, ch)) = kr[j];
-                *reinterpret_cast<u32x4*>(vb + v_place<DP>(r, ch)) = BIAS && out[j] == -INFINITY ? u32x4{0, 0, 0, 0} : vr[j];
+                const int i = tid + j * NT;
+                *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, v_mask[j]) ? u32x4{0, 0, 0, 0} : vr[j];
             }
-            if (BIAS && tid < TK) bias[tid] = add;
+            if (BIAS && tid < TK) bias[tid] = row_key < keys ? key_bias(a, row_mask) : -INFINITY;
         }
-        __device__ __forceinline__ Scales scales(bool) const { return {}; }
+        __device__ __forceinline__ bool any_key(int from, int to) const {
+            for (int i = from; i < to; ++i)
+                if (!is_out(a, mask_word(a, mask, i))) return true;
+            return false;
+        }
+        __device__ __forceinline__ Scales scales(int) const { return {}; }
     };
 };
 
@@ -110,7 +153,9 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     CrossArgs s{};
     s.k = (const uint16_t*)k; s.v = (const uint16_t*)v;
     s.q_bs = q_bs; s.o_bs = o_bs; s.k_bs = k_bs; s.k_rs = k_rs; s.k_hs = k_hs; s.v_bs = v_bs; s.v_rs = v_rs; s.v_hs = v_hs;
-    s.lq = lq; s.lk = lk; s.aligned = sixteen(k, k_bs, k_rs, k_hs) && sixteen(v, v_bs, v_rs, v_hs);
+    // (and rows of a tile within 32-bit offsets of its first)
+    const bool near = k_rs < (1 << 23) && v_rs < (1 << 23) && k_rs >= 0 && v_rs >= 0;
+    s.lq = lq; s.lk = lk; s.aligned = near && sixteen(k, k_bs, k_rs, k_hs) && sixteen(v, v_bs, v_rs, v_hs);
     s.k_lens = k_lens; s.mask = mask; s.mask_kind = mask_kind; s.mask_bs = mask_bs;
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == DT_BF16) return mask_kind ? launch_dim<Dense<DT_BF16, true>>(p, c, s, st) : launch_dim<Dense<DT_BF16, false>>(p, c, s, st);

@@ -24,11 +24,11 @@ struct Codes {
     // iv is 2^16 / A, so that sums of both ends of A's range, 2^-90 and 2^128, stay ordinary numbers; a smaller A counts as 2^-90, and as
     // 2^-60 of the largest so far, so that p' does not leave fp32
     static constexpr float kOut = 65536.f / 127.f;
-    template <int N> struct Scales {
-        float ks[N], lvs[N], ivs[N];
-        __device__ float k(int i) const { return ks[i]; }
-        __device__ float lv(int i) const { return lvs[i]; }
-        __device__ float iv(int i) const { return ivs[i]; }
+    struct Scales {
+        float ks[2], lvs[2], ivs[2];
+        __device__ float k(int h) const { return ks[h]; }
+        __device__ float lv(int h) const { return lvs[h]; }
+        __device__ float iv(int h) const { return ivs[h]; }
     };
     static __device__ __forceinline__ Problem problem(const Args& a, const Common& c, int id) {
         const int s = id / c.hk, head = id - s * c.hk;
@@ -44,26 +44,30 @@ struct Codes {
         return p;
     }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int ROW = DP / 16, CH = TK * ROW / NT, NS = TK / kBlock;
+        static constexpr int ROW = DP / 16, CH = TK * ROW / NT;
         const Args& a;
         const int32_t* table;
-        int tid, lane, keys, d, hk, head, window = -1;
-        int pid;                         // of block 64 * window + lane, and its scales
-        float ks, lv, iv, top = 0.f;
+        int tid, lane, keys, d, hk, head;
+        int k_window = -1, v_window = -1, s_window = -1;
+        int k_page, v_page;              // of block 64 * window + lane
+        float ks, lv, iv, top = 0.f;     // its scales
         u32x4 kr[CH], vr[CH];
-        Scales<NS> now, next;
         __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_)
             : a(a_), tid(tid_), lane(threadIdx.x & 63), keys(p.keys), d(c.d), hk(c.hk) {
             const int s = id / c.hk;
             head = id - s * c.hk;
             table = a.table + (int64_t)s * a.table_cols;
         }
+        // the page of a block, 0 for one that none holds: what is read there counts for nothing, or for NaN
+        __device__ __forceinline__ int page(int block) const {
+            const int p = page_of(table, a.table_cols, a.n_pages, a.page_shift, block);
+            return p < 0 ? 0 : p;
+        }
         __device__ __forceinline__ void look(int w) {
-            window = w;
-            const int block = 64 * w + lane, page = page_of(table, a.table_cols, a.n_pages, a.page_shift, block);
-            const bool there = block < (keys + kBlock - 1) / kBlock, ok = page >= 0;
-            pid = there && ok ? page : 0;
-            const int64_t i = scale_at(pid, hk, head, a.page_shift, block);
+            s_window = w;
+            const int block = 64 * w + lane, p = page_of(table, a.table_cols, a.n_pages, a.page_shift, block);
+            const bool there = block < (keys + kBlock - 1) / kBlock, ok = p >= 0;
+            const int64_t i = scale_at(there && ok ? p : 0, hk, head, a.page_shift, block);
             // a block of no page, or whose values are no numbers, makes the scores NaN: rows that do not see it put -inf there
             const float A = there && ok ? a.vs[i] : 0.f;
             const bool good = A >= 0.f && A < INFINITY;
@@ -74,39 +78,56 @@ struct Codes {
             lv = __builtin_amdgcn_logf(u);
             iv = 65536.f / u;
         }
-        __device__ __forceinline__ void load(int t) {
-            const int b0 = t * NS;
-            if (b0 >> 6 != window) look(b0 >> 6);
-            now = next;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                next.ks[i] = u2f(__builtin_amdgcn_readlane(f2u(ks), (b0 + i) & 63));
-                next.lvs[i] = u2f(__builtin_amdgcn_readlane(f2u(lv), (b0 + i) & 63));
-                next.ivs[i] = u2f(__builtin_amdgcn_readlane(f2u(iv), (b0 + i) & 63));
-            }
+        // TK rows from key0, a multiple of 32 that may lie before the first, where block 0 is read instead
+        __device__ __forceinline__ void rows(u32x4 (&x)[CH], const int8_t* codes, int& window, int& pages, int key0) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
-                const int i = tid + j * NT, r = i / ROW, ch = i % ROW, token = t * TK + r;
-                const int page = __builtin_amdgcn_readlane(pid, __builtin_amdgcn_readfirstlane(token >> 4) & 63);
-                const int64_t at = ((((int64_t)page * hk + head) << a.page_shift) + (token & ((1 << a.page_shift) - 1))) * d + 16 * ch;
-                const bool there = 16 * ch < d;
-                kr[j] = there ? *reinterpret_cast<const u32x4*>(a.k + at) : u32x4{0, 0, 0, 0};
-                vr[j] = there ? *reinterpret_cast<const u32x4*>(a.v + at) : u32x4{0, 0, 0, 0};
-            }
-        }
-        __device__ __forceinline__ void write(uint8_t* kb, uint8_t* vb, float*) {
-#pragma unroll
-            for (int j = 0; j < CH; ++j) {
-                const int i = tid + j * NT, r = i / ROW, ch = i % ROW;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    *reinterpret_cast<u32x4*>(kb + k_place<DP>(r, 2 * ch + e)) = bytes_to_f16(kr[j][2 * e], kr[j][2 * e + 1]);
-                    *reinterpret_cast<u32x4*>(vb + v_place<DP>(r, 2 * ch + e)) = bytes_to_f16(vr[j][2 * e], vr[j][2 * e + 1]);
+                const int i = tid + j * NT, token = key0 + i / ROW, ch = i % ROW;
+                // the rows that a wave loads at once lie in one block: a scalar base and 32-bit offsets
+                const int b = __builtin_amdgcn_readfirstlane(token >> 4), block = b < 0 ? 0 : b;
+                if (block >> 6 != window) {
+                    window = block >> 6;
+                    pages = page(64 * window + lane);
                 }
+                const int64_t at = codes_at(__builtin_amdgcn_readlane(pages, block & 63), hk, head, a.page_shift, block, d);
+                const uint32_t in = (token & (kBlock - 1)) * d + 16 * ch;
+                x[j] = 16 * ch < d ? *reinterpret_cast<const u32x4*>(codes + at + in) : u32x4{0, 0, 0, 0};
             }
         }
-        // of the tile that is multiplied next; `ahead`: the one behind it has been asked for already
-        __device__ __forceinline__ Scales<NS> scales(bool ahead) const { return ahead ? now : next; }
+        __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, k_window, k_page, key0); }
+        __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, v_window, v_page, key0); }
+        __device__ __forceinline__ void write_k(uint8_t* kb) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int i = tid + j * NT;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, 2 * (i % ROW) + e)) = bytes_to_f16(kr[j][2 * e], kr[j][2 * e + 1]);
+            }
+        }
+        __device__ __forceinline__ void write_v(uint8_t* vb, float*) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int i = tid + j * NT;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, 2 * (i % ROW) + e)) = bytes_to_f16(vr[j][2 * e], vr[j][2 * e + 1]);
+            }
+        }
+        __device__ bool any_key(int, int) const { return true; }
+        // of the 32 keys from key0
+        __device__ __forceinline__ Scales scales(int key0) {
+            const int block = __builtin_amdgcn_readfirstlane(key0 >> 4);
+            if (block >> 6 != s_window) look(block >> 6);
+            Scales r;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                r.ks[h] = u2f(__builtin_amdgcn_readlane(f2u(ks), (block + h) & 63));
+                r.lvs[h] = u2f(__builtin_amdgcn_readlane(f2u(lv), (block + h) & 63));
+                r.ivs[h] = u2f(__builtin_amdgcn_readlane(f2u(iv), (block + h) & 63));
+            }
+            return r;
+        }
     };
 };
 
