@@ -1,7 +1,7 @@
 // Attention of query rows to stored states: the kernel that cross_attn.hip (16-bit keys and values) and kv8_attn.hip (pages of 8-bit
 // codes) share.  What differs is where a tile of keys and values comes from: a Source.
 //
-//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(x_j - base),   x_j = c s_j + bias_j (in units of log2),   s_j = q . k_j
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(x_j - base),   x_j = c s_j (in units of log2),   s_j = q . k_j + bias_j / scale
 //
 // One pass over the keys with a running base (the maximum so far, moved only when a row outgrows it by 2^kLag) and sum, both in fp32.
 //
@@ -60,14 +60,13 @@ __device__ __forceinline__ float half_sum(float v) {
 // Key, within a block of 32, of accumulator register i in the half wave g.
 __device__ __forceinline__ constexpr int key_of(int i, int g) { return (i & 3) + 8 * (i >> 2) + 4 * g; }
 
-// Byte position of an 8-element chunk of a staged row, rows of DP 16-bit elements.  K rows are read 16 bytes a lane, 16 rows at a time:
-// the XOR spreads one chunk of 16 rows over all banks.  V rows are read by the transposing read, four rows of 64 bytes at a time.
-template <int DP> __device__ __forceinline__ int k_place(int row, int chunk) {
-    return row * (2 * DP) + 16 * (chunk ^ (DP == 64 ? (row >> 1) & 7 : row & 15));
-}
-template <int DP> __device__ __forceinline__ int v_place(int row, int chunk) {
-    return row * (2 * DP) + 16 * (chunk ^ (DP == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2));
-}
+// A staged tile's rows of DP 16-bit elements, and byte positions in it.  K rows are read 16 bytes a lane, 16 rows at a time: 16 bytes behind
+// each row spread one chunk of 16 rows over all banks.  V rows are read by the transposing read, 64 bytes of four rows at a time: 64 bytes
+// behind each row.  (An XOR of the chunk does the same without the room, but costs an instruction a read where a constant offset is free.)
+template <int DP> constexpr int kRowK = 2 * DP + 16;
+template <int DP> constexpr int kRowV = 2 * DP + 64;
+template <int DP> __device__ __forceinline__ int k_place(int row, int chunk) { return row * kRowK<DP> + 16 * chunk; }
+template <int DP> __device__ __forceinline__ int v_place(int row, int chunk) { return row * kRowV<DP> + 16 * chunk; }
 
 // Eight signed bytes as f16, exactly: 0x6400 | u is 1024 + u in f16, and codes are u - 128.
 __device__ __forceinline__ u32x4 bytes_to_f16(uint32_t lo, uint32_t hi) {
@@ -93,11 +92,21 @@ struct Common {
     int hk, group, d, q_dt;
     int row_tiles, problems, splits;   // grid: row_tiles * problems (batch x hk) * splits
     int aligned;                       // q rows start on 16 bytes (bit 0), o rows on 8 (bit 1)
-    float c;                           // scale * log2 e, its sign in `negate`
-    int negate;
+    float c;                           // |scale| log2 e; 1 where that is 0
+    uint32_t q_and, q_xor;             // what q's words take: a negative scale flips their signs, a scale of 0 makes them 0
     float* part;                       // [splits][problems][rows padded to tiles][DP + 2] where splits > 1
     int rows_padded;
 };
+
+inline void set_scale(Common& c, float scale) {
+    c.c = fabsf(scale) * kLog2e;
+    c.q_and = 0xffffffffu;
+    c.q_xor = scale < 0.f ? 0x80008000u : 0u;
+    if (c.c == 0.f) {
+        c.c = 1.f;
+        c.q_and = c.q_xor = 0u;
+    }
+}
 
 __device__ __forceinline__ u32x4 load8(const uint16_t* p, bool aligned) {
     if (aligned) return *reinterpret_cast<const u32x4*>(p);
@@ -151,7 +160,6 @@ template <class Src, int DP, int RW> struct Lanes {
                 for (int s = 0; s < KS; ++s) qf[w][s] = 16 * s + 8 * g < a.d ? load8(qp + 16 * s + 8 * g, false) : u32x4{0, 0, 0, 0};
             }
         }
-        const uint32_t flip = a.negate ? 0x80008000u : 0u;
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             // The 8-bit source multiplies f16: rows are scaled by a power of two there.
@@ -167,13 +175,13 @@ template <class Src, int DP, int RW> struct Lanes {
                 for (int s = 0; s < KS; ++s) {
                     u32x4 f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) f[i] = pack_f16x2(ldexpf(elem(qf[w][s], 2 * i, a.q_dt), -e), ldexpf(elem(qf[w][s], 2 * i + 1, a.q_dt), -e)) ^ flip;
+                    for (int i = 0; i < 4; ++i) f[i] = pack_f16x2(ldexpf(elem(qf[w][s], 2 * i, a.q_dt), -e), ldexpf(elem(qf[w][s], 2 * i + 1, a.q_dt), -e)) & a.q_and ^ a.q_xor;
                     qf[w][s] = f;
                 }
                 c[w] = ldexpf(c[w], e);
             } else {
 #pragma unroll
-                for (int s = 0; s < KS; ++s) qf[w][s] ^= flip;
+                for (int s = 0; s < KS; ++s) qf[w][s] = qf[w][s] & a.q_and ^ a.q_xor;
             }
             base[w] = -INFINITY;
             sum[w] = 0.f;
@@ -182,19 +190,29 @@ template <class Src, int DP, int RW> struct Lanes {
         }
     }
 
-    // Scores of 32 keys; `k`: the place of the lane's first chunk in LDS, the others are an XOR away.
-    __device__ __forceinline__ void scores(f16acc (&s)[RW], const uint8_t* lds, int k) const {
+    // Scores of 32 keys; `k`: the lane's first chunk in LDS.  A key's bias is what its score starts with, in units of the score: -inf for one
+    // that is out or past the end, whose K is numbers.
+    __device__ __forceinline__ void scores(f16acc (&s)[RW], const uint8_t* k, const float* bias, int g) const {
+        f16acc from{};
+        if constexpr (Src::kBias)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const f32x4 add = *reinterpret_cast<const f32x4*>(bias + key_of(i, g));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) from[i + e] = add[e];
+            }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const u32x4 kf = *reinterpret_cast<const u32x4*>(lds + (k ^ (32 * ks)));
+            const u32x4 kf = *reinterpret_cast<const u32x4*>(k + 32 * ks);
 #pragma unroll
-            for (int w = 0; w < RW; ++w) s[w] = mfma<DT>(kf, qf[w][ks], ks == 0 ? f16acc{} : s[w]);
+            for (int w = 0; w < RW; ++w) s[w] = mfma<DT>(kf, qf[w][ks], ks == 0 ? from : s[w]);
         }
     }
-    // The largest x = c s + bias of 32 keys, and the base moved where a row outgrew it.  kc: what a score is multiplied with, of each 16 keys.
+    // The largest x of 32 keys, and the base moved where a row outgrew it.  kc: what a score is multiplied with, of each 16 keys;
+    // from: what is taken off that.
     // full: every row of the wave sees every key.
     template <class Scales>
-    __device__ __forceinline__ void raise(f16acc (&s)[RW], float (&kc)[RW][2], const Scales& sc, const float* bias, int key0, bool full, int g) {
+    __device__ __forceinline__ void raise(f16acc (&s)[RW], float (&kc)[RW][2], float (&from)[RW], const Scales& sc, int key0, bool full, int g) {
         if (Src::kNormalize && sc.k(0) + sc.k(1) != sc.k(0) + sc.k(1))      // a block without numbers
 #pragma unroll
             for (int w = 0; w < RW; ++w)
@@ -210,28 +228,15 @@ template <class Src, int DP, int RW> struct Lanes {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             float top = -INFINITY;
-            if constexpr (Src::kBias) {
-                // keys that are out, or past the end, have a bias of -inf and scores that are numbers
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const f32x4 add = *reinterpret_cast<const f32x4*>(bias + key_of(i, g));
+            for (int h = 0; h < 2; ++h) {
+                // never 0, so that -inf stays that (a product of 0 comes from scores of 0, or a scale of 0)
+                const float k = c[w] * sc.k(h);
+                kc[w][h] = k > 1.17549435e-38f ? k : 1.17549435e-38f;
+                float m = s[w][8 * h];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[w][i + e] = fmaf(s[w][i + e], c[w], add[e]);
-                        top = fmaxf(top, s[w][i + e]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    // never 0, so that -inf stays that (a product of 0 comes from scores of 0, or a scale of 0)
-                    const float k = c[w] * sc.k(h);
-                    kc[w][h] = k > 1.17549435e-38f ? k : 1.17549435e-38f;
-                    float m = s[w][8 * h];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) m = fmaxf(m, s[w][8 * h + i]);
-                    top = fmaxf(top, fmaf(m, kc[w][h], sc.lv(h)));
-                }
+                for (int i = 1; i < 8; ++i) m = fmaxf(m, s[w][8 * h + i]);
+                top = fmaxf(top, fmaf(m, kc[w][h], sc.lv(h)));
             }
             top = half_max(top);
             if (__any(top > base[w] + kLag)) {
@@ -241,14 +246,22 @@ template <class Src, int DP, int RW> struct Lanes {
 #pragma unroll
                 for (int i = 0; i < DB; ++i) acc[w][i] *= f;
             }
+            from[w] = base[w] == -INFINITY ? 0.f : base[w];
+            // far out (a bias like the type's lowest value) a fused c s - base would show how base was rounded: the rounded product does not
+            if (Src::kBias && __any(fabsf(from[w]) > 262144.f)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[w][i] = s[w][i] * kc[w][i >> 3] - from[w];
+                kc[w][0] = kc[w][1] = 1.f;
+                from[w] = 0.f;
+            }
         }
     }
     // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.
-    template <class Scales> __device__ __forceinline__ void probs(u32x4 (&p)[RW], const f16acc (&s)[RW], const float (&kc)[RW][2], const Scales& sc, int h) {
+    template <class Scales> __device__ __forceinline__ void probs(u32x4 (&p)[RW], const f16acc (&s)[RW], const float (&kc)[RW][2], const float (&from)[RW], const Scales& sc, int h) {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
-            const float off = sc.lv(h) - (base[w] == -INFINITY ? 0.f : base[w]);
-            const auto prob = [&](float x) { return __builtin_amdgcn_exp2f(Src::kBias ? x + off : fmaf(x, kc[w][h], off)); };
+            const float off = sc.lv(h) - from[w];
+            const auto prob = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, kc[w][h], off)); };
             float part = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
@@ -259,13 +272,13 @@ template <class Src, int DP, int RW> struct Lanes {
         }
     }
     // acc += V^T p for those 16 keys; `v`: the lane's place in the first of their rows.
-    __device__ __forceinline__ void values(const u32x4 (&p)[RW], const uint8_t* lds, int v) {
+    __device__ __forceinline__ void values(const u32x4 (&p)[RW], const uint8_t* v) {
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
             u32x2 half[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                half[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + (v ^ (64 * i)) + 8 * j * (2 * DP))));
+                half[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + 64 * i + 8 * j * kRowV<DP>)));
             const u32x4 vf = {half[0][0], half[0][1], half[1][0], half[1][1]};
 #pragma unroll
             for (int w = 0; w < RW; ++w) acc[w][i] = mfma<DT>(vf, p[w], acc[w][i]);
@@ -300,12 +313,12 @@ __device__ __forceinline__ void share_of(int end, int tk, int splits, int split,
     }
 }
 
-// Many rows: four waves of 32 RW rows on the same keys, 64 at a time in two buffers.  A block's scores are multiplied under the
-// exponentials of the block before, so K runs 32 keys ahead of V: tile t is keys 64 t + 32 .. of K and 64 t .. of V.
-template <class Src, int DP, int RW>
-__global__ __launch_bounds__(256, DP * RW >= 256 ? 1 : 2) void tiles_kernel(const Common a, const typename Src::Args sa) {
-    constexpr int TK = 64, TILE = TK * DP * 2, WR = 32 * RW;
-    __shared__ __align__(16) uint8_t lds[4 * TILE];
+// Many rows: QW waves of 32 RW rows on the same keys, 32 NB at a time in two buffers: a tile is on its way into registers while the one
+// before goes into LDS and the one before that is multiplied.
+template <class Src, int DP, int RW, int QW, int NB, int OCC>
+__global__ __launch_bounds__(64 * QW, DP * RW >= 256 ? 1 : 2) void tiles_kernel(const Common a, const typename Src::Args sa) {
+    constexpr int TK = 32 * NB, WR = 32 * RW, TILE_K = TK * kRowK<DP>, TILE_V = TK * kRowV<DP>;
+    __shared__ __align__(16) uint8_t lds[2 * (TILE_K + TILE_V)];
     __shared__ __align__(16) float bias[Src::kBias ? 2 * TK : 4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
@@ -313,58 +326,58 @@ __global__ __launch_bounds__(256, DP * RW >= 256 ? 1 : 2) void tiles_kernel(cons
     id /= a.row_tiles;
     const int split = id % a.splits, problem = id / a.splits;
     const Problem pr = Src::problem(sa, a, problem);
-    const int rows = pr.tokens * a.group, r0 = row_tile * (4 * WR);
+    const int rows = pr.tokens * a.group, r0 = row_tile * (QW * WR);
     if (r0 >= rows) return;     // the whole workgroup: rows of a shorter sequence
+    int t0, t1;
+    share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + QW * WR) - 1) / a.group), TK, a.splits, split, t0, t1);
+    typename Src::template Stage<DP, TK, 64 * QW> st(sa, a, problem, pr, threadIdx.x);
+    if (t0 < t1) {
+        st.load_k(t0 * TK);
+        st.load_v(t0 * TK);
+    }
     Lanes<Src, DP, RW> L;
     L.start(a, pr, r0 + wave * WR, rows, lane);
-    int t0, t1;
-    share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + 4 * WR) - 1) / a.group), TK, a.splits, split, t0, t1);
 
-    typename Src::template Stage<DP, TK, 256> st(sa, a, problem, pr, threadIdx.x);
-    // K in the first two tiles of LDS, V in the others
-    int at_k = lane_k<DP>(lane), at_v = 2 * TILE + lane_v<DP>(lane);
-    f16acc s[2][RW];
+    uint8_t *kb = lds, *vb = lds + 2 * TILE_K;                       // the tile that is multiplied
+    uint8_t *kn = lds + TILE_K, *vn = lds + 2 * TILE_K + TILE_V;     // and the one behind it
+    float *tb = bias, *tn = bias + (Src::kBias ? TK : 0);
+    const int at_k = lane_k<DP>(lane), at_v = lane_v<DP>(lane);
     if (t0 < t1) {
-        st.load_k(t0 * TK - 32);        // its second half: the first block
-        st.write_k(lds + TILE);
-        st.load_k(t0 * TK + 32);
-        st.load_v(t0 * TK);
-        __syncthreads();
-        L.scores(s[0], lds, at_k + TILE + 32 * 2 * DP);
-        st.write_k(lds);
-        st.write_v(lds + 2 * TILE, bias);
+        st.write_k(kb);
+        st.write_v(vb, tb);
         if (t0 + 1 < t1) {
-            st.load_k(t0 * TK + TK + 32);
+            st.load_k(t0 * TK + TK);
             st.load_v(t0 * TK + TK);
         }
         __syncthreads();
     }
-    int flip = 0;
     for (int t = t0; t < t1; ++t) {
-        const float* const tb = bias + (Src::kBias ? flip * TK : 0);
-        const bool full = (t + 1) * TK <= L.all_see;
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const auto sc = st.scales(t * TK + 32 * b);
-            float kc[RW][2];
-            L.raise(s[b], kc, sc, tb + 32 * b, t * TK + 32 * b, full, g);
-            L.scores(s[1 - b], lds, at_k + 32 * b * (2 * DP));
-            u32x4 p[2][RW];
+        for (int b = 0; b < NB; ++b) {
+            const int key0 = t * TK + 32 * b;
+            const auto sc = st.scales(key0);
+            f16acc s[RW];
+            float kc[RW][2], from[RW];
+            L.scores(s, kb + at_k + 32 * b * kRowK<DP>, tb + 32 * b, g);
+            L.raise(s, kc, from, sc, key0, key0 + 32 <= L.all_see, g);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) L.probs(p[h], s[b], kc, sc, h);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) L.values(p[h], lds, at_v + (32 * b + 16 * h) * (2 * DP));
+            for (int h = 0; h < 2; ++h) {
+                u32x4 p[RW];
+                L.probs(p, s, kc, from, sc, h);
+                L.values(p, vb + at_v + (32 * b + 16 * h) * kRowV<DP>);
+            }
         }
-        flip ^= 1;
-        at_k ^= TILE;
-        at_v ^= TILE;
-        st.write_k(lds + flip * TILE);
-        st.write_v(lds + (2 + flip) * TILE, bias + (Src::kBias ? flip * TK : 0));
+        // (behind the last tile the registers hold it still, and nothing reads where it goes)
+        st.write_k(kn);
+        st.write_v(vn, tn);
         if (t + 2 < t1) {
-            st.load_k((t + 2) * TK + 32);
+            st.load_k((t + 2) * TK);
             st.load_v((t + 2) * TK);
         }
         __syncthreads();
+        uint8_t* const k = kb; kb = kn; kn = k;
+        uint8_t* const v = vb; vb = vn; vn = v;
+        float* const f = tb; tb = tn; tn = f;
     }
     L.finish(st, t0 * TK, min(t1 * TK, pr.keys));
 
@@ -405,8 +418,8 @@ __global__ __launch_bounds__(256, DP * RW >= 256 ? 1 : 2) void tiles_kernel(cons
 // Few rows: KW waves on the same 32, each with keys of its own, 32 at a time through its own piece of LDS; no barrier until they meet.
 template <class Src, int DP, int KW>
 __global__ __launch_bounds__(64 * KW, DP >= 256 ? 1 : 2) void few_kernel(const Common a, const typename Src::Args sa) {
-    constexpr int TK = 32, TILE = TK * DP * 2, DB = DP / 32;
-    __shared__ __align__(16) uint8_t lds[KW * 2 * TILE];
+    constexpr int TK = 32, TILE_K = TK * kRowK<DP>, TILE = TILE_K + TK * kRowV<DP>, DB = DP / 32;
+    __shared__ __align__(16) uint8_t lds[KW * TILE];
     __shared__ __align__(16) float bias[Src::kBias ? KW * TK : 4];
     __shared__ float stat[KW * 64];
     const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
@@ -417,8 +430,6 @@ __global__ __launch_bounds__(64 * KW, DP >= 256 ? 1 : 2) void few_kernel(const C
     const Problem pr = Src::problem(sa, a, problem);
     const int rows = pr.tokens * a.group, r0 = row_tile * 32;
     if (r0 >= rows) return;
-    Lanes<Src, DP, 1> L;
-    L.start(a, pr, r0, rows, lane);
     int t0, t1;
     share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + 32) - 1) / a.group), TK, a.splits, split, t0, t1);
     {
@@ -427,36 +438,38 @@ __global__ __launch_bounds__(64 * KW, DP >= 256 ? 1 : 2) void few_kernel(const C
         t1 = min(t1, t0 + share);
     }
     typename Src::template Stage<DP, TK, 64> st(sa, a, problem, pr, lane);
-    uint8_t* const mine = lds + kw * (2 * TILE);
+    uint8_t* const mine = lds + kw * TILE;
     float* const my_bias = bias + (Src::kBias ? kw * TK : 0);
     const auto fence = [] {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    const int at_k = lane_k<DP>(lane), at_v = TILE + lane_v<DP>(lane);
+    const int at_k = lane_k<DP>(lane), at_v = TILE_K + lane_v<DP>(lane);
     if (t0 < t1) {
         st.load_k(t0 * TK);
         st.load_v(t0 * TK);
     }
+    Lanes<Src, DP, 1> L;
+    L.start(a, pr, r0, rows, lane);
     for (int t = t0; t < t1; ++t) {
         const auto sc = st.scales(t * TK);
         fence();
         st.write_k(mine);
-        st.write_v(mine + TILE, my_bias);
+        st.write_v(mine + TILE_K, my_bias);
         if (t + 1 < t1) {
             st.load_k((t + 1) * TK);
             st.load_v((t + 1) * TK);
         }
         fence();
         f16acc s[1];
-        float kc[1][2];
-        L.scores(s, mine, at_k);
-        L.raise(s, kc, sc, my_bias, t * TK, (t + 1) * TK <= L.all_see, g);
+        float kc[1][2], from[1];
+        L.scores(s, mine + at_k, my_bias, g);
+        L.raise(s, kc, from, sc, t * TK, (t + 1) * TK <= L.all_see, g);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             u32x4 p[1];
-            L.probs(p, s, kc, sc, h);
-            L.values(p, mine, at_v + 16 * h * (2 * DP));
+            L.probs(p, s, kc, from, sc, h);
+            L.values(p, mine + at_v + 16 * h * kRowV<DP>);
         }
     }
     L.finish(st, t0 * TK, min(t1 * TK, pr.keys));
@@ -547,13 +560,14 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
     const int dp = padded_dim(d);
     p.few = rows <= 32;
     p.rows = p.few ? 32 : 128;
-    if (!p.few && dp < 256 && getenv("RW2")) p.rows = 256;
+    if (!p.few && dp < 256 && getenv("QW8")) p.rows = 256;
     p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
     const int64_t groups = p.row_tiles * problems, want = 2 * (int64_t)device_cu_count();
     const int64_t least = p.few ? 256 : 512;       // keys that are worth a workgroup
     int64_t s = groups >= want ? 1 : (want + groups - 1) / (groups > 0 ? groups : 1);
     const int64_t most = keys / least > 1 ? keys / least : 1;
     p.splits = (int)(s < most ? s : most);
+    if (getenv("SPL")) p.splits = atoi(getenv("SPL"));
     p.bytes = p.splits > 1 ? 4 * p.splits * problems * p.row_tiles * p.rows * (dp + 2) : 0;
     return p;
 }
@@ -563,8 +577,11 @@ template <class Src, int DP> inline int launch(const Plan& p, Common& a, const t
     if (grid > 0x7fffffff) return -1;
     constexpr int KW = DP == 256 ? 2 : 4;
     if (p.few) few_kernel<Src, DP, KW><<<(int)grid, 64 * KW, 0, stream>>>(a, sa);
-    else if (p.rows == 128) tiles_kernel<Src, DP, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
-    else if constexpr (DP < 256) tiles_kernel<Src, DP, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if (p.rows == 128) { if (getenv("NB2")) tiles_kernel<Src, DP, 1, 4, 2, DP == 64 ? 4 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+       else tiles_kernel<Src, DP, 1, 4, 1, DP == 64 ? 4 : 2><<<(int)grid, 256, 0, stream>>>(a, sa); }
+    else if (getenv("NB2")) tiles_kernel<Src, DP, 1, 8, 2, DP == 64 ? 4 : 2><<<(int)grid, 512, 0, stream>>>(a, sa);
+    else tiles_kernel<Src, DP, 1, 8, 1, DP == 64 ? 4 : 2><<<(int)grid, 512, 0, stream>>>(a, sa);
     KCHECK();
     if (p.splits > 1) {
         join_kernel<Src, DP><<<a.problems * a.rows_padded, DP, 0, stream>>>(a, sa);

@@ -13,18 +13,19 @@ struct CrossArgs {
     const void* mask;
     int mask_kind;          // 1: bytes, 0 = out; 2: f32, added to the logits
     int64_t mask_bs;
+    float per_score, most;  // a bias in units of the score, and its largest magnitude: still a number in units of log2
 };
 
-// What a key's mask holds, and what that adds to its exponent (in units of log2): -inf takes the key out.  A finite bias stays finite, so
-// that the type's lowest value is what it is in the formula: a logit like any other.
+// What a key's mask holds, and what that adds to its score: -inf takes the key out.  A finite bias stays finite, so that the type's lowest
+// value is what it is in the formula: a logit like any other.
 __device__ __forceinline__ uint32_t mask_word(const CrossArgs& a, const void* mask, int key) {
     return a.mask_kind == 1 ? ((const uint8_t*)mask)[key] : ((const uint32_t*)mask)[key];
 }
 __device__ __forceinline__ bool is_out(const CrossArgs& a, uint32_t w) { return w == (a.mask_kind == 1 ? 0u : 0xff800000u); }
 __device__ __forceinline__ float key_bias(const CrossArgs& a, uint32_t w) {
     if (a.mask_kind == 1) return w ? 0.f : -INFINITY;
-    const float b = u2f(w), x = b * kLog2e;
-    return fabsf(b) < INFINITY && fabsf(x) == INFINITY ? copysignf(3.402823466e38f, b) : x;
+    const float b = u2f(w), x = b * a.per_score;
+    return fabsf(b) < INFINITY && !(fabsf(x) < a.most) ? copysignf(a.most, b) : x;
 }
 
 template <int DTYPE, bool BIAS> struct Dense {
@@ -48,7 +49,10 @@ template <int DTYPE, bool BIAS> struct Dense {
         return p;
     }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int CH = TK * DP / 8 / NT, ROW = DP / 8;
+        static constexpr int ROW = DP / 8, CH = (TK * ROW + NT - 1) / NT;
+        static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
+        static_assert(kAll || (CH == 1 && TK <= NT), "some threads are without a piece");
+        __device__ __forceinline__ bool mine() const { return kAll || tid < TK * ROW; }
         const Args& a;
         const uint16_t *k, *v;
         const void* mask;
@@ -64,6 +68,7 @@ template <int DTYPE, bool BIAS> struct Dense {
         }
         // K rows from key0 (which may lie before the first) into registers; V rows with what their keys' masks say
         __device__ __forceinline__ void rows(u32x4 (&x)[CH], const uint16_t* p, int64_t rs, int key0) {
+            if (!mine()) return;
             if (a.aligned && d == DP && key0 >= 0 && key0 + TK <= keys) {     // whole rows of 16-byte pieces: a scalar base and 32-bit offsets
                 const char* const at = (const char*)(p + (int64_t)key0 * rs);
 #pragma unroll
@@ -81,7 +86,7 @@ template <int DTYPE, bool BIAS> struct Dense {
         }
         __device__ __forceinline__ void load_k(int key0) {
             rows(kr, k, a.k_rs, key0);
-            if (BIAS)
+            if (BIAS && mine())
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
                     const int key = key0 + (tid + j * NT) / ROW;
@@ -91,6 +96,7 @@ template <int DTYPE, bool BIAS> struct Dense {
         __device__ __forceinline__ void load_v(int key0) {
             rows(vr, v, a.v_rs, key0);
             if (BIAS) {
+                if (mine())
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
                     const int key = key0 + (tid + j * NT) / ROW;
@@ -105,14 +111,14 @@ template <int DTYPE, bool BIAS> struct Dense {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
-                *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, k_mask[j]) ? u32x4{0, 0, 0, 0} : kr[j];
+                if (mine()) *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, k_mask[j]) ? u32x4{0, 0, 0, 0} : kr[j];
             }
         }
         __device__ __forceinline__ void write_v(uint8_t* vb, float* bias) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
-                *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, v_mask[j]) ? u32x4{0, 0, 0, 0} : vr[j];
+                if (mine()) *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, v_mask[j]) ? u32x4{0, 0, 0, 0} : vr[j];
             }
             if (BIAS && tid < TK) bias[tid] = row_key < keys ? key_bias(a, row_mask) : -INFINITY;
         }
@@ -149,8 +155,11 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
     c.row_tiles = p.row_tiles; c.problems = b * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
     c.aligned = (sixteen(q, q_bs, q_rs, q_hs) ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_bs | o_rs | o_hs) % 4 == 0 ? 2 : 0);
-    c.c = fabsf(scale) * kLog2e; c.negate = scale < 0.f; c.part = (float*)ws;
+    set_scale(c, scale);
+    c.part = (float*)ws;
     CrossArgs s{};
+    s.per_score = (float)(1.4426950408889634 / c.c);
+    s.most = 3e38f / (c.c > 1.f ? c.c : 1.f);
     s.k = (const uint16_t*)k; s.v = (const uint16_t*)v;
     s.q_bs = q_bs; s.o_bs = o_bs; s.k_bs = k_bs; s.k_rs = k_rs; s.k_hs = k_hs; s.v_bs = v_bs; s.v_rs = v_rs; s.v_hs = v_hs;
     // (and rows of a tile within 32-bit offsets of its first)

@@ -44,7 +44,10 @@ struct Codes {
         return p;
     }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int ROW = DP / 16, CH = TK * ROW / NT;
+        static constexpr int ROW = DP / 16, CH = (TK * ROW + NT - 1) / NT;
+        static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
+        static_assert(kAll || (CH == 1 && TK * ROW % 64 == 0), "whole waves are without a piece");
+        __device__ __forceinline__ bool mine() const { return kAll || tid < TK * ROW; }
         const Args& a;
         const int32_t* table;
         int tid, lane, keys, d, hk, head;
@@ -80,6 +83,7 @@ struct Codes {
         }
         // TK rows from key0, a multiple of 32 that may lie before the first, where block 0 is read instead
         __device__ __forceinline__ void rows(u32x4 (&x)[CH], const int8_t* codes, int& window, int& pages, int key0) {
+            if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT, token = key0 + i / ROW, ch = i % ROW;
@@ -97,6 +101,7 @@ struct Codes {
         __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, k_window, k_page, key0); }
         __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, v_window, v_page, key0); }
         __device__ __forceinline__ void write_k(uint8_t* kb) {
+            if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
@@ -106,6 +111,7 @@ struct Codes {
             }
         }
         __device__ __forceinline__ void write_v(uint8_t* vb, float*) {
+            if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
@@ -154,7 +160,8 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
     c.row_tiles = p.row_tiles; c.problems = n * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
     c.aligned = ((uintptr_t)q % 16 == 0 && (q_rs | q_hs) % 8 == 0 ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_rs | o_hs) % 4 == 0 ? 2 : 0);
-    c.c = fabsf(scale) * kLog2e; c.negate = scale < 0.f; c.part = (float*)ws;
+    set_scale(c, scale);
+    c.part = (float*)ws;
     CacheArgs s{k, v, k_scale, v_scale, starts, lens, table, rows, most, n_pages, __builtin_ctz(page), table_cols, causal != 0};
     return launch_dim<Codes>(p, c, s, (hipStream_t)stream);
 }

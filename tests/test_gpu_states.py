@@ -98,6 +98,7 @@ def test_cross_attn(shape, dtype):
     _cross_check(ql.cross_attn(q, k, v, scale, None, keep), q, k, v, scale, None, keep, what="mask")
     bias = torch.where(torch.rand(b, lk, device=DEV, generator=_gen(3)) < 0.2, -math.inf, 2 * torch.randn(b, lk, device=DEV, generator=_gen(4)))
     _cross_check(ql.cross_attn(q, k, v, -scale, lens, bias), q, k, v, -scale, lens, bias, what="bias, lengths and a negative scale")
+    _cross_check(ql.cross_attn(q, k, v, 0.0, lens, bias), q, k, v, 0.0, lens, bias, what="no scale")
 
 
 @pytest.mark.parametrize("lq", [1, 40, 150])
