@@ -19,7 +19,6 @@
 #include "common.hpp"
 
 #include <math.h>
-#include <stdlib.h>
 
 namespace states {
 
@@ -190,54 +189,61 @@ template <class Src, int DP, int RW> struct Lanes {
         }
     }
 
-    // Scores of 32 keys; `k`: the lane's first chunk in LDS.  A key's bias is what its score starts with, in units of the score: -inf for one
-    // that is out or past the end, whose K is numbers.
-    __device__ __forceinline__ void scores(f16acc (&s)[RW], const uint8_t* k, const float* bias, int g) const {
-        f16acc from{};
-        if constexpr (Src::kBias)
+    // Scores of NB blocks of 32 keys; `k`: the lane's first chunk in LDS.  A key's bias is what its score starts with, in units of the score:
+    // -inf for one that is out or past the end, whose K is numbers.
+    template <int NB> __device__ __forceinline__ void scores(f16acc (&s)[NB][RW], const uint8_t* k, const float* bias, int g) const {
+        f16acc from[NB];
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const f32x4 add = *reinterpret_cast<const f32x4*>(bias + key_of(i, g));
+        for (int b = 0; b < NB; ++b) {
+            from[b] = f16acc{};
+            if constexpr (Src::kBias)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) from[i + e] = add[e];
-            }
+                for (int i = 0; i < 16; i += 4) {
+                    const f32x4 add = *reinterpret_cast<const f32x4*>(bias + 32 * b + key_of(i, g));
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const u32x4 kf = *reinterpret_cast<const u32x4*>(k + 32 * ks);
-#pragma unroll
-            for (int w = 0; w < RW; ++w) s[w] = mfma<DT>(kf, qf[w][ks], ks == 0 ? from : s[w]);
+                    for (int e = 0; e < 4; ++e) from[b][i + e] = add[e];
+                }
         }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const u32x4 kf = *reinterpret_cast<const u32x4*>(k + 32 * b * kRowK<DP> + 32 * ks);
+#pragma unroll
+                for (int w = 0; w < RW; ++w) s[b][w] = mfma<DT>(kf, qf[w][ks], ks == 0 ? from[b] : s[b][w]);
+            }
     }
-    // The largest x of 32 keys, and the base moved where a row outgrew it.  kc: what a score is multiplied with, of each 16 keys;
-    // from: what is taken off that.
-    // full: every row of the wave sees every key.
-    template <class Scales>
-    __device__ __forceinline__ void raise(f16acc (&s)[RW], float (&kc)[RW][2], float (&from)[RW], const Scales& sc, int key0, bool full, int g) {
-        if (Src::kNormalize && sc.k(0) + sc.k(1) != sc.k(0) + sc.k(1))      // a block without numbers
+    // The largest x of NB blocks of 32 keys from key0, and the base moved where a row outgrew it.  kc: what a score is multiplied with, of
+    // each 16 keys; from: what is taken off that.  plain: every row of the wave sees every key, and every block is numbers.
+    template <int NB, class Scales>
+    __device__ __forceinline__ void raise(f16acc (&s)[NB][RW], float (&kc)[RW][2 * NB], float (&from)[RW], const Scales& sc, int key0, bool plain, int g) {
+        if (!Src::kBias && !plain) {
 #pragma unroll
-            for (int w = 0; w < RW; ++w)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (sc.k(i >> 3) != sc.k(i >> 3)) s[w][i] = NAN;
-        if (!Src::kBias && !full)
+                for (int w = 0; w < RW; ++w)
 #pragma unroll
-            for (int w = 0; w < RW; ++w)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (key0 + key_of(i, g) >= limit[w]) s[w][i] = -INFINITY;
+                    for (int i = 0; i < 16; ++i) {
+                        if (Src::kNormalize && sc.k(2 * b + (i >> 3)) != sc.k(2 * b + (i >> 3))) s[b][w][i] = NAN;      // a block without numbers
+                        if (key0 + 32 * b + key_of(i, g) >= limit[w]) s[b][w][i] = -INFINITY;
+                    }
+        }
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
-            float top = -INFINITY;
+            float tops[2 * NB];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                // never 0, so that -inf stays that (a product of 0 comes from scores of 0, or a scale of 0)
+            for (int h = 0; h < 2 * NB; ++h) {
+                // never 0, so that -inf stays that (a block of zeros has scores of 0)
                 const float k = c[w] * sc.k(h);
                 kc[w][h] = k > 1.17549435e-38f ? k : 1.17549435e-38f;
-                float m = s[w][8 * h];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) m = fmaxf(m, s[w][8 * h + i]);
-                top = fmaxf(top, fmaf(m, kc[w][h], sc.lv(h)));
+                const f16acc& x = s[h >> 1][w];
+                const int i = 8 * (h & 1);
+                const float m = fmaxf(fmaxf(fmaxf(fmaxf(x[i], x[i + 1]), x[i + 2]), fmaxf(fmaxf(x[i + 3], x[i + 4]), x[i + 5])), fmaxf(x[i + 6], x[i + 7]));
+                tops[h] = fmaf(m, kc[w][h], sc.lv(h));
             }
+            float top = tops[0];
+#pragma unroll
+            for (int h = 1; h < 2 * NB; ++h) top = fmaxf(top, tops[h]);
             top = half_max(top);
             if (__any(top > base[w] + kLag)) {
                 const float nb = fmaxf(base[w], top), f = base[w] == -INFINITY ? 0.f : exp2f(base[w] - nb);
@@ -250,24 +256,29 @@ template <class Src, int DP, int RW> struct Lanes {
             // far out (a bias like the type's lowest value) a fused c s - base would show how base was rounded: the rounded product does not
             if (Src::kBias && __any(fabsf(from[w]) > 262144.f)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[w][i] = s[w][i] * kc[w][i >> 3] - from[w];
-                kc[w][0] = kc[w][1] = 1.f;
+                for (int h = 0; h < 2 * NB; ++h) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s[h >> 1][w][8 * (h & 1) + i] = s[h >> 1][w][8 * (h & 1) + i] * kc[w][h] - from[w];
+                    kc[w][h] = 1.f;
+                }
                 from[w] = 0.f;
             }
         }
     }
     // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.
-    template <class Scales> __device__ __forceinline__ void probs(u32x4 (&p)[RW], const f16acc (&s)[RW], const float (&kc)[RW][2], const float (&from)[RW], const Scales& sc, int h) {
+    template <int NB, class Scales>
+    __device__ __forceinline__ void probs(u32x4 (&p)[RW], const f16acc (&s)[NB][RW], const float (&kc)[RW][2 * NB], const float (&from)[RW], const Scales& sc, int h) {
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
             const float off = sc.lv(h) - from[w];
-            const auto prob = [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, kc[w][h], off)); };
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][w][8 * (h & 1) + i], kc[w][h], off));
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) p[w][i / 2] = pack2<DT>(e[i], e[i + 1]);
             float part = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                p[w][i / 2] = pack2<DT>(prob(s[w][8 * h + i]), prob(s[w][8 * h + i + 1]));
-                part = add2<DT>(p[w][i / 2], part);
-            }
+            for (int i = 0; i < 4; ++i) part = add2<DT>(p[w][i], part);
             sum[w] = fmaf(part, sc.iv(h), sum[w]);
         }
     }
@@ -302,6 +313,16 @@ template <int DP> __device__ __forceinline__ int lane_v(int lane) {
     return v_place<DP>(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
 }
 
+// The scales of a tile from block h0 on.
+template <class Scales> struct Part {
+    const Scales& all;
+    const int h0;
+    __device__ __forceinline__ float k(int h) const { return all.k(h0 + h); }
+    __device__ __forceinline__ float lv(int h) const { return all.lv(h0 + h); }
+    __device__ __forceinline__ float iv(int h) const { return all.iv(h0 + h); }
+};
+template <class Scales> __device__ __forceinline__ Part<Scales> part_of(const Scales& all, int h0) { return {all, h0}; }
+
 // Which tiles of TK keys a workgroup takes.
 __device__ __forceinline__ void share_of(int end, int tk, int splits, int split, int& t0, int& t1) {
     t0 = 0;
@@ -315,8 +336,8 @@ __device__ __forceinline__ void share_of(int end, int tk, int splits, int split,
 
 // Many rows: QW waves of 32 RW rows on the same keys, 32 NB at a time in two buffers: a tile is on its way into registers while the one
 // before goes into LDS and the one before that is multiplied.
-template <class Src, int DP, int RW, int QW, int NB, int OCC>
-__global__ __launch_bounds__(64 * QW, DP * RW >= 256 ? 1 : 2) void tiles_kernel(const Common a, const typename Src::Args sa) {
+template <class Src, int DP, int RW, int QW, int NB, int SB, int OCC>
+__global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, const typename Src::Args sa) {
     constexpr int TK = 32 * NB, WR = 32 * RW, TILE_K = TK * kRowK<DP>, TILE_V = TK * kRowV<DP>;
     __shared__ __align__(16) uint8_t lds[2 * (TILE_K + TILE_V)];
     __shared__ __align__(16) float bias[Src::kBias ? 2 * TK : 4];
@@ -343,8 +364,8 @@ __global__ __launch_bounds__(64 * QW, DP * RW >= 256 ? 1 : 2) void tiles_kernel(
     float *tb = bias, *tn = bias + (Src::kBias ? TK : 0);
     const int at_k = lane_k<DP>(lane), at_v = lane_v<DP>(lane);
     if (t0 < t1) {
-        st.write_k(kb);
-        st.write_v(vb, tb);
+        st.write_k(kb, tb);
+        st.write_v(vb);
         if (t0 + 1 < t1) {
             st.load_k(t0 * TK + TK);
             st.load_v(t0 * TK + TK);
@@ -352,24 +373,25 @@ __global__ __launch_bounds__(64 * QW, DP * RW >= 256 ? 1 : 2) void tiles_kernel(
         __syncthreads();
     }
     for (int t = t0; t < t1; ++t) {
+        const auto all = st.scales(t * TK);
+        const bool plain = st.numbers() && (t + 1) * TK <= L.all_see;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int key0 = t * TK + 32 * b;
-            const auto sc = st.scales(key0);
-            f16acc s[RW];
-            float kc[RW][2], from[RW];
+        for (int b = 0; b < NB; b += SB) {
+            const auto sc = part_of(all, 2 * b);
+            f16acc s[SB][RW];
+            float kc[RW][2 * SB], from[RW];
             L.scores(s, kb + at_k + 32 * b * kRowK<DP>, tb + 32 * b, g);
-            L.raise(s, kc, from, sc, key0, key0 + 32 <= L.all_see, g);
+            L.raise(s, kc, from, sc, t * TK + 32 * b, plain, g);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2 * SB; ++h) {
                 u32x4 p[RW];
                 L.probs(p, s, kc, from, sc, h);
                 L.values(p, vb + at_v + (32 * b + 16 * h) * kRowV<DP>);
             }
         }
         // (behind the last tile the registers hold it still, and nothing reads where it goes)
-        st.write_k(kn);
-        st.write_v(vn, tn);
+        st.write_k(kn, tn);
+        st.write_v(vn);
         if (t + 2 < t1) {
             st.load_k((t + 2) * TK);
             st.load_v((t + 2) * TK);
@@ -454,17 +476,17 @@ __global__ __launch_bounds__(64 * KW, DP >= 256 ? 1 : 2) void few_kernel(const C
     for (int t = t0; t < t1; ++t) {
         const auto sc = st.scales(t * TK);
         fence();
-        st.write_k(mine);
-        st.write_v(mine + TILE_K, my_bias);
+        st.write_k(mine, my_bias);
+        st.write_v(mine + TILE_K);
         if (t + 1 < t1) {
             st.load_k((t + 1) * TK);
             st.load_v((t + 1) * TK);
         }
         fence();
-        f16acc s[1];
+        f16acc s[1][1];
         float kc[1][2], from[1];
         L.scores(s, mine + at_k, my_bias, g);
-        L.raise(s, kc, from, sc, t * TK, (t + 1) * TK <= L.all_see, g);
+        L.raise(s, kc, from, sc, t * TK, st.numbers() && (t + 1) * TK <= L.all_see, g);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             u32x4 p[1];
@@ -549,39 +571,60 @@ __global__ __launch_bounds__(DP) void join_kernel(const Common a, const typename
     *op = a.q_dt == DT_BF16 ? f_to_bf16(r) : f_to_f16(r);
 }
 
-// How a call runs: rows of 32 with the keys over a workgroup's waves, or tiles of more rows; and over how many workgroups the keys of a row go.
+// How a call runs: 32 rows with the keys over a workgroup's waves, or tiles of 128 or 256 rows; and over how many workgroups the keys of a
+// row go.
 struct Plan {
-    int few, rows, row_tiles, splits;
+    int rows, row_tiles, splits;
     int64_t bytes;     // workspace
 };
 inline int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
+inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp) {
     Plan p;
-    const int dp = padded_dim(d);
-    p.few = rows <= 32;
-    p.rows = p.few ? 32 : 128;
-    if (!p.few && dp < 256 && getenv("QW8")) p.rows = 256;
-    p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
-    const int64_t groups = p.row_tiles * problems, want = 2 * (int64_t)device_cu_count();
-    const int64_t least = p.few ? 256 : 512;       // keys that are worth a workgroup
-    int64_t s = groups >= want ? 1 : (want + groups - 1) / (groups > 0 ? groups : 1);
-    const int64_t most = keys / least > 1 ? keys / least : 1;
-    p.splits = (int)(s < most ? s : most);
-    if (getenv("SPL")) p.splits = atoi(getenv("SPL"));
-    p.bytes = p.splits > 1 ? 4 * p.splits * problems * p.row_tiles * p.rows * (dp + 2) : 0;
+    p.rows = tile;
+    p.row_tiles = (int)((rows + tile - 1) / tile);
+    p.splits = splits;
+    p.bytes = splits > 1 ? 4 * splits * problems * p.row_tiles * tile * (dp + 2) : 0;
     return p;
+}
+inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
+    const int dp = padded_dim(d);
+    const int64_t cus = device_cu_count();
+    if (rows <= 32) {
+        const int64_t want = 2 * cus, most = keys / 256 > 1 ? keys / 256 : 1;
+        const int64_t s = problems >= want ? 1 : (want + problems - 1) / (problems > 0 ? problems : 1);
+        return plan_of(32, (int)(s < most ? s : most), rows, problems, dp);
+    }
+    // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts
+    Plan best{};
+    double least = 0.;
+    for (int tile = 128; tile <= (dp == 256 ? 128 : 256); tile *= 2) {
+        const int64_t slots = cus * (dp == 256 ? 1 : dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 ? 2 : 1), groups = (rows + tile - 1) / tile * problems;
+        const double start = tile == 128 ? 7. : 10., each = tile == 128 ? 2.6 : 2.4;
+        for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 512); ++s) {
+            const int64_t rounds = (groups * s + slots - 1) / slots, tiles = (keys + 63) / 64;
+            const double us = rounds * (start + each * ((tiles + s - 1) / s)) + (s == 1 ? 0. : 5. + 1e-6 * 4. * (dp + 2) * rows * problems * (2 * s) / 4.);
+            if (best.rows == 0 || us < least) {
+                least = us;
+                best = plan_of(tile, s, rows, problems, dp);
+            }
+        }
+    }
+    return best;
 }
 
 template <class Src, int DP> inline int launch(const Plan& p, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid > 0x7fffffff) return -1;
     constexpr int KW = DP == 256 ? 2 : 4;
-    if (p.few) few_kernel<Src, DP, KW><<<(int)grid, 64 * KW, 0, stream>>>(a, sa);
-    else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
-    else if (p.rows == 128) { if (getenv("NB2")) tiles_kernel<Src, DP, 1, 4, 2, DP == 64 ? 4 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
-       else tiles_kernel<Src, DP, 1, 4, 1, DP == 64 ? 4 : 2><<<(int)grid, 256, 0, stream>>>(a, sa); }
-    else if (getenv("NB2")) tiles_kernel<Src, DP, 1, 8, 2, DP == 64 ? 4 : 2><<<(int)grid, 512, 0, stream>>>(a, sa);
-    else tiles_kernel<Src, DP, 1, 8, 1, DP == 64 ? 4 : 2><<<(int)grid, 512, 0, stream>>>(a, sa);
+    if (p.rows == 32) few_kernel<Src, DP, KW><<<(int)grid, 64 * KW, 0, stream>>>(a, sa);
+    else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if constexpr (DP == 128) {
+        if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 2, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+        else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
+    } else {
+        if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 4><<<(int)grid, 256, 0, stream>>>(a, sa);
+        else tiles_kernel<Src, DP, 1, 8, 2, 1, 4><<<(int)grid, 512, 0, stream>>>(a, sa);
+    }
     KCHECK();
     if (p.splits > 1) {
         join_kernel<Src, DP><<<a.problems * a.rows_padded, DP, 0, stream>>>(a, sa);

@@ -66,10 +66,10 @@ template <int DTYPE, bool BIAS> struct Dense {
             v = a.v + b * a.v_bs + head * a.v_hs;
             mask = a.mask_kind == 1 ? (const void*)((const uint8_t*)a.mask + b * a.mask_bs) : (const void*)((const float*)a.mask + b * a.mask_bs);
         }
-        // K rows from key0 (which may lie before the first) into registers; V rows with what their keys' masks say
+        // rows from key0 on into registers, and what their keys' masks say; past the end zeros
         __device__ __forceinline__ void rows(u32x4 (&x)[CH], const uint16_t* p, int64_t rs, int key0) {
             if (!mine()) return;
-            if (a.aligned && d == DP && key0 >= 0 && key0 + TK <= keys) {     // whole rows of 16-byte pieces: a scalar base and 32-bit offsets
+            if (a.aligned && d == DP && key0 + TK <= keys) {     // whole rows of 16-byte pieces: a scalar base and 32-bit offsets
                 const char* const at = (const char*)(p + (int64_t)key0 * rs);
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
@@ -80,7 +80,7 @@ template <int DTYPE, bool BIAS> struct Dense {
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
                     const int i = tid + j * NT, key = key0 + i / ROW, ch = i % ROW;
-                    x[j] = key >= 0 && key < keys && 8 * ch < d ? load8(p + key * rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
+                    x[j] = key < keys && 8 * ch < d ? load8(p + key * rs + 8 * ch, a.aligned) : u32x4{0, 0, 0, 0};
                 }
             }
         }
@@ -90,8 +90,12 @@ template <int DTYPE, bool BIAS> struct Dense {
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
                     const int key = key0 + (tid + j * NT) / ROW;
-                    k_mask[j] = key >= 0 && key < keys ? mask_word(a, mask, key) : 1u;
+                    k_mask[j] = key < keys ? mask_word(a, mask, key) : 1u;
                 }
+            if (BIAS && tid < TK) {
+                row_key = key0 + tid;
+                row_mask = row_key < keys ? mask_word(a, mask, row_key) : 1u;
+            }
         }
         __device__ __forceinline__ void load_v(int key0) {
             rows(vr, v, a.v_rs, key0);
@@ -102,31 +106,30 @@ template <int DTYPE, bool BIAS> struct Dense {
                     const int key = key0 + (tid + j * NT) / ROW;
                     v_mask[j] = key < keys ? mask_word(a, mask, key) : 1u;
                 }
-                row_key = key0 + tid;
-                if (tid < TK) row_mask = row_key < keys ? mask_word(a, mask, row_key) : 1u;
             }
         }
         // a key that is out has probability 0, and its value must be a number for the product to leave it out, its score for the bias to
-        __device__ __forceinline__ void write_k(uint8_t* kb) {
+        __device__ __forceinline__ void write_k(uint8_t* kb, float* bias) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
                 if (mine()) *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, k_mask[j]) ? u32x4{0, 0, 0, 0} : kr[j];
             }
+            if (BIAS && tid < TK) bias[tid] = row_key < keys ? key_bias(a, row_mask) : -INFINITY;
         }
-        __device__ __forceinline__ void write_v(uint8_t* vb, float* bias) {
+        __device__ __forceinline__ void write_v(uint8_t* vb) {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
                 if (mine()) *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, v_mask[j]) ? u32x4{0, 0, 0, 0} : vr[j];
             }
-            if (BIAS && tid < TK) bias[tid] = row_key < keys ? key_bias(a, row_mask) : -INFINITY;
         }
         __device__ __forceinline__ bool any_key(int from, int to) const {
             for (int i = from; i < to; ++i)
                 if (!is_out(a, mask_word(a, mask, i))) return true;
             return false;
         }
+        __device__ __forceinline__ bool numbers() const { return true; }
         __device__ __forceinline__ Scales scales(int) const { return {}; }
     };
 };

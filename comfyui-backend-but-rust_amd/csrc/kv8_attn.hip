@@ -24,8 +24,8 @@ struct Codes {
     // iv is 2^16 / A, so that sums of both ends of A's range, 2^-90 and 2^128, stay ordinary numbers; a smaller A counts as 2^-90, and as
     // 2^-60 of the largest so far, so that p' does not leave fp32
     static constexpr float kOut = 65536.f / 127.f;
-    struct Scales {
-        float ks[2], lvs[2], ivs[2];
+    template <int N> struct Scales {
+        float ks[N], lvs[N], ivs[N];
         __device__ float k(int h) const { return ks[h]; }
         __device__ float lv(int h) const { return lvs[h]; }
         __device__ float iv(int h) const { return ivs[h]; }
@@ -54,6 +54,7 @@ struct Codes {
         int k_window = -1, v_window = -1, s_window = -1;
         int k_page, v_page;              // of block 64 * window + lane
         float ks, lv, iv, top = 0.f;     // its scales
+        bool all_numbers;                // of the window
         u32x4 kr[CH], vr[CH];
         __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_)
             : a(a_), tid(tid_), lane(threadIdx.x & 63), keys(p.keys), d(c.d), hk(c.hk) {
@@ -78,17 +79,18 @@ struct Codes {
             // the A of p' and of the sum's division: any will do where all values are 0
             top = fmaxf(top, wave_max_f32(good ? A : 0.f));
             const float u = top == 0.f ? 1.f : A > 0.f && good ? fmaxf(A, fmaxf(top * 0x1p-60f, 0x1p-90f)) : top;
+            all_numbers = !__any(ks != ks);
             lv = __builtin_amdgcn_logf(u);
             iv = 65536.f / u;
         }
-        // TK rows from key0, a multiple of 32 that may lie before the first, where block 0 is read instead
+        // TK rows from key0, a multiple of 32
         __device__ __forceinline__ void rows(u32x4 (&x)[CH], const int8_t* codes, int& window, int& pages, int key0) {
             if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT, token = key0 + i / ROW, ch = i % ROW;
                 // the rows that a wave loads at once lie in one block: a scalar base and 32-bit offsets
-                const int b = __builtin_amdgcn_readfirstlane(token >> 4), block = b < 0 ? 0 : b;
+                const int block = __builtin_amdgcn_readfirstlane(token >> 4);
                 if (block >> 6 != window) {
                     window = block >> 6;
                     pages = page(64 * window + lane);
@@ -100,7 +102,7 @@ struct Codes {
         }
         __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, k_window, k_page, key0); }
         __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, v_window, v_page, key0); }
-        __device__ __forceinline__ void write_k(uint8_t* kb) {
+        __device__ __forceinline__ void write_k(uint8_t* kb, float*) {
             if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
@@ -110,7 +112,7 @@ struct Codes {
                     *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, 2 * (i % ROW) + e)) = bytes_to_f16(kr[j][2 * e], kr[j][2 * e + 1]);
             }
         }
-        __device__ __forceinline__ void write_v(uint8_t* vb, float*) {
+        __device__ __forceinline__ void write_v(uint8_t* vb) {
             if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
@@ -121,13 +123,14 @@ struct Codes {
             }
         }
         __device__ bool any_key(int, int) const { return true; }
-        // of the 32 keys from key0
-        __device__ __forceinline__ Scales scales(int key0) {
+        __device__ __forceinline__ bool numbers() const { return all_numbers; }
+        // of the TK keys from key0
+        __device__ __forceinline__ Scales<TK / kBlock> scales(int key0) {
             const int block = __builtin_amdgcn_readfirstlane(key0 >> 4);
             if (block >> 6 != s_window) look(block >> 6);
-            Scales r;
+            Scales<TK / kBlock> r;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < TK / kBlock; ++h) {
                 r.ks[h] = u2f(__builtin_amdgcn_readlane(f2u(ks), (block + h) & 63));
                 r.lvs[h] = u2f(__builtin_amdgcn_readlane(f2u(lv), (block + h) & 63));
                 r.ivs[h] = u2f(__builtin_amdgcn_readlane(f2u(iv), (block + h) & 63));
