@@ -437,141 +437,286 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
     }
 }
 
-// Few rows: KW waves on the same 32, each with keys of its own, 32 at a time through its own piece of LDS; no barrier until they meet.
-template <class Src, int DP, int KW>
-__global__ __launch_bounds__(64 * KW, DP >= 256 ? 1 : 2) void few_kernel(const Common a, const typename Src::Args sa) {
-    constexpr int TK = 32, TILE_K = TK * kRowK<DP>, TILE = TILE_K + TK * kRowV<DP>, DB = DP / 32;
-    __shared__ __align__(16) uint8_t lds[KW * TILE];
+// Few rows, the form for single tokens: KW waves on the same 16 RT rows, each with 32 keys of its own at a time and no barrier until their
+// results meet.  What counts is the keys' way in: K goes from memory straight into the fragments of v_mfma_f32_16x16x32 (lane: key
+// lane % 16, channels in the order of Source::q_chunk), V through the wave's own piece of LDS, where it is turned.  Lanes hold row lane % 16 and
+// keys 4 (lane / 16) .. + 3 of each 16, which is, in order, what the product with V takes, if that counts its keys so.
+template <int DT> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (DT == DT_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// The largest / the sum of the four lanes of a row.
+__device__ __forceinline__ float quarter_max(float v) {
+    const auto s = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+    return half_max(fmaxf(u2f(s[0]), u2f(s[1])));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+    const auto s = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
+    return half_sum(u2f(s[0]) + u2f(s[1]));
+}
+
+template <class Src, int DP, int KW, int RT, int OCC>
+__global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const typename Src::Args sa) {
+    constexpr int TK = 32, TILE = TK * kRowV<DP>, KS = DP / 32, DB = DP / 16, R = 16 * RT, DT = Src::DT;
+    constexpr int MEET = R * DP * 4;      // a wave's numerators
+    __shared__ __align__(16) uint8_t lds[KW * (TILE > MEET ? TILE : MEET)];
     __shared__ __align__(16) float bias[Src::kBias ? KW * TK : 4];
-    __shared__ float stat[KW * 64];
-    const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+    __shared__ float stat[KW * 2 * R];
+    const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, gg = lane >> 4;
     int id = xcd_contiguous(blockIdx.x, gridDim.x);
     const int row_tile = id % a.row_tiles;
     id /= a.row_tiles;
     const int split = id % a.splits, problem = id / a.splits;
     const Problem pr = Src::problem(sa, a, problem);
-    const int rows = pr.tokens * a.group, r0 = row_tile * 32;
+    const int rows = pr.tokens * a.group, r0 = row_tile * R;
     if (r0 >= rows) return;
     int t0, t1;
-    share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + 32) - 1) / a.group), TK, a.splits, split, t0, t1);
+    share_of(min(pr.keys, pr.limit0 + (min(rows, r0 + R) - 1) / a.group), TK, a.splits, split, t0, t1);
     {
         const int share = (t1 - t0 + KW - 1) / KW;
         t0 = min(t1, t0 + kw * share);
         t1 = min(t1, t0 + share);
     }
     typename Src::template Stage<DP, TK, 64> st(sa, a, problem, pr, lane);
+    if (t0 < t1) {
+        st.load_fragments(t0 * TK);
+        st.load_v(t0 * TK);
+    }
+
+    int row[RT], token[RT], head[RT], limit[RT];
+    u32x4 qf[RT][KS];
+    float c[RT], base[RT], sum[RT];
+    f32x4 acc[RT][DB];
+#pragma unroll
+    for (int w = 0; w < RT; ++w) {
+        row[w] = r0 + 16 * w + col;
+        const int r = row[w] < rows ? row[w] : rows - 1;
+        token[w] = r / a.group;
+        head[w] = r - token[w] * a.group;
+        limit[w] = min(pr.keys, pr.limit0 + token[w]);
+        c[w] = a.c;
+        const uint16_t* qp = (const uint16_t*)a.q + pr.q_at + token[w] * a.q_rs + head[w] * a.q_hs;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int at = 8 * Src::q_chunk(s, gg);
+            qf[w][s] = at < a.d ? load8(qp + at, a.aligned & 1) : u32x4{0, 0, 0, 0};
+        }
+    }
+    const int all_see = min(pr.keys, pr.limit0 + min(rows - 1, r0) / a.group);
+#pragma unroll
+    for (int w = 0; w < RT; ++w) {
+        if constexpr (Src::kNormalize) {
+            float m = 0.f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(elem(qf[w][s], i, a.q_dt)));
+            m = quarter_max(m);
+            const int e = m > 0.f && m < INFINITY ? ilogbf(m) : 0;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                u32x4 f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = pack_f16x2(ldexpf(elem(qf[w][s], 2 * i, a.q_dt), -e), ldexpf(elem(qf[w][s], 2 * i + 1, a.q_dt), -e)) & a.q_and ^ a.q_xor;
+                qf[w][s] = f;
+            }
+            c[w] = ldexpf(c[w], e);
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[w][s] = qf[w][s] & a.q_and ^ a.q_xor;
+        }
+        base[w] = -INFINITY;
+        sum[w] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) acc[w][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
     uint8_t* const mine = lds + kw * TILE;
     float* const my_bias = bias + (Src::kBias ? kw * TK : 0);
     const auto fence = [] {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    const int at_k = lane_k<DP>(lane), at_v = TILE_K + lane_v<DP>(lane);
-    if (t0 < t1) {
-        st.load_k(t0 * TK);
-        st.load_v(t0 * TK);
-    }
-    Lanes<Src, DP, 1> L;
-    L.start(a, pr, r0, rows, lane);
+    const int at_v = v_place<DP>(4 * gg + (col >> 2), (col & 3) >> 1) + 8 * (col & 1);
     for (int t = t0; t < t1; ++t) {
         const auto sc = st.scales(t * TK);
         fence();
-        st.write_k(mine, my_bias);
-        st.write_v(mine + TILE_K);
-        if (t + 1 < t1) {
-            st.load_k((t + 1) * TK);
-            st.load_v((t + 1) * TK);
-        }
+        st.write_v(mine);
+        st.write_bias(my_bias);
+        if (t + 1 < t1) st.load_v((t + 1) * TK);
         fence();
-        f16acc s[1][1];
-        float kc[1][2], from[1];
-        L.scores(s, mine + at_k, my_bias, g);
-        L.raise(s, kc, from, sc, t * TK, st.numbers() && (t + 1) * TK <= L.all_see, g);
+        f32x4 s[RT][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4 p[1];
-            L.probs(p, s, kc, from, sc, h);
-            L.values(p, mine + at_v + 16 * h * kRowV<DP>);
+        for (int w = 0; w < RT; ++w)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if constexpr (Src::kBias) s[w][b] = *reinterpret_cast<const f32x4*>(my_bias + 16 * b + 4 * gg);
+                else s[w][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const u32x4 kf = st.fragment(b, ks);
+#pragma unroll
+                for (int w = 0; w < RT; ++w) s[w][b] = mfma16<DT>(kf, qf[w][ks], s[w][b]);
+            }
+        if (t + 1 < t1) st.load_fragments((t + 1) * TK);
+        const bool plain = st.numbers() && (t + 1) * TK <= all_see;
+        u32x4 p[RT];
+#pragma unroll
+        for (int w = 0; w < RT; ++w) {
+            float kc[2], top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                if (!Src::kBias && !plain) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (Src::kNormalize && sc.k(b) != sc.k(b)) s[w][b][i] = NAN;
+                        if (t * TK + 16 * b + 4 * gg + i >= limit[w]) s[w][b][i] = -INFINITY;
+                    }
+                }
+                const float k = c[w] * sc.k(b);
+                kc[b] = k > 1.17549435e-38f ? k : 1.17549435e-38f;
+                top = fmaxf(top, fmaf(fmaxf(fmaxf(s[w][b][0], s[w][b][1]), fmaxf(s[w][b][2], s[w][b][3])), kc[b], sc.lv(b)));
+            }
+            top = quarter_max(top);
+            if (__any(top > base[w] + kLag)) {
+                const float nb = fmaxf(base[w], top), f = base[w] == -INFINITY ? 0.f : exp2f(base[w] - nb);
+                base[w] = nb;
+                sum[w] *= f;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) acc[w][i] *= f;
+            }
+            float from = base[w] == -INFINITY ? 0.f : base[w];
+            if (Src::kBias && __any(fabsf(from) > 262144.f)) {      // as in Lanes::raise
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    s[w][b] = s[w][b] * kc[b] - from;
+                    kc[b] = 1.f;
+                }
+                from = 0.f;
+            }
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const float off = sc.lv(b) - from;
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[w][b][i], kc[b], off));
+                p[w][2 * b] = pack2<DT>(e[0], e[1]);
+                p[w][2 * b + 1] = pack2<DT>(e[2], e[3]);
+                sum[w] = fmaf(add2<DT>(p[w][2 * b + 1], add2<DT>(p[w][2 * b], 0.f)), sc.iv(b), sum[w]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+            u32x2 half[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                half[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(mine + at_v + 16 * j * kRowV<DP> + 32 * i)));
+            const u32x4 vf = {half[0][0], half[0][1], half[1][0], half[1][1]};
+#pragma unroll
+            for (int w = 0; w < RT; ++w) acc[w][i] = mfma16<DT>(vf, p[w], acc[w][i]);
         }
     }
-    L.finish(st, t0 * TK, min(t1 * TK, pr.keys));
+#pragma unroll
+    for (int w = 0; w < RT; ++w) {
+        sum[w] = quarter_sum(sum[w]);
+        if (Src::kBias && base[w] == -INFINITY && sum[w] != sum[w] && !st.any_key(t0 * TK, min(t1 * TK, pr.keys))) {     // q is no number, and saw nothing
+            sum[w] = 0.f;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) acc[w][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
 
+    // register j of block i: channel 16 i + 4 gg + j
+    __syncthreads();
+    float* const mo = reinterpret_cast<float*>(lds + kw * MEET);
+#pragma unroll
+    for (int w = 0; w < RT; ++w) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mo[(16 * i + 4 * gg + j) * R + 16 * w + col] = acc[w][i][j];
+        if (gg == 0) {
+            stat[kw * 2 * R + 16 * w + col] = base[w];
+            stat[kw * 2 * R + R + 16 * w + col] = sum[w];
+        }
+    }
+    __syncthreads();
+    // a thread per row and piece of four channels
     const int64_t part_at = ((int64_t)split * a.problems + problem) * a.rows_padded;
-    __syncthreads();
-    float* const mo = reinterpret_cast<float*>(lds) + kw * 32 * DP;
+    for (int i = threadIdx.x; i < R * (DP / 4); i += 64 * KW) {
+        const int ch = 4 * (i % (DP / 4)), rr = i / (DP / 4), r = r0 + rr;
+        if (r >= rows) break;
+        float nb = -INFINITY, wt[KW], l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < DB; ++i)
+        for (int k = 0; k < KW; ++k) nb = fmaxf(nb, stat[k * 2 * R + rr]);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) mo[(32 * i + key_of(j, g)) * 32 + col] = L.acc[0][i][j];
-    if (g == 0) {
-        stat[kw * 64 + col] = L.base[0];
-        stat[kw * 64 + 32 + col] = L.sum[0];
-    }
-    __syncthreads();
-    // every wave adds a part of the channels: DP / KW of them for its lane's row
-    float nb = -INFINITY, w[KW];
-#pragma unroll
-    for (int k = 0; k < KW; ++k) nb = fmaxf(nb, stat[k * 64 + col]);
-    float l = 0.f;
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-        const float b = stat[k * 64 + col];
-        w[k] = b == -INFINITY ? 0.f : exp2f(b - nb);
-        l = fmaf(stat[k * 64 + 32 + col], w[k], l);
-    }
-    if (L.row[0] >= rows) return;
-    constexpr int EACH = DP / KW / 2;      // channels of a lane
-    const int d0 = kw * (DP / KW) + g * EACH;
-    const float inv = l == 0.f ? 0.f : Src::kOut / l;
-    uint16_t* const op = (uint16_t*)a.o + pr.o_at + L.token[0] * a.o_rs + L.head[0] * a.o_hs;
-    float* const pp = a.part + (part_at + L.row[0]) * (DP + 2);
-#pragma unroll
-    for (int j = 0; j < EACH; j += 4) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            v[e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < KW; ++k) v[e] = fmaf(reinterpret_cast<const float*>(lds)[(k * DP + d0 + j + e) * 32 + col], w[k], v[e]);
+        for (int k = 0; k < KW; ++k) {
+            const float b = stat[k * 2 * R + rr];
+            wt[k] = b == -INFINITY ? 0.f : exp2f(b - nb);
+            l = fmaf(stat[k * 2 * R + R + rr], wt[k], l);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < KW; ++k) v[e] = fmaf(reinterpret_cast<const float*>(lds + k * MEET)[(ch + e) * R + rr], wt[k], v[e]);
         if (a.splits > 1) {
+            float* const pp = a.part + (part_at + r) * (DP + 2);
+            *reinterpret_cast<f32x2*>(pp + ch) = f32x2{v[0], v[1]};
+            *reinterpret_cast<f32x2*>(pp + ch + 2) = f32x2{v[2], v[3]};
+            if (ch == 0) *reinterpret_cast<f32x2*>(pp + DP) = f32x2{nb, l};
+        } else if (ch < a.d) {
+            const float inv = l == 0.f ? 0.f : Src::kOut / l;
+            const int tk = r / a.group;
+            uint16_t* const op = (uint16_t*)a.o + pr.o_at + tk * a.o_rs + (r - tk * a.group) * a.o_hs + ch;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pp[d0 + j + e] = v[e];
-        } else if (d0 + j < a.d) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) op[d0 + j + e] = a.q_dt == DT_BF16 ? f_to_bf16(v[e] * inv) : f_to_f16(v[e] * inv);
+            for (int e = 0; e < 4; ++e) op[e] = a.q_dt == DT_BF16 ? f_to_bf16(v[e] * inv) : f_to_f16(v[e] * inv);
         }
-    }
-    if (a.splits > 1 && kw == 0 && g == 0) {
-        pp[DP] = nb;
-        pp[DP + 1] = l;
     }
 }
 
 // The parts of rows whose keys several workgroups shared, added in the order of the keys: one workgroup of DP threads per row.
 template <class Src, int DP>
-__global__ __launch_bounds__(DP) void join_kernel(const Common a, const typename Src::Args sa) {
-    const int row = blockIdx.x % a.rows_padded, problem = blockIdx.x / a.rows_padded;
+__global__ __launch_bounds__(DP) void join_kernel(const Common a, const typename Src::Args sa, int rows_most) {
+    __shared__ float weight[64];
+    const int row = blockIdx.x % rows_most, problem = blockIdx.x / rows_most, ch = threadIdx.x;
     const Problem pr = Src::problem(sa, a, problem);
     if (row >= pr.tokens * a.group) return;
-    const int token = row / a.group, head = row - token * a.group, ch = threadIdx.x;
     const float* const p = a.part + ((int64_t)problem * a.rows_padded + row) * (DP + 2);
     const int64_t step = (int64_t)a.problems * a.rows_padded * (DP + 2);
-    float nb = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) nb = fmaxf(nb, p[s * step + DP]);
-    float v = 0.f, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float b = p[s * step + DP], w = b == -INFINITY ? 0.f : exp2f(b - nb);
-        v = fmaf(p[s * step + ch], w, v);
-        l = fmaf(p[s * step + DP + 1], w, l);
+    float inv = 0.f;
+    if (ch < 64) {      // a lane per part
+        const f32x2 s = ch < a.splits ? *reinterpret_cast<const f32x2*>(p + ch * step + DP) : f32x2{-INFINITY, 0.f};
+        const float nb = wave_max_f32(s[0]), w = s[0] == -INFINITY ? 0.f : exp2f(s[0] - nb);
+        weight[ch] = w;
+        const float l = (float)wave_sum_f64((double)(s[1] * w));
+        inv = l == 0.f ? 0.f : Src::kOut / l;
     }
+    __shared__ float scale;
+    if (ch == 0) scale = inv;
+    float v = 0.f;
+    __syncthreads();
+    int s = 0;
+    for (; s + 8 <= a.splits; s += 8) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = p[(s + i) * step + ch];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v = fmaf(x[i], weight[s + i], v);
+    }
+    for (; s < a.splits; ++s) v = fmaf(p[s * step + ch], weight[s], v);
     if (ch >= a.d) return;
-    const float r = l == 0.f ? 0.f : v * (Src::kOut / l);
+    const float r = scale == 0.f ? 0.f : v * scale;
+    const int token = row / a.group, head = row - token * a.group;
     uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + head * a.o_hs + ch;
     *op = a.q_dt == DT_BF16 ? f_to_bf16(r) : f_to_f16(r);
 }
 
-// How a call runs: 32 rows with the keys over a workgroup's waves, or tiles of 128 or 256 rows; and over how many workgroups the keys of a
+// How a call runs: 16 or 32 rows with the keys over a workgroup's waves, or tiles of 128 or 256 rows; and over how many workgroups the keys of a
 // row go.
 struct Plan {
     int rows, row_tiles, splits;
@@ -590,9 +735,11 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
     const int dp = padded_dim(d);
     const int64_t cus = device_cu_count();
     if (rows <= 32) {
-        const int64_t want = 2 * cus, most = keys / 256 > 1 ? keys / 256 : 1;
-        const int64_t s = problems >= want ? 1 : (want + problems - 1) / (problems > 0 ? problems : 1);
-        return plan_of(32, (int)(s < most ? s : most), rows, problems, dp);
+        const int tile = rows <= 16 ? 16 : 32;
+        const int64_t want = 4 * cus, most = (keys + 127) / 128;
+        int64_t s = problems >= want ? 1 : (want + problems - 1) / (problems > 0 ? problems : 1);
+        if (s > 64) s = 64;
+        return plan_of(tile, (int)(s < most ? s : most > 1 ? most : 1), rows, problems, dp);
     }
     // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts
     Plan best{};
@@ -612,11 +759,11 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
     return best;
 }
 
-template <class Src, int DP> inline int launch(const Plan& p, Common& a, const typename Src::Args& sa, hipStream_t stream) {
+template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
-    if (grid > 0x7fffffff) return -1;
-    constexpr int KW = DP == 256 ? 2 : 4;
-    if (p.rows == 32) few_kernel<Src, DP, KW><<<(int)grid, 64 * KW, 0, stream>>>(a, sa);
+    if (grid > 0x7fffffff || a.problems * rows > 0x7fffffff) return -1;
+    if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if (p.rows == 32) few_kernel<Src, DP, 4, 2, DP == 256 ? 1 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 128) {
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 2, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
@@ -627,16 +774,16 @@ template <class Src, int DP> inline int launch(const Plan& p, Common& a, const t
     }
     KCHECK();
     if (p.splits > 1) {
-        join_kernel<Src, DP><<<a.problems * a.rows_padded, DP, 0, stream>>>(a, sa);
+        join_kernel<Src, DP><<<(int)(a.problems * rows), DP, 0, stream>>>(a, sa, (int)rows);
         KCHECK();
     }
     return 0;
 }
-template <class Src> inline int launch_dim(const Plan& p, Common& a, const typename Src::Args& sa, hipStream_t stream) {
+template <class Src> inline int launch_dim(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     switch (padded_dim(a.d)) {
-        case 64: return launch<Src, 64>(p, a, sa, stream);
-        case 128: return launch<Src, 128>(p, a, sa, stream);
-        default: return launch<Src, 256>(p, a, sa, stream);
+        case 64: return launch<Src, 64>(p, rows, a, sa, stream);
+        case 128: return launch<Src, 128>(p, rows, a, sa, stream);
+        default: return launch<Src, 256>(p, rows, a, sa, stream);
     }
 }
 

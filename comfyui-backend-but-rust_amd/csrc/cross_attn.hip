@@ -48,6 +48,8 @@ template <int DTYPE, bool BIAS> struct Dense {
         p.limit0 = p.keys;
         return p;
     }
+    // the chunk of 8 channels that step s of the product of few rows takes from lanes 16 gg ..
+    static __device__ __forceinline__ int q_chunk(int s, int gg) { return 4 * s + gg; }
     template <int DP, int TK, int NT> struct Stage {
         static constexpr int ROW = DP / 8, CH = (TK * ROW + NT - 1) / NT;
         static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
@@ -57,7 +59,7 @@ template <int DTYPE, bool BIAS> struct Dense {
         const uint16_t *k, *v;
         const void* mask;
         int tid, keys, d;
-        u32x4 kr[CH], vr[CH];
+        u32x4 kr[CH], vr[CH];      // (for few rows kr are the fragments, [16 keys][step])
         uint32_t k_mask[BIAS ? CH : 1], v_mask[BIAS ? CH : 1], row_mask;     // as they lie in memory: looked at when they have arrived
         int row_key;
         __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_) : a(a_), tid(tid_), keys(p.keys), d(c.d) {
@@ -96,6 +98,31 @@ template <int DTYPE, bool BIAS> struct Dense {
                 row_key = key0 + tid;
                 row_mask = row_key < keys ? mask_word(a, mask, row_key) : 1u;
             }
+        }
+        __device__ __forceinline__ void load_fragments(int key0) {
+            static_assert(NT != 64 || CH == 2 * (DP / 32), "32 keys of a wave");
+            const int col = tid & 15, gg = tid >> 4;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int key = key0 + 16 * b + col;
+                const uint16_t* const at = k + (key < keys ? key : 0) * a.k_rs + 8 * gg;
+                if (a.aligned && d == DP) {
+#pragma unroll
+                    for (int s = 0; s < DP / 32; ++s) kr[b * (DP / 32) + s] = load8(at + 32 * s, true);
+                } else {
+#pragma unroll
+                    for (int s = 0; s < DP / 32; ++s) kr[b * (DP / 32) + s] = 32 * s + 8 * gg < d ? load8(at + 32 * s, a.aligned) : u32x4{0, 0, 0, 0};
+                }
+                if (BIAS) k_mask[b] = key < keys ? mask_word(a, mask, key) : a.mask_kind == 1 ? 0u : 0xff800000u;     // past the end: out
+            }
+            if (BIAS && tid < TK) {
+                row_key = key0 + tid;
+                row_mask = row_key < keys ? mask_word(a, mask, row_key) : 1u;
+            }
+        }
+        __device__ __forceinline__ u32x4 fragment(int b, int s) const { return BIAS && is_out(a, k_mask[b]) ? u32x4{0, 0, 0, 0} : kr[b * (DP / 32) + s]; }
+        __device__ __forceinline__ void write_bias(float* bias) {
+            if (BIAS && tid < TK) bias[tid] = row_key < keys ? key_bias(a, row_mask) : -INFINITY;
         }
         __device__ __forceinline__ void load_v(int key0) {
             rows(vr, v, a.v_rs, key0);
@@ -170,6 +197,6 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     s.lq = lq; s.lk = lk; s.aligned = near && sixteen(k, k_bs, k_rs, k_hs) && sixteen(v, v_bs, v_rs, v_hs);
     s.k_lens = k_lens; s.mask = mask; s.mask_kind = mask_kind; s.mask_bs = mask_bs;
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == DT_BF16) return mask_kind ? launch_dim<Dense<DT_BF16, true>>(p, c, s, st) : launch_dim<Dense<DT_BF16, false>>(p, c, s, st);
-    return mask_kind ? launch_dim<Dense<DT_F16, true>>(p, c, s, st) : launch_dim<Dense<DT_F16, false>>(p, c, s, st);
+    if (dtype == DT_BF16) return mask_kind ? launch_dim<Dense<DT_BF16, true>>(p, (int64_t)lq * (h / hk), c, s, st) : launch_dim<Dense<DT_BF16, false>>(p, (int64_t)lq * (h / hk), c, s, st);
+    return mask_kind ? launch_dim<Dense<DT_F16, true>>(p, (int64_t)lq * (h / hk), c, s, st) : launch_dim<Dense<DT_F16, false>>(p, (int64_t)lq * (h / hk), c, s, st);
 }

@@ -43,6 +43,8 @@ struct Codes {
         p.limit0 = a.causal ? sp.len - sp.count + 1 : p.keys;
         return p;
     }
+    // the chunk of 8 channels that step s of the product of few rows takes from lanes 16 gg ..: half of the 16 codes of a load
+    static __device__ __forceinline__ int q_chunk(int s, int gg) { return 8 * (s >> 1) + 2 * gg + (s & 1); }
     template <int DP, int TK, int NT> struct Stage {
         static constexpr int ROW = DP / 16, CH = (TK * ROW + NT - 1) / NT;
         static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
@@ -102,6 +104,27 @@ struct Codes {
         }
         __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, k_window, k_page, key0); }
         __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, v_window, v_page, key0); }
+        __device__ __forceinline__ void load_fragments(int key0) {
+            static_assert(NT != 64 || CH == 2 * (DP / 64), "32 keys of a wave");
+            const int col = tid & 15, gg = tid >> 4;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int block = __builtin_amdgcn_readfirstlane(key0 >> 4) + b;
+                if (block >> 6 != k_window) {
+                    k_window = block >> 6;
+                    k_page = page(64 * k_window + lane);
+                }
+                const int8_t* const at = a.k + codes_at(__builtin_amdgcn_readlane(k_page, block & 63), hk, head, a.page_shift, block, d);
+#pragma unroll
+                for (int i = 0; i < DP / 64; ++i)
+                    kr[b * (DP / 64) + i] = 64 * i + 16 * gg < d ? *reinterpret_cast<const u32x4*>(at + (uint32_t)(col * d + 64 * i + 16 * gg)) : u32x4{0, 0, 0, 0};
+            }
+        }
+        __device__ __forceinline__ u32x4 fragment(int b, int s) const {
+            const u32x4 c = kr[b * (DP / 64) + s / 2];
+            return bytes_to_f16(c[2 * (s & 1)], c[2 * (s & 1) + 1]);
+        }
+        __device__ __forceinline__ void write_bias(float*) {}
         __device__ __forceinline__ void write_k(uint8_t* kb, float*) {
             if (!mine()) return;
 #pragma unroll
@@ -166,5 +189,5 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     set_scale(c, scale);
     c.part = (float*)ws;
     CacheArgs s{k, v, k_scale, v_scale, starts, lens, table, rows, most, n_pages, __builtin_ctz(page), table_cols, causal != 0};
-    return launch_dim<Codes>(p, c, s, (hipStream_t)stream);
+    return launch_dim<Codes>(p, (int64_t)most * (h / hk), c, s, (hipStream_t)stream);
 }
