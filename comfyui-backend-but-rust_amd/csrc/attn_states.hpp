@@ -731,15 +731,31 @@ inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp
     p.bytes = splits > 1 ? 4 * splits * problems * p.row_tiles * tile * (dp + 2) : 0;
     return p;
 }
-inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d) {
+// bytes: of a key's or value's element.
+inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int bytes) {
     const int dp = padded_dim(d);
     const int64_t cus = device_cu_count();
     if (rows <= 32) {
-        const int tile = rows <= 16 ? 16 : 32;
-        const int64_t want = 4 * cus, most = (keys + 127) / 128;
-        int64_t s = problems >= want ? 1 : (want + problems - 1) / (problems > 0 ? problems : 1);
-        if (s > 64) s = 64;
-        return plan_of(tile, (int)(s < most ? s : most > 1 ? most : 1), rows, problems, dp);
+        // In microseconds: a workgroup starts and ends in 4; 32 keys of a wave take 1.65 at least (1 x 1369 keys x 64 heads of 72 channels in one
+        // part 22.6 in all), and longer where the waves of a CU together ask for more than its share of the copy rate, 20 KB a microsecond,
+        // of which CUs with few waves reach less (12 x 32749 keys x 8 heads of 128 codes: 3 parts 183, 5 parts 138, 8 parts, which are one
+        // full round, 130, 16 parts 136); a wave beside others on its CU takes a little more; joining 3.
+        const int tile = rows <= 16 ? 16 : 32, per_cu = dp == 256 ? 1 : tile == 32 || (bytes > 1 && dp == 128) ? 2 : 3;
+        const int64_t slots = cus * per_cu, tiles = (keys + 31) / 32;
+        const double full = per_cu * 4 * 32. * d * 2 * bytes / 20e3;
+        int best = 1;
+        double least = 0.;
+        for (int s = 1; s <= 64 && (s == 1 || s <= tiles); ++s) {
+            const int64_t rounds = (problems * s + slots - 1) / slots, each = ((tiles + s - 1) / s + 3) / 4;
+            const double busy = problems * s >= slots ? 1. : (double)(problems * s) / slots, shared = full * busy / (0.85 + 0.15 * busy), step = shared > 1.65 ? shared : 1.65;
+            const int64_t in_one = (tiles + s - 1) / s;
+            const double us = rounds * (4. + each * step + 0.25 * (in_one < 4 ? in_one : 4)) + (s == 1 ? 0. : 3. + 0.02 * s + 4e-6 * (dp + 2) * rows * problems * s / 2.);
+            if (s == 1 || us < least) {
+                least = us;
+                best = s;
+            }
+        }
+        return plan_of(tile, best, rows, problems, dp);
     }
     // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts
     Plan best{};

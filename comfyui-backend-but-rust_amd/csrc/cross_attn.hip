@@ -165,7 +165,7 @@ template <int DTYPE, bool BIAS> struct Dense {
 
 GPU_API int64_t gpu_cross_attn_workspace(int b, int lq, int lk, int h, int hk, int head_dim) {
     if (b <= 0 || lq <= 0 || lk <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256) return 0;
-    return make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim).bytes;
+    return make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim, 2).bytes;
 }
 
 GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void* o, void* ws, int b, int lq, int lk, int h, int hk,
@@ -177,7 +177,7 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     if (mask_kind < 0 || mask_kind > 2 || (mask_kind != 0 && !mask && lk > 0) || !(fabsf(scale) < INFINITY)) return -1;
     if (b == 0 || lq == 0) return 0;
     if ((int64_t)lq * (h / hk) > 0x7fffff00 || (int64_t)b * hk > 0x7fffffff || !q || !o || (lk > 0 && (!k || !v))) return -1;
-    const Plan p = make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim);
+    const Plan p = make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim, 2);
     if (p.bytes && (!ws || (uintptr_t)ws % 16 != 0)) return -1;
     const auto sixteen = [](const void* at, int64_t s0, int64_t s1, int64_t s2) { return (uintptr_t)at % 16 == 0 && (s0 | s1 | s2) % 8 == 0; };
     Common c{};

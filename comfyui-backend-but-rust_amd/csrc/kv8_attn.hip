@@ -167,7 +167,7 @@ struct Codes {
 
 GPU_API int64_t gpu_kv8_attn_workspace(int n, int most, int h, int hk, int head_dim, int page, int table_cols) {
     if (n <= 0 || most <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256 || table_cols <= 0 || page <= 0) return 0;
-    return make_plan((int64_t)most * (h / hk), (int64_t)n * hk, (int64_t)table_cols * page, head_dim).bytes;
+    return make_plan((int64_t)most * (h / hk), (int64_t)n * hk, (int64_t)table_cols * page, head_dim, 1).bytes;
 }
 
 GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* o, int64_t o_rs, int64_t o_hs, void* ws, const int8_t* k,
@@ -179,7 +179,7 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     if (!rows_ok(starts, lens, table, table_cols, n, rows, most)) return -1;
     if (n == 0 || rows == 0 || most == 0) return 0;
     if (!q || !o || (int64_t)most * (h / hk) > 0x7fffff00 || (int64_t)n * hk > 0x7fffffff) return -1;
-    const Plan p = make_plan((int64_t)most * (h / hk), (int64_t)n * hk, (int64_t)table_cols * page, head_dim);
+    const Plan p = make_plan((int64_t)most * (h / hk), (int64_t)n * hk, (int64_t)table_cols * page, head_dim, 1);
     if (p.bytes && (!ws || (uintptr_t)ws % 16 != 0)) return -1;
     Common c{};
     c.q = q; c.o = o; c.q_rs = q_rs; c.q_hs = q_hs; c.o_rs = o_rs; c.o_hs = o_hs;
