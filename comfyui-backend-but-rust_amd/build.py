@@ -75,7 +75,7 @@ def drop_calls():
 
 
 def build_calls():
-    """The Python calls that are native code (csrc/py_linear.cpp): host code only, against torch's headers and libgpu_kernels.so."""
+    """The Python calls that are native code (csrc/py_linear.cpp with py_states.hpp): host code only, against torch's headers and libgpu_kernels.so."""
     drop_calls()
     torch = _torch()
     if torch is None:
@@ -100,9 +100,10 @@ def _older(out, deps):
 def stale():
     """Whether an output is missing or older than what it is made from: each by its own time, since a later one's compilation may have failed."""
     include = os.path.join(os.path.dirname(HERE), "include")
-    kernels = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".hpp"))] + [os.path.join(include, "gpu_api.h")]
+    kernels = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hip", ".hpp")) and not f.startswith("py_")] + [os.path.join(include, "gpu_api.h")]
+    calls = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.startswith("py_")]
     return (_older(OUT, kernels) or _older(BLAS_OUT, [os.path.join(CSRC, "blas_gemm.cpp"), os.path.join(include, "gpu_blas_api.h")]) or
-            (_torch() is not None and _older(calls_out(), [os.path.join(CSRC, "py_linear.cpp"), os.path.join(include, "gpu_api.h"), OUT])))
+            (_torch() is not None and _older(calls_out(), [*calls, os.path.join(include, "gpu_api.h"), OUT])))
 
 
 def build(force=True):

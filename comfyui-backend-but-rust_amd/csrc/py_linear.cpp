@@ -9,7 +9,9 @@
 #include <ATen/ops/empty.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -67,7 +69,14 @@ PyObject* linear_w8a8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-PyMethodDef methods[] = {{"linear_w8a8", (PyCFunction)(void (*)(void))linear_w8a8, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+}  // namespace
+
+#include "py_states.hpp"
+
+namespace {
+
+#define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {CALL(linear_w8a8), CALL(cross_attn), CALL(kv8_attn), CALL(kv8_store), CALL(kv8_read), CALL(kv8_copy_pages), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

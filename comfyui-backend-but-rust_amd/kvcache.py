@@ -77,6 +77,12 @@ def _heads(t, heads, dim, what, device):
 
 def store(cache, rows, k, v):
     """The rows of k and v ([rows, heads, d], bf16 or f16) become the last tokens of their sequences."""
+    if qlinear._pycalls is None or qlinear._pycalls.kv8_store(k, v, *cache, *rows) is None:
+        _store(cache, rows, k, v)
+
+
+def _store(cache, rows, k, v):
+    """The calls in Python, here and below: what the native ones leave to them, and every refusal."""
     pages, heads, page, dim = _cache(cache, 4)
     dev = cache.k.device
     _heads(k, heads, dim, "k", dev); _heads(v, heads, dim, "v", dev)
@@ -91,6 +97,11 @@ def store(cache, rows, k, v):
 def read(cache, rows, tokens, dtype=torch.bfloat16):
     """The last tokens of the sequences as (k, v), each [tokens, heads, d]; tokens: all rows of the call, rows.starts[-1].  Rows of no
     sequence are left uninitialised."""
+    kv = None if qlinear._pycalls is None else qlinear._pycalls.kv8_read(*cache, *rows, tokens, dtype)
+    return _read(cache, rows, tokens, dtype) if kv is None else kv
+
+
+def _read(cache, rows, tokens, dtype):
     pages, heads, page, dim = _cache(cache, 4)
     dev = cache.k.device
     if dtype not in qlinear._TORCH_DT:
@@ -107,6 +118,11 @@ def read(cache, rows, tokens, dtype=torch.bfloat16):
 def attn(q, cache, rows, scale, causal=True, out=None):
     """softmax(scale * q k^T) v over the stored tokens: q [rows, h, d] (bf16 or f16), h a multiple of the cache's heads.  Causal: a row sees the
     tokens up to its own place; otherwise all that its sequence holds.  Rows of no sequence are left as they are in `out`."""
+    o = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.kv8_attn(q, *cache, *rows, float(scale), bool(causal))
+    return _attn(q, cache, rows, scale, causal, out) if o is None else o
+
+
+def _attn(q, cache, rows, scale, causal, out):
     pages, heads, page, dim = _cache(cache, 4)
     dev = cache.k.device
     _heads(q, None, dim, "q", dev)
@@ -131,6 +147,11 @@ def attn(q, cache, rows, scale, causal=True, out=None):
 def copy_pages(cache, src, dst):
     """Pages src[i] -> dst[i] (int32 tensors on the cache's device), scales and all layers included.  No page may be named twice in dst, or in
     both: the copies run side by side."""
+    if qlinear._pycalls is None or qlinear._pycalls.kv8_copy_pages(*cache, src, dst) is None:
+        _copy_pages(cache, src, dst)
+
+
+def _copy_pages(cache, src, dst):
     layered = cache.k.dim() == 5
     shape = _cache(cache, 5 if layered else 4)
     pages, heads, page, dim = shape[-4:]

@@ -415,6 +415,12 @@ def cross_attn(q, k, v, scale, k_lens=None, mask=None):
     """softmax(scale * q k^T + mask) v over an encoder's states: q [b, lq, h, d], k, v [b, lk, hk, d] (bf16 or f16, any strides with a dense last
     axis, h a multiple of hk, d a multiple of 8 up to 256) -> [b, lq, h, d].  k_lens (int32 [b]): item i has that many keys.  mask
     [lk] or [b, lk]: bool, False takes a key out, or float32, added to the logits, -inf takes it out.  A row without keys gives zeros."""
+    o = None if _pycalls is None else _pycalls.cross_attn(q, k, v, float(scale), k_lens, mask)
+    return _cross_attn(q, k, v, scale, k_lens, mask) if o is None else o
+
+
+def _cross_attn(q, k, v, scale, k_lens, mask):
+    """The call in Python: what the native one leaves to it, and every refusal."""
     b, lq, h, d = q.shape
     if k.dim() != 4 or k.shape != v.shape or k.shape[0] != b or k.shape[3] != d or k.shape[2] == 0 or h % k.shape[2]:
         raise ValueError("q [b, lq, h, d] and k, v [b, lk, hk, d] do not fit: %s, %s and %s" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))

@@ -498,6 +498,35 @@ def test_streams_and_graphs():
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
 
 
+def test_native_calls_take_what_the_python_side_takes(monkeypatch):
+    """The calls through csrc/py_states.hpp and the same calls in Python: the same bits, and none of them left to the other side."""
+    ql, kv = pkg("qlinear"), pkg("kvcache")
+    lens = [700, 33]
+    cache, table, _ = _filled(lens, 2, 64, 32, 71)
+    rows = _rows(kv, [3, 1], lens, table)
+    g = _gen(72)
+    q, x, y = (torch.randn(4, h, 64, device=DEV, generator=g).bfloat16() for h in (4, 2, 2))
+    layered = kv.new_cache(6, 2, 64, 32, 3)
+    for t in layered:
+        t.copy_(torch.randint(-100, 100, t.shape, device=DEV, generator=g))
+    cq, ck, cv = _cross_inputs(2, 5, 70, 2, 1, 64, torch.float16, 73)
+    masks = [None, torch.rand(70, device=DEV, generator=g) < 0.5, torch.randn(2, 70, device=DEV, generator=g)]
+
+    def calls():
+        kv.store(cache, rows, x, y)
+        kv.copy_pages(layered, _i32([1, 2]), _i32([4, 0]))
+        return [kv.attn(q, cache, rows, 0.125), kv.attn(q, cache, rows, 1, False), *kv.read(cache, rows, 4), *kv.read(cache, rows, 4, torch.float32), *cache, *layered.layer(2),
+                *(ql.cross_attn(cq, ck, cv, 0.125, _i32([70, 4]), m) for m in masks), ql.cross_attn(cq[:, ::2], ck, cv, 1)]
+
+    assert ql._pycalls is not None
+    with monkeypatch.context() as m:
+        for module, name in ((kv, "_store"), (kv, "_read"), (kv, "_attn"), (kv, "_copy_pages"), (ql, "_cross_attn")):
+            m.setattr(module, name, lambda *a, **k: pytest.fail("left to the Python side"))
+        native = [t.clone() for t in calls()]
+    monkeypatch.setattr(ql, "_pycalls", None)
+    assert all(torch.equal(a, b) for a, b in zip(native, calls()))
+
+
 def test_refusals_with_gpu_tensors():
     ql, kv = pkg("qlinear"), pkg("kvcache")
     q, k, v = _cross_inputs(1, 4, 6, 2, 2, 64, torch.bfloat16, 61)
