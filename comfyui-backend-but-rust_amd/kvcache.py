@@ -162,3 +162,140 @@ def _copy_pages(cache, src, dst):
     with qlinear._on(dev) as s:
         ffi.k("gpu_kv8_copy_pages", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
               shape[0] if layered else 1, pages, page, heads, dim, src.data_ptr(), dst.data_ptr(), src.shape[0], s)
+
+
+class CacheFull(RuntimeError):
+    pass
+
+
+class Sequences:
+    """Which pages hold which sequence: taken as sequences grow, shared by forks, copied before a shared one is written, given back, moved down.
+
+    The book is kept on the host; what a call needs of it goes to the device with the call, and pages are moved by queued copies.  All calls on
+    the cache are made on one stream, or ordered by the caller.  Pages' contents stay when they are given back: nothing reads them before they are
+    written again.  Nothing here can be captured into a graph (a captured call's Rows are tensors that the program fills itself)."""
+
+    def __init__(self, cache):
+        self.cache = cache
+        self.page = cache.k.shape[-2]
+        self._users = [0] * cache.k.shape[-4]
+        self._unused = list(range(len(self._users)))[::-1]      # the lowest is taken first
+        self._seqs = {}                                         # id -> [pages, length]
+        self._ids = 0
+
+    def add(self):
+        """A new, empty sequence."""
+        self._ids += 1
+        self._seqs[self._ids] = [[], 0]
+        return self._ids
+
+    def length(self, seq):
+        return self._seqs[seq][1]
+
+    def pages(self, seq):
+        return list(self._seqs[seq][0])
+
+    @property
+    def unused(self):
+        """Pages that nobody holds."""
+        return len(self._unused)
+
+    def fork(self, seq):
+        """A new sequence of the same tokens, in the same pages until one of the two writes."""
+        pages, length = self._seqs[seq]
+        new = self.add()
+        self._seqs[new] = [list(pages), length]
+        for p in pages:
+            self._users[p] += 1
+        return new
+
+    def truncate(self, seq, length):
+        """Drops the tokens from `length` on."""
+        s = self._seqs[seq]
+        if not 0 <= length <= s[1]:
+            raise ValueError("sequence %d has %d tokens, not %d" % (seq, s[1], length))
+        keep = -(-length // self.page)
+        self._give_back(s[0][keep:])
+        del s[0][keep:]
+        s[1] = length
+
+    def free(self, seq):
+        self._give_back(self._seqs.pop(seq)[0])
+
+    def extend(self, seqs, counts):
+        """Room for counts[i] more tokens at the end of seqs[i]; returns the Rows that store them, and that attend as them.  Raises CacheFull,
+        and changes nothing, where the pages do not suffice."""
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
+            raise ValueError("extend wants every sequence once, and a count of tokens for each")
+        need, users = 0, dict()
+        for s, c in zip(seqs, counts):
+            pages, length = self._seqs[s]
+            need += -(-(length + c) // self.page) - len(pages)
+            if c and length % self.page:
+                last = pages[-1]
+                users[last] = users.get(last, self._users[last]) - 1
+                need += users[last] > 0     # somebody else has it still: this one writes into a copy
+        if need > len(self._unused):
+            raise CacheFull("%d pages wanted, %d unused" % (need, len(self._unused)))
+        src, dst = [], []
+        for s, c in zip(seqs, counts):
+            entry = self._seqs[s]
+            pages, length = entry
+            if c and length % self.page and self._users[pages[-1]] > 1:
+                self._users[pages[-1]] -= 1
+                src.append(pages[-1])
+                pages[-1] = self._take()
+                dst.append(pages[-1])
+            while len(pages) * self.page < length + c:
+                pages.append(self._take())
+            entry[1] = length + c
+        self._copy(src, dst)
+        return self.rows(seqs, counts)
+
+    def rows(self, seqs, counts):
+        """Rows of counts[i] queries each to what seqs[i] hold: their last tokens (causal), or rows of something else (not causal)."""
+        n, cols = len(seqs), max([len(self._seqs[s][0]) for s in seqs] + [1])
+        starts = [0]
+        for c in counts:
+            starts.append(starts[-1] + c)
+        flat = starts + [self._seqs[s][1] for s in seqs]
+        for s in seqs:
+            pages = self._seqs[s][0]
+            flat += pages + [-1] * (cols - len(pages))
+        t = self._upload(flat)
+        return Rows(t[:n + 1], t[n + 1:2 * n + 1], t[2 * n + 1:].view(n, cols), max([0, *counts]))
+
+    def compact(self):
+        """Moves pages down into unused ones until the used ones are the lowest; returns how many moved.  Rows made before name the old places."""
+        used = [p for p, u in enumerate(self._users) if u]
+        dst = [p for p in range(len(used)) if not self._users[p]]
+        src = used[len(used) - len(dst):]
+        where = dict(zip(src, dst))
+        self._copy(src, dst)
+        for a, b in where.items():
+            self._users[a], self._users[b] = 0, self._users[a]
+        for entry in self._seqs.values():
+            entry[0] = [where.get(p, p) for p in entry[0]]
+        self._unused = list(range(len(used), len(self._users)))[::-1]
+        return len(src)
+
+    def _take(self):
+        p = self._unused.pop()
+        self._users[p] = 1
+        return p
+
+    def _give_back(self, pages):
+        for p in pages:
+            self._users[p] -= 1
+            if not self._users[p]:
+                self._unused.append(p)
+
+    def _copy(self, src, dst):
+        for i in range(0, len(src), 32768):
+            t = self._upload(src[i:i + 32768] + dst[i:i + 32768])
+            n = t.shape[0] // 2
+            copy_pages(self.cache, t[:n], t[n:])
+
+    def _upload(self, numbers):
+        dev = self.cache.k.device
+        return torch.tensor(numbers, dtype=torch.int32, pin_memory=dev.type == "cuda").to(dev, non_blocking=True)

@@ -186,6 +186,8 @@ class Model:
         self.amax = [[torch.zeros(heads, 0, dtype=torch.float64) for _ in range(2)] for _ in range(seqs)]
 
     def append(self, s, k, v):
+        if not k.shape[0]:
+            return
         for w, x in enumerate((k, v)):
             x = x.double().cpu().transpose(0, 1)               # [heads, new, dim]
             c, a = self.codes[s][w], self.amax[s][w]
@@ -496,6 +498,62 @@ def test_streams_and_graphs():
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+def test_a_run_of_them_together():
+    """Two prompts through two layers: stored, attended, forked, grown token by token, an encoder's states attended from the cache, one freed,
+    pages moved: at every step what a plain implementation over each sequence's own tokens gives."""
+    ql, kv = pkg("qlinear"), pkg("kvcache")
+    layers, heads, h, dim, g = 2, 2, 4, 64, _gen(81)
+    seqs = kv.Sequences(kv.new_cache(40, heads, dim, 16, layers))
+    models = {}
+
+    def step(ids, counts, causal=True):
+        rows = seqs.extend(ids, counts)
+        for layer in range(layers):
+            cache = seqs.cache.layer(layer)
+            k, v = (torch.randn(sum(counts), heads, dim, device=DEV, generator=g).bfloat16() for _ in range(2))
+            q = torch.randn(sum(counts), h, dim, device=DEV, generator=g).bfloat16()
+            kv.store(cache, rows, k, v)
+            o = kv.attn(q, cache, rows, 0.125, causal)
+            at = 0
+            for s, c in zip(ids, counts):
+                models[s][layer].append(0, k[at:at + c], v[at:at + c])
+                _attn_check(o[at:at + c], q[at:at + c], models[s][layer], [c], [seqs.length(s)], 0.125, causal, "sequence %d layer %d" % (s, layer))
+                at += c
+
+    def copy_of(ms):
+        out = [Model(heads, dim, 1) for _ in ms]
+        for a, b in zip(out, ms):
+            a.codes, a.amax = [[t.clone() for t in w] for w in b.codes], [[t.clone() for t in w] for w in b.amax]
+        return out
+
+    a, b = seqs.add(), seqs.add()
+    for s in (a, b):
+        models[s] = [Model(heads, dim, 1) for _ in range(layers)]
+    step([a, b], [100, 37])
+    step([b, a], [1, 1])
+    c = seqs.fork(a)
+    models[c] = copy_of(models[a])
+    for _ in range(3):
+        step([a, b, c], [1, 1, 1])
+    step([c], [30])
+    seqs.free(b)
+    assert seqs.compact() > 0
+    step([a, c], [2, 1])
+    states = seqs.add()     # an encoder's states, attended by rows that are none of its tokens, and the same in 16 bits
+    models[states] = [Model(heads, dim, 1) for _ in range(layers)]
+    step([states], [77], causal=False)
+    rows = seqs.rows([states, a], [200, 3])
+    q = torch.randn(203, h, dim, device=DEV, generator=g).bfloat16()
+    cache = seqs.cache.layer(1)
+    o = kv.attn(q, cache, rows, 0.125, causal=False)
+    _attn_check(o[:200], q[:200], models[states][1], [200], [77], 0.125, False, "states")
+    _attn_check(o[200:], q[200:], models[a][1], [3], [seqs.length(a)], 0.125, False, "all of a")
+    k, v = kv.read(cache, seqs.rows([states], [77]), 77)
+    k16, v16 = (t.double()[None] for t in (k, v))
+    x = ql.cross_attn(q[None, :200], k[None], v[None], 0.125)
+    _cross_check(x, q[None, :200], k16, v16, 0.125, what="read back")
 
 
 def test_native_calls_take_what_the_python_side_takes(monkeypatch):

@@ -126,3 +126,92 @@ def test_device_data_becomes_addresses_inside_the_cache(tmp_path):
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-ftrapv", "-I",
                            os.path.join(ROOT, "comfyui-backend-but-rust_amd", "csrc"), str(src), "-o", exe])
     assert subprocess.check_output([exe], text=True) == "ok\n"
+
+
+def _host_copy(cache, src, dst):
+    src, dst = src.tolist(), dst.tolist()
+    assert not set(src) & set(dst) and len(set(dst)) == len(dst)
+    axis = cache.k.dim() - 4
+    for t in cache:
+        t.index_copy_(axis, torch.tensor(dst), t.index_select(axis, torch.tensor(src)))
+
+
+def _write(seqs, rows, ids, held, first):
+    """Marks every new token in its place, as a store would."""
+    k = seqs.cache.k
+    for i, s in enumerate(ids):
+        n = int(rows.starts[i + 1] - rows.starts[i])
+        for j in range(n):
+            t = int(rows.lens[i]) - n + j
+            held[s].append((first + j) % 120 + 1)
+            k[..., int(rows.table[i, t // seqs.page]), 0, t % seqs.page, 0] = held[s][-1]
+        first += n
+    return first
+
+
+def _holds(seqs, s, held):
+    k = seqs.cache.k.flatten(0, -5)[0] if seqs.cache.k.dim() == 5 else seqs.cache.k
+    return [int(k[seqs.pages(s)[t // seqs.page], 0, t % seqs.page, 0]) for t in range(seqs.length(s))] == held[s]
+
+
+@pytest.mark.parametrize("layers", [None, 2])
+def test_sequences_share_copy_and_move_pages(layers, monkeypatch):
+    """Forks, cuts, ends, growth and compaction in any order: every sequence keeps its own tokens, and no page is lost."""
+    import random
+    kv = pkg("kvcache")
+    monkeypatch.setattr(kv, "copy_pages", _host_copy)
+    for seed in range(6):
+        rng = random.Random(seed)
+        seqs = kv.Sequences(kv.new_cache(24, 1, 16, 16, layers, device="cpu"))
+        held, first = {}, 0
+        for _ in range(150):
+            what = rng.choice(("add", "extend", "extend", "extend", "fork", "fork", "truncate", "free", "compact"))
+            ids = sorted(held)
+            if what == "add" or not ids:
+                held[seqs.add()] = []
+            elif what == "fork":
+                s = rng.choice(ids)
+                held[seqs.fork(s)] = list(held[s])
+            elif what == "truncate":
+                s = rng.choice(ids)
+                held[s] = held[s][:rng.randint(0, len(held[s]))]
+                seqs.truncate(s, len(held[s]))
+            elif what == "free":
+                s = rng.choice(ids)
+                seqs.free(s)
+                del held[s]
+            elif what == "compact":
+                seqs.compact()
+                used = {p for s in held for p in seqs.pages(s)}
+                assert used == set(range(len(used)))
+            else:
+                some = rng.sample(ids, rng.randint(1, min(4, len(ids))))
+                counts = [rng.choice((0, 1, 1, 5, 16, 40)) for _ in some]
+                before = (seqs.unused, [seqs.pages(s) for s in ids], [seqs.length(s) for s in ids])
+                try:
+                    rows = seqs.extend(some, counts)
+                except kv.CacheFull:
+                    assert before == (seqs.unused, [seqs.pages(s) for s in ids], [seqs.length(s) for s in ids])
+                    continue
+                assert rows.most == max(counts) and rows.starts.tolist()[-1] == sum(counts)
+                first = _write(seqs, rows, some, held, first)
+            assert all(seqs.length(s) == len(h) and _holds(seqs, s, held) for s, h in held.items()), (seed, what)
+            assert seqs.unused == 24 - len({p for s in held for p in seqs.pages(s)})
+        for s in list(held):
+            seqs.free(s)
+        assert seqs.unused == 24
+
+
+def test_sequences_refuse():
+    kv = pkg("kvcache")
+    seqs = kv.Sequences(kv.new_cache(2, 1, 16, 16, device="cpu"))
+    a = seqs.add()
+    for bad in (lambda: seqs.extend([a, a], [1, 1]), lambda: seqs.extend([a], [1, 2]), lambda: seqs.extend([a], [-1]), lambda: seqs.truncate(a, 1), lambda: seqs.truncate(a, -1)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(kv.CacheFull):
+        seqs.extend([a], [33])
+    with pytest.raises(KeyError):
+        seqs.free(a + 1)
+    rows = seqs.rows([a], [0])
+    assert rows.table.shape == (1, 1) and rows.table.item() == -1 and rows.most == 0
