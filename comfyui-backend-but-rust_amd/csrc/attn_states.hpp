@@ -33,6 +33,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // Rows may outgrow their base by 2^kLag before numerator and denominator are rescaled: far from the ends of fp32, and of the f16 that
 // probabilities are rounded to (2^15.99).
 constexpr float kLag = 6.f;
+// Where probabilities are f16 they are 2^kShift times as large, up to 2^15: below 2^-23 of the base they are subnormal, and rounded by 2^-34 of it.
+template <int DT> constexpr float kShift = DT == DT_F16 ? 9.f : 0.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DT> __device__ __forceinline__ f16acc mfma(u32x4 a, u32x4 b, f16acc c) {
@@ -129,7 +131,7 @@ __device__ __forceinline__ int xcd_contiguous(int b, int n) {
 // The rows of a wave: which they are, their queries, and what they have so far.
 template <class Src, int DP, int RW> struct Lanes {
     static constexpr int KS = DP / 16, DB = DP / 32, DT = Src::DT;
-    int row[RW], token[RW], head[RW], limit[RW];     // of the lane; it sees keys below `limit`
+    int limit[RW];                                   // the lane's rows see keys below
     int all_see;                                     // every row of the wave sees the keys below
     u32x4 qf[RW][KS];                                // in the order of the products' channels
     float c[RW], base[RW], sum[RW];
@@ -138,19 +140,13 @@ template <class Src, int DP, int RW> struct Lanes {
     // rows from r0 on, of `rows`
     __device__ __forceinline__ void start(const Common& a, const Problem& pr, int r0, int rows, int lane) {
         const int col = lane & 31, g = lane >> 5;
-#pragma unroll
-        for (int w = 0; w < RW; ++w) {
-            row[w] = r0 + 32 * w + col;
-            const int r = row[w] < rows ? row[w] : rows - 1;
-            token[w] = r / a.group;
-            head[w] = r - token[w] * a.group;
-            limit[w] = min(pr.keys, pr.limit0 + token[w]);
-        }
         all_see = min(pr.keys, pr.limit0 + min(rows - 1, r0) / a.group);
 #pragma unroll
         for (int w = 0; w < RW; ++w) {
+            const int r = min(r0 + 32 * w + col, rows - 1), token = r / a.group, head = r - token * a.group;
+            limit[w] = min(pr.keys, pr.limit0 + token);
             c[w] = a.c;
-            const uint16_t* qp = (const uint16_t*)a.q + pr.q_at + token[w] * a.q_rs + head[w] * a.q_hs;
+            const uint16_t* qp = (const uint16_t*)a.q + pr.q_at + token * a.q_rs + head * a.q_hs;
             if (a.aligned & 1) {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) qf[w][s] = 16 * s + 8 * g < a.d ? load8(qp + 16 * s + 8 * g, true) : u32x4{0, 0, 0, 0};
@@ -252,7 +248,7 @@ template <class Src, int DP, int RW> struct Lanes {
 #pragma unroll
                 for (int i = 0; i < DB; ++i) acc[w][i] *= f;
             }
-            from[w] = base[w] == -INFINITY ? 0.f : base[w];
+            from[w] = base[w] == -INFINITY ? 0.f : base[w] - kShift<DT>;
             // far out (a bias like the type's lowest value) a fused c s - base would show how base was rounded: the rounded product does not
             if (Src::kBias && __any(fabsf(from[w]) > 262144.f)) {
 #pragma unroll
@@ -264,6 +260,24 @@ template <class Src, int DP, int RW> struct Lanes {
                 from[w] = 0.f;
             }
         }
+    }
+    // What the sum of NB blocks lacks in probs(), which adds the probabilities as they are rounded (half the instructions), for keys whose A
+    // differ much: what is subnormal beside the largest p' may be a large probability of a small A.
+    template <int NB, class Scales>
+    __device__ __forceinline__ void mend_sum(const f16acc (&s)[NB][RW], const float (&kc)[RW][2 * NB], const float (&from)[RW], const Scales& sc) {
+#pragma unroll
+        for (int w = 0; w < RW; ++w)
+#pragma unroll
+            for (int h = 0; h < 2 * NB; ++h) {
+                float lost = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][w][8 * (h & 1) + i], kc[w][h], sc.lv(h) - from[w]));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][w][8 * (h & 1) + i + 1], kc[w][h], sc.lv(h) - from[w]));
+                    lost += p0 + p1 - add2<DT>(pack2<DT>(p0, p1), 0.f);
+                }
+                sum[w] = fmaf(lost, sc.iv(h), sum[w]);
+            }
     }
     // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.
     template <int NB, class Scales>
@@ -382,6 +396,7 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
             float kc[RW][2 * SB], from[RW];
             L.scores(s, kb + at_k + 32 * b * kRowK<DP>, tb + 32 * b, g);
             L.raise(s, kc, from, sc, t * TK + 32 * b, plain, g);
+            if (Src::kNormalize && __builtin_expect(!st.even(), 0)) L.mend_sum(s, kc, from, sc);
 #pragma unroll
             for (int h = 0; h < 2 * SB; ++h) {
                 u32x4 p[RW];
@@ -407,9 +422,10 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
     const int64_t part_at = ((int64_t)split * a.problems + problem) * a.rows_padded;
 #pragma unroll
     for (int w = 0; w < RW; ++w) {
-        if (L.row[w] >= rows) continue;
+        const int row = r0 + wave * WR + 32 * w + (lane & 31), token = row / a.group, head = row - token * a.group;
+        if (row >= rows) continue;
         if (a.splits > 1) {
-            float* const pp = a.part + (part_at + L.row[w]) * (DP + 2);
+            float* const pp = a.part + (part_at + row) * (DP + 2);
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -418,7 +434,7 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
             continue;
         }
         const float inv = L.sum[w] == 0.f ? 0.f : Src::kOut / L.sum[w];
-        uint16_t* const op = (uint16_t*)a.o + pr.o_at + L.token[w] * a.o_rs + L.head[w] * a.o_hs;
+        uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + head * a.o_hs;
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -590,7 +606,7 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
 #pragma unroll
                 for (int i = 0; i < DB; ++i) acc[w][i] *= f;
             }
-            float from = base[w] == -INFINITY ? 0.f : base[w];
+            float from = base[w] == -INFINITY ? 0.f : base[w] - kShift<DT>;
             if (Src::kBias && __any(fabsf(from) > 262144.f)) {      // as in Lanes::raise
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
@@ -607,7 +623,7 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
                 for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[w][b][i], kc[b], off));
                 p[w][2 * b] = pack2<DT>(e[0], e[1]);
                 p[w][2 * b + 1] = pack2<DT>(e[2], e[3]);
-                sum[w] = fmaf(add2<DT>(p[w][2 * b + 1], add2<DT>(p[w][2 * b], 0.f)), sc.iv(b), sum[w]);
+                sum[w] = fmaf(Src::kNormalize ? (e[0] + e[1]) + (e[2] + e[3]) : add2<DT>(p[w][2 * b + 1], add2<DT>(p[w][2 * b], 0.f)), sc.iv(b), sum[w]);
             }
         }
 #pragma unroll
@@ -679,41 +695,50 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
     }
 }
 
-// The parts of rows whose keys several workgroups shared, added in the order of the keys: one workgroup of DP threads per row.
+// The parts of rows whose keys several workgroups shared, added in the order of the keys: a wave per row, first a lane per part, then DP / 64
+// channels a lane.
 template <class Src, int DP>
-__global__ __launch_bounds__(DP) void join_kernel(const Common a, const typename Src::Args sa, int rows_most) {
-    __shared__ float weight[64];
-    const int row = blockIdx.x % rows_most, problem = blockIdx.x / rows_most, ch = threadIdx.x;
+__global__ __launch_bounds__(256) void join_kernel(const Common a, const typename Src::Args sa, int rows_most) {
+    constexpr int E = DP / 64;
+    typedef float fe __attribute__((ext_vector_type(E)));
+    const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), problem = id / rows_most, row = id - problem * rows_most;
+    if (problem >= a.problems) return;
     const Problem pr = Src::problem(sa, a, problem);
     if (row >= pr.tokens * a.group) return;
     const float* const p = a.part + ((int64_t)problem * a.rows_padded + row) * (DP + 2);
     const int64_t step = (int64_t)a.problems * a.rows_padded * (DP + 2);
-    float inv = 0.f;
-    if (ch < 64) {      // a lane per part
-        const f32x2 s = ch < a.splits ? *reinterpret_cast<const f32x2*>(p + ch * step + DP) : f32x2{-INFINITY, 0.f};
-        const float nb = wave_max_f32(s[0]), w = s[0] == -INFINITY ? 0.f : exp2f(s[0] - nb);
-        weight[ch] = w;
-        const float l = (float)wave_sum_f64((double)(s[1] * w));
-        inv = l == 0.f ? 0.f : Src::kOut / l;
-    }
-    __shared__ float scale;
-    if (ch == 0) scale = inv;
-    float v = 0.f;
-    __syncthreads();
-    int s = 0;
-    for (; s + 8 <= a.splits; s += 8) {
-        float x[8];
+    const f32x2 s = lane < a.splits ? *reinterpret_cast<const f32x2*>(p + lane * step + DP) : f32x2{-INFINITY, 0.f};
+    fe x[8];      // eight parts on their way at once, the first before the weights are known
+    const auto load = [&](int i) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = p[(s + i) * step + ch];
+        for (int j = 0; j < 8; ++j) {
+            x[j] = fe{};
+            if (i + j < a.splits)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v = fmaf(x[i], weight[s + i], v);
+                for (int e = 0; e < E; ++e) x[j][e] = p[(i + j) * step + E * lane + e];
+        }
+    };
+    load(0);
+    const float nb = wave_max_f32(s[0]), w = s[0] == -INFINITY ? 0.f : exp2f(s[0] - nb);
+    const float l = (float)wave_sum_f64((double)(s[1] * w)), inv = l == 0.f ? 0.f : Src::kOut / l;
+    fe v{};
+    for (int i = 0; i < a.splits; i += 8) {
+        if (i) load(i);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float wj = u2f(__builtin_amdgcn_readlane(f2u(w), (i + j) & 63));      // 0 behind the last part
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = fmaf(x[j][e], wj, v[e]);
+        }
     }
-    for (; s < a.splits; ++s) v = fmaf(p[s * step + ch], weight[s], v);
-    if (ch >= a.d) return;
-    const float r = scale == 0.f ? 0.f : v * scale;
     const int token = row / a.group, head = row - token * a.group;
-    uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + head * a.o_hs + ch;
-    *op = a.q_dt == DT_BF16 ? f_to_bf16(r) : f_to_f16(r);
+    uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + head * a.o_hs + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (E * lane + e < a.d) {
+            const float r = inv == 0.f ? 0.f : v[e] * inv;
+            op[e] = a.q_dt == DT_BF16 ? f_to_bf16(r) : f_to_f16(r);
+        }
 }
 
 // How a call runs: 16 or 32 rows with the keys over a workgroup's waves, or tiles of 128 or 256 rows; and over how many workgroups the keys of a
@@ -740,14 +765,14 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         // part 22.6 in all), and longer where the waves of a CU together ask for more than its share of the copy rate, 20 KB a microsecond,
         // of which CUs with few waves reach less (12 x 32749 keys x 8 heads of 128 codes: 3 parts 183, 5 parts 138, 8 parts, which are one
         // full round, 130, 16 parts 136); a wave beside others on its CU takes a little more; joining 3.
-        const int tile = rows <= 16 ? 16 : 32, per_cu = dp == 256 ? 1 : tile == 32 || (bytes > 1 && dp == 128) ? 2 : 3;
-        const int64_t slots = cus * per_cu, tiles = (keys + 31) / 32;
+        const int tile = rows <= 16 || dp == 256 ? 16 : 32, per_cu = dp == 256 ? 1 : tile == 32 || (bytes > 1 && dp == 128) ? 2 : 3;
+        const int64_t slots = cus * per_cu, tiles = (keys + 31) / 32, groups = problems * ((rows + tile - 1) / tile);
         const double full = per_cu * 4 * 32. * d * 2 * bytes / 20e3;
         int best = 1;
         double least = 0.;
         for (int s = 1; s <= 64 && (s == 1 || s <= tiles); ++s) {
-            const int64_t rounds = (problems * s + slots - 1) / slots, each = ((tiles + s - 1) / s + 3) / 4;
-            const double busy = problems * s >= slots ? 1. : (double)(problems * s) / slots, shared = full * busy / (0.85 + 0.15 * busy), step = shared > 1.65 ? shared : 1.65;
+            const int64_t rounds = (groups * s + slots - 1) / slots, each = ((tiles + s - 1) / s + 3) / 4;
+            const double busy = groups * s >= slots ? 1. : (double)(groups * s) / slots, shared = full * busy / (0.85 + 0.15 * busy), step = shared > 1.65 ? shared : 1.65;
             const int64_t in_one = (tiles + s - 1) / s;
             const double us = rounds * (4. + each * step + 0.25 * (in_one < 4 ? in_one : 4)) + (s == 1 ? 0. : 3. + 0.02 * s + 4e-6 * (dp + 2) * rows * problems * s / 2.);
             if (s == 1 || us < least) {
@@ -779,8 +804,8 @@ template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Comm
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid > 0x7fffffff || a.problems * rows > 0x7fffffff) return -1;
     if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
-    else if (p.rows == 32) few_kernel<Src, DP, 4, 2, DP == 256 ? 1 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if (p.rows == 32) few_kernel<Src, DP, 4, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 128) {
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 2, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
@@ -790,7 +815,7 @@ template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Comm
     }
     KCHECK();
     if (p.splits > 1) {
-        join_kernel<Src, DP><<<(int)(a.problems * rows), DP, 0, stream>>>(a, sa, (int)rows);
+        join_kernel<Src, DP><<<(int)((a.problems * rows + 3) / 4), 256, 0, stream>>>(a, sa, (int)rows);
         KCHECK();
     }
     return 0;

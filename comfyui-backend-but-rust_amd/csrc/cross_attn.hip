@@ -157,6 +157,7 @@ template <int DTYPE, bool BIAS> struct Dense {
             return false;
         }
         __device__ __forceinline__ bool numbers() const { return true; }
+        __device__ __forceinline__ bool even() const { return true; }
         __device__ __forceinline__ Scales scales(int) const { return {}; }
     };
 };

@@ -21,9 +21,9 @@ struct Codes {
     typedef CacheArgs Args;
     static constexpr int DT = DT_F16;
     static constexpr bool kBias = false, kNormalize = true;
-    // iv is 2^16 / A, so that sums of both ends of A's range, 2^-90 and 2^128, stay ordinary numbers; a smaller A counts as 2^-90, and as
+    // iv is 16 / A, so that sums of both ends of A's range, 2^-90 and 2^128, stay ordinary numbers; a smaller A counts as 2^-90, and as
     // 2^-60 of the largest so far, so that p' does not leave fp32
-    static constexpr float kOut = 65536.f / 127.f;
+    static constexpr float kOut = 16.f / 127.f;
     template <int N> struct Scales {
         float ks[N], lvs[N], ivs[N];
         __device__ float k(int h) const { return ks[h]; }
@@ -53,10 +53,10 @@ struct Codes {
         const Args& a;
         const int32_t* table;
         int tid, lane, keys, d, hk, head;
-        int k_window = -1, v_window = -1, s_window = -1;
-        int k_page, v_page;              // of block 64 * window + lane
+        int window = -1, s_window = -1;
+        int pages;                       // of block 64 * window + lane
         float ks, lv, iv, top = 0.f;     // its scales
-        bool all_numbers;                // of the window
+        bool all_numbers, all_even;      // of the window
         u32x4 kr[CH], vr[CH];
         __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_)
             : a(a_), tid(tid_), lane(threadIdx.x & 63), keys(p.keys), d(c.d), hk(c.hk) {
@@ -83,10 +83,11 @@ struct Codes {
             const float u = top == 0.f ? 1.f : A > 0.f && good ? fmaxf(A, fmaxf(top * 0x1p-60f, 0x1p-90f)) : top;
             all_numbers = !__any(ks != ks);
             lv = __builtin_amdgcn_logf(u);
-            iv = 65536.f / u;
+            iv = 16.f / u;
+            all_even = !__any(u < top * 0x1p-4f);
         }
         // TK rows from key0, a multiple of 32
-        __device__ __forceinline__ void rows(u32x4 (&x)[CH], const int8_t* codes, int& window, int& pages, int key0) {
+        __device__ __forceinline__ void rows(u32x4 (&x)[CH], const int8_t* codes, int key0) {
             if (!mine()) return;
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
@@ -102,19 +103,19 @@ struct Codes {
                 x[j] = 16 * ch < d ? *reinterpret_cast<const u32x4*>(codes + at + in) : u32x4{0, 0, 0, 0};
             }
         }
-        __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, k_window, k_page, key0); }
-        __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, v_window, v_page, key0); }
+        __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, key0); }
+        __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, key0); }
         __device__ __forceinline__ void load_fragments(int key0) {
             static_assert(NT != 64 || CH == 2 * (DP / 64), "32 keys of a wave");
             const int col = tid & 15, gg = tid >> 4;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 const int block = __builtin_amdgcn_readfirstlane(key0 >> 4) + b;
-                if (block >> 6 != k_window) {
-                    k_window = block >> 6;
-                    k_page = page(64 * k_window + lane);
+                if (block >> 6 != window) {
+                    window = block >> 6;
+                    pages = page(64 * window + lane);
                 }
-                const int8_t* const at = a.k + codes_at(__builtin_amdgcn_readlane(k_page, block & 63), hk, head, a.page_shift, block, d);
+                const int8_t* const at = a.k + codes_at(__builtin_amdgcn_readlane(pages, block & 63), hk, head, a.page_shift, block, d);
 #pragma unroll
                 for (int i = 0; i < DP / 64; ++i)
                     kr[b * (DP / 64) + i] = 64 * i + 16 * gg < d ? *reinterpret_cast<const u32x4*>(at + (uint32_t)(col * d + 64 * i + 16 * gg)) : u32x4{0, 0, 0, 0};
@@ -147,6 +148,7 @@ struct Codes {
         }
         __device__ bool any_key(int, int) const { return true; }
         __device__ __forceinline__ bool numbers() const { return all_numbers; }
+        __device__ __forceinline__ bool even() const { return all_even; }
         // of the TK keys from key0
         __device__ __forceinline__ Scales<TK / kBlock> scales(int key0) {
             const int block = __builtin_amdgcn_readfirstlane(key0 >> 4);

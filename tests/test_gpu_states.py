@@ -3,8 +3,12 @@
 
 The cache's codes and scales are whole-number work and must be equal.  Attention outputs are held to bounds that count roundings, each off by at
 most half a step u (bf16 2^-8, f16 2^-11, fp32 2^-24 relative to the value):
-  the output's rounding                              u_out |o|
-  probabilities, rounded for the product with V      u_p sum p |v| / sum p      (f16: those below 2^-14 of the largest 2^-25 of it, each)
+  the output's rounding                              u_out |o|, or half the type's smallest step (f16: 2^-25) where that is more
+  probabilities, rounded for the product with V      u_p sum p |v| / sum p
+  ... in f16, where they are subnormal               n 2^-34 max_j p_j A_j / sum p: they are held in units of 2^-9 times a base that is at most the
+                                                     largest p_j A_j, A_j the magnitude that the kernel counts into p (1, or the block's), and
+                                                     round by 2^-25 of a unit; the cache's sum takes them rounded where no A is below 1/16 of
+                                                     the largest: n 2^-30 of the sum
   scores, fp32 sums of d products in any order       |dx| <= (d + 8) 2^-24 (scale max_j sum_i |q_i k_ji| + |bias|) in the exponent, in numerator
                                                      and denominator: 2 |dx| sum p |v| / sum p; exp2 itself 2^-22 likewise
   the sums over n keys                               (n + 8) 2^-23 sum p |v| / sum p
@@ -26,7 +30,8 @@ def _gen(seed):
 
 
 def _reference(q, k, v, scale, keep, bias, u_p, u_out, tiny):
-    """One head in 64 bits: q [m, d], k, v [l, d], keep bool [m, l], bias [l] -> (o, bound), both [m, d]."""
+    """One head in 64 bits: q [m, d], k, v [l, d], keep bool [m, l], bias [l] -> (o, bound), both [m, d].  tiny: the
+    A_j of f16 probabilities, or None."""
     q, k, v = q.double(), k.double(), v.double()
     keep = keep & ~torch.isneginf(bias)
     k, v = (torch.where(keep.any(0)[:, None], t, 0.0) for t in (k, v))     # a key that nobody sees may hold anything
@@ -43,8 +48,8 @@ def _reference(q, k, v, scale, keep, bias, u_p, u_out, tiny):
         size = size.amax(-1, keepdim=True) + torch.where(torch.isinf(bias), 0.0, bias.abs().clamp(max=1e4)).max()
     d, n = q.shape[1], k.shape[0]
     dx = (d + 8) * 2.0 ** -24 * size + 2.0 ** -22 if n else 0.0
-    low = n * 2.0 ** -25 * tiny * (p[:, :, None] * v.abs()).amax(1) / l if n and tiny and q.shape[0] * n * d < 2 ** 28 else (n * 2.0 ** -25 * tiny * v.abs().amax(0) / l if n else 0.0)
-    return o, u_out * o.abs() + (u_p + 2 * dx + (n + 8) * 2.0 ** -23) * mass + low + 1e-30
+    low = n * (2.0 ** -34 * (p * tiny).amax(-1, keepdim=True) / l + 2.0 ** -30 * mass) if n and tiny is not None else 0.0
+    return o, (u_out * o.abs()).clamp(min=2.0 ** -25 if u_out == U[torch.float16] else 0.0) + (u_p + 2 * dx + (n + 8) * 2.0 ** -23) * mass + low + 1e-30
 
 
 def _check(got, want, bound, what):
@@ -75,7 +80,7 @@ def _cross_check(o, q, k, v, scale, k_lens=None, mask=None, what=""):
             else:
                 bias = row.double()
         for j in range(h):
-            want, bound = _reference(q[i, :, j], k[i, :, j * hk // h], v[i, :, j * hk // h], scale, keep, bias, U[q.dtype], U[q.dtype], 1.0 if q.dtype == torch.float16 else 0.0)
+            want, bound = _reference(q[i, :, j], k[i, :, j * hk // h], v[i, :, j * hk // h], scale, keep, bias, U[q.dtype], U[q.dtype], v.double().nan_to_num(0, 0, 0).abs().max() if q.dtype == torch.float16 and lk else None)
             _check(o[i, :, j], want, bound, "%s item %d head %d" % (what, i, j))
 
 
@@ -369,9 +374,10 @@ def _attn_check(o, q, model, new, lens, scale, causal, what=""):
         k, v = model.values(s, 0)[:l], model.values(s, 1)[:l]
         pos = torch.arange(l - m, l, device=DEV) if causal else torch.full((m,), l, device=DEV)
         keep = torch.arange(l, device=DEV) <= pos[:, None]
+        tiny = model.amax[s][1].repeat_interleave(16, 1)[:, :l].to(DEV)
         for j in range(h if m else 0):
             # q rows are scaled to f16: what lies 2^14 below the row's largest rounds by 2^-25 of it, less than the sums' own roundings
-            want, bound = _reference(q[at:at + m, j], k[:, j * heads // h], v[:, j * heads // h], scale, keep, torch.zeros(l, dtype=torch.float64, device=DEV), U[torch.float16], U[q.dtype], 1.0)
+            want, bound = _reference(q[at:at + m, j], k[:, j * heads // h], v[:, j * heads // h], scale, keep, torch.zeros(l, dtype=torch.float64, device=DEV), U[torch.float16], U[q.dtype], tiny[j * heads // h])
             _check(o[at:at + m, j], want, bound, "%s sequence %d head %d" % (what, s, j))
         at += m
 
@@ -409,6 +415,23 @@ def test_cache_attn_scales_of_all_sizes(new):
         model.append(0, k, v)
         q = (q_size * torch.randn(new, 2, 64, device=DEV, generator=g)).bfloat16()
         _attn_check(kv.attn(q, cache, _rows(kv, [new], lens, table), 0.125, True), q, model, [new], lens, 0.125, True, "%g %g %g" % (q_size, k_size, v_size))
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_cache_attn_small_values_with_most_of_the_probability(new):
+    """Blocks whose values are 2^-30 of others' hold nearly all of the probability: their keys' p A is subnormal, their sum is not."""
+    kv = pkg("kvcache")
+    g, lens = _gen(14), [1600]
+    cache, table = kv.new_cache(50, 1, 64, 32), _table(lens, 32, 50, 1)
+    k = (0.05 * torch.randn(1600, 1, 64, device=DEV, generator=g)).bfloat16()
+    v = torch.randn(1600, 1, 64, device=DEV, generator=g)
+    v[16:] *= 2.0 ** -30
+    v = v.bfloat16()
+    kv.store(cache, _rows(kv, lens, lens, table), k, v)
+    model = Model(1, 64, 1)
+    model.append(0, k, v)
+    q = torch.randn(new, 2, 64, device=DEV, generator=g).bfloat16()
+    _attn_check(kv.attn(q, cache, _rows(kv, [new], lens, table), 0.125, True), q, model, [new], lens, 0.125, True)
 
 
 def test_cache_attn_strided_rows():
