@@ -12,7 +12,7 @@
 // key_of() does.  Probabilities never cross lanes.  V is read from LDS with the transposing 16-bit read, which turns four keys times
 // 16 channels, so it is staged as it lies in memory.
 //
-// A workgroup is four waves with rows of their own on the same keys (tiles_kernel), or several on the same 32 rows and different keys,
+// A workgroup is waves with rows of their own on the same keys (tiles_kernel), or four waves on the same 16 or 32 rows and different keys,
 // whose results meet in LDS (few_kernel).  Where that leaves CUs idle, several workgroups share a row's keys and leave numerators,
 // denominators and bases in the workspace.
 #pragma once
@@ -99,8 +99,9 @@ struct Common {
     int rows_padded;
 };
 
-inline void set_scale(Common& c, float scale) {
-    c.c = fabsf(scale) * kLog2e;
+// A |scale| log2 e below `least` counts as 0.
+inline void set_scale(Common& c, float scale, float least) {
+    c.c = fabsf(scale) * kLog2e < least ? 0.f : fabsf(scale) * kLog2e;
     c.q_and = 0xffffffffu;
     c.q_xor = scale < 0.f ? 0x80008000u : 0u;
     if (c.c == 0.f) {
@@ -349,7 +350,18 @@ __device__ __forceinline__ void share_of(int end, int tk, int splits, int split,
 }
 
 // Many rows: QW waves of 32 RW rows on the same keys, 32 NB at a time in two buffers: a tile is on its way into registers while the one
-// before goes into LDS and the one before that is multiplied.
+// before goes into LDS and the one before that is multiplied, SB blocks of 32 keys per step of the softmax.
+//
+// 4 * d operations a pair on the matrix pipes, one exponential a pair beside them.  2 x 1024 new tokens of 32 heads behind 7168 stored ones
+// (223 GFLOP) take 274 us, 0.81 PFLOP/s where an 8192-cubed product of the vendor's library reaches 1.23; matrix pipes 41 % and vector
+// pipes 54 % busy at 1.7 GHz under the power limit, and the two hardly overlap: a probe shows a product of another wave keeping vector
+// instructions from issue for 11 of its 32 cycles (v_dot2 for all of them).  Head dim 64 (frame of 2025 tokens to 16200, f16, 16 heads):
+// vector pipes 75 % busy, 199 us.
+// Eight waves on a tile spend half the instructions on staging, conversion to f16 above all, that four do (289 us against 325), but few rows
+// do not fill them; 64 keys per softmax step with one branch 285 against 289; sums of rounded pairs (v_dot2) against additions 270 and
+// 284.  Not kept: scores of the next keys between the exponentials, left to the compiler (292) or held there by sched_barrier (310); two
+// groups of waves half a tile apart (288 at best, 312); two row blocks a wave, which halve the reads of LDS but leave one wave a SIMD at head
+// dim 128 (440) or fewer at 64 (252 against 210).
 template <class Src, int DP, int RW, int QW, int NB, int SB, int OCC>
 __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, const typename Src::Args sa) {
     constexpr int TK = 32 * NB, WR = 32 * RW, TILE_K = TK * kRowK<DP>, TILE_V = TK * kRowV<DP>;
@@ -457,6 +469,8 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
 // results meet.  What counts is the keys' way in: K goes from memory straight into the fragments of v_mfma_f32_16x16x32 (lane: key
 // lane % 16, channels in the order of Source::q_chunk), V through the wave's own piece of LDS, where it is turned.  Lanes hold row lane % 16 and
 // keys 4 (lane / 16) .. + 3 of each 16, which is, in order, what the product with V takes, if that counts its keys so.
+// 12 tokens to 16 to 32 thousand keys of 8 heads of 128 codes each: 131 us with the joining, 4.7 TB/s, where a copy reaches 5.2; in the 32 x 32 x 16
+// form with K through LDS, twice the registers and half the waves, 203.  One token to 613 keys: 10 us, of which 3.5 are the second launch.
 template <int DT> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     if constexpr (DT == DT_BF16)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -695,8 +709,8 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
     }
 }
 
-// The parts of rows whose keys several workgroups shared, added in the order of the keys: a wave per row, first a lane per part, then DP / 64
-// channels a lane.
+// The parts of rows whose keys several workgroups shared, added in the order of the keys, so every call gives the same bits: a wave per row,
+// first a lane per part, then DP / 64 channels a lane.  Two trips to memory: 3.5 us for a few rows, 13.7 for 4 parts of 32400 rows of 64.
 template <class Src, int DP>
 __global__ __launch_bounds__(256) void join_kernel(const Common a, const typename Src::Args sa, int rows_most) {
     constexpr int E = DP / 64;
@@ -785,7 +799,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
     // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts
     Plan best{};
     double least = 0.;
-    for (int tile = 128; tile <= (dp == 256 ? 128 : 256); tile *= 2) {
+    for (int tile = 128; tile <= (dp == 256 || rows <= 128 ? 128 : 256); tile *= 2) {
         const int64_t slots = cus * (dp == 256 ? 1 : dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 ? 2 : 1), groups = (rows + tile - 1) / tile * problems;
         const double start = tile == 128 ? 7. : 10., each = tile == 128 ? 2.6 : 2.4;
         for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 512); ++s) {
@@ -802,7 +816,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
 
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
-    if (grid > 0x7fffffff || a.problems * rows > 0x7fffffff) return -1;
+    if (grid * 512 > 0xffffffff || a.problems * rows * 64 > 0xffffffff) return -1;      // threads of a launch
     if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if (p.rows == 32) few_kernel<Src, DP, 4, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);

@@ -177,7 +177,7 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     if (b < 0 || lq < 0 || lk < 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256 || head_dim % 8 != 0) return -1;
     if (mask_kind < 0 || mask_kind > 2 || (mask_kind != 0 && !mask && lk > 0) || !(fabsf(scale) < INFINITY)) return -1;
     if (b == 0 || lq == 0) return 0;
-    if ((int64_t)lq * (h / hk) > 0x7fffff00 || (int64_t)b * hk > 0x7fffffff || !q || !o || (lk > 0 && (!k || !v))) return -1;
+    if ((int64_t)lq * (h / hk) > 0x7ffff000 || (int64_t)b * hk > 0x7fffffff || !q || !o || (lk > 0 && (!k || !v))) return -1;
     const Plan p = make_plan((int64_t)lq * (h / hk), (int64_t)b * hk, lk, head_dim, 2);
     if (p.bytes && (!ws || (uintptr_t)ws % 16 != 0)) return -1;
     const auto sixteen = [](const void* at, int64_t s0, int64_t s1, int64_t s2) { return (uintptr_t)at % 16 == 0 && (s0 | s1 | s2) % 8 == 0; };
@@ -186,7 +186,8 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
     c.row_tiles = p.row_tiles; c.problems = b * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
     c.aligned = (sixteen(q, q_bs, q_rs, q_hs) ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_bs | o_rs | o_hs) % 4 == 0 ? 2 : 0);
-    set_scale(c, scale);
+    // with a bias, which is counted in units of the score, scales from which it would leave fp32 are none
+    set_scale(c, scale, mask_kind == 2 ? 1e-30f : 1.17549435e-38f);
     c.part = (float*)ws;
     CrossArgs s{};
     s.per_score = (float)(1.4426950408889634 / c.c);
@@ -200,4 +201,12 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == DT_BF16) return mask_kind ? launch_dim<Dense<DT_BF16, true>>(p, (int64_t)lq * (h / hk), c, s, st) : launch_dim<Dense<DT_BF16, false>>(p, (int64_t)lq * (h / hk), c, s, st);
     return mask_kind ? launch_dim<Dense<DT_F16, true>>(p, (int64_t)lq * (h / hk), c, s, st) : launch_dim<Dense<DT_F16, false>>(p, (int64_t)lq * (h / hk), c, s, st);
+}
+
+GPU_API int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t keys, int head_dim, int bytes, int32_t* out) {
+    if (rows <= 0 || problems <= 0 || keys < 0 || head_dim <= 0 || head_dim > 256 || (bytes != 1 && bytes != 2) || !out) return -1;
+    const Plan p = make_plan(rows, problems, keys, head_dim, bytes);
+    out[0] = p.rows;
+    out[1] = p.splits;
+    return 0;
 }

@@ -49,5 +49,5 @@ inline bool cache_ok(const void* k, const void* v, const void* ks, const void* v
            (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)ks % 4 == 0 && (uintptr_t)vs % 4 == 0;
 }
 inline bool rows_ok(const void* starts, const void* lens, const void* table, int cols, int n, int rows, int most) {
-    return n >= 0 && rows >= 0 && most >= 0 && cols > 0 && (n == 0 || (starts && lens && table));
+    return n >= 0 && rows >= 0 && most >= 0 && (n == 0 || (cols > 0 && starts && lens && table));
 }

@@ -180,7 +180,7 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     if (!cache_ok(k, v, k_scale, v_scale, n_pages, page, hk, head_dim) || h <= 0 || h % hk != 0 || !(fabsf(scale) < INFINITY)) return -1;
     if (!rows_ok(starts, lens, table, table_cols, n, rows, most)) return -1;
     if (n == 0 || rows == 0 || most == 0) return 0;
-    if (!q || !o || (int64_t)most * (h / hk) > 0x7fffff00 || (int64_t)n * hk > 0x7fffffff) return -1;
+    if (!q || !o || (int64_t)most * (h / hk) > 0x7ffff000 || (int64_t)n * hk > 0x7fffffff) return -1;
     const Plan p = make_plan((int64_t)most * (h / hk), (int64_t)n * hk, (int64_t)table_cols * page, head_dim, 1);
     if (p.bytes && (!ws || (uintptr_t)ws % 16 != 0)) return -1;
     Common c{};
@@ -188,7 +188,7 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
     c.row_tiles = p.row_tiles; c.problems = n * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
     c.aligned = ((uintptr_t)q % 16 == 0 && (q_rs | q_hs) % 8 == 0 ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_rs | o_hs) % 4 == 0 ? 2 : 0);
-    set_scale(c, scale);
+    set_scale(c, scale, 1.17549435e-38f);
     c.part = (float*)ws;
     CacheArgs s{k, v, k_scale, v_scale, starts, lens, table, rows, most, n_pages, __builtin_ctz(page), table_cols, causal != 0};
     return launch_dim<Codes>(p, (int64_t)most * (h / hk), c, s, (hipStream_t)stream);

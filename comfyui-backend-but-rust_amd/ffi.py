@@ -52,6 +52,7 @@ SIGNATURES = {
     "gpu_int8_attn_key_bias": [_P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32] + [_I64] * 12 + [_F32, _P, _P],
     "gpu_cross_attn": [_I32, _P, _P, _P, _P, _P] + [_I32] * 6 + [_I64] * 12 + [_F32, _P, _P, _I32, _I64, _P],
     "gpu_cross_attn_workspace": [_I32] * 6,
+    "gpu_internal_states_plan": [_I64, _I64, _I64, _I32, _I32, _P],
     "gpu_kv8_store": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 6 + [_P],
     "gpu_kv8_read": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 6 + [_P],
     "gpu_kv8_attn": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 7 + [_F32, _I32, _P],

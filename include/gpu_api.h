@@ -317,7 +317,8 @@ int64_t gpu_w6a8_group_gemm_scratch(const void* Wp, int64_t M, int64_t N, int64_
  * j / (h / hk).  head_dim a multiple of 8 up to 256.  Rows that start on 16 bytes (o: 8) take wide loads, others work too.
  * k_lens: int32 [b] on the device or null (all lk); values outside 0..lk count as the nearer end.  mask: null (mask_kind 0), bytes [b, lk], 0 = the
  * key is out (1), or f32 [b, lk] added to the logits, -inf = out (2); rows mask_bs elements apart (0: one row for all), 32-bit elements on 4 bytes.
- * A key that is out counts as absent whatever k and v hold there; a row without keys gives zeros.  Scores, probabilities' sums and
+ * A key that is out counts as absent whatever k and v hold there; a row without keys gives zeros.  With f32 masks a |scale| below
+ * 7e-31 counts as 0.  Scores, probabilities' sums and
  * outputs are held in fp32, the probabilities rounded to the row type for the product with v.
  * ws: gpu_cross_attn_workspace bytes (0: null will do), 16-byte aligned, in use until the work queued here has run.
  * Returns -1 for sizes, a scale that is not finite, or pointers that do not fit this. */
@@ -330,6 +331,7 @@ int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void*
 /* A paged cache of keys and values in 8 bits.
  *   k, v              int8 [n_pages, hk, page, d], 16-byte aligned; page a power of two from 16 to 4096, d a multiple of 16 up to 256
  *   k_scale, v_scale  f32 [n_pages, hk, page / 16]: A, the largest magnitude of the 16 tokens' values of that head; a code c stands for c * A / 127
+ *                     (where A is 0 the codes are)
  *   starts int32 [n + 1], lens int32 [n], table int32 [n, table_cols], all on the device: rows starts[s] .. starts[s + 1] of the call's
  *     row tensors are the LAST tokens of sequence s, which holds lens[s] tokens (the new ones among them, at most 2^30); its token t is slot
  *     t % page of page table[s, t / page].  rows: rows of the row tensors, none behind it is touched; most: the most rows of one
@@ -360,6 +362,11 @@ int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* o, 
                  float scale, int causal, void* stream);
 int gpu_kv8_copy_pages(int8_t* ck, int8_t* cv, float* k_scale, float* v_scale, int layers, int n_pages, int page, int hk, int head_dim,
                        const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times
+ * key-value heads) of `rows` (query tokens times query heads of a key-value head, the most of any) over `keys`: out[0] = rows of a workgroup (16 and 32:
+ * its waves share them, 128 and 256: a wave has 32), out[1] = workgroups that share a row's keys. */
+int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t keys, int head_dim, int bytes, int32_t* out);
 
 /* Test and tuning hook: force the GEMM kernel family.  1, 2 = 128x128 and 64x64 register-staged tiles; 5 = weights straight
  * into registers, for M <= 128; 7 = four waves multiply what four others fetch, 128x64 to 128x192 tiles, K split where they are few;

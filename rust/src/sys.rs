@@ -104,6 +104,7 @@ extern "C" {
         rows: i32, most: i32, h: i32, hk: i32, head_dim: i32, scale: f32, causal: i32, stream: PM) -> i32;
     pub fn gpu_kv8_copy_pages(ck: PM, cv: PM, k_scale: PM, v_scale: PM, layers: i32, n_pages: i32, page: i32,
         hk: i32, head_dim: i32, src: P, dst: P, n: i32, stream: PM) -> i32;
+    pub fn gpu_internal_states_plan(rows: i64, problems: i64, keys: i64, head_dim: i32, bytes: i32, out: PM) -> i32;
     pub fn gpu_int8_gemm_force_config(cfg: i32) -> i32;
     pub fn gpu_internal_int8_gemm_plan(m: i64, n: i64, k: i64, start: i32, aligned: i32, out: PM) -> i32;
     pub fn gpu_mfma_layout_probe(out: PM, stream: PM) -> i32;

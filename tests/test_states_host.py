@@ -1,5 +1,6 @@
 """Attention to stored states without a GPU: refusals of the C ABI and of the Python side, and the arithmetic that turns device data into
 addresses, compiled for the host."""
+import ctypes
 import os
 import subprocess
 
@@ -34,7 +35,7 @@ def _move(name, dtype=2, a=P, b=P, s=128, k=P, v=P, ks=P, vs=P, pages=4, page=64
 
 CACHE = [({"k": 0}, -1), ({"v": P + 8}, -1), ({"ks": 0}, -1), ({"vs": P + 2}, -1), ({"pages": 0}, -1), ({"page": 48}, -1), ({"page": 8}, -1), ({"page": 8192}, -1), ({"hk": 0}, -1),
          ({"d": 72}, -1), ({"d": 272}, -1), ({"d": 0}, -1), ({"starts": 0}, -1), ({"lens": 0}, -1), ({"table": 0}, -1), ({"cols": 0}, -1), ({"n": -1}, -1), ({"rows": -1}, -1), ({"most": -1}, -1),
-         ({"n": 0}, 0), ({"rows": 0}, 0), ({"most": 0}, 0)]
+         ({"n": 0}, 0), ({"n": 0, "cols": 0, "table": 0}, 0), ({"rows": 0}, 0), ({"most": 0}, 0)]
 
 
 @pytest.mark.parametrize("args,code", CACHE + [({"dtype": 0}, -4), ({"h": 3}, -1), ({"scale": float("nan")}, -1), ({"q": 0}, -1), ({"o": 0}, -1), ({"cols": 1 << 16, "ws": 0}, -1)])
@@ -66,6 +67,25 @@ def test_workspaces():
     assert w(2, 4096, 77, 10, 10, 64) == 0 and w(0, 1, 1, 1, 1, 64) == 0 and w(1, 1, 100, 3, 2, 64) == 0
     assert w(1, 1, 1 << 16, 8, 8, 128) % 16 == 0 and w(1, 1, 1 << 16, 8, 8, 128) > 0
     assert ffi.lib.gpu_kv8_attn_workspace(1, 1, 32, 8, 128, 64, 1024) > 0 and ffi.lib.gpu_kv8_attn_workspace(1, 1, 32, 8, 128, 64, 1) == 0
+
+
+def _plan(rows, problems, keys, d, bytes):
+    out = (ctypes.c_int32 * 2)()
+    ffi.k("gpu_internal_states_plan", rows, problems, keys, d, bytes, ctypes.cast(out, ctypes.c_void_p))
+    return tuple(out)
+
+
+@pytest.mark.parametrize("case,plan", [
+    ((4096, 20, 77, 64, 2), (128, 1)),          # SDXL's prompt keys: short, many rows
+    ((8192, 40, 512, 128, 2), (128, 1)),        # 142 us against 149 with tiles of 256 rows
+    ((1111, 48, 4608, 128, 2), (256, 1)),       # 175 against 191; in two parts 217 to 230
+    ((4096, 16, 8192, 128, 1), (256, 1)),       # 284 against 324; in two parts 336
+    ((2025, 16, 16256, 64, 1), (256, 4)),       # 200 against 218 in two parts, 357 in one
+    ((4, 96, 32752, 128, 1), (16, 8)),          # one full round: 130 against 138 and 154 in 5 and 6 parts
+    ((1, 64, 1369, 72, 2), (16, 6)), ((20, 8, 4096, 128, 1), (32, 32)), ((33, 1, 64, 256, 2), (128, 1)), ((1, 1, 0, 8, 2), (16, 1)), ((1, 2000, 100000, 128, 1), (16, 8)), ((200, 1, 1010, 128, 2), (256, 1)), ((128, 1, 1010, 128, 2), (128, 1))])
+def test_attention_forms_where_they_were_measured(case, plan):
+    """For 256 CUs, which is what a host without a device is taken for."""
+    assert _plan(*case) == plan
 
 
 def test_python_side_refuses_host_tensors():
