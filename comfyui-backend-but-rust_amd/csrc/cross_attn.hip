@@ -66,13 +66,17 @@ template <int DTYPE, bool BIAS> struct Dense {
             const int b = id / c.hk, head = id - b * c.hk;
             k = a.k + b * a.k_bs + head * a.k_hs;
             v = a.v + b * a.v_bs + head * a.v_hs;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) kr[j] = vr[j] = u32x4{0, 0, 0, 0};
             mask = a.mask_kind == 1 ? (const void*)((const uint8_t*)a.mask + b * a.mask_bs) : (const void*)((const float*)a.mask + b * a.mask_bs);
         }
         // rows from key0 on into registers, and what their keys' masks say; past the end zeros
         __device__ __forceinline__ void rows(u32x4 (&x)[CH], const uint16_t* p, int64_t rs, int key0) {
             if (!mine()) return;
-            if (a.aligned && d == DP && key0 + TK <= keys) {     // whole rows of 16-byte pieces: a scalar base and 32-bit offsets
+            static_assert(NT % ROW == 0, "a thread's pieces are of one chunk");
+            if (a.aligned && key0 + TK <= keys) {     // 16-byte pieces: a scalar base and 32-bit offsets; behind the head dim they stay 0
                 const char* const at = (const char*)(p + (int64_t)key0 * rs);
+                if (8 * (tid % ROW) < d)
 #pragma unroll
                 for (int j = 0; j < CH; ++j) {
                     const int i = tid + j * NT;
@@ -106,12 +110,13 @@ template <int DTYPE, bool BIAS> struct Dense {
             for (int b = 0; b < 2; ++b) {
                 const int key = key0 + 16 * b + col;
                 const uint16_t* const at = k + (key < keys ? key : 0) * a.k_rs + 8 * gg;
-                if (a.aligned && d == DP) {
+                if (a.aligned) {
 #pragma unroll
-                    for (int s = 0; s < DP / 32; ++s) kr[b * (DP / 32) + s] = load8(at + 32 * s, true);
+                    for (int s = 0; s < DP / 32; ++s)
+                        if (32 * s + 8 * gg < d) kr[b * (DP / 32) + s] = load8(at + 32 * s, true);
                 } else {
 #pragma unroll
-                    for (int s = 0; s < DP / 32; ++s) kr[b * (DP / 32) + s] = 32 * s + 8 * gg < d ? load8(at + 32 * s, a.aligned) : u32x4{0, 0, 0, 0};
+                    for (int s = 0; s < DP / 32; ++s) if (32 * s + 8 * gg < d) kr[b * (DP / 32) + s] = load8(at + 32 * s, false);
                 }
                 if (BIAS) k_mask[b] = key < keys ? mask_word(a, mask, key) : a.mask_kind == 1 ? 0u : 0xff800000u;     // past the end: out
             }

@@ -63,6 +63,8 @@ struct Codes {
             const int s = id / c.hk;
             head = id - s * c.hk;
             table = a.table + (int64_t)s * a.table_cols;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) kr[j] = vr[j] = u32x4{0, 0, 0, 0};     // behind the head dim they stay 0
         }
         // the page of a block, 0 for one that none holds: what is read there counts for nothing, or for NaN
         __device__ __forceinline__ int page(int block) const {
@@ -100,7 +102,7 @@ struct Codes {
                 }
                 const int64_t at = codes_at(__builtin_amdgcn_readlane(pages, block & 63), hk, head, a.page_shift, block, d);
                 const uint32_t in = (token & (kBlock - 1)) * d + 16 * ch;
-                x[j] = 16 * ch < d ? *reinterpret_cast<const u32x4*>(codes + at + in) : u32x4{0, 0, 0, 0};
+                if (16 * ch < d) x[j] = *reinterpret_cast<const u32x4*>(codes + at + in);
             }
         }
         __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, key0); }
@@ -118,7 +120,7 @@ struct Codes {
                 const int8_t* const at = a.k + codes_at(__builtin_amdgcn_readlane(pages, block & 63), hk, head, a.page_shift, block, d);
 #pragma unroll
                 for (int i = 0; i < DP / 64; ++i)
-                    kr[b * (DP / 64) + i] = 64 * i + 16 * gg < d ? *reinterpret_cast<const u32x4*>(at + (uint32_t)(col * d + 64 * i + 16 * gg)) : u32x4{0, 0, 0, 0};
+                    if (64 * i + 16 * gg < d) kr[b * (DP / 64) + i] = *reinterpret_cast<const u32x4*>(at + (uint32_t)(col * d + 64 * i + 16 * gg));
             }
         }
         __device__ __forceinline__ u32x4 fragment(int b, int s) const {
