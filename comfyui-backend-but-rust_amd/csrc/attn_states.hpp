@@ -713,7 +713,7 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
 // first a lane per part, then DP / 64 channels a lane.  Two trips to memory: 3.5 us for a few rows, 13.7 for 4 parts of 32400 rows of 64.
 template <class Src, int DP>
 __global__ __launch_bounds__(256) void join_kernel(const Common a, const typename Src::Args sa, int rows_most) {
-    constexpr int E = DP / 64;
+    constexpr int E = DP / 64;      // channels of a lane
     typedef float fe __attribute__((ext_vector_type(E)));
     const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), problem = id / rows_most, row = id - problem * rows_most;
     if (problem >= a.problems) return;
@@ -761,7 +761,8 @@ struct Plan {
     int rows, row_tiles, splits;
     int64_t bytes;     // workspace
 };
-inline int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+// Kernels are built for these; 192 keeps two waves a SIMD, which 256 cannot (2 x 4096 x 4096 x 16 heads of 160: 444 us against 703 padded to 256).
+inline int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp) {
     Plan p;
     p.rows = tile;
@@ -779,7 +780,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         // part 22.6 in all), and longer where the waves of a CU together ask for more than its share of the copy rate, 20 KB a microsecond,
         // of which CUs with few waves reach less (12 x 32749 keys x 8 heads of 128 codes: 3 parts 183, 5 parts 138, 8 parts, which are one
         // full round, 130, 16 parts 136); a wave beside others on its CU takes a little more; joining 3.
-        const int tile = rows <= 16 || dp == 256 ? 16 : 32, per_cu = dp == 256 ? 1 : tile == 32 || (bytes > 1 && dp == 128) ? 2 : 3;
+        const int tile = rows <= 16 || dp >= 192 ? 16 : 32, per_cu = dp == 256 || (bytes > 1 && dp == 192) ? 1 : tile == 32 || dp == 192 || (bytes > 1 && dp == 128) ? 2 : 3;
         const int64_t slots = cus * per_cu, tiles = (keys + 31) / 32, groups = problems * ((rows + tile - 1) / tile);
         const double full = per_cu * 4 * 32. * d * 2 * bytes / 20e3;
         int best = 1;
@@ -817,9 +818,12 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid * 512 > 0xffffffff || a.problems * rows * 64 > 0xffffffff) return -1;      // threads of a launch
-    if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+    if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : DP == 192 ? (Src::kNormalize ? 2 : 1) : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
-    else if (p.rows == 32) few_kernel<Src, DP, 4, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if constexpr (DP == 192) {
+        if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+        else tiles_kernel<Src, DP, 1, 8, 2, 1, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
+    } else if (p.rows == 32) few_kernel<Src, DP, 4, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 128) {
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 2, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
@@ -838,6 +842,7 @@ template <class Src> inline int launch_dim(const Plan& p, int64_t rows, Common& 
     switch (padded_dim(a.d)) {
         case 64: return launch<Src, 64>(p, rows, a, sa, stream);
         case 128: return launch<Src, 128>(p, rows, a, sa, stream);
+        case 192: return launch<Src, 192>(p, rows, a, sa, stream);
         default: return launch<Src, 256>(p, rows, a, sa, stream);
     }
 }

@@ -51,7 +51,7 @@ template <int DTYPE, bool BIAS> struct Dense {
     // the chunk of 8 channels that step s of the product of few rows takes from lanes 16 gg ..
     static __device__ __forceinline__ int q_chunk(int s, int gg) { return 4 * s + gg; }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int ROW = DP / 8, CH = (TK * ROW + NT - 1) / NT;
+        static constexpr int ROW = DP == 192 ? 32 : DP / 8, CH = (TK * ROW + NT - 1) / NT;      // a power of two threads to a row
         static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
         static_assert(kAll || (CH == 1 && TK <= NT), "some threads are without a piece");
         __device__ __forceinline__ bool mine() const { return kAll || tid < TK * ROW; }
@@ -104,7 +104,7 @@ template <int DTYPE, bool BIAS> struct Dense {
             }
         }
         __device__ __forceinline__ void load_fragments(int key0) {
-            static_assert(NT != 64 || CH == 2 * (DP / 32), "32 keys of a wave");
+            static_assert(NT != 64 || CH >= 2 * (DP / 32), "32 keys of a wave");
             const int col = tid & 15, gg = tid >> 4;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -145,7 +145,7 @@ template <int DTYPE, bool BIAS> struct Dense {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
-                if (mine()) *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, k_mask[j]) ? u32x4{0, 0, 0, 0} : kr[j];
+                if (mine() && i % ROW < DP / 8) *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, k_mask[j]) ? u32x4{0, 0, 0, 0} : kr[j];
             }
             if (BIAS && tid < TK) bias[tid] = row_key < keys ? key_bias(a, row_mask) : -INFINITY;
         }
@@ -153,7 +153,7 @@ template <int DTYPE, bool BIAS> struct Dense {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
-                if (mine()) *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, v_mask[j]) ? u32x4{0, 0, 0, 0} : vr[j];
+                if (mine() && i % ROW < DP / 8) *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, i % ROW)) = BIAS && is_out(a, v_mask[j]) ? u32x4{0, 0, 0, 0} : vr[j];
             }
         }
         __device__ __forceinline__ bool any_key(int from, int to) const {

@@ -46,7 +46,7 @@ struct Codes {
     // the chunk of 8 channels that step s of the product of few rows takes from lanes 16 gg ..: half of the 16 codes of a load
     static __device__ __forceinline__ int q_chunk(int s, int gg) { return 8 * (s >> 1) + 2 * gg + (s & 1); }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int ROW = DP / 16, CH = (TK * ROW + NT - 1) / NT;
+        static constexpr int ROW = DP == 192 ? 16 : DP / 16, CH = (TK * ROW + NT - 1) / NT;      // a power of two threads to a row
         static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
         static_assert(kAll || (CH == 1 && TK * ROW % 64 == 0), "whole waves are without a piece");
         __device__ __forceinline__ bool mine() const { return kAll || tid < TK * ROW; }
@@ -108,7 +108,7 @@ struct Codes {
         __device__ __forceinline__ void load_k(int key0) { rows(kr, a.k, key0); }
         __device__ __forceinline__ void load_v(int key0) { rows(vr, a.v, key0); }
         __device__ __forceinline__ void load_fragments(int key0) {
-            static_assert(NT != 64 || CH == 2 * (DP / 64), "32 keys of a wave");
+            static_assert(NT != 64 || CH >= 2 * (DP / 64), "32 keys of a wave");
             const int col = tid & 15, gg = tid >> 4;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -133,6 +133,7 @@ struct Codes {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
+                if (i % ROW >= DP / 16) continue;
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     *reinterpret_cast<u32x4*>(kb + k_place<DP>(i / ROW, 2 * (i % ROW) + e)) = bytes_to_f16(kr[j][2 * e], kr[j][2 * e + 1]);
@@ -143,6 +144,7 @@ struct Codes {
 #pragma unroll
             for (int j = 0; j < CH; ++j) {
                 const int i = tid + j * NT;
+                if (i % ROW >= DP / 16) continue;
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                     *reinterpret_cast<u32x4*>(vb + v_place<DP>(i / ROW, 2 * (i % ROW) + e)) = bytes_to_f16(vr[j][2 * e], vr[j][2 * e + 1]);
