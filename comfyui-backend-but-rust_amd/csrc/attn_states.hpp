@@ -63,9 +63,9 @@ __device__ __forceinline__ constexpr int key_of(int i, int g) { return (i & 3) +
 
 // A staged tile's rows of DP 16-bit elements, and byte positions in it.  K rows are read 16 bytes a lane, 16 rows at a time: 16 bytes behind
 // each row spread one chunk of 16 rows over all banks.  V rows are read by the transposing read, 64 bytes of four rows at a time: 64 bytes
-// behind each row.  (An XOR of the chunk does the same without the room, but costs an instruction a read where a constant offset is free.)
+// behind each row, 128 where 64 would end on the first bank again.  (An XOR of the chunk does the same without the room, but costs an instruction a read where a constant offset is free.)
 template <int DP> constexpr int kRowK = 2 * DP + 16;
-template <int DP> constexpr int kRowV = 2 * DP + 64;
+template <int DP> constexpr int kRowV = DP == 96 ? 320 : 2 * DP + 64;
 template <int DP> __device__ __forceinline__ int k_place(int row, int chunk) { return row * kRowK<DP> + 16 * chunk; }
 template <int DP> __device__ __forceinline__ int v_place(int row, int chunk) { return row * kRowV<DP> + 16 * chunk; }
 
@@ -713,7 +713,7 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
 // first a lane per part, then DP / 64 channels a lane.  Two trips to memory: 3.5 us for a few rows, 13.7 for 4 parts of 32400 rows of 64.
 template <class Src, int DP>
 __global__ __launch_bounds__(256) void join_kernel(const Common a, const typename Src::Args sa, int rows_most) {
-    constexpr int E = DP / 64;      // channels of a lane
+    constexpr int E = (DP + 63) / 64;      // channels of a lane
     typedef float fe __attribute__((ext_vector_type(E)));
     const int lane = threadIdx.x & 63, id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), problem = id / rows_most, row = id - problem * rows_most;
     if (problem >= a.problems) return;
@@ -727,7 +727,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Common a, const typenam
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             x[j] = fe{};
-            if (i + j < a.splits)
+            if (i + j < a.splits && (DP % 64 == 0 || E * lane < DP))
 #pragma unroll
                 for (int e = 0; e < E; ++e) x[j][e] = p[(i + j) * step + E * lane + e];
         }
@@ -761,8 +761,9 @@ struct Plan {
     int rows, row_tiles, splits;
     int64_t bytes;     // workspace
 };
-// Kernels are built for these; 192 keeps two waves a SIMD, which 256 cannot (2 x 4096 x 4096 x 16 heads of 160: 444 us against 703 padded to 256).
-inline int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
+// Kernels are built for these.  192 keeps two waves a SIMD, which 256 cannot (2 x 4096 x 4096 x 16 heads of 160: 444 us against 703); 96 three
+// with tiles of 128 rows (2 x 4096 x 77 x 10 heads of 80: 13.7 us against 19.2 padded to 128; 2 x 4096 x 4096 x 8: 113 against 125).
+inline int padded_dim(int d, int64_t rows) { return d <= 64 ? 64 : d <= 96 && rows > 32 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp) {
     Plan p;
     p.rows = tile;
@@ -773,7 +774,7 @@ inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp
 }
 // bytes: of a key's or value's element.
 inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int bytes) {
-    const int dp = padded_dim(d);
+    const int dp = padded_dim(d, rows);
     const int64_t cus = device_cu_count();
     if (rows <= 32) {
         // In microseconds: a workgroup starts and ends in 4; 32 keys of a wave take 1.65 at least (1 x 1369 keys x 64 heads of 72 channels in one
@@ -801,7 +802,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
     Plan best{};
     double least = 0.;
     for (int tile = 128; tile <= (dp == 256 || rows <= 128 ? 128 : 256); tile *= 2) {
-        const int64_t slots = cus * (dp == 256 ? 1 : dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 ? 2 : 1), groups = (rows + tile - 1) / tile * problems;
+        const int64_t slots = cus * (dp == 256 ? 1 : dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 ? (dp == 96 ? 3 : 2) : 1), groups = (rows + tile - 1) / tile * problems;
         const double start = tile == 128 ? 7. : 10., each = tile == 128 ? 2.6 : 2.4;
         for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 512); ++s) {
             const int64_t rounds = (groups * s + slots - 1) / slots, tiles = (keys + 63) / 64;
@@ -818,7 +819,10 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid * 512 > 0xffffffff || a.problems * rows * 64 > 0xffffffff) return -1;      // threads of a launch
-    if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : DP == 192 ? (Src::kNormalize ? 2 : 1) : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
+    if constexpr (DP == 96) {
+        if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 3><<<(int)grid, 256, 0, stream>>>(a, sa);
+        else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
+    } else if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : DP == 192 ? (Src::kNormalize ? 2 : 1) : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
     else if constexpr (DP == 192) {
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
@@ -839,8 +843,9 @@ template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Comm
     return 0;
 }
 template <class Src> inline int launch_dim(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
-    switch (padded_dim(a.d)) {
+    switch (padded_dim(a.d, rows)) {
         case 64: return launch<Src, 64>(p, rows, a, sa, stream);
+        case 96: return launch<Src, 96>(p, rows, a, sa, stream);
         case 128: return launch<Src, 128>(p, rows, a, sa, stream);
         case 192: return launch<Src, 192>(p, rows, a, sa, stream);
         default: return launch<Src, 256>(p, rows, a, sa, stream);

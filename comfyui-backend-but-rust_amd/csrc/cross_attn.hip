@@ -51,7 +51,7 @@ template <int DTYPE, bool BIAS> struct Dense {
     // the chunk of 8 channels that step s of the product of few rows takes from lanes 16 gg ..
     static __device__ __forceinline__ int q_chunk(int s, int gg) { return 4 * s + gg; }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int ROW = DP == 192 ? 32 : DP / 8, CH = (TK * ROW + NT - 1) / NT;      // a power of two threads to a row
+        static constexpr int ROW = DP == 192 ? 32 : DP == 96 ? 16 : DP / 8, CH = (TK * ROW + NT - 1) / NT;      // a power of two threads to a row
         static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
         static_assert(kAll || (CH == 1 && TK <= NT), "some threads are without a piece");
         __device__ __forceinline__ bool mine() const { return kAll || tid < TK * ROW; }

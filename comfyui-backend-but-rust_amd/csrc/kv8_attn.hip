@@ -46,7 +46,7 @@ struct Codes {
     // the chunk of 8 channels that step s of the product of few rows takes from lanes 16 gg ..: half of the 16 codes of a load
     static __device__ __forceinline__ int q_chunk(int s, int gg) { return 8 * (s >> 1) + 2 * gg + (s & 1); }
     template <int DP, int TK, int NT> struct Stage {
-        static constexpr int ROW = DP == 192 ? 16 : DP / 16, CH = (TK * ROW + NT - 1) / NT;      // a power of two threads to a row
+        static constexpr int ROW = DP == 192 ? 16 : DP == 96 ? 8 : DP / 16, CH = (TK * ROW + NT - 1) / NT;      // a power of two threads to a row
         static constexpr bool kAll = TK * ROW % NT == 0;      // every thread has a piece of every load
         static_assert(kAll || (CH == 1 && TK * ROW % 64 == 0), "whole waves are without a piece");
         __device__ __forceinline__ bool mine() const { return kAll || tid < TK * ROW; }
