@@ -92,7 +92,7 @@ struct Common {
     int64_t q_rs, q_hs, o_rs, o_hs;    // element strides of tokens and heads
     int hk, group, d, q_dt;
     int row_tiles, problems, splits;   // grid: row_tiles * problems (batch x hk) * splits
-    int aligned;                       // q rows start on 16 bytes (bit 0), o rows on 8 (bit 1)
+    int aligned;                       // rows start on 16 bytes: q's (bit 0), o's (bit 1)
     float c;                           // |scale| log2 e; 1 where that is 0
     uint32_t q_and, q_xor;             // what q's words take: a negative scale flips their signs, a scale of 0 makes them 0
     float* part;                       // [splits][problems][rows padded to tiles][DP + 2] where splits > 1
@@ -353,10 +353,10 @@ __device__ __forceinline__ void share_of(int end, int tk, int splits, int split,
 // before goes into LDS and the one before that is multiplied, SB blocks of 32 keys per step of the softmax.
 //
 // 4 * d operations a pair on the matrix pipes, one exponential a pair beside them.  2 x 1024 new tokens of 32 heads behind 7168 stored ones
-// (223 GFLOP) take 274 us, 0.81 PFLOP/s where an 8192-cubed product of the vendor's library reaches 1.23; matrix pipes 41 % and vector
+// (223 GFLOP) take 272 us, 0.82 PFLOP/s where an 8192-cubed product of the vendor's library reaches 1.23; matrix pipes 41 % and vector
 // pipes 54 % busy at 1.7 GHz under the power limit, and the two hardly overlap: a probe shows a product of another wave keeping vector
 // instructions from issue for 11 of its 32 cycles (v_dot2 for all of them).  Head dim 64 (frame of 2025 tokens to 16200, f16, 16 heads):
-// vector pipes 75 % busy, 199 us.
+// vector pipes 75 % busy, 193 us.
 // Eight waves on a tile spend half the instructions on staging, conversion to f16 above all, that four do (289 us against 325), but few rows
 // do not fill them; 64 keys per softmax step with one branch 285 against 289; sums of rounded pairs (v_dot2) against additions 270 and
 // 284.  Not kept: scores of the next keys between the exponentials, left to the compiler (292) or held there by sched_barrier (310); two
@@ -450,17 +450,23 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                const int at = 32 * i + key_of(j, g);
-                if (at >= a.d) continue;
-                float v[4];
+            for (int j = 0; j < 16; j += 8) {
+                if (32 * i + 2 * j >= a.d) continue;
+                uint32_t u[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = L.acc[w][i][j + e] * inv;
-                const u32x2 u = a.q_dt == DT_BF16 ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])} : u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
-                if (a.aligned & 2) *reinterpret_cast<u32x2*>(op + at) = u;
+                for (int e = 0; e < 4; ++e) {
+                    const float x = L.acc[w][i][j + 2 * e] * inv, y = L.acc[w][i][j + 2 * e + 1] * inv;
+                    u[e] = a.q_dt == DT_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                }
+                // of 16 channels a half wave has 0 .. 3 and 8 .. 11, or the others: each takes half from the other and has 8 in a row
+                const auto s0 = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
+                const u32x4 eight = {s0[0], s1[0], s0[1], s1[1]};
+                const int at = 32 * i + 2 * j + 8 * g;
+                if (at >= a.d) continue;
+                if (a.aligned & 2) *reinterpret_cast<u32x4*>(op + at) = eight;
                 else
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) op[at + e] = (uint16_t)(u[e >> 1] >> 16 * (e & 1));
+                    for (int e = 0; e < 8; ++e) op[at + e] = (uint16_t)(eight[e >> 1] >> 16 * (e & 1));
             }
     }
 }
@@ -469,7 +475,7 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
 // results meet.  What counts is the keys' way in: K goes from memory straight into the fragments of v_mfma_f32_16x16x32 (lane: key
 // lane % 16, channels in the order of Source::q_chunk), V through the wave's own piece of LDS, where it is turned.  Lanes hold row lane % 16 and
 // keys 4 (lane / 16) .. + 3 of each 16, which is, in order, what the product with V takes, if that counts its keys so.
-// 12 tokens to 16 to 32 thousand keys of 8 heads of 128 codes each: 131 us with the joining, 4.7 TB/s, where a copy reaches 5.2; in the 32 x 32 x 16
+// 12 tokens to 16 to 32 thousand keys of 8 heads of 128 codes each: 130 us with the joining, 4.8 TB/s, where a copy reaches 5.2; in the 32 x 32 x 16
 // form with K through LDS, twice the registers and half the waves, 203.  One token to 613 keys: 10 us, of which 3.5 are the second launch.
 template <int DT> __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     if constexpr (DT == DT_BF16)

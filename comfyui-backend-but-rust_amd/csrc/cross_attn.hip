@@ -190,7 +190,7 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
     c.q = q; c.o = o; c.q_rs = q_rs; c.q_hs = q_hs; c.o_rs = o_rs; c.o_hs = o_hs;
     c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
     c.row_tiles = p.row_tiles; c.problems = b * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
-    c.aligned = (sixteen(q, q_bs, q_rs, q_hs) ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_bs | o_rs | o_hs) % 4 == 0 ? 2 : 0);
+    c.aligned = (sixteen(q, q_bs, q_rs, q_hs) ? 1 : 0) | (sixteen(o, o_bs, o_rs, o_hs) ? 2 : 0);
     // with a bias, which is counted in units of the score, scales from which it would leave fp32 are none
     set_scale(c, scale, mask_kind == 2 ? 1e-30f : 1.17549435e-38f);
     c.part = (float*)ws;

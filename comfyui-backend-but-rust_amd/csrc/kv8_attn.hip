@@ -191,7 +191,7 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     c.q = q; c.o = o; c.q_rs = q_rs; c.q_hs = q_hs; c.o_rs = o_rs; c.o_hs = o_hs;
     c.hk = hk; c.group = h / hk; c.d = head_dim; c.q_dt = dtype;
     c.row_tiles = p.row_tiles; c.problems = n * hk; c.splits = p.splits; c.rows_padded = p.row_tiles * p.rows;
-    c.aligned = ((uintptr_t)q % 16 == 0 && (q_rs | q_hs) % 8 == 0 ? 1 : 0) | ((uintptr_t)o % 8 == 0 && (o_rs | o_hs) % 4 == 0 ? 2 : 0);
+    c.aligned = ((uintptr_t)q % 16 == 0 && (q_rs | q_hs) % 8 == 0 ? 1 : 0) | ((uintptr_t)o % 16 == 0 && (o_rs | o_hs) % 8 == 0 ? 2 : 0);
     set_scale(c, scale, 1.17549435e-38f);
     c.part = (float*)ws;
     CacheArgs s{k, v, k_scale, v_scale, starts, lens, table, rows, most, n_pages, __builtin_ctz(page), table_cols, causal != 0};
