@@ -314,7 +314,7 @@ int64_t gpu_w6a8_group_gemm_scratch(const void* Wp, int64_t M, int64_t N, int64_
 /* Cross attention to an encoder's states, 16-bit throughout: o = softmax(scale * q k^T + bias) v per head, where batch item i attends
  * to the keys j < k_lens[i] that its mask leaves.  dtype DT_F16 or DT_BF16 (others -4) for q [b, lq, h, d], k, v [b, lk, hk, d] and o
  * [b, lq, h, d]; element strides per batch item, token and head (bs, rs, hs), the last axis dense; query head j uses key-value head
- * j / (h / hk).  head_dim a multiple of 8 up to 256.  Rows that start on 16 bytes (o: 8) take wide loads, others work too.
+ * j / (h / hk).  head_dim a multiple of 8 up to 256.  Rows that start on 16 bytes take wide loads and stores, others work too.
  * k_lens: int32 [b] on the device or null (all lk); values outside 0..lk count as the nearer end.  mask: null (mask_kind 0), bytes [b, lk], 0 = the
  * key is out (1), or f32 [b, lk] added to the logits, -inf = out (2); rows mask_bs elements apart (0: one row for all), 32-bit elements on 4 bytes.
  * A key that is out counts as absent whatever k and v hold there; a row without keys gives zeros.  With f32 masks a |scale| below
