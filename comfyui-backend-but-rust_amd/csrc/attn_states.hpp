@@ -767,7 +767,8 @@ struct Plan {
     int rows, row_tiles, splits;
     int64_t bytes;     // workspace
 };
-// Kernels are built for these.  192 keeps two waves a SIMD, which 256 cannot (2 x 4096 x 4096 x 16 heads of 160: 444 us against 703); 96 three
+// Kernels are built for these.  192 and 256 rows of 256 keep two waves a SIMD, 128 rows
+// of 256 cannot (2 x 4096 x 4096 x 16 heads of 160: 444 us against 703 in those, 8 of 256: 278 against 366); 96 keeps three
 // with tiles of 128 rows (2 x 4096 x 77 x 10 heads of 80: 13.7 us against 19.2 padded to 128; 2 x 4096 x 4096 x 8: 113 against 125).
 inline int padded_dim(int d, int64_t rows) { return d <= 64 ? 64 : d <= 96 && rows > 32 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp) {
@@ -804,12 +805,13 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         }
         return plan_of(tile, best, rows, problems, dp);
     }
-    // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts
+    // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts; head dims above 192 measured by
+    // themselves (4 x 638 x 6, 72 heads of 256: tiles of 128 rows 84, of 256 62; 1 x 962 x 773 x 20: 64 and 75)
     Plan best{};
     double least = 0.;
-    for (int tile = 128; tile <= (dp == 256 || rows <= 128 ? 128 : 256); tile *= 2) {
-        const int64_t slots = cus * (dp == 256 ? 1 : dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 ? (dp == 96 ? 3 : 2) : 1), groups = (rows + tile - 1) / tile * problems;
-        const double start = tile == 128 ? 7. : 10., each = tile == 128 ? 2.6 : 2.4;
+    for (int tile = 128; tile <= (rows <= 128 ? 128 : 256); tile *= 2) {
+        const int64_t slots = cus * (dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 && dp < 256 ? (dp == 96 ? 3 : 2) : 1), groups = (rows + tile - 1) / tile * problems;
+        const double start = (tile == 128 ? 7. : 10.) + (dp == 256 ? 6. : 0.), each = dp == 256 ? (tile == 128 ? 2.7 : 4.2) : tile == 128 ? 2.6 : 2.4;
         for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 512); ++s) {
             const int64_t rounds = (groups * s + slots - 1) / slots, tiles = (keys + 63) / 64;
             const double us = rounds * (start + each * ((tiles + s - 1) / s)) + (s == 1 ? 0. : 5. + 1e-6 * 4. * (dp + 2) * rows * problems * (2 * s) / 4.);
@@ -829,7 +831,10 @@ template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Comm
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 3><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
     } else if (p.rows == 16) few_kernel<Src, DP, 4, 1, DP == 256 ? 1 : DP == 192 ? (Src::kNormalize ? 2 : 1) : Src::kNormalize || DP == 64 ? 3 : 2><<<(int)grid, 256, 0, stream>>>(a, sa);
-    else if constexpr (DP == 256) tiles_kernel<Src, DP, 1, 4, 2, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
+    else if constexpr (DP == 256) {
+        if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, Src::kNormalize ? 2 : 1, 1, 1><<<(int)grid, 256, 0, stream>>>(a, sa);
+        else tiles_kernel<Src, DP, 1, 8, 1, 1, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
+    }
     else if constexpr (DP == 192) {
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 1, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
