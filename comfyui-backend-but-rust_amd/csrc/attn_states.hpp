@@ -765,6 +765,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Common a, const typenam
 // row go.
 struct Plan {
     int rows, row_tiles, splits;
+    int blocks = 1;    // of 32 keys that a tile of 128 rows of head dims to 64 takes at a time
     int64_t bytes;     // workspace
 };
 // Kernels are built for these.  192 and 256 rows of 256 keep two waves a SIMD, 128 rows
@@ -818,6 +819,9 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
             if (best.rows == 0 || us < least) {
                 least = us;
                 best = plan_of(tile, s, rows, problems, dp);
+                // Two where no CU has more than one: 16 x 2048 rows, 512 keys 15.6 us against 18.5; with four on a CU the smaller tile's
+                // are ahead, 120 x 8 heads of 120 rows and 1024 keys 66 against 70.
+                best.blocks = groups * s <= cus && keys > 64 ? 2 : 1;
             }
         }
     }
@@ -843,7 +847,8 @@ template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Comm
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 2, 2, 2><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);
     } else {
-        if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 4><<<(int)grid, 256, 0, stream>>>(a, sa);
+        if (p.rows == 128 && p.blocks == 1) tiles_kernel<Src, DP, 1, 4, 1, 1, 4><<<(int)grid, 256, 0, stream>>>(a, sa);
+        else if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 2, 2, 3><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 1, 4><<<(int)grid, 512, 0, stream>>>(a, sa);
     }
     KCHECK();

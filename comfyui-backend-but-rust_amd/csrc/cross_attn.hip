@@ -213,5 +213,6 @@ GPU_API int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t key
     const Plan p = make_plan(rows, problems, keys, head_dim, bytes);
     out[0] = p.rows;
     out[1] = p.splits;
+    out[2] = padded_dim(head_dim, rows) == 64 && p.rows == 128 ? p.blocks : 0;
     return 0;
 }

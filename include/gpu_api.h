@@ -365,7 +365,8 @@ int gpu_kv8_copy_pages(int8_t* ck, int8_t* cv, float* k_scale, float* v_scale, i
 
 /* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times
  * key-value heads) of `rows` (query tokens times query heads of a key-value head, the most of any) over `keys`: out[0] = rows of a workgroup (16 and 32:
- * its waves share them, 128 and 256: a wave has 32), out[1] = workgroups that share a row's keys. */
+ * its waves share them, 128 and 256: a wave has 32), out[1] = workgroups that share a row's keys,
+ * out[2] = blocks of 32 keys at a time where there is a choice (128 rows, head dims to 64; else 0). */
 int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t keys, int head_dim, int bytes, int32_t* out);
 
 /* Test and tuning hook: force the GEMM kernel family.  1, 2 = 128x128 and 64x64 register-staged tiles; 5 = weights straight

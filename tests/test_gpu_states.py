@@ -90,7 +90,7 @@ CROSS = [(1, 1, 1, 1, 1, 8), (2, 1, 300, 4, 4, 64), (1, 3, 77, 6, 2, 128), (2, 3
          (1, 24, 3000, 1, 1, 64), (2, 20, 60, 1, 1, 128), (1, 24, 3000, 1, 1, 96), (1, 130, 3000, 1, 1, 128), (1, 200, 1010, 2, 2, 64), (1, 257, 1000, 1, 1, 128),
          (1, 150, 20000, 1, 1, 64), (1, 150, 20000, 1, 1, 128),
          (1, 60, 65, 1, 1, 96), (1, 70, 3000, 1, 1, 72), (2, 257, 1000, 1, 1, 88), (1, 150, 20000, 1, 1, 80), (1, 20, 60, 1, 1, 72), (1, 9, 60, 1, 1, 192), (1, 5, 3000, 2, 2, 136), (1, 60, 70, 2, 2, 168), (1, 60, 3000, 1, 1, 256), (1, 257, 1000, 1, 1, 144), (1, 150, 20000, 1, 1, 176),
-         (1, 300, 70, 86, 86, 248), (1, 130, 2050, 65, 65, 240)]
+         (1, 300, 70, 86, 86, 248), (1, 130, 2050, 65, 65, 240), (1, 33, 200, 260, 260, 16)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
@@ -395,7 +395,8 @@ ATTN = [([1], [1], 1, 1, 16, 16), ([1, 1, 1], [5, 700, 64], 4, 2, 128, 64), ([3,
         ([20], [50], 1, 1, 128, 16), ([20], [3000], 1, 1, 112, 16), ([1, 1], [60, 9], 2, 1, 128, 16), ([1], [40], 1, 1, 256, 16), ([40], [60], 1, 1, 240, 16),
         ([200, 9], [1008, 1], 1, 1, 64, 16), ([300], [1000], 1, 1, 128, 16), ([150], [20000], 1, 1, 64, 64), ([75], [20000], 2, 1, 128, 64),
         ([60, 3], [65, 9], 1, 1, 96, 16), ([70], [3000], 1, 1, 80, 32), ([257], [1000], 2, 2, 96, 16), ([150], [20000], 1, 1, 80, 64), ([9], [60], 1, 1, 192, 16), ([5], [3000], 2, 2, 144, 32), ([60, 2], [70, 33], 2, 2, 160, 16), ([60], [3000], 1, 1, 176, 16), ([257], [1000], 1, 1, 192, 16),
-        ([150], [20000], 1, 1, 176, 64), ([300], [320], 86, 86, 240, 16), ([130], [2048], 65, 65, 256, 64)]
+        ([150], [20000], 1, 1, 176, 64), ([300], [320], 86, 86, 240, 16), ([130], [2048], 65, 65, 256, 64),
+        ([33], [208], 260, 260, 16, 16)]
 
 
 def test_the_cases_reach_every_form():
@@ -403,18 +404,21 @@ def test_the_cases_reach_every_form():
     and not."""
     import ctypes
     ffi = pkg("ffi")
-    out, dp = (ctypes.c_int32 * 2)(), lambda d, rows: 96 if 64 < d <= 96 and rows > 32 else -(-d // 64) * 64
+    out, dp = (ctypes.c_int32 * 3)(), lambda d, rows: 96 if 64 < d <= 96 and rows > 32 else -(-d // 64) * 64
     want = {(p, r, s) for p in (64, 96, 128, 192, 256) for r in (16, 32, 128, 256) for s in (False, True) if (p != 96 or r > 32) and (p < 192 or r != 32)}
-    seen = {1: set(), 2: set()}
+    seen, blocks = {1: set(), 2: set()}, {(by, n) for by in (1, 2) for n in (1, 2)}
     for b, lq, lk, h, hk, d in CROSS:
         ffi.k("gpu_internal_states_plan", lq * (h // hk), b * hk, lk, d, 2, ctypes.cast(out, ctypes.c_void_p))
+        blocks.discard((2, out[2]) if lk > 64 else None)
         seen[2].add((dp(d, lq * (h // hk)), out[0], out[1] > 1))
     for new, lens, h, heads, dim, page in ATTN:
         cols = max(-(-l // page) for l in lens)
         ffi.k("gpu_internal_states_plan", max(new) * (h // heads), len(lens) * heads, cols * page, dim, 1, ctypes.cast(out, ctypes.c_void_p))
+        blocks.discard((1, out[2]) if max(lens) > 64 else None)
         seen[1].add((dp(dim, max(new) * (h // heads)), out[0], out[1] > 1))
     assert seen[2] >= want, sorted(want - seen[2])
     assert seen[1] >= want, sorted(want - seen[1])
+    assert not blocks, blocks
 
 
 @pytest.mark.parametrize("causal", [True, False], ids=["causal", "all"])
