@@ -806,15 +806,22 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         }
         return plan_of(tile, best, rows, problems, dp);
     }
-    // microseconds: a workgroup's start and end, its tile of 64 keys with the CU full, and the joining of parts; head dims above 192 measured by
-    // themselves (4 x 638 x 6, 72 heads of 256: tiles of 128 rows 84, of 256 62; 1 x 962 x 773 x 20: 64 and 75)
+    // In microseconds: a workgroup's start and end; 64 keys of it alone on its CU (4 x 150 x 584, 6 heads of 128: 20 in all; 2 x 512 x 800, 8 heads: 24)
+    // or among as many as fit; and the joining of parts, which at 128 keys a part still pays where most CUs would idle (100 new tokens of 8 heads behind
+    // 800: 16 us in parts, 31 in one; 4 x 83 x 524, 20 heads of 168: 28 and 45).
     Plan best{};
     double least = 0.;
     for (int tile = 128; tile <= (rows <= 128 ? 128 : 256); tile *= 2) {
-        const int64_t slots = cus * (dp == 64 ? (tile == 128 ? 4 : 2) : tile == 128 && dp < 256 ? (dp == 96 ? 3 : 2) : 1), groups = (rows + tile - 1) / tile * problems;
-        const double start = (tile == 128 ? 7. : 10.) + (dp == 256 ? 6. : 0.), each = dp == 256 ? (tile == 128 ? 2.7 : 4.2) : tile == 128 ? 2.6 : 2.4;
-        for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 512); ++s) {
-            const int64_t rounds = (groups * s + slots - 1) / slots, tiles = (keys + 63) / 64;
+        const bool small = tile == 128;
+        const int fit = small ? (dp == 64 ? 4 : dp == 96 ? 3 : dp == 256 ? 1 : 2) : dp == 64 ? 2 : 1;
+        const int64_t slots = cus * fit, groups = (rows + tile - 1) / tile * problems, tiles = (keys + 63) / 64;
+        const double start = (small ? 7. : 13.) + (dp == 256 ? 6. : 0.);
+        // (of head dims to 64, where a CU has one, with 64 keys at a time)
+        const double alone = dp == 256 ? (small ? 3.7 : 4.2) : dp == 192 ? (small ? 4.2 : 3.3) : !small ? (dp == 64 ? 1.55 : dp == 96 ? 1.6 : bytes > 1 ? 1.9 : 2.2) : dp == 64 ? 1.7 : dp == 96 ? 2.1 : bytes > 1 ? 1.3 : 1.75;
+        const double full = dp >= 192 || (dp > 64 && !small) ? alone : small ? 2.6 : 2.4;
+        for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 128); ++s) {
+            const int64_t rounds = (groups * s + slots - 1) / slots, on_one = rounds > 1 ? fit : (groups * s + cus - 1) / cus;
+            const double share = full * on_one / fit, each = dp == 64 && small && on_one == 1 ? 1.2 : share > alone ? share : alone;
             const double us = rounds * (start + each * ((tiles + s - 1) / s)) + (s == 1 ? 0. : 5. + 1e-6 * 4. * (dp + 2) * rows * problems * (2 * s) / 4.);
             if (best.rows == 0 || us < least) {
                 least = us;

@@ -90,7 +90,9 @@ CROSS = [(1, 1, 1, 1, 1, 8), (2, 1, 300, 4, 4, 64), (1, 3, 77, 6, 2, 128), (2, 3
          (1, 24, 3000, 1, 1, 64), (2, 20, 60, 1, 1, 128), (1, 24, 3000, 1, 1, 96), (1, 130, 3000, 1, 1, 128), (1, 200, 1010, 2, 2, 64), (1, 257, 1000, 1, 1, 128),
          (1, 150, 20000, 1, 1, 64), (1, 150, 20000, 1, 1, 128),
          (1, 60, 65, 1, 1, 96), (1, 70, 3000, 1, 1, 72), (2, 257, 1000, 1, 1, 88), (1, 150, 20000, 1, 1, 80), (1, 20, 60, 1, 1, 72), (1, 9, 60, 1, 1, 192), (1, 5, 3000, 2, 2, 136), (1, 60, 70, 2, 2, 168), (1, 60, 3000, 1, 1, 256), (1, 257, 1000, 1, 1, 144), (1, 150, 20000, 1, 1, 176),
-         (1, 300, 70, 86, 86, 248), (1, 130, 2050, 65, 65, 240), (1, 33, 200, 260, 260, 16)]
+         (1, 300, 70, 86, 86, 248), (1, 130, 2050, 65, 65, 240), (1, 33, 200, 260, 260, 16),
+         (1, 1030, 2050, 86, 86, 64), (1, 130, 20000, 65, 65, 48), (1, 8200, 1030, 3, 3, 96), (1, 130, 4100, 86, 86, 128), (1, 130, 1030, 129, 129, 112),
+         (1, 8200, 600, 3, 3, 192), (1, 130, 70, 1, 1, 256)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
@@ -396,7 +398,8 @@ ATTN = [([1], [1], 1, 1, 16, 16), ([1, 1, 1], [5, 700, 64], 4, 2, 128, 64), ([3,
         ([200, 9], [1008, 1], 1, 1, 64, 16), ([300], [1000], 1, 1, 128, 16), ([150], [20000], 1, 1, 64, 64), ([75], [20000], 2, 1, 128, 64),
         ([60, 3], [65, 9], 1, 1, 96, 16), ([70], [3000], 1, 1, 80, 32), ([257], [1000], 2, 2, 96, 16), ([150], [20000], 1, 1, 80, 64), ([9], [60], 1, 1, 192, 16), ([5], [3000], 2, 2, 144, 32), ([60, 2], [70, 33], 2, 2, 160, 16), ([60], [3000], 1, 1, 176, 16), ([257], [1000], 1, 1, 192, 16),
         ([150], [20000], 1, 1, 176, 64), ([300], [320], 86, 86, 240, 16), ([130], [2048], 65, 65, 256, 64),
-        ([33], [208], 260, 260, 16, 16)]
+        ([33], [208], 260, 260, 16, 16), ([40, 7], [120, 60], 1, 1, 128, 16), ([1030], [2050], 86, 86, 64, 64), ([130], [20000], 65, 65, 48, 64), ([130], [1030], 192, 3, 96, 64),
+        ([130], [2050], 86, 86, 128, 64), ([130], [1030], 129, 129, 112, 16), ([130], [600], 192, 3, 192, 32), ([130], [130], 1, 1, 256, 16)]
 
 
 def test_the_cases_reach_every_form():

@@ -82,7 +82,8 @@ def _plan(rows, problems, keys, d, bytes):
     ((4096, 16, 8192, 128, 1), (256, 1)),       # 284 against 324; in two parts 336
     ((2025, 16, 16256, 64, 1), (256, 4)),       # 200 against 218 in two parts, 357 in one
     ((4, 96, 32752, 128, 1), (16, 8)),          # one full round: 130 against 138 and 154 in 5 and 6 parts
-    ((1, 64, 1369, 72, 2), (16, 6)), ((20, 8, 4096, 128, 1), (32, 32)), ((33, 1, 64, 256, 2), (128, 1)), ((1, 1, 0, 8, 2), (16, 1)), ((1, 2000, 100000, 128, 1), (16, 8)), ((200, 1, 1010, 128, 2), (256, 1)), ((128, 1, 1010, 128, 2), (128, 1))])
+    ((1, 64, 1369, 72, 2), (16, 6)), ((20, 8, 4096, 128, 1), (32, 32)), ((33, 1, 64, 256, 2), (128, 1)), ((1, 1, 0, 8, 2), (16, 1)), ((1, 2000, 100000, 128, 1), (16, 8)), ((200, 1, 1010, 128, 2), (128, 6)), ((96, 24, 4608, 128, 2), (128, 9)),
+    ((1024, 16, 1000, 192, 2), (128, 4)), ((83, 80, 524, 168, 2), (128, 3)), ((962, 20, 773, 256, 2), (128, 1)), ((2004, 132, 225, 256, 2), (256, 1)), ((4096, 16, 1024, 72, 2), (256, 1))])
 def test_attention_forms_where_they_were_measured(case, plan):
     """For 256 CUs, which is what a host without a device is taken for."""
     assert _plan(*case) == plan
