@@ -835,6 +835,9 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
     return best;
 }
 
+// Waves a SIMD (the last argument) are what the registers of a form allow without spilling more than a few; blocks of 32 keys a tile follow: one where
+// two would cost a workgroup its place (head dims to 64 and 96 with 128 rows: 4 and 3 on a CU; 192), two elsewhere.  At 256 with 128 rows, one wave a SIMD
+// either way: 16-bit keys one at a time (4 x 638 x 6, 72 heads: 84 us against 98 with two), codes two (the last 1024 of 2 x 4096 tokens, 16 over 4 heads: 234 against 246).
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid * 512 > 0xffffffff || a.problems * rows * 64 > 0xffffffff) return -1;      // threads of a launch
