@@ -835,7 +835,8 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
     return best;
 }
 
-// Waves a SIMD (the last argument) are what the registers of a form allow without spilling more than a few; blocks of 32 keys a tile follow: one where
+// Waves a SIMD (the last argument) are what the registers of a form allow, spilling a few at most (codes at 256 with 256 rows 66, and
+// ahead all the same: 2025 rows of 8 heads of 240 to 8100, 200 us against 248 with 128 rows); blocks of 32 keys a tile follow: one where
 // two would cost a workgroup its place (head dims to 64 and 96 with 128 rows: 4 and 3 on a CU; 192), two elsewhere.  At 256 with 128 rows, one wave a SIMD
 // either way: 16-bit keys one at a time (4 x 638 x 6, 72 heads: 84 us against 98 with two), codes two (the last 1024 of 2 x 4096 tokens, 16 over 4 heads: 234 against 246).
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
