@@ -780,10 +780,13 @@ inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp
     p.bytes = splits > 1 ? 4 * splits * problems * p.row_tiles * tile * (dp + 2) : 0;
     return p;
 }
+// A launch has fewer than 2^32 threads: workgroups of 512 at most, and rows that the join can take, four in 256.
+constexpr int64_t kMostGroups = 0xffffffff / 512, kMostJoined = 0xffffffff / 256 * 4;
 // bytes: of a key's or value's element.
 inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int bytes) {
     const int dp = padded_dim(d, rows);
     const int64_t cus = device_cu_count();
+    const auto can = [&](int64_t groups, int s) { return s == 1 || (groups * s <= kMostGroups && rows * problems <= kMostJoined); };
     if (rows <= 32) {
         // In microseconds: a workgroup starts and ends in 4; 32 keys of a wave take 1.65 at least (1 x 1369 keys x 64 heads of 72 channels in one
         // part 22.6 in all), and longer where the waves of a CU together ask for more than its share of the copy rate, 20 KB a microsecond,
@@ -794,7 +797,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         const double full = per_cu * 4 * 32. * d * 2 * bytes / 20e3;
         int best = 1;
         double least = 0.;
-        for (int s = 1; s <= 64 && (s == 1 || s <= tiles); ++s) {
+        for (int s = 1; s <= 64 && (s == 1 || s <= tiles) && can(groups, s); ++s) {
             const int64_t rounds = (groups * s + slots - 1) / slots, each = ((tiles + s - 1) / s + 3) / 4;
             const double busy = groups * s >= slots ? 1. : (double)(groups * s) / slots, shared = full * busy / (0.85 + 0.15 * busy), step = shared > 1.65 ? shared : 1.65;
             const int64_t in_one = (tiles + s - 1) / s;
@@ -815,11 +818,12 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         const bool small = tile == 128;
         const int fit = small ? (dp == 64 ? 4 : dp == 96 ? 3 : dp == 256 ? 1 : 2) : dp == 64 ? 2 : 1;
         const int64_t slots = cus * fit, groups = (rows + tile - 1) / tile * problems, tiles = (keys + 63) / 64;
+        if (small && rows > 128 && groups > kMostGroups) continue;
         const double start = (small ? 7. : 13.) + (dp == 256 ? 6. : 0.);
         // (of head dims to 64, where a CU has one, with 64 keys at a time)
         const double alone = dp == 256 ? (small ? 3.7 : 4.2) : dp == 192 ? (small ? 4.2 : 3.3) : !small ? (dp == 64 ? 1.55 : dp == 96 ? 1.6 : bytes > 1 ? 1.9 : 2.2) : dp == 64 ? 1.7 : dp == 96 ? 2.1 : bytes > 1 ? 1.3 : 1.75;
         const double full = dp >= 192 || (dp > 64 && !small) ? alone : small ? 2.6 : 2.4;
-        for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 128); ++s) {
+        for (int s = 1; s <= 16 && (s == 1 || keys >= (int64_t)s * 128) && can(groups, s); ++s) {
             const int64_t rounds = (groups * s + slots - 1) / slots, on_one = rounds > 1 ? fit : (groups * s + cus - 1) / cus;
             const double share = full * on_one / fit, each = dp == 64 && small && on_one == 1 ? 1.2 : share > alone ? share : alone;
             const double us = rounds * (start + each * ((tiles + s - 1) / s)) + (s == 1 ? 0. : 5. + 1e-6 * 4. * (dp + 2) * rows * problems * (2 * s) / 4.);
@@ -841,7 +845,7 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
 // either way: 16-bit keys one at a time (4 x 638 x 6, 72 heads: 84 us against 98 with two), codes two (the last 1024 of 2 x 4096 tokens, 16 over 4 heads: 234 against 246).
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
-    if (grid * 512 > 0xffffffff || a.problems * rows * 64 > 0xffffffff) return -1;      // threads of a launch
+    if (grid > kMostGroups) return -1;
     if constexpr (DP == 96) {
         if (p.rows == 128) tiles_kernel<Src, DP, 1, 4, 1, 1, 3><<<(int)grid, 256, 0, stream>>>(a, sa);
         else tiles_kernel<Src, DP, 1, 8, 2, 2, 2><<<(int)grid, 512, 0, stream>>>(a, sa);

@@ -211,6 +211,7 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
 GPU_API int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t keys, int head_dim, int bytes, int32_t* out) {
     if (rows <= 0 || problems <= 0 || keys < 0 || head_dim <= 0 || head_dim > 256 || (bytes != 1 && bytes != 2) || !out) return -1;
     const Plan p = make_plan(rows, problems, keys, head_dim, bytes);
+    if (p.row_tiles * problems * p.splits > kMostGroups) return -1;
     out[0] = p.rows;
     out[1] = p.splits;
     out[2] = padded_dim(head_dim, rows) == 64 && p.rows == 128 ? p.blocks : 0;

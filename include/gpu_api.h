@@ -321,7 +321,8 @@ int64_t gpu_w6a8_group_gemm_scratch(const void* Wp, int64_t M, int64_t N, int64_
  * 7e-31 counts as 0.  Scores, probabilities' sums and
  * outputs are held in fp32, the probabilities rounded to the row type for the product with v.
  * ws: gpu_cross_attn_workspace bytes (0: null will do), 16-byte aligned, in use until the work queued here has run.
- * Returns -1 for sizes, a scale that is not finite, or pointers that do not fit this. */
+ * Returns -1 for sizes, a scale that is not finite, or pointers that do not fit this, and for more than 8388607 workgroups: b * hk, times
+ * lq * h / hk in tiles of 256 rows (up to 32 rows: of 16). */
 int64_t gpu_cross_attn_workspace(int b, int lq, int lk, int h, int hk, int head_dim);
 int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void* o, void* ws, int b, int lq, int lk, int h, int hk,
                    int head_dim, int64_t q_bs, int64_t q_rs, int64_t q_hs, int64_t k_bs, int64_t k_rs, int64_t k_hs, int64_t v_bs,
@@ -345,7 +346,8 @@ int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void*
  * gpu_kv8_read gives the rows back in dtype (any): code * A / 127.  Rows on 8 bytes (f32: 16), strides multiples of 4 (-1).
  * gpu_kv8_attn: o = softmax(scale * q k^T) v for the rows of q [rows, h, d] (DT_F16 or DT_BF16); row i of a sequence's m sees the tokens
  *   0 .. lens[s] - m + i (causal) or all lens[s].  A row that sees none gives zeros.  ws: gpu_kv8_attn_workspace bytes (0: null will do),
- *   16-byte aligned, in use until the work queued here has run.
+ *   16-byte aligned, in use until the work queued here has run.  At most 8388607 workgroups (-1): n * hk, times most * h / hk in tiles of
+ *   256 rows (up to 32 rows: of 16).
  * gpu_kv8_copy_pages copies pages src[i] -> dst[i] (int32 on the device, n <= 65535) with their scales in each of `layers` caches that lie
  *   one behind the other in every array.  Numbers that are no page are left out.  No page may be named twice in dst, or in both.
  * All return -4 for a dtype they do not take, -1 for sizes and pointers that do not fit the above (n <= 65535 in store and read). */
@@ -366,7 +368,7 @@ int gpu_kv8_copy_pages(int8_t* ck, int8_t* cv, float* k_scale, float* v_scale, i
 /* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times
  * key-value heads) of `rows` (query tokens times query heads of a key-value head, the most of any) over `keys`: out[0] = rows of a workgroup (16 and 32:
  * its waves share them, 128 and 256: a wave has 32), out[1] = workgroups that share a row's keys,
- * out[2] = blocks of 32 keys at a time where there is a choice (128 rows, head dims to 64; else 0). */
+ * out[2] = blocks of 32 keys at a time where there is a choice (128 rows, head dims to 64; else 0).  -1 for what those refuse. */
 int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t keys, int head_dim, int bytes, int32_t* out);
 
 /* Test and tuning hook: force the GEMM kernel family.  1, 2 = 128x128 and 64x64 register-staged tiles; 5 = weights straight
