@@ -35,6 +35,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr float kLag = 6.f;
 // Where probabilities are f16 they are 2^kShift times as large, up to 2^15: below 2^-23 of the base they are subnormal, and rounded by 2^-34 of it.
 template <int DT> constexpr float kShift = DT == DT_F16 ? 9.f : 0.f;
+// The least log2 of a value block's A that a row's base counts (8-bit codes).
+constexpr float kLeast = -90.f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DT> __device__ __forceinline__ f16acc mfma(u32x4 a, u32x4 b, f16acc c) {
@@ -58,6 +60,28 @@ __device__ __forceinline__ float half_sum(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
     return u2f(s[0]) + u2f(s[1]);
 }
+// Sixteen times the sum of 2^(x - from), x = kc s, of N scores from `at` on: by their own largest, so that nothing leaves fp32 which counts.
+template <int N, class Scores> __device__ __forceinline__ float sum_of(const Scores& s, int at, float kc, float from) {
+    float m = s[at], sum = 0.f;
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, s[at + i]);
+    m = fmaxf(m * kc, -3e38f);      // (-inf of all: each is 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[at + i], kc, -m));
+    const float e = fmaxf(m - from + 4.f, -200.f), whole = floorf(e);
+    return sum * ldexpf(__builtin_amdgcn_exp2f(e - whole), (int)whole);
+}
+// What sums and numerators take when their base gives way to a new one: 2^d, d = base - now.  With 8-bit codes bases of the same scores differ as
+// far as the A of values do, and sums of a small base are large: 2^d alone would leave fp32, so they take 2^(d / 2) twice.
+template <class Src> struct Rebase {
+    float f;
+    __device__ __forceinline__ Rebase(float base, float now) {
+        const float d = base == -INFINITY ? -INFINITY : base - now;     // no keys yet: nothing
+        f = exp2f(Src::kNormalize ? 0.5f * d : d);
+    }
+    __device__ __forceinline__ float whole() const { return Src::kNormalize ? f * f : f; }
+    __device__ __forceinline__ float add(float to, float sum) const { return fmaf(Src::kNormalize ? sum * f : sum, f, to); }
+};
 // Key, within a block of 32, of accumulator register i in the half wave g.
 __device__ __forceinline__ constexpr int key_of(int i, int g) { return (i & 3) + 8 * (i >> 2) + 4 * g; }
 
@@ -211,9 +235,10 @@ template <class Src, int DP, int RW> struct Lanes {
             }
     }
     // The largest x of NB blocks of 32 keys from key0, and the base moved where a row outgrew it.  kc: what a score is multiplied with, of
-    // each 16 keys; from: what is taken off that.  plain: every row of the wave sees every key, and every block is numbers.
+    // each 16 keys; from: what is taken off that.  plain: every row of the wave sees every key, and every block is numbers.  even: no A is
+    // below 2^kLeast.
     template <int NB, class Scales>
-    __device__ __forceinline__ void raise(f16acc (&s)[NB][RW], float (&kc)[RW][2 * NB], float (&from)[RW], const Scales& sc, int key0, bool plain, int g) {
+    __device__ __forceinline__ void raise(f16acc (&s)[NB][RW], float (&kc)[RW][2 * NB], float (&from)[RW], const Scales& sc, int key0, bool plain, bool even, int g) {
         if (!Src::kBias && !plain) {
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -241,11 +266,18 @@ template <class Src, int DP, int RW> struct Lanes {
             float top = tops[0];
 #pragma unroll
             for (int h = 1; h < 2 * NB; ++h) top = fmaxf(top, tops[h]);
+            if (Src::kNormalize && __builtin_expect(!even, 0))
+#pragma unroll
+                for (int h = 0; h < 2 * NB; ++h)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaf(s[h >> 1][w][8 * (h & 1) + i], kc[w][h], kLeast));
             top = half_max(top);
             if (__any(top > base[w] + kLag)) {
-                const float nb = fmaxf(base[w], top), f = base[w] == -INFINITY ? 0.f : exp2f(base[w] - nb);
+                const float nb = fmaxf(base[w], top);
+                const Rebase<Src> by(base[w], nb);
+                const float f = by.whole();
                 base[w] = nb;
-                sum[w] *= f;
+                sum[w] = by.add(0.f, sum[w]);
 #pragma unroll
                 for (int i = 0; i < DB; ++i) acc[w][i] *= f;
             }
@@ -262,23 +294,13 @@ template <class Src, int DP, int RW> struct Lanes {
             }
         }
     }
-    // What the sum of NB blocks lacks in probs(), which adds the probabilities as they are rounded (half the instructions), for keys whose A
-    // differ much: what is subnormal beside the largest p' may be a large probability of a small A.
-    template <int NB, class Scales>
-    __device__ __forceinline__ void mend_sum(const f16acc (&s)[NB][RW], const float (&kc)[RW][2 * NB], const float (&from)[RW], const Scales& sc) {
+    // The sum of NB blocks where probs() adds none of it, their A being uneven: what is subnormal or nothing beside the largest p' may be a
+    // large probability of a small A.
+    template <int NB> __device__ __forceinline__ void add_sum(const f16acc (&s)[NB][RW], const float (&kc)[RW][2 * NB], const float (&from)[RW]) {
 #pragma unroll
         for (int w = 0; w < RW; ++w)
 #pragma unroll
-            for (int h = 0; h < 2 * NB; ++h) {
-                float lost = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][w][8 * (h & 1) + i], kc[w][h], sc.lv(h) - from[w]));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][w][8 * (h & 1) + i + 1], kc[w][h], sc.lv(h) - from[w]));
-                    lost += p0 + p1 - add2<DT>(pack2<DT>(p0, p1), 0.f);
-                }
-                sum[w] = fmaf(lost, sc.iv(h), sum[w]);
-            }
+            for (int h = 0; h < 2 * NB; ++h) sum[w] += sum_of<8>(s[h >> 1][w], 8 * (h & 1), kc[w][h], from[w]);
     }
     // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.
     template <int NB, class Scales>
@@ -407,8 +429,8 @@ __global__ __launch_bounds__(64 * QW, OCC) void tiles_kernel(const Common a, con
             f16acc s[SB][RW];
             float kc[RW][2 * SB], from[RW];
             L.scores(s, kb + at_k + 32 * b * kRowK<DP>, tb + 32 * b, g);
-            L.raise(s, kc, from, sc, t * TK + 32 * b, plain, g);
-            if (Src::kNormalize && __builtin_expect(!st.even(), 0)) L.mend_sum(s, kc, from, sc);
+            L.raise(s, kc, from, sc, t * TK + 32 * b, plain, st.even(), g);
+            if (Src::kNormalize && __builtin_expect(!st.even(), 0)) L.add_sum(s, kc, from);
 #pragma unroll
             for (int h = 0; h < 2 * SB; ++h) {
                 u32x4 p[RW];
@@ -616,13 +638,17 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
                 }
                 const float k = c[w] * sc.k(b);
                 kc[b] = k > 1.17549435e-38f ? k : 1.17549435e-38f;
-                top = fmaxf(top, fmaf(fmaxf(fmaxf(s[w][b][0], s[w][b][1]), fmaxf(s[w][b][2], s[w][b][3])), kc[b], sc.lv(b)));
+                const float m = fmaxf(fmaxf(s[w][b][0], s[w][b][1]), fmaxf(s[w][b][2], s[w][b][3]));
+                top = fmaxf(top, fmaf(m, kc[b], sc.lv(b)));
+                if (Src::kNormalize && __builtin_expect(!st.even(), 0)) top = fmaxf(top, fmaf(m, kc[b], kLeast));
             }
             top = quarter_max(top);
             if (__any(top > base[w] + kLag)) {
-                const float nb = fmaxf(base[w], top), f = base[w] == -INFINITY ? 0.f : exp2f(base[w] - nb);
+                const float nb = fmaxf(base[w], top);
+                const Rebase<Src> by(base[w], nb);
+                const float f = by.whole();
                 base[w] = nb;
-                sum[w] *= f;
+                sum[w] = by.add(0.f, sum[w]);
 #pragma unroll
                 for (int i = 0; i < DB; ++i) acc[w][i] *= f;
             }
@@ -637,6 +663,7 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
             }
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
+                if (Src::kNormalize && __builtin_expect(!st.even(), 0)) sum[w] += sum_of<4>(s[w][b], 0, kc[b], from);      // as in Lanes::add_sum
                 const float off = sc.lv(b) - from;
                 float e[4];
 #pragma unroll
@@ -692,9 +719,9 @@ __global__ __launch_bounds__(64 * KW, OCC) void few_kernel(const Common a, const
         for (int k = 0; k < KW; ++k) nb = fmaxf(nb, stat[k * 2 * R + rr]);
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
-            const float b = stat[k * 2 * R + rr];
-            wt[k] = b == -INFINITY ? 0.f : exp2f(b - nb);
-            l = fmaf(stat[k * 2 * R + R + rr], wt[k], l);
+            const Rebase<Src> by(stat[k * 2 * R + rr], nb);
+            wt[k] = by.whole();
+            l = by.add(l, stat[k * 2 * R + R + rr]);
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -739,8 +766,8 @@ __global__ __launch_bounds__(256) void join_kernel(const Common a, const typenam
         }
     };
     load(0);
-    const float nb = wave_max_f32(s[0]), w = s[0] == -INFINITY ? 0.f : exp2f(s[0] - nb);
-    const float l = (float)wave_sum_f64((double)(s[1] * w)), inv = l == 0.f ? 0.f : Src::kOut / l;
+    const Rebase<Src> by(s[0], wave_max_f32(s[0]));
+    const float w = by.whole(), l = (float)wave_sum_f64((double)by.add(0.f, s[1])), inv = l == 0.f ? 0.f : Src::kOut / l;
     fe v{};
     for (int i = 0; i < a.splits; i += 8) {
         if (i) load(i);

@@ -16,13 +16,14 @@ struct CacheArgs {
 // Codes are exact in f16, so the products take f16 operands whatever q is: a row of q is scaled by a power of two, after which bf16 values
 // are f16 values but for those 2^14 below the row's largest, which round like a 32-bit sum would.  The key's scale multiplies the score.  The
 // value's scale A becomes part of the probability, p' = p A <= 2^kLag, by its log2 in the exponent, and the denominator takes the block's
-// sum of p' divided by A again: nothing per element.
+// sum of p' divided by A again: nothing per element.  That holds where the A of 64 blocks are within 1/16 of the largest so far, and not below
+// kLeast; elsewhere p' may vanish beside a p that does not, and the denominator is summed from p itself (Lanes::add_sum).
 struct Codes {
     typedef CacheArgs Args;
     static constexpr int DT = DT_F16;
     static constexpr bool kBias = false, kNormalize = true;
-    // iv is 16 / A, so that sums of both ends of A's range, 2^-90 and 2^128, stay ordinary numbers; a smaller A counts as 2^-90, and as
-    // 2^-60 of the largest so far, so that p' does not leave fp32
+    // iv is 16 / A, so that sums of both ends of A's range, 2^kLeast and 2^128, stay ordinary numbers; a row's base counts a smaller A as
+    // 2^kLeast, so that p, which is 2^-kLeast of the base then, does so too
     static constexpr float kOut = 16.f / 127.f;
     template <int N> struct Scales {
         float ks[N], lvs[N], ivs[N];
@@ -56,7 +57,7 @@ struct Codes {
         int window = -1, s_window = -1;
         int pages;                       // of block 64 * window + lane
         float ks, lv, iv, top = 0.f;     // its scales
-        bool all_numbers, all_even;      // of the window
+        bool all_numbers, all_even;      // of the window: no block without numbers; iv in use
         u32x4 kr[CH], vr[CH];
         __device__ Stage(const Args& a_, const Common& c, int id, const Problem& p, int tid_)
             : a(a_), tid(tid_), lane(threadIdx.x & 63), keys(p.keys), d(c.d), hk(c.hk) {
@@ -82,11 +83,12 @@ struct Codes {
             ks = !there ? 0.f : ok && good ? a.ks[i] * (1.f / 127.f) : NAN;
             // the A of p' and of the sum's division: any will do where all values are 0
             top = fmaxf(top, wave_max_f32(good ? A : 0.f));
-            const float u = top == 0.f ? 1.f : A > 0.f && good ? fmaxf(A, fmaxf(top * 0x1p-60f, 0x1p-90f)) : top;
+            const float u = top == 0.f ? 1.f : A > 0.f && good ? A : top;
             all_numbers = !__any(ks != ks);
-            lv = __builtin_amdgcn_logf(u);
-            iv = 16.f / u;
-            all_even = !__any(u < top * 0x1p-4f);
+            lv = u < 0x1p-64f ? __builtin_amdgcn_logf(u * 0x1p64f) - 64.f : __builtin_amdgcn_logf(u);      // the instruction takes ordinary numbers
+            all_even = !__any(u < fmaxf(top * 0x1p-4f, 0x1p-90f));
+            static_assert(kLeast == -90.f, "which is where iv ends");
+            iv = all_even ? 16.f / u : 0.f;
         }
         // TK rows from key0, a multiple of 32
         __device__ __forceinline__ void rows(u32x4 (&x)[CH], const int8_t* codes, int key0) {

@@ -345,7 +345,8 @@ int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void*
  *   earlier forgets what it held.  A value that is not finite makes A, and so all of the block, NaN.  No two sequences of a call may write one block.
  * gpu_kv8_read gives the rows back in dtype (any): code * A / 127.  Rows on 8 bytes (f32: 16), strides multiples of 4 (-1).
  * gpu_kv8_attn: o = softmax(scale * q k^T) v for the rows of q [rows, h, d] (DT_F16 or DT_BF16); row i of a sequence's m sees the tokens
- *   0 .. lens[s] - m + i (causal) or all lens[s].  A row that sees none gives zeros.  ws: gpu_kv8_attn_workspace bytes (0: null will do),
+ *   0 .. lens[s] - m + i (causal) or all lens[s].  A row that sees none gives zeros.  Probabilities times their value's A are rounded to f16,
+ *   and at least in units of 2^-34 of the row's largest such product, in which an A below 2^-90 counts as that.  ws: gpu_kv8_attn_workspace bytes (0: null will do),
  *   16-byte aligned, in use until the work queued here has run.  At most 8388607 workgroups (-1): n * hk, times most * h / hk in tiles of
  *   256 rows (up to 32 rows: of 16).
  * gpu_kv8_copy_pages copies pages src[i] -> dst[i] (int32 on the device, n <= 65535) with their scales in each of `layers` caches that lie

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from conftest import pkg
-from test_gpu_states import DEV, _attn_check, _cross_check, _filled, _gen, _rows
+from test_gpu_states import DEV, Model, U, _attn_check, _check, _cross_check, _filled, _gen, _reference, _rows, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +32,54 @@ def test_cross_attn_with_more_rows_than_a_join_takes():
     o = ql.cross_attn(one.expand(-1, 524288, -1, -1), k, v, 0.3)
     _cross_check(o[:, :1], one, k, v, 0.3)
     assert bool((o == o[:, :1]).all())
+
+
+def _values_check(q, k, v, new, causal, unit, what):
+    """Attention over one sequence of these keys and values, in units of `unit` (a power of two, of each row) against the formula.  Beside the
+    roundings that test_gpu_states.py counts, p A is held in f16 in units of 2^-34 of the row's largest, in which an A below 2^-90 counts as that."""
+    kv = pkg("kvcache")
+    length, heads, dim = k.shape
+    pages = -(-length // 64) + 1
+    cache, table = kv.new_cache(pages, heads, dim, 64), _table([length], 64, pages, 1)
+    kv.store(cache, _rows(kv, [length], [length], table), k, v)
+    model = Model(heads, dim, 1)
+    model.append(0, k, v)
+    o = kv.attn(q, cache, _rows(kv, [new], [length], table), 0.125, causal).double() / unit[:, None, None]
+    pos = torch.arange(length - new, length, device=DEV) if causal else torch.full((new,), length, device=DEV)
+    values, keys = model.values(0, 1), model.values(0, 0)
+    amax = model.amax[0][1].repeat_interleave(16, 1)[:, :length].to(DEV).clamp(min=2.0 ** -90)
+    for j in range(q.shape[1]):
+        i = j * heads // q.shape[1]
+        for u in unit.unique().tolist():
+            rows = unit == u
+            keep = (torch.arange(length, device=DEV) <= pos[:, None])[rows]
+            want, bound = _reference(q[rows, j], keys[:, i], values[:, i] / u, 0.125, keep, torch.zeros(length, dtype=torch.float64, device=DEV), U[torch.float16], U[q.dtype], amax[i] / u)
+            _check(o[rows, j], want, bound, "%s head %d" % (what, j))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 240])
+@pytest.mark.parametrize("new,length", [(1, 200), (1, 9000), (50, 200), (200, 300), (70, 9000)])
+def test_cache_attn_values_far_below_and_above_each_other(new, length, dim):
+    """Values near 1e-30; rows that see such values alone, before tokens whose values are 2^180 of theirs; values 2^-90 of others' that hold all
+    but e^-60 of the probability; the largest of bf16 beside the smallest."""
+    g = _gen(95)
+    q = torch.randn(new, 2, dim, device=DEV, generator=g).bfloat16()
+    k, v = (torch.randn(length, 1, dim, device=DEV, generator=g).bfloat16() for _ in range(2))
+    one = torch.ones(new, dtype=torch.float64, device=DEV)
+    for causal in (True, False):
+        _values_check(q, k, (v.float() * 1e-30).bfloat16(), new, causal, one * 2.0 ** -100, "1e-30")
+        some = torch.where(torch.arange(length, device=DEV) % 48 < 16, 0.0, 1e-28)[:, None, None]
+        _values_check(q, k, (v.float() * some).bfloat16(), new, causal, one * 2.0 ** -93, "zeros beside 1e-28")
+    first = length - (new + 1) // 2      # the later half of the rows' own tokens, or the last one's
+    huge = torch.where(torch.arange(length, device=DEV) // 16 * 16 >= first, 1e30, 1e-25)[:, None, None]
+    sees = torch.arange(length - new, length, device=DEV) >= (first + 15) // 16 * 16
+    _values_check(q, k, (v.float() * huge).bfloat16(), new, True, torch.where(sees, 2.0 ** 100, 2.0 ** -83), "before 1e30")
+    # one direction of the keys decides: the tokens of every third block have logits 60 above the others'
+    q[..., 0], k[..., 0] = 16.0, 0.0
+    third = torch.arange(length, device=DEV) // 16 % 3 == 0
+    k[third, :, 0] = 30.0
+    weak = torch.where(third, 1e-25, 100.0)[:, None, None]
+    _values_check(q, k, (v.float() * weak).bfloat16(), new, False, one * 2.0 ** -83, "probable and small")
+    k[third, :, 0] = 88.0
+    weak = torch.where(third, 1e-38, 1e38)[:, None, None]
+    _values_check(q, k, (v.float() * weak).clamp(-3.38e38, 3.38e38).bfloat16(), new, False, one * 2.0 ** -127, "ends of bf16")
