@@ -318,8 +318,9 @@ int64_t gpu_w6a8_group_gemm_scratch(const void* Wp, int64_t M, int64_t N, int64_
  * k_lens: int32 [b] on the device or null (all lk); values outside 0..lk count as the nearer end.  mask: null (mask_kind 0), bytes [b, lk], 0 = the
  * key is out (1), or f32 [b, lk] added to the logits, -inf = out (2); rows mask_bs elements apart (0: one row for all), 32-bit elements on 4 bytes.
  * A key that is out counts as absent whatever k and v hold there; a row without keys gives zeros.  With f32 masks a |scale| below
- * 7e-31 counts as 0.  Scores, probabilities' sums and
- * outputs are held in fp32, the probabilities rounded to the row type for the product with v.
+ * 7e-31 counts as 0, and biases beyond the least of 7e37 |scale| and 5e37 keep their order, but where they differ by less than 1e-5 of
+ * themselves they may count as equal.  Scores, probabilities' sums and outputs are held in fp32, the probabilities rounded to the row
+ * type for the product with v.
  * ws: gpu_cross_attn_workspace bytes (0: null will do), 16-byte aligned, in use until the work queued here has run.
  * Returns -1 for sizes, a scale that is not finite, or pointers that do not fit this, and for more than 8388607 workgroups: b * hk, times
  * lq * h / hk in tiles of 256 rows (up to 32 rows: of 16). */

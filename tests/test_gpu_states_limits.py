@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from conftest import pkg
-from test_gpu_states import DEV, Model, U, _attn_check, _check, _cross_check, _filled, _gen, _reference, _rows, _table
+from test_gpu_states import DEV, Model, U, _attn_check, _check, _cross_check, _cross_inputs, _filled, _gen, _reference, _rows, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,37 @@ def test_cache_attn_values_far_below_and_above_each_other(new, length, dim):
     k[third, :, 0] = 88.0
     weak = torch.where(third, 1e-38, 1e38)[:, None, None]
     _values_check(q, k, (v.float() * weak).clamp(-3.38e38, 3.38e38).bfloat16(), new, False, one * 2.0 ** -127, "ends of bf16")
+
+
+@pytest.mark.parametrize("scale", [0.125, -2.0, 1e-3, 40.0, 1e-25])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("lq,lk", [(1, 130), (40, 70), (150, 300), (1, 3000)])
+def test_cross_attn_very_large_biases_keep_their_order(lq, lk, dtype, scale):
+    """A row whose biases are all far out, where q k^T is nothing beside them: the key with the largest has all of the probability, keys of
+    the same bias share it, here and between ordinary keys and far ones."""
+    ql = pkg("qlinear")
+    q, k, v = _cross_inputs(1, lq, lk, 2, 1, 64, dtype, 94)
+    low = torch.finfo(torch.float32).min
+    best, second = lk // 3, lk - 1
+
+    def winner(row, keys):
+        o = ql.cross_attn(q, k, v, scale, None, torch.tensor(row, device=DEV, dtype=torch.float32))[0].double()
+        want = v[0, keys, 0].double().mean(0)
+        # probabilities alike, rounded once and summed as rounded: the sums' roundings and the output's
+        assert ((o - want).abs() <= 2 * U[dtype] * v[0, keys, 0].double().abs().mean(0)).all(), (row[best], row[second], row[0])
+
+    for rest, at_best in ((low, -1e38), (low, -3.3e38), (-3.4e38, -3.39e38), (-2.9e38, -2.2e38), (-1e38, -4e37), (3e37, 3e38), (1e38, -low), (low, -low), (low, -1e30), (-1e31, -1e30)):
+        row = [rest] * lk
+        row[best] = at_best
+        winner(row, [best])
+        row[second] = at_best
+        winner(row, [best, second])
+    # one of them after another, in steps of 1e-4
+    steps = [-3.4e38 * (1 - 1e-4 * i) for i in range(lk)]
+    winner(steps, [lk - 1])
+    winner(steps[::-1], [0])
+    winner([-x for x in steps], [0])
+    row = [-x for x in steps[::-1]]
+    row[second] = -3.4e38
+    row[:2] = [-torch.inf, 0.0]
+    winner(row, [lk - 2])
