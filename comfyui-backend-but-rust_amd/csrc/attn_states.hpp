@@ -807,6 +807,8 @@ inline Plan plan_of(int tile, int splits, int64_t rows, int64_t problems, int dp
     p.bytes = splits > 1 ? 4 * splits * problems * p.row_tiles * tile * (dp + 2) : 0;
     return p;
 }
+// Query tokens and keys of a problem: a position some tiles past the last key, and the sum of two, stay 32-bit numbers.
+constexpr int kMostLength = 1 << 30;
 // A launch has fewer than 2^32 threads: workgroups of 512 at most, and rows that the join can take, four in 256.
 constexpr int64_t kMostGroups = 0xffffffff / 512, kMostJoined = 0xffffffff / 256 * 4;
 // bytes: of a key's or value's element.

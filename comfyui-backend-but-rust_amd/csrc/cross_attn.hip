@@ -190,6 +190,7 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
                            const void* mask, int mask_kind, int64_t mask_bs, void* stream) {
     if (dtype != DT_F16 && dtype != DT_BF16) return -4;
     if (b < 0 || lq < 0 || lk < 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256 || head_dim % 8 != 0) return -1;
+    if (lq > kMostLength || lk > kMostLength) return -1;
     if (mask_kind < 0 || mask_kind > 2 || (mask_kind != 0 && !mask && lk > 0) || !(fabsf(scale) < INFINITY)) return -1;
     if (b == 0 || lq == 0) return 0;
     if ((int64_t)lq * (h / hk) > 0x7ffff000 || (int64_t)b * hk > 0x7fffffff || !q || !o || (lk > 0 && (!k || !v))) return -1;
@@ -223,7 +224,7 @@ GPU_API int gpu_cross_attn(int dtype, const void* q, const void* k, const void* 
 }
 
 GPU_API int gpu_internal_states_plan(int64_t rows, int64_t problems, int64_t keys, int head_dim, int bytes, int32_t* out) {
-    if (rows <= 0 || problems <= 0 || keys < 0 || head_dim <= 0 || head_dim > 256 || (bytes != 1 && bytes != 2) || !out) return -1;
+    if (rows <= 0 || problems <= 0 || keys < 0 || head_dim <= 0 || head_dim > 256 || (bytes != 1 && bytes != 2) || !out || (bytes == 2 && keys > kMostLength)) return -1;
     const Plan p = make_plan(rows, problems, keys, head_dim, bytes);
     if (p.row_tiles * problems * p.splits > kMostGroups) return -1;
     out[0] = p.rows;

@@ -6,6 +6,8 @@ namespace {
 
 using namespace states;
 
+static_assert(kMostTokens <= kMostLength, "positions stay 32-bit numbers");
+
 struct CacheArgs {
     const int8_t *k, *v;
     const float *ks, *vs;
@@ -186,7 +188,7 @@ GPU_API int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, v
     if (!cache_ok(k, v, k_scale, v_scale, n_pages, page, hk, head_dim) || h <= 0 || h % hk != 0 || !(fabsf(scale) < INFINITY)) return -1;
     if (!rows_ok(starts, lens, table, table_cols, n, rows, most)) return -1;
     if (n == 0 || rows == 0 || most == 0) return 0;
-    if (!q || !o || (int64_t)most * (h / hk) > 0x7ffff000 || (int64_t)n * hk > 0x7fffffff) return -1;
+    if (!q || !o || most > kMostLength || (int64_t)most * (h / hk) > 0x7ffff000 || (int64_t)n * hk > 0x7fffffff) return -1;
     const Plan p = make_plan((int64_t)most * (h / hk), (int64_t)n * hk, (int64_t)table_cols * page, head_dim, 1);
     if (p.bytes && (!ws || (uintptr_t)ws % 16 != 0)) return -1;
     Common c{};

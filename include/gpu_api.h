@@ -314,7 +314,7 @@ int64_t gpu_w6a8_group_gemm_scratch(const void* Wp, int64_t M, int64_t N, int64_
 /* Cross attention to an encoder's states, 16-bit throughout: o = softmax(scale * q k^T + bias) v per head, where batch item i attends
  * to the keys j < k_lens[i] that its mask leaves.  dtype DT_F16 or DT_BF16 (others -4) for q [b, lq, h, d], k, v [b, lk, hk, d] and o
  * [b, lq, h, d]; element strides per batch item, token and head (bs, rs, hs), the last axis dense; query head j uses key-value head
- * j / (h / hk).  head_dim a multiple of 8 up to 256.  Rows that start on 16 bytes take wide loads and stores, others work too.
+ * j / (h / hk).  lq and lk at most 2^30, head_dim a multiple of 8 up to 256.  Rows that start on 16 bytes take wide loads and stores, others work too.
  * k_lens: int32 [b] on the device or null (all lk); values outside 0..lk count as the nearer end.  mask: null (mask_kind 0), bytes [b, lk], 0 = the
  * key is out (1), or f32 [b, lk] added to the logits, -inf = out (2); rows mask_bs elements apart (0: one row for all), 32-bit elements on 4 bytes.
  * A key that is out counts as absent whatever k and v hold there; a row without keys gives zeros.  With f32 masks a |scale| below
@@ -348,7 +348,7 @@ int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void*
  * gpu_kv8_attn: o = softmax(scale * q k^T) v for the rows of q [rows, h, d] (DT_F16 or DT_BF16); row i of a sequence's m sees the tokens
  *   0 .. lens[s] - m + i (causal) or all lens[s].  A row that sees none gives zeros.  Probabilities times their value's A are rounded to f16,
  *   and at least in units of 2^-34 of the row's largest such product, in which an A below 2^-90 counts as that.  ws: gpu_kv8_attn_workspace bytes (0: null will do),
- *   16-byte aligned, in use until the work queued here has run.  At most 8388607 workgroups (-1): n * hk, times most * h / hk in tiles of
+ *   16-byte aligned, in use until the work queued here has run.  most at most 2^30, and 8388607 workgroups (-1): n * hk, times most * h / hk in tiles of
  *   256 rows (up to 32 rows: of 16).
  * gpu_kv8_copy_pages copies pages src[i] -> dst[i] (int32 on the device, n <= 65535) with their scales in each of `layers` caches that lie
  *   one behind the other in every array.  Numbers that are no page are left out.  No page may be named twice in dst, or in both.

@@ -117,3 +117,13 @@ def test_cross_attn_very_large_biases_keep_their_order(lq, lk, dtype, scale):
     row[second] = -3.4e38
     row[:2] = [-torch.inf, 0.0]
     winner(row, [lk - 2])
+
+
+def test_cross_attn_as_many_keys_as_it_takes():
+    """2^30 keys that are one key: sums of ones up to 2^22 a wave are exact, and so is what joins them."""
+    ql = pkg("qlinear")
+    one = torch.ones(1, 1, 1, 64, device=DEV, dtype=torch.bfloat16)
+    many = one.expand(1, 1 << 30, 1, 64)
+    assert bool((ql.cross_attn(one, many, many, 0.125) == 1).all())
+    lens = torch.tensor([(1 << 30) - 5], dtype=torch.int32, device=DEV)
+    assert bool((ql.cross_attn(one, many, many, 0.125, lens) == 1).all())

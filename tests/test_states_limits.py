@@ -49,3 +49,18 @@ def test_plans_end_where_launches_do():
             for by in (1, 2):
                 rc, (tile, parts) = _plan((1 << 26) // problems, problems, keys, 64, by)
                 assert rc == 0 and parts == 1, (problems, keys, by)
+
+
+def test_lengths_end_at_two_to_the_thirty():
+    """Positions of keys, a few tiles past the last, and of rows behind them stay 32-bit numbers."""
+    assert _cross(1, 64, (1 << 30) + 1, 1, 1, 8) == -1 and _cross(1, 64, (1 << 31) - 1, 1, 1, 8) == -1
+    assert _cross(1, (1 << 30) + 1, 64, 1, 1, 8) == -1
+    assert _plan(64, 1, (1 << 30) + 1, 8, 2)[0] == -1 and _plan(64, 1, 1 << 30, 8, 2)[0] == 0
+    assert _cache(1, (1 << 30) + 1, 1, 1) == -1
+    # a table may be wider than any sequence is long
+    assert _plan(64, 1, 1 << 36, 64, 1)[0] == 0
+
+
+@no_device
+def test_lengths_up_to_two_to_the_thirty_pass():
+    assert _cross(1, 64, 1 << 30, 1, 1, 8) > 0 and _cross(1, 1 << 30, 64, 1, 1, 8) > 0 and _cache(1, 1 << 30, 1, 1) > 0
