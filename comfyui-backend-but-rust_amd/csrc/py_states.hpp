@@ -5,10 +5,12 @@
 
 namespace {
 
-// A tensor whose memory a kernel may read: on the current device, without a gradient to record.
+// A tensor whose memory a kernel may read: on the current device, without a gradient to record or a tangent to carry on.
 const at::Tensor* given(PyObject* o) {
     const at::Tensor* t = plain(o);
-    return t && t->is_cuda() && t->layout() == at::kStrided && t->device().index() == c10::hip::current_device() && !(t->requires_grad() && at::GradMode::is_enabled()) ? t : nullptr;
+    if (!t || !t->is_cuda() || t->layout() != at::kStrided || t->device().index() != c10::hip::current_device()) return nullptr;
+    if (t->requires_grad() && at::GradMode::is_enabled()) return nullptr;
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined() ? nullptr : t;
 }
 bool ints(const at::Tensor* t, int64_t dims) { return t && t->scalar_type() == at::kInt && t->dim() == dims && t->is_contiguous(); }
 bool half_type(const at::Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }

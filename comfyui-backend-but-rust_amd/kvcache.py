@@ -3,7 +3,8 @@ an encoder's states over all steps of a sampler, the frames of a stream, the tok
 
 `Cache` names the device arrays, `Rows` which rows of a call belong to which sequence and where its tokens lie; both are plain tuples, so a
 program may keep the tensors as it likes.  The formats and what every call does with them stand in include/gpu_api.h.  Nothing here waits for
-the GPU; calls are queued on the current stream of the tensors' device.  There is no backward pass: inputs that ask for gradients are refused.
+the GPU; calls are queued on the current stream of the tensors' device.  There is no backward pass and no forward mode: inputs that ask for
+gradients or carry tangents are refused.
 """
 from typing import NamedTuple
 

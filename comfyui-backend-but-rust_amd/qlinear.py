@@ -51,6 +51,8 @@ def _on(device):
 def _no_grad(t, what):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s asks for gradients, and this call has no backward pass: detach it, or call under torch.no_grad()" % what)
+    if torch._C._is_fwd_grad_enabled() and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError("%s carries a tangent, and this call has no forward mode: detach it, or call under torch.inference_mode()" % what)
 
 
 def _ptr(t):

@@ -127,3 +127,25 @@ def test_cross_attn_as_many_keys_as_it_takes():
     assert bool((ql.cross_attn(one, many, many, 0.125) == 1).all())
     lens = torch.tensor([(1 << 30) - 5], dtype=torch.int32, device=DEV)
     assert bool((ql.cross_attn(one, many, many, 0.125, lens) == 1).all())
+
+
+def test_dual_tensors_are_refused():
+    """Forward mode has no rule here any more than reverse mode: a tangent is not dropped in silence, on neither side of the native calls."""
+    ql, kv, ad = pkg("qlinear"), pkg("kvcache"), torch.autograd.forward_ad
+    q, k, v = _cross_inputs(1, 4, 6, 2, 2, 64, torch.bfloat16, 61)
+    bias = torch.zeros(6, device=DEV)
+    cache, table, _ = _filled([20], 2, 64, 16, 62)
+    rows = _rows(kv, [4], [20], table)
+    x, out = q[0], torch.empty_like(q[0])
+    ql.cross_attn(q, k, v, 0.125, None, bias)
+    with ad.dual_level():
+        dual = lambda t: ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ql.cross_attn(dual(q), k, v, 0.125), lambda: ql.cross_attn(q, dual(k), v, 0.125), lambda: ql.cross_attn(q, k, dual(v), 0.125),
+                     lambda: ql.cross_attn(q, k, v, 0.125, None, dual(bias)), lambda: kv.attn(dual(x), cache, rows, 0.125), lambda: kv.attn(x, cache, rows, 0.125, True, dual(out)),
+                     lambda: kv.store(cache, rows, dual(x), x), lambda: kv.store(cache, rows, x, dual(x))):
+            with pytest.raises(ValueError, match="carries a tangent"):
+                call()
+        want = ql.cross_attn(q, k, v, 0.125)
+        assert torch.equal(ql.cross_attn(dual(q).detach(), k, v, 0.125), want)
+        with torch.inference_mode():
+            assert torch.equal(ql.cross_attn(dual(q), k, v, 0.125), want)

@@ -64,3 +64,22 @@ def test_lengths_end_at_two_to_the_thirty():
 @no_device
 def test_lengths_up_to_two_to_the_thirty_pass():
     assert _cross(1, 64, 1 << 30, 1, 1, 8) > 0 and _cross(1, 1 << 30, 64, 1, 1, 8) > 0 and _cache(1, 1 << 30, 1, 1) > 0
+
+
+def test_inputs_that_carry_derivatives_are_refused():
+    ql, ad = pkg("qlinear"), torch.autograd.forward_ad
+    x = torch.ones(3)
+    ql._no_grad(x, "x")
+    with pytest.raises(ValueError, match="x asks for gradients"):
+        ql._no_grad(x.clone().requires_grad_(), "x")
+    with ad.dual_level():
+        dual = ad.make_dual(x, x)
+        with pytest.raises(ValueError, match="x carries a tangent"):
+            ql._no_grad(dual, "x")
+        with torch.no_grad(), pytest.raises(ValueError, match="x carries a tangent"):      # which is reverse mode's alone
+            ql._no_grad(dual, "x")
+        with torch.inference_mode():
+            ql._no_grad(dual, "x")
+        ql._no_grad(dual.detach(), "x")
+        ql._no_grad(x, "x")
+    ql._no_grad(dual, "x")
