@@ -52,9 +52,10 @@ def _cache(cache, dims):
     if v.dtype != torch.int8 or v.shape != k.shape or v.device != k.device or not v.is_contiguous():
         raise ValueError("cache.v must be like cache.k, got %s %s" % (v.dtype, tuple(v.shape)))
     want = k.shape[:-2] + (k.shape[-2] // BLOCK,)
-    for t in (cache.k_scale, cache.v_scale):
+    for t, what in ((cache.k_scale, "cache.k_scale"), (cache.v_scale, "cache.v_scale")):
         if t.dtype != torch.float32 or t.shape != want or t.device != k.device or not t.is_contiguous():
             raise ValueError("the cache's scales must be contiguous float32 %s on its device, got %s %s" % (tuple(want), t.dtype, tuple(t.shape)))
+        qlinear._no_grad(t, what)
     return k.shape
 
 

@@ -149,3 +149,23 @@ def test_dual_tensors_are_refused():
         assert torch.equal(ql.cross_attn(dual(q).detach(), k, v, 0.125), want)
         with torch.inference_mode():
             assert torch.equal(ql.cross_attn(dual(q), k, v, 0.125), want)
+
+
+def test_scales_that_carry_derivatives_are_refused():
+    """The cache's scales are numbers that a gradient could be asked for; the calls have none to give."""
+    kv, ad = pkg("kvcache"), torch.autograd.forward_ad
+    cache, table, _ = _filled([20], 2, 64, 16, 63)
+    rows = _rows(kv, [4], [20], table)
+    x = torch.randn(4, 2, 64, device=DEV, generator=_gen(64)).bfloat16()
+    one, two = (torch.tensor([i], dtype=torch.int32, device=DEV) for i in (0, 1))
+    with ad.dual_level():
+        for name in ("k_scale", "v_scale"):
+            scale = getattr(cache, name)
+            for t, what in ((scale.clone().requires_grad_(), "asks for gradients"), (ad.make_dual(scale.clone(), scale), "carries a tangent")):
+                bad = cache._replace(**{name: t})
+                for call in (lambda: kv.store(bad, rows, x, x), lambda: kv.read(bad, rows, 4), lambda: kv.attn(x, bad, rows, 0.125), lambda: kv.copy_pages(bad, one, two)):
+                    with pytest.raises(ValueError, match=name + " " + what):
+                        call()
+    trained = cache._replace(k_scale=cache.k_scale.clone().requires_grad_())
+    with torch.no_grad():
+        assert torch.equal(kv.attn(x, trained, rows, 0.125), kv.attn(x, cache, rows, 0.125))
