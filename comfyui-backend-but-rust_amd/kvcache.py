@@ -256,6 +256,8 @@ class Sequences:
 
     def rows(self, seqs, counts):
         """Rows of counts[i] queries each to what seqs[i] hold: their last tokens (causal), or rows of something else (not causal)."""
+        if len(seqs) != len(counts) or any(c < 0 for c in counts):
+            raise ValueError("rows wants a count of rows for every sequence, got %d sequences and counts %s" % (len(seqs), list(counts)))
         n, cols = len(seqs), max([len(self._seqs[s][0]) for s in seqs] + [1])
         starts = [0]
         for c in counts:

@@ -83,3 +83,18 @@ def test_inputs_that_carry_derivatives_are_refused():
         ql._no_grad(dual.detach(), "x")
         ql._no_grad(x, "x")
     ql._no_grad(dual, "x")
+
+
+def test_sequences_rows_want_a_count_for_each():
+    """Too few counts made starts of some of the lengths, and lengths of the table."""
+    kv = pkg("kvcache")
+    seqs = kv.Sequences(kv.new_cache(4, 1, 16, 16, device="cpu"))
+    a, b = seqs.add(), seqs.add()
+    seqs.extend([a, b], [20, 3])
+    for counts in ([1], [1, 2, 3], [], [1, -1]):
+        with pytest.raises(ValueError, match="a count of rows"):
+            seqs.rows([a, b], counts)
+    rows = seqs.rows([a, b, a], [2, 0, 7])      # (a sequence may be attended twice)
+    assert rows.starts.tolist() == [0, 2, 2, 9] and rows.lens.tolist() == [20, 3, 20] and rows.table.shape == (3, 2) and rows.most == 7
+    rows = seqs.rows([], [])
+    assert rows.starts.tolist() == [0] and rows.lens.shape == (0,) and rows.table.shape == (0, 1) and rows.most == 0
