@@ -169,3 +169,85 @@ def test_scales_that_carry_derivatives_are_refused():
     trained = cache._replace(k_scale=cache.k_scale.clone().requires_grad_())
     with torch.no_grad():
         assert torch.equal(kv.attn(x, trained, rows, 0.125), kv.attn(x, cache, rows, 0.125))
+
+
+def _attended_and_crossed(new, seed):
+    """A cache call and a cross call whose keys are shared by workgroups, with what they read: both are functions of device data alone."""
+    ql, kv = pkg("qlinear"), pkg("kvcache")
+    lens = [2500, 900]
+    cache, table, _ = _filled(lens, 2, 64, 32, seed)
+    rows = _rows(kv, [new, new], lens, table)
+    g = _gen(seed + 1)
+    q = torch.randn(2 * new, 8, 64, device=DEV, generator=g).bfloat16()
+    cq, ck, cv = _cross_inputs(2, new, 2500, 4, 2, 64, torch.float16, seed + 2)
+    k_lens = torch.tensor([2500, 77], dtype=torch.int32, device=DEV)
+    mask = torch.rand(2, 2500, device=DEV, generator=g) < 0.5
+    return (q, cache, rows, cq, k_lens, mask), lambda: [kv.attn(q, cache, rows, 0.125), ql.cross_attn(cq, ck, cv, 0.125, k_lens, mask)]
+
+
+@pytest.mark.parametrize("new", [1, 24, 60])
+def test_two_graphs_follow_lengths_tables_and_masks(new):
+    """What device data hold when a replay runs counts, not what they held at the capture; two graphs in turn, eager calls between them."""
+    sets = [_attended_and_crossed(new, seed) for seed in (101, 111)]
+    for _, call in sets:
+        call()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _, call in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call())
+    for step, (lens, k_lens) in enumerate((([2500, 900], [2500, 77]), ([61, 2400], [0, 2500]), ([1700, 60], [3, 1300]), ([60, 60], [2500, 2499]))):
+        for (q, cache, rows, cq, at, mask), _ in sets:
+            q.normal_()
+            cq.normal_()
+            rows.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+            rows.table.copy_(rows.table.flip(0) if step == 2 else rows.table)
+            at.copy_(torch.tensor(k_lens, dtype=torch.int32))
+            mask.logical_not_()
+        for i in (1, 0, 1):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        got = [[t.clone() for t in o] for o in outs]
+        want = [call() for _, call in sets]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for x, y in zip(a, b):
+                # (tokens that a table does not hold are NaN)
+                assert torch.equal(x.view(torch.int16), y.view(torch.int16)), (step, new)
+
+
+@pytest.mark.parametrize("new", [1, 24, 60])
+def test_two_streams_at_once(new):
+    sets = [_attended_and_crossed(new, seed) for seed in (121, 131)]
+    want = [call() for _, call in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[] for _ in sets]
+    for _ in range(5):
+        for i, (_, call) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(call())
+    torch.cuda.synchronize()
+    for many, once in zip(got, want):
+        assert all(torch.equal(x, y) for o in many for x, y in zip(o, once))
+
+
+@pytest.mark.parametrize("new", [1, 24, 70])
+def test_pages_in_several_tables_and_outputs_in_the_queries_place(new):
+    """Sequences that begin with the same pages; outputs written over the queries that they come from; a bound above the longest's rows."""
+    kv = pkg("kvcache")
+    cache, table, model = _filled([640], 2, 64, 32, 141)
+    lens = [640, 300, 77]
+    both = table.expand(3, -1).contiguous()
+    q = torch.randn(3 * new, 8, 64, device=DEV, generator=_gen(142)).bfloat16()
+    rows = _rows(kv, [new] * 3, lens, both)
+    want = kv.attn(q, cache, rows, 0.125)
+    for i, l in enumerate(lens):
+        _attn_check(want[i * new:(i + 1) * new], q[i * new:(i + 1) * new], model, [new], [l], 0.125, True, "sequence %d" % i)
+    place = q.clone()
+    assert kv.attn(place, cache, rows, 0.125, out=place) is place and torch.equal(place, want)
+    more = rows._replace(most=new + 200)
+    for i, l in enumerate(lens):
+        o = kv.attn(q, cache, more, 0.125)[i * new:(i + 1) * new]
+        _attn_check(o, q[i * new:(i + 1) * new], model, [new], [l], 0.125, True, "bound, sequence %d" % i)
