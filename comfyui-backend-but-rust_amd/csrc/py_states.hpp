@@ -9,6 +9,7 @@ namespace {
 const at::Tensor* given(PyObject* o) {
     const at::Tensor* t = plain(o);
     if (!t || !t->is_cuda() || t->layout() != at::kStrided || t->device().index() != c10::hip::current_device()) return nullptr;
+    if (!t->unsafeGetTensorImpl()->autograd_meta()) return t;      // which both would be part of
     if (t->requires_grad() && at::GradMode::is_enabled()) return nullptr;
     return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined() ? nullptr : t;
 }
