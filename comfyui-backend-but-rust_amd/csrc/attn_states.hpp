@@ -302,7 +302,9 @@ template <class Src, int DP, int RW> struct Lanes {
 #pragma unroll
             for (int h = 0; h < 2 * NB; ++h) sum[w] += sum_of<8>(s[h >> 1][w], 8 * (h & 1), kc[w][h], from[w]);
     }
-    // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.
+    // Probabilities of 16 of the keys (h), rounded and in pairs, and their sum.  The product with V takes 16-bit operands, so they are rounded to V's type
+    // (codes: f16), each by 2^-8 (bf16) or 2^-11 of itself at most; the sum is of them as rounded, which takes half the
+    // instructions and leaves out what all keys lose alike.
     template <int NB, class Scales>
     __device__ __forceinline__ void probs(u32x4 (&p)[RW], const f16acc (&s)[NB][RW], const float (&kc)[RW][2 * NB], const float (&from)[RW], const Scales& sc, int h) {
 #pragma unroll
@@ -375,10 +377,10 @@ __device__ __forceinline__ void share_of(int end, int tk, int splits, int split,
 // before goes into LDS and the one before that is multiplied, SB blocks of 32 keys per step of the softmax.
 //
 // 4 * d operations a pair on the matrix pipes, one exponential a pair beside them.  2 x 1024 new tokens of 32 heads behind 7168 stored ones
-// (223 GFLOP) take 272 us, 0.82 PFLOP/s where an 8192-cubed product of the vendor's library reaches 1.23; matrix pipes 41 % and vector
-// pipes 54 % busy at 1.7 GHz under the power limit, and the two hardly overlap: a probe shows a product of another wave keeping vector
+// (223 GFLOP) take 274 us, 0.81 PFLOP/s where an 8192-cubed product of the vendor's library reaches 1.23; matrix pipes 41 % and vector
+// pipes 51 % busy at 1.7 GHz under the power limit, and the two hardly overlap: a probe shows a product of another wave keeping vector
 // instructions from issue for 11 of its 32 cycles (v_dot2 for all of them).  Head dim 64 (frame of 2025 tokens to 16200, f16, 16 heads):
-// vector pipes 75 % busy, 193 us.
+// vector pipes 78 % busy, 189 us.
 // Eight waves on a tile spend half the instructions on staging, conversion to f16 above all, that four do (289 us against 325), but few rows
 // do not fill them; 64 keys per softmax step with one branch 285 against 289; sums of rounded pairs (v_dot2) against additions 270 and
 // 284.  Not kept: scores of the next keys between the exponentials, left to the compiler (292) or held there by sched_barrier (310); two
@@ -820,7 +822,8 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
         // In microseconds: a workgroup starts and ends in 4; 32 keys of a wave take 1.65 at least (1 x 1369 keys x 64 heads of 72 channels in one
         // part 22.6 in all), and longer where the waves of a CU together ask for more than its share of the copy rate, 20 KB a microsecond,
         // of which CUs with few waves reach less (12 x 32749 keys x 8 heads of 128 codes: 3 parts 183, 5 parts 138, 8 parts, which are one
-        // full round, 130, 16 parts 136); a wave beside others on its CU takes a little more; joining 3.
+        // full round, 130, 16 parts 136); a wave beside others on its CU takes a little more; joining 3.  per_cu is the workgroups that share a CU in
+        // this reckoning, and what registers and LDS allow but for head dims to 64, where 4 or 5 would fit (3 with 32 rows): not measured there.
         const int tile = rows <= 16 || dp >= 192 ? 16 : 32, per_cu = dp == 256 || (bytes > 1 && dp == 192) ? 1 : tile == 32 || dp == 192 || (bytes > 1 && dp == 128) ? 2 : 3;
         const int64_t slots = cus * per_cu, tiles = (keys + 31) / 32, groups = problems * ((rows + tile - 1) / tile);
         const double full = per_cu * 4 * 32. * d * 2 * bytes / 20e3;
@@ -868,10 +871,10 @@ inline Plan make_plan(int64_t rows, int64_t problems, int64_t keys, int d, int b
     return best;
 }
 
-// Waves a SIMD (the last argument) are what the registers of a form allow, spilling a few at most (codes at 256 with 256 rows 66, and
-// ahead all the same: 2025 rows of 8 heads of 240 to 8100, 200 us against 248 with 128 rows); blocks of 32 keys a tile follow: one where
+// Waves a SIMD (the last argument) are what the registers of a form allow, spilling a few at most (codes at 256 with 256 rows 40, and
+// ahead all the same: 2025 rows of 8 heads of 240 to 8100, 173 us against 247 with 128 rows); blocks of 32 keys a tile follow: one where
 // two would cost a workgroup its place (head dims to 64 and 96 with 128 rows: 4 and 3 on a CU; 192), two elsewhere.  At 256 with 128 rows, one wave a SIMD
-// either way: 16-bit keys one at a time (4 x 638 x 6, 72 heads: 84 us against 98 with two), codes two (the last 1024 of 2 x 4096 tokens, 16 over 4 heads: 234 against 246).
+// either way: 16-bit keys one at a time (4 x 638 x 6, 72 heads: 84 us against 98 with two), codes two (the last 1024 of 2 x 4096 tokens, 16 over 4 heads: 235 against 251).
 template <class Src, int DP> inline int launch(const Plan& p, int64_t rows, Common& a, const typename Src::Args& sa, hipStream_t stream) {
     const int64_t grid = (int64_t)p.row_tiles * a.problems * p.splits;
     if (grid > kMostGroups) return -1;

@@ -30,7 +30,7 @@ class Rows(NamedTuple):
     starts: torch.Tensor        # int32 [n + 1]: rows starts[s] .. starts[s + 1] of a call are the last tokens of sequence s
     lens: torch.Tensor          # int32 [n]: tokens that the sequence holds, the new ones among them
     table: torch.Tensor         # int32 [n, pages of a sequence]: token t lies in page table[s, t // page]
-    most: int                   # rows of the sequence that has the most in this call
+    most: int                   # rows of the sequence that has the most in this call, or a bound; one below that misplaces the rows above it
 
 
 def new_cache(pages, heads, dim, page=64, layers=None, device="cuda:0"):
@@ -119,7 +119,8 @@ def _read(cache, rows, tokens, dtype):
 
 def attn(q, cache, rows, scale, causal=True, out=None):
     """softmax(scale * q k^T) v over the stored tokens: q [rows, h, d] (bf16 or f16), h a multiple of the cache's heads.  Causal: a row sees the
-    tokens up to its own place; otherwise all that its sequence holds.  Rows of no sequence are left as they are in `out`."""
+    tokens up to its own place; otherwise all that its sequence holds.  Rows of no sequence are left as they are in `out`.  rows.most decides how
+    all of the call runs: single tokens and long pieces of prompts are better two calls."""
     o = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.kv8_attn(q, *cache, *rows, float(scale), bool(causal))
     return _attn(q, cache, rows, scale, causal, out) if o is None else o
 

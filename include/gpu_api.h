@@ -337,7 +337,8 @@ int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void*
  *   starts int32 [n + 1], lens int32 [n], table int32 [n, table_cols], all on the device: rows starts[s] .. starts[s + 1] of the call's
  *     row tensors are the LAST tokens of sequence s, which holds lens[s] tokens (the new ones among them, at most 2^30); its token t is slot
  *     t % page of page table[s, t / page].  rows: rows of the row tensors, none behind it is touched; most: the most rows of one
- *     sequence (those above it are left out).  Sequences without rows, and without tokens, are fine.  An entry of the table that is no page
+ *     sequence, or a bound.  It must not be too small: of a sequence with more rows the first `most` are taken for its LAST tokens (stored at, or
+ *     attending from, their places), the others are left out.  Sequences without rows, and without tokens, are fine.  An entry of the table that is no page
  *     (outside 0 .. n_pages - 1, or beyond table_cols) is never accessed: tokens there are not stored, read back as NaN, and make NaN
  *     of every attention row that sees them.
  * gpu_kv8_store writes the rows of k and v (DT_F16 or DT_BF16, element strides of tokens and heads, dense last axis) at their places.  Per block
@@ -348,8 +349,9 @@ int gpu_cross_attn(int dtype, const void* q, const void* k, const void* v, void*
  * gpu_kv8_attn: o = softmax(scale * q k^T) v for the rows of q [rows, h, d] (DT_F16 or DT_BF16); row i of a sequence's m sees the tokens
  *   0 .. lens[s] - m + i (causal) or all lens[s].  A row that sees none gives zeros.  Probabilities times their value's A are rounded to f16,
  *   and at least in units of 2^-34 of the row's largest such product, in which an A below 2^-90 counts as that.  ws: gpu_kv8_attn_workspace bytes (0: null will do),
- *   16-byte aligned, in use until the work queued here has run.  most at most 2^30, and 8388607 workgroups (-1): n * hk, times most * h / hk in tiles of
- *   256 rows (up to 32 rows: of 16).
+ *   16-byte aligned, in use until the work queued here has run.  At most 2^30 for most, and 8388607 workgroups (-1): n * hk, times
+ *   most * h / hk in tiles of 256 rows (up to 32 rows: of 16).  `most` decides for all sequences how the call runs: single tokens beside a
+ *   prompt piece wait for tiles made for the piece and share no keys, so a batch of both is better made two calls, of the tokens and of the pieces.
  * gpu_kv8_copy_pages copies pages src[i] -> dst[i] (int32 on the device, n <= 65535) with their scales in each of `layers` caches that lie
  *   one behind the other in every array.  Numbers that are no page are left out.  No page may be named twice in dst, or in both.
  * All return -4 for a dtype they do not take, -1 for sizes and pointers that do not fit the above (n <= 65535 in store and read). */
