@@ -58,6 +58,10 @@ SIGNATURES = {
     "gpu_kv8_attn": [_I32, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _P, _P, _I32, _I32, _P, _P, _P] + [_I32] * 7 + [_F32, _I32, _P],
     "gpu_kv8_attn_workspace": [_I32] * 7,
     "gpu_kv8_copy_pages": [_P, _P, _P, _P] + [_I32] * 5 + [_P, _P, _I32, _P],
+    "gpu_fp8_quant_rows": [_I32, _I32, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _F32, _P, _P, _I64, _I32, _I32, _P],
+    "gpu_fp8_gemm": [_P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _P],
+    "gpu_rope": [_I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _F32, _I32, _I32, _P],
+    "gpu_prompt_attn": [_I32] + [_P, _I64, _I64] * 4 + [_P, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P],
     "gpu_internal_act_probe": [_I32, _P, _P, _I32, _P],
     "gpu_internal_geglu_form": [_I32, _I32],
     "gpu_internal_cvt_pk_u8_probe": [_P, _P, _I32, _P],

@@ -451,3 +451,65 @@ def _cross_attn(q, k, v, scale, k_lens, mask):
               q.stride(2), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), o.stride(0), o.stride(1), o.stride(2),
               float(scale), _ptr(k_lens), _ptr(mask), kind, bs, s)
     return o
+
+
+_FP8_ROWS = {"plain": ffi.PRO_PLAIN, "rms": ffi.PRO_RMS, "swiglu": ffi.PRO_SWIGLU}
+GROUP = 128         # columns that share a scale in the e4m3 format
+
+
+def fp8_quant_rows(x, prologue="plain", norm_w=None, eps=0.0, resid=None, out=None):
+    """Rows as e4m3 codes with a scale for each group of 128 columns: (q [M, K] float8_e4m3fn, scales float32 [ceil(K / 128), M]), and with a
+    residual also the sum x + resid in x's type, (q, scales, sum).  x and resid: [M, K] bf16, f16 or f32, any row stride.  "rms": the rows are
+    normed, with weight norm_w (float32 [K]) and eps; "swiglu": x is [M, 2K], silu of its first half times the second.  out: where the sum goes
+    instead of a new tensor; it may be x or resid."""
+    if x.dim() != 2 or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1) or x.dtype not in _TORCH_DT:
+        raise ValueError("x must be a 2-D bfloat16, float16 or float32 CUDA tensor with a dense last axis, got %s %s with strides %s" % (x.dtype, tuple(x.shape), x.stride()))
+    if prologue not in _FP8_ROWS:
+        raise ValueError("prologue must be one of %s, got %r" % (sorted(_FP8_ROWS), prologue))
+    M, K = x.shape
+    if prologue == "swiglu":
+        if K % 2 or resid is not None:
+            raise ValueError("swiglu takes rows of two halves and no residual, got %d columns" % K)
+        K //= 2
+    if (norm_w is not None) != (prologue == "rms") or (out is not None and resid is None):
+        raise ValueError("norm_w belongs to the rms prologue, out to a residual")
+    for t, shape, dtype, what in ((resid, (M, K), x.dtype, "resid"), (out, (M, K), x.dtype, "out"), (norm_w, (K,), torch.float32, "norm_w")):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != x.device or (shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError("%s must be %s %s on x's device with a dense last axis, got %s %s with strides %s on %s" % (what, dtype, shape, t.dtype, tuple(t.shape), t.stride(), t.device))
+    for t, what in ((x, "x"), (resid, "resid"), (norm_w, "norm_w"), (out, "out")):
+        if t is not None:
+            _no_grad(t, what)
+    q = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((-(-K // GROUP), M), dtype=torch.float32, device=x.device)
+    total = None if resid is None else torch.empty((M, K), dtype=x.dtype, device=x.device) if out is None else out
+    with _on(x.device) as s:
+        ffi.k("gpu_fp8_quant_rows", _TORCH_DT[x.dtype], _FP8_ROWS[prologue], _ptr(x), x.stride(0), _ptr(resid), 0 if resid is None else resid.stride(0), _ptr(total),
+              0 if total is None else total.stride(0), K, _ptr(norm_w), float(eps), _ptr(q), _ptr(scales), M, M, K, s)
+    return (q, scales) if total is None else (q, scales, total)
+
+
+def fp8_gemm(A, W, xs, ws, bias=None, out_dtype=torch.bfloat16, D=None):
+    """A . W^T of e4m3 operands with block scales: A [M, K] and xs float32 [ceil(K / 128), M] as fp8_quant_rows gives them, W [N, K] with ws
+    float32 [ceil(N / 128), ceil(K / 128)], a scale for each block of 128 x 128; bias [N] in out_dtype."""
+    if A.dim() != 2 or W.dim() != 2 or A.shape[1] != W.shape[1]:
+        raise ValueError("A [M,K] and W [N,K] must share K, got %s and %s" % (tuple(A.shape), tuple(W.shape)))
+    M, K = A.shape
+    N = W.shape[0]
+    G = -(-K // GROUP)
+    D = torch.empty((M, N), dtype=out_dtype, device=A.device) if D is None else D
+    _dense(A, W, ws, bias, D)
+    _want(A, torch.float8_e4m3fn, "A"); _want(W, torch.float8_e4m3fn, "W"); _want(xs, torch.float32, "xs"); _want(ws, torch.float32, "ws"); _want(bias, out_dtype, "bias"); _want(D, out_dtype, "D")
+    if out_dtype not in _TORCH_DT:
+        raise ValueError("out_dtype must be bfloat16, float16 or float32, got %s" % out_dtype)
+    if xs.shape != (G, M) or (M > 1 and xs.stride(1) != 1) or (G > 1 and xs.stride(0) < M) or ws.shape != (-(-N // GROUP), G):
+        raise ValueError("xs must be [%d, %d] with a dense last axis and ws [%d, %d], got %s with strides %s and %s" % (G, M, -(-N // GROUP), G, tuple(xs.shape), xs.stride(), tuple(ws.shape)))
+    if (bias is not None and bias.shape != (N,)) or D.shape != (M, N):
+        raise ValueError("bias must be [%d] and D [%d, %d]" % (N, M, N))
+    for t, what in ((A, "A"), (W, "W"), (xs, "xs"), (ws, "ws"), (bias, "bias"), (D, "D")):
+        if t is not None:
+            if t.device != A.device:
+                raise ValueError("%s must be on A's device, got %s and %s" % (what, t.device, A.device))
+            _no_grad(t, what)
+    with _on(A.device) as s:
+        ffi.k("gpu_fp8_gemm", _ptr(A), _ptr(W), _ptr(xs), xs.stride(0) if G > 1 else M, _ptr(ws), _ptr(bias), _ptr(D), M, N, K, _TORCH_DT[out_dtype], s)
+    return D

@@ -369,6 +369,45 @@ int gpu_kv8_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* o, 
 int gpu_kv8_copy_pages(int8_t* ck, int8_t* cv, float* k_scale, float* v_scale, int layers, int n_pages, int page, int hk, int head_dim,
                        const int32_t* src, const int32_t* dst, int n, void* stream);
 
+/* Rows as e4m3 codes (OCP: largest 448, no infinities) with a scale for each group of 128 columns, the operands of gpu_fp8_gemm.
+ *   s = T(x + resid), stored to sum, where resid is not null (then sum is not either; PRO_PLAIN and PRO_RMS), else x
+ *   n = s (PRO_PLAIN), s * norm_w / sqrt(mean(s^2) + eps) over the row (PRO_RMS), or silu(x) * x[up_offset ..] (PRO_SWIGLU), in fp32
+ *   A = max(largest |n| of the group, 2^-100), scales[g * scales_stride + m] = A / 448, q[m, k] = e4m3(n * (448 / A)), nearest even
+ * x, resid, sum: T[M, stride], dtype bf16, f16 or f32 (else -4), dense rows at any stride; sum may be x or resid, with its stride.
+ * norm_w f32 [K].  q [M, K], 8-byte aligned; scales f32 [ceil(K / 128), scales_stride], scales_stride >= M; the last group may be part of one.
+ * A group that holds a NaN or an infinity stands for NaN throughout.  K a multiple of 16 (-1) up to 32768 (-2); -3 prologue. */
+int gpu_fp8_quant_rows(int dtype, int prologue, const void* x, int64_t x_stride, const void* resid, int64_t resid_stride, void* sum,
+                       int64_t sum_stride, int64_t up_offset, const float* norm_w, float eps, void* q, float* scales,
+                       int64_t scales_stride, int M, int K, void* stream);
+
+/* D[m, n] = Out(sum_g xs[g * xs_stride + m] * ws[n / 128, g] * (sum over the group's k of A[m, k] * W[n, k]) + bias[n]): A [M, K] and W [N, K] e4m3,
+ * K-contiguous, 16-byte aligned; groups of 128 along K; xs f32 [groups, xs_stride], ws f32 [ceil(N / 128), groups]; the last group and
+ * the last block of rows of W may be parts.  bias Out[N] or null.  Out by out_dt (-4).  K a multiple of 16 (-1).  Sums in fp32, but that for 16-bit
+ * outputs the matrix instruction cuts the products of each eight k off at 2^-13 of the largest one's power of two (1.5e-5 of the result on normally
+ * distributed operands). */
+int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_stride, const float* ws, const void* bias, void* D, int64_t M,
+                 int64_t N, int64_t K, int out_dt, void* stream);
+
+/* Rotary positions.  Of every head of q [T, h, d] and k [T, hk, d] (dtype bf16, f16 or f32, else -4; element strides of tokens and heads, dense
+ * last axis) the first `rot` channels are pairs, (j, j + rot / 2) or, interleaved, (2j, 2j + 1); pair j of token t turns by the angle
+ * positions[t] * freqs[j] (radians; 64 bits), (a, b) -> factor * (a cos - b sin, a sin + b cos); the other channels stay.  With q_norm or k_norm
+ * (f32 [d]) the heads of that side are first divided by sqrt(mean(x^2) + eps) over d and multiplied by it.  fp32 throughout, rounded
+ * once.  Outputs may be the inputs, with their strides.  d and rot multiples of 4, d up to 256, up to 65536 heads (-1); either side may have 0 heads. */
+int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, int64_t qo_rs, int64_t qo_hs, int h, const void* k,
+             int64_t k_rs, int64_t k_hs, void* k_out, int64_t ko_rs, int64_t ko_hs, int hk, const int32_t* positions, const double* freqs,
+             int rot, int interleaved, float factor, const float* q_norm, const float* k_norm, float eps, int T, int head_dim, void* stream);
+
+/* Attention over whole prompts that lie one behind the other: rows starts[s] .. starts[s + 1] of q [tokens, h, d], k and v [tokens, hk, d] and o
+ * [tokens, h, d] are prompt s (int32 [n + 1] on the device); o = softmax(scale * q k^T) v within it, over the keys up to the row's own
+ * (causal) or all.  dtype DT_F16 or DT_BF16 (-4); element strides of tokens and heads, dense last axis; query head j uses key-value head
+ * j / (h / hk).  Rows of no prompt are left as they are.  starts that do not grow are brought into 0 .. tokens: rows may then be left
+ * out, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key makes it NaN, a value its channel NaN or
+ * infinite.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
+ * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 128 rows or more, and n) (-1). */
+int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
+                    int64_t v_rs, int64_t v_hs, void* o, int64_t o_rs, int64_t o_hs, const int32_t* starts, int n, int tokens, int h, int hk,
+                    int head_dim, float scale, int causal, void* stream);
+
 /* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times
  * key-value heads) of `rows` (query tokens times query heads of a key-value head, the most of any) over `keys`: out[0] = rows of a workgroup (16 and 32:
  * its waves share them, 128 and 256: a wave has 32), out[1] = workgroups that share a row's keys,

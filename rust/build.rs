@@ -10,6 +10,7 @@ use std::process::Command;
 const UNITS: &[&str] = &[
     "quant_rows.hip", "prologue_rows.hip", "weight_formats.hip", "act_tables.hip", "int8_gemm.hip", "w6.hip",
     "w6_requant.hip", "w6a8_group_gemm.hip", "attn_int8.hip", "cross_attn.hip", "kv8.hip", "kv8_attn.hip",
+    "fp8_rows.hip", "fp8_gemm.hip", "rope.hip", "prompt_attn.hip",
 ];
 
 fn run(cmd: &mut Command) {
