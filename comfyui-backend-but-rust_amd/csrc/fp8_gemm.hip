@@ -138,7 +138,197 @@ __global__ void __launch_bounds__(256, 2) fp8_gemm_kernel(const Fp8Gemm p) {
         for (int j = 0; j < 4; ++j) store_four<OUT_DT>(p, m0 + wm + 16 * i + row, n0 + wn + 16 * j + 4 * part, acc[i][j]);
 }
 
+// ---- tiles by DMA ----------------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ void dma16(uint32_t lds_dst, uint32_t lane_off, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(lane_off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(uint32_t lds_dst, uint32_t lane_off, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_dst), "v"(lane_off), "s"(base) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ int lane_now() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
+// A wave's FM x FN tiles, first row mw, first column nb: rounded, passed 32 rows at a time through `wl`, LDS of its own (32 rows of its columns;
+// 16-byte chunks swizzled by row), and stored in whole row segments, 16 bytes a lane.
+template <int OUT_DT, int FM, int FN>
+__device__ __forceinline__ void store_wave_tile(const Fp8Gemm& p, uint8_t* wl, const v4f (&acc)[FN][FM], int mw, int nb, int lane) {
+    static_assert(OUT_DT != DT_F32, "16-bit outputs");
+    const int row = lane & 15, part = lane >> 4;
+    if (!p.rows_ok) {
+#pragma unroll
+        for (int in = 0; in < FN; ++in)
+#pragma unroll
+            for (int im = 0; im < FM; ++im) store_four<OUT_DT>(p, mw + 16 * im + row, nb + 16 * in + 4 * part, acc[in][im]);
+        return;
+    }
+    constexpr int CPR = 2 * FN, RPI = 64 / CPR;      // 16-byte chunks of a row, rows of a store instruction
+    float bv[FN][4];
+#pragma unroll
+    for (int in = 0; in < FN; ++in)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) bv[in][c] = p.bias && nb + 16 * in + 4 * part + c < p.N ? ld_dt<OUT_DT>(p.bias, nb + 16 * in + 4 * part + c) : 0.f;
+#pragma unroll
+    for (int ip = 0; ip < FM / 2; ++ip) {
+#pragma unroll
+        for (int hm = 0; hm < 2; ++hm) {
+            const int r = 16 * hm + row;
+#pragma unroll
+            for (int in = 0; in < FN; ++in) {
+                const v4f x = acc[in][2 * ip + hm];
+                float v[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[c] = x[c] + bv[in][c];
+                uint8_t* const to = wl + r * (16 * CPR) + (((2 * in + (part >> 1)) ^ (r & (CPR - 1))) << 4) + 8 * (part & 1);
+                *reinterpret_cast<uint2*>(to) = OUT_DT == DT_BF16 ? make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])) : make_uint2(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]));
+            }
+        }
+        asm volatile("" ::: "memory");      // a wave's LDS accesses stay in order
+#pragma unroll
+        for (int t = 0; t < 32 / RPI; ++t) {
+            const int r = t * RPI + lane / CPR, c = lane % CPR, m = mw + 32 * ip + r, n = nb + 8 * c;
+            const uint4 v = *reinterpret_cast<const uint4*>(wl + r * (16 * CPR) + ((c ^ (r & (CPR - 1))) << 4));
+            if (m < p.M && n < p.N) *reinterpret_cast<uint4*>((uint16_t*)p.D + (int64_t)m * p.N + n) = v;
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+// A fragment of the group that is not a whole one, straight from memory: 0 behind K.
+__device__ __forceinline__ v8i tail_fragment(const uint8_t* x, int row, int limit, int K, int k0, int part) {
+    const uint8_t* const at = x + (int64_t)min(row, limit - 1) * K + k0;
+    v4i a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    if (k0 + 16 * part < K) a = *reinterpret_cast<const v4i*>(at + 16 * part);
+    if (k0 + 64 + 16 * part < K) b = *reinterpret_cast<const v4i*>(at + 64 + 16 * part);
+    return two(a, b);
+}
+
+// Large sizes: tiles of 256 x 256, eight waves of 128 x 64, two LDS stages: group g + 1 travels while group g is multiplied, one barrier a group.
+constexpr int BIG = 256, BIG_STAGE = BIG * kGroup, BIG_S = 4 * BIG_STAGE, BIG_LDS = BIG_S + 2 * BIG * 4;
+
+template <int OUT_DT>
+__global__ void __launch_bounds__(512, 1) fp8_gemm_big_kernel(const Fp8Gemm p) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+    int tm, tn;
+    tile_of_block((int)blockIdx.x, (int)gridDim.x, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = tm * BIG, n0 = tn * BIG, full = p.K / kGroup;
+    const uint32_t lds_base = (uint32_t)(uintptr_t)smem;
+    constexpr int FM = 8, FN = 4;
+
+    // The lower waves fetch: 8-row blocks wn + 4 j of W and of A, the swizzle on the memory's side, and the scales of rows 64 wn ..
+    const uint32_t lrow = (uint32_t)lane >> 3, K = (uint32_t)p.K;
+    const uint32_t chunk = ((lane & 7) ^ (((wn & 1) << 2) | (lrow >> 1))) * 16, drow = wn * 8 + lrow;
+    const uint32_t w_last = (uint32_t)min(BIG - 1, p.N - 1 - n0), a_last = (uint32_t)min(BIG - 1, p.M - 1 - m0);
+    const uint32_t s_off = 4u * min((uint32_t)(64 * wn + lane), a_last);
+    const uint8_t *const a_base = p.A + (int64_t)m0 * p.K, *const w_base = p.W + (int64_t)n0 * p.K;
+    const float* const s_base = p.xs + m0;
+    constexpr int NDMA = 17;
+    const auto dma = [&](int g, int j) {      // groups past the end fetch the last one again, which nothing reads
+        const int gc = g < full ? g : full - 1, stage = g & 1;
+        if (j < 8) dma16(lds_base + (2 + stage) * BIG_STAGE + (wn + 4 * j) * 1024, __umul24(min(drow + 32 * j, w_last), K) + chunk, w_base + (int64_t)gc * kGroup);
+        else if (j < 16) dma16(lds_base + stage * BIG_STAGE + (wn + 4 * (j - 8)) * 1024, __umul24(min(drow + 32 * (j - 8), a_last), K) + chunk, a_base + (int64_t)gc * kGroup);
+        else dma4(lds_base + BIG_S + stage * (BIG * 4) + wn * 256, s_off, s_base + gc * p.xs_rs);
+    };
+    const int frow = lane & 15, part = lane >> 4;
+    const int fsw = (part ^ ((frow >> 1) & 7)) << 4, aoff = (wm * 128 + frow) * kGroup + fsw, woff = (wn * 64 + frow) * kGroup + fsw;
+    // (waves whose columns lie behind N take any block's scales)
+    const float* const ws = p.ws + (int64_t)min((n0 + wn * 64) / kGroup, (p.N - 1) / kGroup) * p.groups;
+
+    v4f sums[2][FN], acc[FN][FM];      // a group's sums of a row tile and of the one before
+    float s[2];
+#pragma unroll
+    for (int in = 0; in < FN; ++in) {
+        sums[1][in] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int im = 0; im < FM; ++im) acc[in][im] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    s[1] = 0.f;
+    const auto fold = [&](int buf, int in, int im) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[in][im][c] = fmaf(sums[buf][in][c], s[buf], acc[in][im][c]);
+    };
+    // No branch inside: the compiler would move the folds behind it.
+    const auto loop = [&](auto fetches_tag) {
+        constexpr bool fetches = decltype(fetches_tag)::value;
+        if constexpr (fetches) {
+#pragma unroll
+            for (int j = 0; j < NDMA; ++j) dma(0, j);
+            wait_vmcnt<0>();
+        }
+        __syncthreads();
+        for (int g = 0; g < full; ++g) {
+            const uint8_t *sa = smem + (g & 1) * BIG_STAGE, *sw = smem + (2 + (g & 1)) * BIG_STAGE;
+            const float* const sx = reinterpret_cast<const float*>(smem + BIG_S + (g & 1) * (BIG * 4)) + wm * 128 + frow;
+            const float wg = ws[g];
+            v8i fw[FN], fa[2];
+            const auto read = [&](const uint8_t* from, int off) { return two(*reinterpret_cast<const v4i*>(from + off), *reinterpret_cast<const v4i*>(from + (off ^ 64))); };
+            fa[0] = read(sa, aoff);
+#pragma unroll
+            for (int in = 0; in < FN; ++in) fw[in] = read(sw, woff + in * 16 * kGroup);
+            SCHED_FENCE();
+#pragma unroll
+            for (int in = 0; in < FN; ++in) fold(1, in, FM - 1);      // the last row tile of the group before, under the first reads of this one
+            SCHED_FENCE();
+#pragma unroll
+            for (int im = 0; im < FM; ++im) {
+                if (im + 1 < FM) fa[(im + 1) & 1] = read(sa, aoff + (im + 1) * 16 * kGroup);
+                s[im & 1] = sx[16 * im] * wg;
+#pragma unroll
+                for (int in = 0; in < FN; ++in) sums[im & 1][in] = mfma(fw[in], fa[im & 1], v4f{0.f, 0.f, 0.f, 0.f});
+                SCHED_FENCE();
+#pragma unroll
+                for (int in = 0; in < FN; ++in) {
+                    const int j = im * 3 + in;
+                    if (im > 0) fold((im - 1) & 1, in, im - 1);
+                    SCHED_FENCE();
+                    if (fetches && in < 3 && j < NDMA) dma(g + 1, j);      // the stage last read before the previous barrier
+                    SCHED_FENCE();
+                }
+            }
+            if constexpr (fetches) wait_vmcnt<0>();
+            __syncthreads();
+        }
+    };
+    if (wm == 0) loop(std::true_type{});
+    else loop(std::false_type{});
+#pragma unroll
+    for (int in = 0; in < FN; ++in) fold(1, in, FM - 1);
+    if (p.K > full * kGroup) {
+        const int k0 = full * kGroup, r = lane_now() & 15, c = lane_now() >> 4;
+        v8i fw[FN];
+#pragma unroll
+        for (int in = 0; in < FN; ++in) fw[in] = tail_fragment(p.W, n0 + wn * 64 + 16 * in + r, p.N, p.K, k0, c);
+#pragma unroll
+        for (int im = 0; im < FM; ++im) {
+            const int m = m0 + wm * 128 + 16 * im + r;
+            const v8i fa = tail_fragment(p.A, m, p.M, p.K, k0, c);
+            s[0] = p.xs[full * p.xs_rs + min(m, p.M - 1)] * ws[full];
+#pragma unroll
+            for (int in = 0; in < FN; ++in) sums[0][in] = mfma(fw[in], fa, v4f{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int in = 0; in < FN; ++in) fold(0, in, im);
+        }
+    }
+    // (the stages are idle; the lane number is taken anew so that the loop does not keep it)
+    store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * 128, n0 + wn * 64, lane_now());
+}
+
+template <int OUT_DT> int launch_big(Fp8Gemm p, hipStream_t st) {
+    const auto kern = fp8_gemm_big_kernel<OUT_DT>;
+    static PerDeviceOnce once;
+    if (const int e = allow_dynamic_lds((const void*)kern, BIG_LDS, once)) return e;
+    p.tiles_m = (p.M + BIG - 1) / BIG;
+    p.tiles_n = (p.N + BIG - 1) / BIG;
+    if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 512) return -1;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(512), BIG_LDS, st, p);
+    KCHECK();
+    return 0;
+}
+
 template <int OUT_DT> int launch(Fp8Gemm p, hipStream_t st) {
+    if constexpr (OUT_DT != DT_F32)
+        if (p.K >= kGroup && p.K < (1 << 23) && p.M >= 512 && p.N >= 512) return launch_big<OUT_DT>(p, st);
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = (p.N + 127) / 128;
     if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 256) return -1;

@@ -143,7 +143,7 @@ def _product(a, w, xs, ws, bias, dtype):
 
 
 GEMM = [(1, 1, 16), (1, 128, 128), (3, 5, 144), (16, 128, 256), (17, 130, 400), (64, 256, 1024), (5, 1000, 4096), (128, 128, 128), (129, 127, 2640), (100, 520, 1152), (256, 512, 2048),
-        (300, 264, 640), (1000, 1000, 384), (513, 777, 256)]
+        (300, 264, 640), (1000, 1000, 384), (513, 777, 256), (700, 600, 1168), (512, 1040, 128), (769, 520, 4224)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=name)
