@@ -31,7 +31,15 @@ struct Fp8Gemm {
     int M, N, K, groups;
     int tiles_m, tiles_n;
     int rows_ok;      // rows of D start on 16 bytes
+    int slices;       // workgroups that share an output's K
+    float* planes;    // [slices][M][N] where those are several
 };
+// Groups g0 .. g1 of slice `s`.
+__device__ __forceinline__ void slice_of(int groups, int slices, int s, int& g0, int& g1) {
+    const int share = (groups + slices - 1) / slices;
+    g0 = min(groups, s * share);
+    g1 = min(groups, g0 + share);
+}
 
 // Both operands in the instruction's lane order: row lane % 16, and of its 128 bytes the 16-byte chunks lane / 16 and 4 + lane / 16.  (Which
 // k a lane holds does not matter as long as both operands agree.)
@@ -61,6 +69,16 @@ template <int OUT_DT> __device__ __forceinline__ void store_four(const Fp8Gemm& 
         for (int j = 0; j < 4; ++j)
             if (n + j < p.N) st_dt<OUT_DT>(p.D, at + j, v[j]);
     }
+}
+
+__device__ __forceinline__ void store_plane(const Fp8Gemm& p, int slice, int m, int n, v4f v) {
+    if (m >= p.M || n >= p.N) return;
+    float* const to = p.planes + ((int64_t)slice * p.M + m) * p.N + n;
+    if (p.N % 4 == 0) *reinterpret_cast<v4f*>(to) = v;
+    else
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) to[j] = v[j];
 }
 
 // Any sizes: tiles of 128 x 128, four waves of 64 x 64, a group at a time through registers into one of two LDS stages.
@@ -148,6 +166,26 @@ __device__ __forceinline__ void dma4(uint32_t lds_dst, uint32_t lane_off, const 
 }
 template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 __device__ __forceinline__ int lane_now() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
+// The scales of a column block's groups from g0 on, for loops that read LDS: a scalar load would have them wait for all of it, so a lane holds a
+// group's, of 64 and of the next 64.  (1024 x 4096 -> 4096 in tiles of 128 x 128: 39.9 us with a scalar load a group, 28.9 without.)
+struct BlockScales {
+    const float* from;
+    int lane, last, at = 0;      // the groups that there are; groups done
+    float now, next;
+    __device__ __forceinline__ BlockScales(const float* ws, int g0, int end, int lane_) : from(ws + g0), lane(lane_), last(end - g0 - 1) {
+        now = from[min(lane, last)];
+        next = from[min(lane + 64, last)];
+    }
+    __device__ __forceinline__ float take() {
+        const float s = u2f(__builtin_amdgcn_readlane(f2u(now), at & 63));
+        if ((++at & 63) == 0) {
+            now = next;
+            next = from[min(at + 64 + lane, last)];
+        }
+        return s;
+    }
+};
 
 // A wave's FM x FN tiles, first row mw, first column nb: rounded, passed 32 rows at a time through `wl`, LDS of its own (32 rows of its columns;
 // 16-byte chunks swizzled by row), and stored in whole row segments, 16 bytes a lane.
@@ -257,10 +295,11 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_big_kernel(const Fp8Gemm p) {
             wait_vmcnt<0>();
         }
         __syncthreads();
+        BlockScales scales(ws, 0, full, lane);
         for (int g = 0; g < full; ++g) {
             const uint8_t *sa = smem + (g & 1) * BIG_STAGE, *sw = smem + (2 + (g & 1)) * BIG_STAGE;
             const float* const sx = reinterpret_cast<const float*>(smem + BIG_S + (g & 1) * (BIG * 4)) + wm * 128 + frow;
-            const float wg = ws[g];
+            const float wg = scales.take();
             v8i fw[FN], fa[2];
             const auto read = [&](const uint8_t* from, int off) { return two(*reinterpret_cast<const v4i*>(from + off), *reinterpret_cast<const v4i*>(from + (off ^ 64))); };
             fa[0] = read(sa, aoff);
@@ -316,19 +355,353 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_big_kernel(const Fp8Gemm p) {
 
 template <int OUT_DT> int launch_big(Fp8Gemm p, hipStream_t st) {
     const auto kern = fp8_gemm_big_kernel<OUT_DT>;
-    static PerDeviceOnce once;
-    if (const int e = allow_dynamic_lds((const void*)kern, BIG_LDS, once)) return e;
     p.tiles_m = (p.M + BIG - 1) / BIG;
     p.tiles_n = (p.N + BIG - 1) / BIG;
     if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 512) return -1;
+    static PerDeviceOnce once;
+    if (const int e = allow_dynamic_lds((const void*)kern, BIG_LDS, once)) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(512), BIG_LDS, st, p);
     KCHECK();
     return 0;
 }
 
-template <int OUT_DT> int launch(Fp8Gemm p, hipStream_t st) {
-    if constexpr (OUT_DT != DT_F32)
-        if (p.K >= kGroup && p.K < (1 << 23) && p.M >= 512 && p.N >= 512) return launch_big<OUT_DT>(p, st);
+// Few tiles: 64 or 128 rows by 128 columns, four waves that multiply (2 x 2 of BM / 2 x 64) and four that do nothing but fetch, into a ring of LDS
+// stages; K in slices over workgroups where the tiles are fewer than CUs.  At the barrier before group g the groups up to g + 1 have landed, so
+// that the first fragments of the next group are read behind the last products of this one; the stage of group g - 1 is fetched into.
+template <int BM> struct Mid {
+    static constexpr int BN = 128, STAGE = (BM + BN) * kGroup, SCALES = 128 * 4, NS = BM == 128 ? 4 : 6, LDS = NS * (STAGE + SCALES);
+    static constexpr int FM = BM / 32, FN = 4, NDMA = (BM + BN) / 32 + 1;      // of a fetching wave and group
+};
+
+template <int BM, int OUT_DT>
+__global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
+    using C = Mid<BM>;
+    constexpr int FM = C::FM, FN = C::FN;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = p.tiles_m * p.tiles_n, slice = blockIdx.x / tiles;
+    int tm, tn;
+    tile_of_block((int)blockIdx.x - slice * tiles, tiles, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * C::BN;
+    int g0, g1;
+    slice_of(p.groups, p.slices, slice, g0, g1);
+    const bool tail = g1 == p.groups && g0 < g1 && p.K % kGroup != 0;
+    const int end = tail ? g1 - 1 : g1, n = end - g0;      // whole groups
+    const auto meet = [] {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (wave >= 4) {
+        if (n <= 0) return;      // (no barrier is waited for then)
+        // 8-row blocks w + 4 j, of A and then of W; the swizzle on the memory's side.  The scales of the rows 64 (w % 2) .., by two waves alike.
+        const int w = wave - 4;
+        const uint32_t lds_base = (uint32_t)(uintptr_t)smem, lrow = (uint32_t)lane >> 3, K = (uint32_t)p.K;
+        const uint32_t chunk = ((lane & 7) ^ (((w & 1) << 2) | (lrow >> 1))) * 16, drow = w * 8 + lrow;
+        const uint32_t w_last = (uint32_t)min(C::BN - 1, p.N - 1 - n0), a_last = (uint32_t)min(BM - 1, p.M - 1 - m0);
+        uint32_t off[C::NDMA - 1];
+#pragma unroll
+        for (int j = 0; j < C::NDMA - 1; ++j) off[j] = (j < BM / 32 ? min(drow + 32 * j, a_last) : min(drow + 32 * (j - BM / 32), w_last)) * K + chunk;
+        const uint32_t s_off = 4u * min((uint32_t)(64 * (w & 1) + lane), a_last);
+        const uint8_t *const a_base = p.A + (int64_t)m0 * p.K, *const w_base = p.W + (int64_t)n0 * p.K;
+        const float* const s_base = p.xs + m0;
+        int put = 0;
+        const auto fetch = [&](int g) {      // groups past the end fetch the last one again, which nothing reads
+            const int gc = g < end ? g : end - 1;
+            const uint32_t to = lds_base + put * C::STAGE + w * 1024;
+#pragma unroll
+            for (int j = 0; j < C::NDMA - 1; ++j) dma16(to + j * 4096, off[j], (j < BM / 32 ? a_base : w_base) + (int64_t)gc * kGroup);
+            dma4(lds_base + C::NS * C::STAGE + put * C::SCALES + (w & 1) * 256, s_off, s_base + gc * p.xs_rs);
+            put = put == C::NS - 1 ? 0 : put + 1;
+        };
+#pragma unroll
+        for (int i = 0; i < C::NS - 1; ++i) fetch(g0 + i);
+        for (int i = 0; i < n; ++i) {
+            wait_vmcnt<(C::NS - 3) * C::NDMA>();
+            meet();
+            if (i + 1 < n) fetch(g0 + i + C::NS - 1);
+        }
+        wait_vmcnt<0>();      // nothing may still be writing this workgroup's LDS when it retires, or is stored through
+        meet();
+        return;
+    }
+    const int wm = wave >> 1, wn = wave & 1, frow = lane & 15, part = lane >> 4;
+    const int fsw = (part ^ ((frow >> 1) & 7)) << 4, aoff = (wm * (BM / 2) + frow) * kGroup + fsw, woff = (BM + wn * 64 + frow) * kGroup + fsw;
+    const float* const ws = p.ws + (int64_t)tn * p.groups;
+    v4f acc[FN][FM], sums[2][FN];
+    float last = 0.f;      // the scale of the row tile that is not folded yet
+#pragma unroll
+    for (int in = 0; in < FN; ++in) {
+        sums[(FM - 1) & 1][in] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int im = 0; im < FM; ++im) acc[in][im] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    const auto fold = [&](int buf, int in, int im, float s) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[in][im][c] = fmaf(sums[buf][in][c], s, acc[in][im][c]);
+    };
+    struct First {      // what a group begins with
+        v8i w[FN], a;
+        float s[FM], ws;
+    };
+    BlockScales scales(ws, g0, n > 0 ? end : g0 + 1, lane);
+    int get = 0;
+    const auto read = [&](const uint8_t* at, int o) { return two(*reinterpret_cast<const v4i*>(at + o), *reinterpret_cast<const v4i*>(at + (o ^ 64))); };
+    const auto begin = [&](First& f) {      // of the stage `get`
+        const uint8_t* const at = smem + get * C::STAGE;
+        const float* const sx = reinterpret_cast<const float*>(smem + C::NS * C::STAGE + get * C::SCALES) + wm * (BM / 2) + frow;
+        f.a = read(at, aoff);
+#pragma unroll
+        for (int in = 0; in < FN; ++in) f.w[in] = read(at, woff + in * 16 * kGroup);
+#pragma unroll
+        for (int im = 0; im < FM; ++im) f.s[im] = sx[16 * im];
+    };
+    const auto group = [&](First& f, First& next) {
+        const uint8_t* const at = smem + get * C::STAGE;
+        get = get == C::NS - 1 ? 0 : get + 1;
+        v8i fa[2];
+        fa[0] = f.a;
+#pragma unroll
+        for (int im = 0; im < FM; ++im) {
+            if (im + 1 < FM) fa[(im + 1) & 1] = read(at, aoff + (im + 1) * 16 * kGroup);
+            else begin(next);
+            SCHED_FENCE();
+            const int done = im ? im - 1 : FM - 1;
+            const float s = im ? f.s[im - 1] * f.ws : last;
+            // the products of this row tile, and the fold of the one before between them
+#pragma unroll
+            for (int in = 0; in < FN; ++in) {
+                const v4f d = mfma(f.w[in], fa[im & 1], v4f{0.f, 0.f, 0.f, 0.f});
+                fold(done & 1, in, done, s);
+                sums[im & 1][in] = d;
+                SCHED_FENCE();
+            }
+        }
+        last = f.s[FM - 1] * f.ws;
+    };
+    static_assert(FM % 2 == 0, "row tiles alternate between two sets of sums");
+    if (n > 0) {
+        First f[2];
+        meet();
+        begin(f[0]);
+        f[0].ws = scales.take();
+        for (int g = g0; g < end; g += 2) {
+            f[1].ws = scales.take();      // (here and not among the products: it has a branch, behind which the compiler would move the folds)
+            group(f[0], f[1]);
+            meet();                       // (behind the last group: the fetching waves' last)
+            if (g + 1 >= end) break;
+            f[0].ws = scales.take();
+            group(f[1], f[0]);
+            meet();
+        }
+#pragma unroll
+        for (int in = 0; in < FN; ++in) fold((FM - 1) & 1, in, FM - 1, last);
+    }
+    if (tail) {
+        const int k0 = end * kGroup;
+        v8i fw[FN];
+#pragma unroll
+        for (int in = 0; in < FN; ++in) fw[in] = tail_fragment(p.W, n0 + wn * 64 + 16 * in + frow, p.N, p.K, k0, part);
+#pragma unroll
+        for (int im = 0; im < FM; ++im) {
+            const int m = m0 + wm * (BM / 2) + 16 * im + frow;
+            const v8i fa = tail_fragment(p.A, m, p.M, p.K, k0, part);
+            const float s = p.xs[end * p.xs_rs + min(m, p.M - 1)] * ws[end];
+#pragma unroll
+            for (int in = 0; in < FN; ++in) {
+                const v4f d = mfma(fw[in], fa, v4f{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[in][im][c] = fmaf(d[c], s, acc[in][im][c]);
+            }
+        }
+    }
+    if (p.slices > 1) {
+#pragma unroll
+        for (int in = 0; in < FN; ++in)
+#pragma unroll
+            for (int im = 0; im < FM; ++im) store_plane(p, slice, m0 + wm * (BM / 2) + 16 * im + frow, n0 + wn * 64 + 16 * in + 4 * part, acc[in][im]);
+    } else store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 64, lane);      // (the stages are idle)
+}
+
+// Few rows: the weights' way in is what counts.  They go from memory straight into the operand of the matrix instruction, as do the rows of A (from
+// the caches): eight waves on the same 16 MT rows and 16 CT columns, each with every eighth group of K, two on their way; the waves' sums meet in
+// LDS and are added in their order.
+template <int MT, int CT, int OUT_DT>
+__global__ void __launch_bounds__(512) fp8_gemm_few_kernel(const Fp8Gemm p) {
+    constexpr int TILES = MT * CT;
+    __shared__ __align__(16) float meet[8 * TILES * 256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = lane & 15, part = lane >> 4;
+    const int slice = blockIdx.x / p.tiles_n, n0 = (blockIdx.x - slice * p.tiles_n) * 16 * CT;
+    int g0, g1;
+    slice_of(p.groups, p.slices, slice, g0, g1);
+    const uint8_t *wp[CT], *ap[MT];
+    const float* sp[MT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) wp[c] = p.W + (int64_t)min(n0 + 16 * c + row, p.N - 1) * p.K + 16 * part;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) ap[m] = p.A + (int64_t)min(16 * m + row, p.M - 1) * p.K + 16 * part, sp[m] = p.xs + min(16 * m + row, p.M - 1);
+    const float* const ws = p.ws + (int64_t)(n0 / kGroup) * p.groups;
+    struct Group {
+        v8i w[CT], a[MT];
+        float s[MT], ws;
+    };
+    const auto load = [&](Group& x, int g) {
+        const int k0 = g * kGroup;
+        const auto at = [&](const uint8_t* q) {
+            if (k0 + kGroup <= p.K) return two(*reinterpret_cast<const v4i*>(q + k0), *reinterpret_cast<const v4i*>(q + k0 + 64));
+            v4i a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+            if (k0 + 16 * part < p.K) a = *reinterpret_cast<const v4i*>(q + k0);
+            if (k0 + 64 + 16 * part < p.K) b = *reinterpret_cast<const v4i*>(q + k0 + 64);
+            return two(a, b);
+        };
+#pragma unroll
+        for (int c = 0; c < CT; ++c) x.w[c] = at(wp[c]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) x.a[m] = at(ap[m]), x.s[m] = sp[m][g * p.xs_rs];
+        x.ws = ws[g];
+    };
+    v4f acc[CT][MT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[c][m] = v4f{0.f, 0.f, 0.f, 0.f};
+    const auto multiply = [&](const Group& x) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                v4f d = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (OUT_DT == DT_F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(x.w[c][e], x.w[c][e + 1]), widen(x.a[m][e], x.a[m][e + 1]), d, 0, 0, 0);
+                } else d = mfma(x.w[c], x.a[m], d);
+                const float s = x.s[m] * x.ws;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[c][m][e] = fmaf(d[e], s, acc[c][m][e]);
+            }
+    };
+    Group x[2];
+    int g = g0 + wave;
+    if (g < g1) load(x[0], g);
+    if (g + 8 < g1) load(x[1], g + 8);
+    for (; g < g1; g += 16) {
+        multiply(x[0]);
+        if (g + 16 < g1) load(x[0], g + 16);
+        if (g + 8 < g1) multiply(x[1]);
+        if (g + 24 < g1) load(x[1], g + 24);
+    }
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) *reinterpret_cast<v4f*>(meet + ((wave * CT + c) * MT + m) * 256 + 4 * lane) = acc[c][m];
+    __syncthreads();
+    for (int i = threadIdx.x; i < TILES * 64; i += 512) {      // four outputs of a row
+        const int tile = i >> 6, l = i & 63, m = 16 * (tile % MT) + (l & 15), n = n0 + 16 * (tile / MT) + 4 * (l >> 4);
+        v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 8; ++w) v += *reinterpret_cast<const v4f*>(meet + (w * TILES + tile) * 256 + 4 * l);
+        if (p.slices > 1) store_plane(p, slice, m, n, v);
+        else store_four<OUT_DT>(p, m, n, v);
+    }
+}
+
+// The planes of a K in slices, added in their order.
+template <int OUT_DT> __global__ void __launch_bounds__(256) fp8_gemm_join_kernel(const Fp8Gemm p) {
+    const int64_t size = (int64_t)p.M * p.N;
+    for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < size; i += 4 * 256 * (int64_t)gridDim.x) {
+        if (p.N % 4 == 0) {
+            v4f v = *reinterpret_cast<const v4f*>(p.planes + i);
+            for (int s = 1; s < p.slices; ++s) v += *reinterpret_cast<const v4f*>(p.planes + s * size + i);
+            const int m = (int)(i / p.N);
+            store_four<OUT_DT>(p, m, (int)(i - (int64_t)m * p.N), v);
+        } else
+            for (int e = 0; e < 4 && i + e < size; ++e) {
+                float v = p.planes[i + e];
+                for (int s = 1; s < p.slices; ++s) v += p.planes[s * size + i + e];
+                const int n = (int)((i + e) % p.N);
+                st_dt<OUT_DT>(p.D, i + e, p.bias ? v + ld_dt<OUT_DT>(p.bias, n) : v);
+            }
+    }
+}
+
+// How a call runs.
+enum Form { kAny, kBig, kMid128, kMid64, kFew };
+struct Plan {
+    int form, slices, ct;
+};
+std::atomic<int> g_force{-1};      // test hook: 100 * form + slices
+
+Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
+    const int64_t cus = device_cu_count(), groups = (K + kGroup - 1) / kGroup;
+    Plan p{kAny, 1, 1};
+    const bool fits = K >= kGroup && K < (1 << 23), half = out_dt != DT_F32;
+    const int force = g_force.load(std::memory_order_relaxed);
+    const auto at_most = [&](int64_t s) { return (int)(s < 1 ? 1 : s > groups ? groups : s > 32 ? 32 : s); };
+    if (force >= 0) {
+        p.form = force / 100;
+        p.slices = at_most(force % 100);
+        if (p.form == kFew && M > 32) p.form = kAny;
+        if ((p.form == kBig || p.form == kMid128 || p.form == kMid64) && !(fits && half)) p.form = kAny;
+        if (p.form == kAny || p.form == kBig) p.slices = 1;
+        if (p.form == kFew) p.ct = N > 16 * cus ? 2 : 1;
+        return p;
+    }
+    if (M <= 32) {
+        p.form = kFew;
+        p.ct = (N + 31) / 32 >= 2 * cus ? 2 : 1;
+        const int64_t tiles = (N + 16 * p.ct - 1) / (16 * p.ct);
+        p.slices = tiles >= cus ? 1 : at_most(groups / 16 < cus / tiles ? groups / 16 : cus / tiles);
+        return p;
+    }
+    if (!fits || !half) return p;
+    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), bm = M <= 64 ? 64 : 128, mid = ((M + bm - 1) / bm) * ((N + 127) / 128);
+    if (M >= 512 && N >= 512 && (big >= cus || mid > 2 * cus)) {
+        p.form = kBig;
+        return p;
+    }
+    p.form = bm == 64 ? kMid64 : kMid128;
+    p.slices = mid >= cus ? 1 : at_most(groups / 4 < cus / mid ? groups / 4 : cus / mid);
+    return p;
+}
+int64_t planes_of(const Plan& p, int64_t M, int64_t N) { return p.slices > 1 ? 4 * p.slices * M * N : 0; }
+
+template <int OUT_DT> int launch_join(const Fp8Gemm& p, hipStream_t st) {
+    const int64_t blocks = ((int64_t)p.M * p.N + 1023) / 1024, most = 8 * (int64_t)device_cu_count();
+    fp8_gemm_join_kernel<OUT_DT><<<(int)(blocks < most ? blocks : most), 256, 0, st>>>(p);
+    KCHECK();
+    return 0;
+}
+template <int BM, int OUT_DT> int launch_mid(Fp8Gemm p, hipStream_t st) {
+    const auto kern = fp8_gemm_mid_kernel<BM, OUT_DT>;
+    p.tiles_m = (p.M + BM - 1) / BM;
+    p.tiles_n = (p.N + 127) / 128;
+    const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.slices;
+    if (grid > 0xffffffffll / 512) return -1;
+    static PerDeviceOnce once;
+    if (const int e = allow_dynamic_lds((const void*)kern, Mid<BM>::LDS, once)) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), Mid<BM>::LDS, st, p);
+    KCHECK();
+    return p.slices > 1 ? launch_join<OUT_DT>(p, st) : 0;
+}
+template <int MT, int CT, int OUT_DT> int launch_few(Fp8Gemm p, hipStream_t st) {
+    p.tiles_n = (p.N + 16 * CT - 1) / (16 * CT);
+    const int64_t grid = (int64_t)p.tiles_n * p.slices;
+    if (grid > 0xffffffffll / 512) return -1;
+    fp8_gemm_few_kernel<MT, CT, OUT_DT><<<(int)grid, 512, 0, st>>>(p);
+    KCHECK();
+    return p.slices > 1 ? launch_join<OUT_DT>(p, st) : 0;
+}
+
+template <int OUT_DT> int launch(Fp8Gemm p, const Plan& plan, hipStream_t st) {
+    p.slices = plan.slices;
+    if (plan.form == kFew) {
+        if (p.M <= 16) return plan.ct == 2 ? launch_few<1, 2, OUT_DT>(p, st) : launch_few<1, 1, OUT_DT>(p, st);
+        return plan.ct == 2 ? launch_few<2, 2, OUT_DT>(p, st) : launch_few<2, 1, OUT_DT>(p, st);
+    }
+    if constexpr (OUT_DT != DT_F32) {
+        if (plan.form == kBig) return launch_big<OUT_DT>(p, st);
+        if (plan.form == kMid128) return launch_mid<128, OUT_DT>(p, st);
+        if (plan.form == kMid64) return launch_mid<64, OUT_DT>(p, st);
+    }
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = (p.N + 127) / 128;
     if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 256) return -1;
@@ -339,18 +712,37 @@ template <int OUT_DT> int launch(Fp8Gemm p, hipStream_t st) {
 
 }  // namespace
 
+GPU_API int64_t gpu_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int out_dt) {
+    if (M <= 0 || N <= 0 || K <= 0 || M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00) return 0;
+    return planes_of(plan_of(M, N, K, out_dt), M, N);
+}
+
 GPU_API int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_stride, const float* ws, const void* bias, void* D,
-                         int64_t M, int64_t N, int64_t K, int out_dt, void* stream) {
+                         void* work, int64_t M, int64_t N, int64_t K, int out_dt, void* stream) {
     if (out_dt != DT_BF16 && out_dt != DT_F16 && out_dt != DT_F32) return -4;
     if (M < 0 || N < 0 || K <= 0 || K % 16 != 0 || M > 0x7fffff00 || N > 0x7fffff00 || K > 0x7fffff00 || xs_stride < M) return -1;
     if (M == 0 || N == 0) return 0;
     const int size = out_dt == DT_F32 ? 4 : 2;
     if (!A || !W || !xs || !ws || !D || (uintptr_t)A % 16 != 0 || (uintptr_t)W % 16 != 0 || (uintptr_t)xs % 4 != 0 || (uintptr_t)ws % 4 != 0 || (uintptr_t)D % size != 0 ||
         (uintptr_t)bias % size != 0) return -1;
+    const Plan plan = plan_of(M, N, K, out_dt);
+    if (plan.slices > 1 && (!work || (uintptr_t)work % 16 != 0)) return -1;
     Fp8Gemm p{};
-    p.A = (const uint8_t*)A; p.W = (const uint8_t*)W; p.xs = xs; p.ws = ws; p.bias = bias; p.D = D; p.xs_rs = xs_stride;
+    p.A = (const uint8_t*)A; p.W = (const uint8_t*)W; p.xs = xs; p.ws = ws; p.bias = bias; p.D = D; p.xs_rs = xs_stride; p.planes = (float*)work;
     p.M = (int)M; p.N = (int)N; p.K = (int)K; p.groups = (int)((K + kGroup - 1) / kGroup);
     p.rows_ok = (uintptr_t)D % 16 == 0 && N * size % 16 == 0;
     const hipStream_t st = (hipStream_t)stream;
-    return out_dt == DT_BF16 ? launch<DT_BF16>(p, st) : out_dt == DT_F16 ? launch<DT_F16>(p, st) : launch<DT_F32>(p, st);
+    return out_dt == DT_BF16 ? launch<DT_BF16>(p, plan, st) : out_dt == DT_F16 ? launch<DT_F16>(p, plan, st) : launch<DT_F32>(p, plan, st);
+}
+
+GPU_API int gpu_internal_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dt, int32_t* out) {
+    if (M <= 0 || N <= 0 || K <= 0 || !out) return -1;
+    const Plan p = plan_of(M, N, K, out_dt);
+    out[0] = p.form;
+    out[1] = p.slices;
+    return 0;
+}
+GPU_API int gpu_internal_fp8_gemm_force(int form_and_slices) {
+    g_force.store(form_and_slices, std::memory_order_relaxed);
+    return 0;
 }

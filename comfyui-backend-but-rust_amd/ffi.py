@@ -59,7 +59,10 @@ SIGNATURES = {
     "gpu_kv8_attn_workspace": [_I32] * 7,
     "gpu_kv8_copy_pages": [_P, _P, _P, _P] + [_I32] * 5 + [_P, _P, _I32, _P],
     "gpu_fp8_quant_rows": [_I32, _I32, _P, _I64, _P, _I64, _P, _I64, _I64, _P, _F32, _P, _P, _I64, _I32, _I32, _P],
-    "gpu_fp8_gemm": [_P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _P],
+    "gpu_fp8_gemm": [_P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I32, _P],
+    "gpu_fp8_gemm_workspace": [_I64, _I64, _I64, _I32],
+    "gpu_internal_fp8_gemm_plan": [_I64, _I64, _I64, _I32, _P],
+    "gpu_internal_fp8_gemm_force": [_I32],
     "gpu_rope": [_I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _F32, _I32, _I32, _P],
     "gpu_prompt_attn": [_I32] + [_P, _I64, _I64] * 4 + [_P, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P],
     "gpu_internal_act_probe": [_I32, _P, _P, _I32, _P],
@@ -97,6 +100,7 @@ def _load():
     lib.gpu_w6a8_group_gemm_scratch.restype = _I64
     lib.gpu_cross_attn_workspace.restype = _I64
     lib.gpu_kv8_attn_workspace.restype = _I64
+    lib.gpu_fp8_gemm_workspace.restype = _I64
     lib.gpu_int8_gemm_static_limit.argtypes = []
     lib.gpu_int8_gemm_static_limit.restype = _I64
     lib.gpu_kernels_build_info.restype = C.c_char_p

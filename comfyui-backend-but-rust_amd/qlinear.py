@@ -511,5 +511,7 @@ def fp8_gemm(A, W, xs, ws, bias=None, out_dtype=torch.bfloat16, D=None):
                 raise ValueError("%s must be on A's device, got %s and %s" % (what, t.device, A.device))
             _no_grad(t, what)
     with _on(A.device) as s:
-        ffi.k("gpu_fp8_gemm", _ptr(A), _ptr(W), _ptr(xs), xs.stride(0) if G > 1 else M, _ptr(ws), _ptr(bias), _ptr(D), M, N, K, _TORCH_DT[out_dtype], s)
+        need = ffi.lib.gpu_fp8_gemm_workspace(M, N, K, _TORCH_DT[out_dtype])
+        work = torch.empty((need,), dtype=torch.uint8, device=A.device) if need else None
+        ffi.k("gpu_fp8_gemm", _ptr(A), _ptr(W), _ptr(xs), xs.stride(0) if G > 1 else M, _ptr(ws), _ptr(bias), _ptr(D), _ptr(work), M, N, K, _TORCH_DT[out_dtype], s)
     return D

@@ -384,9 +384,11 @@ int gpu_fp8_quant_rows(int dtype, int prologue, const void* x, int64_t x_stride,
  * K-contiguous, 16-byte aligned; groups of 128 along K; xs f32 [groups, xs_stride], ws f32 [ceil(N / 128), groups]; the last group and
  * the last block of rows of W may be parts.  bias Out[N] or null.  Out by out_dt (-4).  K a multiple of 16 (-1).  Sums in fp32, but that for 16-bit
  * outputs the matrix instruction cuts the products of each eight k off at 2^-13 of the largest one's power of two (1.5e-5 of the result on normally
- * distributed operands). */
-int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_stride, const float* ws, const void* bias, void* D, int64_t M,
-                 int64_t N, int64_t K, int out_dt, void* stream);
+ * distributed operands).  work: gpu_fp8_gemm_workspace bytes (0: null will do), 16-byte aligned (-1), in use until the work queued here has
+ * run.  A call gives the same bits every time. */
+int64_t gpu_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int out_dt);
+int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_stride, const float* ws, const void* bias, void* D, void* work,
+                 int64_t M, int64_t N, int64_t K, int out_dt, void* stream);
 
 /* Rotary positions.  Of every head of q [T, h, d] and k [T, hk, d] (dtype bf16, f16 or f32, else -4; element strides of tokens and heads, dense
  * last axis) the first `rot` channels are pairs, (j, j + rot / 2) or, interleaved, (2j, 2j + 1); pair j of token t turns by the angle
@@ -407,6 +409,12 @@ int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, 
 int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
                     int64_t v_rs, int64_t v_hs, void* o, int64_t o_rs, int64_t o_hs, const int32_t* starts, int n, int tokens, int h, int hk,
                     int head_dim, float scale, int causal, void* stream);
+
+/* Test hooks, no reference counterpart: how gpu_fp8_gemm runs a size, out[0] = form (0 any size, 1 tiles of 256 x 256, 2 of 128 x 128 and 3 of
+ * 64 x 128 with K in slices, 4 up to 32 rows), out[1] = slices of K; and a form forced on the calls of the process, 100 * form + slices
+ * (-1: by the sizes; 0 where the form does not take the size).  The workspace follows. */
+int gpu_internal_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dt, int32_t* out);
+int gpu_internal_fp8_gemm_force(int form_and_slices);
 
 /* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times
  * key-value heads) of `rows` (query tokens times query heads of a key-value head, the most of any) over `keys`: out[0] = rows of a workgroup (16 and 32:

@@ -107,7 +107,8 @@ extern "C" {
     pub fn gpu_fp8_quant_rows(dtype: i32, prologue: i32, x: P, x_stride: i64, resid: P, resid_stride: i64, sum: PM,
         sum_stride: i64, up_offset: i64, norm_w: P, eps: f32, q: PM, scales: PM, scales_stride: i64, m: i32,
         k: i32, stream: PM) -> i32;
-    pub fn gpu_fp8_gemm(a: P, w: P, xs: P, xs_stride: i64, ws: P, bias: P, d: PM, m: i64, n: i64, k: i64,
+    pub fn gpu_fp8_gemm_workspace(m: i64, n: i64, k: i64, out_dt: i32) -> i64;
+    pub fn gpu_fp8_gemm(a: P, w: P, xs: P, xs_stride: i64, ws: P, bias: P, d: PM, work: PM, m: i64, n: i64, k: i64,
         out_dt: i32, stream: PM) -> i32;
     pub fn gpu_rope(dtype: i32, q: P, q_rs: i64, q_hs: i64, q_out: PM, qo_rs: i64, qo_hs: i64, h: i32, k: P,
         k_rs: i64, k_hs: i64, k_out: PM, ko_rs: i64, ko_hs: i64, hk: i32, positions: P, freqs: P, rot: i32,
@@ -115,6 +116,8 @@ extern "C" {
     pub fn gpu_prompt_attn(dtype: i32, q: P, q_rs: i64, q_hs: i64, k: P, k_rs: i64, k_hs: i64, v: P, v_rs: i64,
         v_hs: i64, o: PM, o_rs: i64, o_hs: i64, starts: P, n: i32, tokens: i32, h: i32, hk: i32, head_dim: i32,
         scale: f32, causal: i32, stream: PM) -> i32;
+    pub fn gpu_internal_fp8_gemm_plan(m: i64, n: i64, k: i64, out_dt: i32, out: PM) -> i32;
+    pub fn gpu_internal_fp8_gemm_force(form_and_slices: i32) -> i32;
     pub fn gpu_internal_states_plan(rows: i64, problems: i64, keys: i64, head_dim: i32, bytes: i32, out: PM) -> i32;
     pub fn gpu_int8_gemm_force_config(cfg: i32) -> i32;
     pub fn gpu_internal_int8_gemm_plan(m: i64, n: i64, k: i64, start: i32, aligned: i32, out: PM) -> i32;

@@ -156,6 +156,25 @@ def test_fp8_gemm(M, N, K, dtype):
         _check(ql.fp8_gemm(a, w, xs, ws, b, dtype), want, bound, "bias" if b is not None else "plain")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=name)
+@pytest.mark.parametrize("form,slices,sizes", [(0, 1, (40, 200, 1040)), (1, 1, (300, 260, 1040)), (1, 1, (20, 30, 128)), (2, 1, (130, 260, 640)), (2, 3, (200, 130, 1296)), (2, 7, (1, 1, 1024)),
+                                               (3, 1, (65, 129, 640)), (3, 2, (64, 128, 400)), (3, 31, (50, 200, 4096)), (4, 1, (31, 70, 1040)), (4, 3, (16, 200, 4112)), (4, 2, (2, 4500, 144)),
+                                               (4, 2, (17, 4500, 400))])
+def test_every_form_of_fp8_gemm(form, slices, sizes, dtype):
+    """Forced on sizes of any kind; where a form does not take a size, the one for any size runs."""
+    ql, ffi = pkg("qlinear"), pkg("ffi")
+    a, w, xs, ws, bias = _operands(*sizes, dtype, 70)
+    want, bound = _product(a, w, xs, ws, bias, dtype)
+    ffi.k("gpu_internal_fp8_gemm_force", 100 * form + slices)
+    try:
+        got = ql.fp8_gemm(a, w, xs, ws, bias, dtype)
+        again = ql.fp8_gemm(a, w, xs, ws, bias, dtype)
+    finally:
+        ffi.k("gpu_internal_fp8_gemm_force", -1)
+    _check(got, want, bound, "form %d" % form)
+    assert torch.equal(got, again)
+
+
 def test_fp8_gemm_layouts_and_odd_values():
     """Scales further apart than they are many, outputs at any address; codes and scales that are no numbers reach their rows and columns only."""
     ql = pkg("qlinear")

@@ -24,14 +24,14 @@ def test_quant_rows_refusals(args, code):
     assert _rows(**args) == code
 
 
-def _gemm(A=P, W=P, xs=P, stride=8, ws=P, bias=0, D=P, M=8, N=8, K=256, dt=2):
-    return ffi.raw("gpu_fp8_gemm", A, W, xs, stride, ws, bias, D, M, N, K, dt, 0)
+def _gemm(A=P, W=P, xs=P, stride=8, ws=P, bias=0, D=P, work=P, M=8, N=8, K=256, dt=2):
+    return ffi.raw("gpu_fp8_gemm", A, W, xs, stride, ws, bias, D, work, M, N, K, dt, 0)
 
 
 @pytest.mark.parametrize("args,code", [({"dt": 3}, -4), ({"dt": -1}, -4), ({"M": -1}, -1), ({"N": -1}, -1), ({"K": 0}, -1), ({"K": 8}, -1), ({"K": 40}, -1), ({"stride": 7}, -1), ({"A": 0}, -1), ({"W": 0}, -1),
                                        ({"xs": 0}, -1), ({"ws": 0}, -1), ({"D": 0}, -1), ({"A": P + 8}, -1), ({"W": P + 4}, -1), ({"xs": P + 2}, -1), ({"ws": P + 1}, -1), ({"D": P + 1}, -1),
                                        ({"D": P + 2, "dt": 0}, -1), ({"bias": P + 1}, -1), ({"M": 1 << 31, "stride": 1 << 31}, -1), ({"N": 1 << 31}, -1), ({"M": 1 << 30, "stride": 1 << 30, "N": 1 << 20}, -1),
-                                       ({"M": 0}, 0), ({"N": 0}, 0)])
+                                       ({"K": 8192, "work": 0}, -1), ({"K": 8192, "work": P + 8}, -1), ({"M": 0}, 0), ({"N": 0}, 0)])
 def test_gemm_refusals(args, code):
     assert _gemm(**args) == code
 
