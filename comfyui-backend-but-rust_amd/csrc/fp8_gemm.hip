@@ -51,6 +51,15 @@ __device__ __forceinline__ v8h widen(int lo, int hi) {
     return __builtin_bit_cast(v8h, v4i{(int)pair(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)), (int)pair(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
                                        (int)pair(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)), (int)pair(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))});
 }
+// A group's sums for outputs of a type.
+template <int OUT_DT> __device__ __forceinline__ v4f product(v8i w, v8i a) {
+    v4f d = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (OUT_DT == DT_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(w[e], w[e + 1]), widen(a[e], a[e + 1]), d, 0, 0, 0);
+        return d;
+    } else return mfma(w, a, d);
+}
 // Chunk c of row r at slot c ^ ((r >> 1) & 7): 16 rows at one chunk lie on 16 of the 64 banks' 16-byte groups.
 __device__ __forceinline__ int place(int row, int chunk) { return row * kGroup + ((chunk ^ ((row >> 1) & 7)) << 4); }
 
@@ -138,11 +147,7 @@ __global__ void __launch_bounds__(256, 2) fp8_gemm_kernel(const Fp8Gemm p) {
             const v8i fw = fragment(sw, wn + 16 * j + row);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                v4f d = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (OUT_DT == DT_F32) {
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(fw[e], fw[e + 1]), widen(fa[i][e], fa[i][e + 1]), d, 0, 0, 0);
-                } else d = mfma(fw, fa[i], d);
+                const v4f d = product<OUT_DT>(fw, fa[i]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(d[e], s[i], acc[i][j][e]);
             }
@@ -459,6 +464,7 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
         const uint8_t* const at = smem + get * C::STAGE;
         get = get == C::NS - 1 ? 0 : get + 1;
         v8i fa[2];
+        v8h wide[FN][4];      // (32-bit outputs)
         fa[0] = f.a;
 #pragma unroll
         for (int im = 0; im < FM; ++im) {
@@ -468,6 +474,24 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
             const int done = im ? im - 1 : FM - 1;
             const float s = im ? f.s[im - 1] * f.ws : last;
             // the products of this row tile, and the fold of the one before between them
+            if constexpr (OUT_DT == DT_F32) {
+                v4f d[FN];
+#pragma unroll
+                for (int in = 0; in < FN; ++in) d[in] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const v8h a = widen(fa[im & 1][2 * e], fa[im & 1][2 * e + 1]);
+#pragma unroll
+                    for (int in = 0; in < FN; ++in) {
+                        if (im == 0) wide[in][e] = widen(f.w[in][2 * e], f.w[in][2 * e + 1]);
+                        d[in] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wide[in][e], a, d[in], 0, 0, 0);
+                        if (e == 3) fold(done & 1, in, done, s);
+                    }
+                }
+#pragma unroll
+                for (int in = 0; in < FN; ++in) sums[im & 1][in] = d[in];
+                SCHED_FENCE();
+            } else
 #pragma unroll
             for (int in = 0; in < FN; ++in) {
                 const v4f d = mfma(f.w[in], fa[im & 1], v4f{0.f, 0.f, 0.f, 0.f});
@@ -508,18 +532,22 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
             const float s = p.xs[end * p.xs_rs + min(m, p.M - 1)] * ws[end];
 #pragma unroll
             for (int in = 0; in < FN; ++in) {
-                const v4f d = mfma(fw[in], fa, v4f{0.f, 0.f, 0.f, 0.f});
+                const v4f d = product<OUT_DT>(fw[in], fa);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[in][im][c] = fmaf(d[c], s, acc[in][im][c]);
             }
         }
     }
-    if (p.slices > 1) {
+    if (p.slices > 1 || OUT_DT == DT_F32) {      // (16 bytes a lane, 64 in a row)
 #pragma unroll
         for (int in = 0; in < FN; ++in)
 #pragma unroll
-            for (int im = 0; im < FM; ++im) store_plane(p, slice, m0 + wm * (BM / 2) + 16 * im + frow, n0 + wn * 64 + 16 * in + 4 * part, acc[in][im]);
-    } else store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 64, lane);      // (the stages are idle)
+            for (int im = 0; im < FM; ++im) {
+                const int m = m0 + wm * (BM / 2) + 16 * im + frow, n = n0 + wn * 64 + 16 * in + 4 * part;
+                if (p.slices > 1) store_plane(p, slice, m, n, acc[in][im]);
+                else store_four<OUT_DT>(p, m, n, acc[in][im]);
+            }
+    } else if constexpr (OUT_DT != DT_F32) store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 64, lane);      // (the stages are idle)
 }
 
 // Few rows: the weights' way in is what counts.  They go from memory straight into the operand of the matrix instruction, as do the rows of A (from
@@ -569,11 +597,7 @@ __global__ void __launch_bounds__(512) fp8_gemm_few_kernel(const Fp8Gemm p) {
         for (int c = 0; c < CT; ++c)
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                v4f d = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (OUT_DT == DT_F32) {
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(x.w[c][e], x.w[c][e + 1]), widen(x.a[m][e], x.a[m][e + 1]), d, 0, 0, 0);
-                } else d = mfma(x.w[c], x.a[m], d);
+                const v4f d = product<OUT_DT>(x.w[c], x.a[m]);
                 const float s = x.s[m] * x.ws;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[c][m][e] = fmaf(d[e], s, acc[c][m][e]);
@@ -630,36 +654,56 @@ struct Plan {
 };
 std::atomic<int> g_force{-1};      // test hook: 100 * form + slices
 
+// Slices of a few rows' K where there are fewer workgroups than CUs: the eight waves of one share 24 groups at least, or the joining costs more than
+// it saves (16 x 4096 -> 1024: 6.3 us in one slice, 6.9 in two; 8 x 12288 -> 512: 11.2 in one, 7.6 in four).  Two column tiles a wave where that
+// leaves two workgroups a CU.
+// Else the smallest sum of rounds of one workgroup a CU, in us: a fixed time, and one for every group of 128, which grows from `alone` with the share of
+// the CUs that are busy (the caches' and the memory's rates) to `full`; slices are joined for 3 us, 0.35 for each, and their planes' way out and
+// in.  Fitted to 117 sizes of 33 to 3000 rows in up to 14 forms each, weights from memory: 0.25 % slower than the best of them in the mean, 7 % at most.
+// 64 rows: 4.2 + 0.36 .. 0.45 (64 x 4096 -> 24576 29 us), 128 rows: 4.5 + 0.50 .. 0.62 (1024 x 4096 -> 4096 24 us; 35 with 64 rows), 256 x 256: 6 + 1.3 ..
+// 1.65 (2048 x 4096 -> 24576 185 us; 270 with 128 rows).  32-bit outputs take tiles of 64 rows, whose fragments leave room for the
+// weights as f16 (1111 x 2640 -> 1000 20 us, 42 in the form for any size), and that form where it has two tiles of its 128 rows a CU (2048 x 4096 ->
+// 4096 87 us, 99).
 Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
     const int64_t cus = device_cu_count(), groups = (K + kGroup - 1) / kGroup;
-    Plan p{kAny, 1, 1};
-    const bool fits = K >= kGroup && K < (1 << 23), half = out_dt != DT_F32;
-    const int force = g_force.load(std::memory_order_relaxed);
+    Plan p{kAny, 1, (N + 31) / 32 >= 2 * cus ? 2 : 1};
+    const bool fits = K >= kGroup && K < (1 << 23);
     const auto at_most = [&](int64_t s) { return (int)(s < 1 ? 1 : s > groups ? groups : s > 32 ? 32 : s); };
+    const int force = g_force.load(std::memory_order_relaxed);
     if (force >= 0) {
         p.form = force / 100;
         p.slices = at_most(force % 100);
-        if (p.form == kFew && M > 32) p.form = kAny;
-        if ((p.form == kBig || p.form == kMid128 || p.form == kMid64) && !(fits && half)) p.form = kAny;
+        if ((p.form == kFew && M > 32) || (p.form != kFew && !fits) || ((p.form == kBig || p.form == kMid128) && out_dt == DT_F32)) p.form = kAny;
         if (p.form == kAny || p.form == kBig) p.slices = 1;
-        if (p.form == kFew) p.ct = N > 16 * cus ? 2 : 1;
         return p;
     }
     if (M <= 32) {
-        p.form = kFew;
-        p.ct = (N + 31) / 32 >= 2 * cus ? 2 : 1;
         const int64_t tiles = (N + 16 * p.ct - 1) / (16 * p.ct);
-        p.slices = tiles >= cus ? 1 : at_most(groups / 16 < cus / tiles ? groups / 16 : cus / tiles);
+        p.form = kFew;
+        p.slices = at_most(groups / 24 < cus / tiles ? groups / 24 : cus / tiles);
         return p;
     }
-    if (!fits || !half) return p;
-    const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), bm = M <= 64 ? 64 : 128, mid = ((M + bm - 1) / bm) * ((N + 127) / 128);
-    if (M >= 512 && N >= 512 && (big >= cus || mid > 2 * cus)) {
-        p.form = kBig;
-        return p;
+    if (!fits || (out_dt == DT_F32 && ((M + 127) / 128) * ((N + 127) / 128) >= 2 * cus)) return p;
+    static const struct {
+        Form form;
+        int bm, bn;
+        double start, alone, full;
+    } forms[] = {{kMid64, 64, 128, 4.2, 0.36, 0.45}, {kMid128, 128, 128, 4.5, 0.50, 0.62}, {kBig, 256, 256, 6.0, 1.3, 1.65}};
+    double least = 0.;
+    for (const auto& f : forms) {
+        if (f.form != kMid64 && out_dt == DT_F32) break;
+        const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
+        for (int s = 1; s == 1 || (f.form != kBig && s <= at_most(groups) && tiles * s <= 2 * cus); ++s) {
+            const int64_t whole = tiles * s / cus, left = tiles * s % cus, steps = (groups + s - 1) / s;
+            const double us = whole * (f.start + f.full * steps) + (left ? f.start + (f.alone + (f.full - f.alone) * left / cus) * steps : 0.) +
+                              (s > 1 ? 3.0 + 0.35 * s + 1.44e-6 * s * M * N : 0.);
+            if (p.form == kAny || us < least) {
+                least = us;
+                p.form = f.form;
+                p.slices = s;
+            }
+        }
     }
-    p.form = bm == 64 ? kMid64 : kMid128;
-    p.slices = mid >= cus ? 1 : at_most(groups / 4 < cus / mid ? groups / 4 : cus / mid);
     return p;
 }
 int64_t planes_of(const Plan& p, int64_t M, int64_t N) { return p.slices > 1 ? 4 * p.slices * M * N : 0; }
@@ -697,10 +741,10 @@ template <int OUT_DT> int launch(Fp8Gemm p, const Plan& plan, hipStream_t st) {
         if (p.M <= 16) return plan.ct == 2 ? launch_few<1, 2, OUT_DT>(p, st) : launch_few<1, 1, OUT_DT>(p, st);
         return plan.ct == 2 ? launch_few<2, 2, OUT_DT>(p, st) : launch_few<2, 1, OUT_DT>(p, st);
     }
+    if (plan.form == kMid64) return launch_mid<64, OUT_DT>(p, st);
     if constexpr (OUT_DT != DT_F32) {
         if (plan.form == kBig) return launch_big<OUT_DT>(p, st);
         if (plan.form == kMid128) return launch_mid<128, OUT_DT>(p, st);
-        if (plan.form == kMid64) return launch_mid<64, OUT_DT>(p, st);
     }
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = (p.N + 127) / 128;
