@@ -75,7 +75,7 @@ def drop_calls():
 
 
 def build_calls():
-    """The Python calls that are native code (csrc/py_linear.cpp with py_states.hpp): host code only, against torch's headers and libgpu_kernels.so."""
+    """The Python calls that are native code (csrc/py_linear.cpp with py_states.hpp and py_prompt.hpp): host code only, against torch's headers and libgpu_kernels.so."""
     drop_calls()
     torch = _torch()
     if torch is None:

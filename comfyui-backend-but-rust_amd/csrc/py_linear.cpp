@@ -73,11 +73,13 @@ PyObject* linear_w8a8(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }  // namespace
 
 #include "py_states.hpp"
+#include "py_prompt.hpp"
 
 namespace {
 
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {CALL(linear_w8a8), CALL(cross_attn), CALL(kv8_attn), CALL(kv8_store), CALL(kv8_read), CALL(kv8_copy_pages), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {CALL(linear_w8a8), CALL(cross_attn), CALL(kv8_attn), CALL(kv8_store), CALL(kv8_read), CALL(kv8_copy_pages), CALL(fp8_quant_rows), CALL(fp8_gemm), CALL(rope),
+                         CALL(prompt_attn), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycalls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

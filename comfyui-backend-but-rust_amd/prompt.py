@@ -42,6 +42,12 @@ def rope(q, k, positions, freqs, interleaved=False, factor=1.0, q_norm=None, k_n
     or into out = (q_out, k_out), which may be q and k.  The first 2 * len(freqs) channels of each head turn, in pairs of both halves or,
     interleaved, of neighbours; freqs float64: radians a token (rope_freqs).  factor scales what turns.  q_norm, k_norm (float32 [d]): each head
     is RMS-normed with that weight and eps first.  Returns (q_out, k_out)."""
+    y = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.rope(q, k, positions, freqs, bool(interleaved), float(factor), q_norm, k_norm, float(eps))
+    return _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out) if y is None else y
+
+
+def _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out):
+    """The call in Python, here and below: what the native one leaves to it, and every refusal."""
     if q.dtype not in qlinear._TORCH_DT:
         raise ValueError("q must be bfloat16, float16 or float32, got %s" % q.dtype)
     _heads(q, None, None, "q", q)
@@ -81,6 +87,11 @@ def attn(q, k, v, starts, scale, causal=True, out=None):
     """softmax(scale * q k^T) v within each prompt: rows starts[s] .. starts[s + 1] (int32 [n + 1] on the device) of q [tokens, h, d] and k, v [tokens,
     hk, d] (bf16 or f16, any strides with a dense last axis, h a multiple of hk, d a multiple of 8 up to 256).  Causal: a row sees the keys up to
     its own.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`."""
+    o = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.prompt_attn(q, k, v, starts, float(scale), bool(causal))
+    return _attn(q, k, v, starts, scale, causal, out) if o is None else o
+
+
+def _attn(q, k, v, starts, scale, causal, out):
     if q.dtype not in _DT:
         raise ValueError("q must be float16 or bfloat16, got %s" % q.dtype)
     _heads(q, None, None, "q", q)

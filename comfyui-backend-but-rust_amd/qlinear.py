@@ -462,6 +462,12 @@ def fp8_quant_rows(x, prologue="plain", norm_w=None, eps=0.0, resid=None, out=No
     residual also the sum x + resid in x's type, (q, scales, sum).  x and resid: [M, K] bf16, f16 or f32, any row stride.  "rms": the rows are
     normed, with weight norm_w (float32 [K]) and eps; "swiglu": x is [M, 2K], silu of its first half times the second.  out: where the sum goes
     instead of a new tensor; it may be x or resid."""
+    y = None if _pycalls is None else _pycalls.fp8_quant_rows(x, _FP8_ROWS.get(prologue, -1), norm_w, float(eps), resid, out)
+    return _fp8_quant_rows(x, prologue, norm_w, eps, resid, out) if y is None else y
+
+
+def _fp8_quant_rows(x, prologue, norm_w, eps, resid, out):
+    """The call in Python, here and below: what the native one leaves to it, and every refusal."""
     if x.dim() != 2 or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1) or x.dtype not in _TORCH_DT:
         raise ValueError("x must be a 2-D bfloat16, float16 or float32 CUDA tensor with a dense last axis, got %s %s with strides %s" % (x.dtype, tuple(x.shape), x.stride()))
     if prologue not in _FP8_ROWS:
@@ -491,6 +497,11 @@ def fp8_quant_rows(x, prologue="plain", norm_w=None, eps=0.0, resid=None, out=No
 def fp8_gemm(A, W, xs, ws, bias=None, out_dtype=torch.bfloat16, D=None):
     """A . W^T of e4m3 operands with block scales: A [M, K] and xs float32 [ceil(K / 128), M] as fp8_quant_rows gives them, W [N, K] with ws
     float32 [ceil(N / 128), ceil(K / 128)], a scale for each block of 128 x 128; bias [N] in out_dtype."""
+    y = None if _pycalls is None else _pycalls.fp8_gemm(A, W, xs, ws, bias, out_dtype, D)
+    return _fp8_gemm(A, W, xs, ws, bias, out_dtype, D) if y is None else y
+
+
+def _fp8_gemm(A, W, xs, ws, bias, out_dtype, D):
     if A.dim() != 2 or W.dim() != 2 or A.shape[1] != W.shape[1]:
         raise ValueError("A [M,K] and W [N,K] must share K, got %s and %s" % (tuple(A.shape), tuple(W.shape)))
     M, K = A.shape
