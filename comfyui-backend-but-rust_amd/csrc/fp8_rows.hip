@@ -33,11 +33,13 @@ struct Fp8Rows {
 constexpr int kPiece = 8;           // columns of a lane at a time: 16 lanes to a group of 128
 constexpr float kLeastA = 0x1p-100f, kTop = 448.f;
 
-template <int DT> __device__ __forceinline__ void load_piece(const void* base, int64_t at, bool wide, float (&v)[kPiece]) {
+// PAST: rows that are read once and do not fit the last-level cache leave what is in it alone.
+template <bool PAST, class V> __device__ __forceinline__ V fetch(const V* p) { return PAST ? __builtin_nontemporal_load(p) : *p; }
+template <int DT, bool PAST> __device__ __forceinline__ void load_piece(const void* base, int64_t at, bool wide, float (&v)[kPiece]) {
     if constexpr (DT == DT_F32) {
         const float* const p = (const float*)base + at;
         if (wide) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+            const f32x4 a = fetch<PAST>(reinterpret_cast<const f32x4*>(p)), b = fetch<PAST>(reinterpret_cast<const f32x4*>(p + 4));
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
         } else {
@@ -47,7 +49,7 @@ template <int DT> __device__ __forceinline__ void load_piece(const void* base, i
     } else {
         const uint16_t* const p = (const uint16_t*)base + at;
         u32x4 w;
-        if (wide) w = *reinterpret_cast<const u32x4*>(p);
+        if (wide) w = fetch<PAST>(reinterpret_cast<const u32x4*>(p));
         else
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
@@ -104,13 +106,15 @@ __device__ __forceinline__ uint32_t row_max_u32(uint32_t v) {
     v = max(v, mv(v, std::integral_constant<int, 0x141>{}));
     return max(v, mv(v, std::integral_constant<int, 0x140>{}));
 }
-// e^-x by the hardware's exp2, off by x 2^-24 and a unit: far below half a step of a code.
+// x / (1 + e^-x) by the hardware's exp2 and reciprocal: off by three units of fp32 and |x| / 3, where half a step of a code is 2^20 of them.  (The rounding of
+// the exponent put back and a Newton step on the reciprocal make that one unit, and the kernel bound by its vector instructions: 4099 x
+// 12288 from f16 48.7 -> 56.4 us.)
 __device__ __forceinline__ float silu(float x) {
     return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896340736f));
 }
 
 // A row is a.wpr waves of C pieces a lane, piece i of lane l at columns 8 (64 (wave + wpr i) + l) ..; a workgroup has rows side by side.
-template <int DT, int PRO, int C>
+template <int DT, int PRO, int C, bool PAST>
 __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Rows a) {
     __shared__ float part[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -127,9 +131,9 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Rows a) {
 #pragma unroll
             for (int j = 0; j < kPiece; ++j) v[i][j] = 0.f;
             if (col >= a.K) continue;
-            load_piece<DT>(a.x, row * a.x_rs + col, a.wide & 1, v[i]);
-            if (PRO == PRO_SWIGLU) load_piece<DT>(a.x, row * a.x_rs + a.up_offset + col, a.wide & 8, up[i]);
-            if (PRO == PRO_RMS) load_piece<DT_F32>(a.norm_w, col, a.wide & 16, w[i]);
+            load_piece<DT, PAST>(a.x, row * a.x_rs + col, a.wide & 1, v[i]);
+            if (PRO == PRO_SWIGLU) load_piece<DT, PAST>(a.x, row * a.x_rs + a.up_offset + col, a.wide & 8, up[i]);
+            if (PRO == PRO_RMS) load_piece<DT_F32, false>(a.norm_w, col, a.wide & 16, w[i]);
         }
         if (PRO != PRO_SWIGLU && a.resid) {
 #pragma unroll
@@ -137,7 +141,7 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Rows a) {
                 const int col = kPiece * (64 * (part_of_row + a.wpr * i) + lane);
                 if (col >= a.K) continue;
                 float r[kPiece];
-                load_piece<DT>(a.resid, row * a.resid_rs + col, a.wide & 2, r);
+                load_piece<DT, PAST>(a.resid, row * a.resid_rs + col, a.wide & 2, r);
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) v[i][j] += r[j];
                 round_store<DT>(a.sum, row * a.sum_rs + col, a.wide & 4, v[i]);
@@ -192,21 +196,27 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Rows a) {
     }
 }
 
-template <int DT, int PRO> int launch(Fp8Rows a, hipStream_t st) {
-    // A wave where its pieces suffice, more waves where rows are few or long: a lane has up to four pieces (RMS up to eight, past 16384 columns)
+// A row's waves have a piece each up to 4096 columns, more of them beyond (RMS at 8192 x 4096, bf16, with a residual, 235 MB: 44.7 us, 5.25 TB/s, as
+// one large copy; 46.9 with two pieces, 49.0 with four).  Calls of 64 MB or more load past the caches: 8192 x 4096 44.7 us, 49.7 without, 16384 x
+// 1024 23.7 and 25.2; 1024 x 5120, which stay in the last-level cache, 11.5 and 11.0.
+template <int DT, int PRO, bool PAST> int launch(Fp8Rows a, hipStream_t st) {
     const int pieces = (a.K + 64 * kPiece - 1) / (64 * kPiece);      // of 512 columns
     int wpr = 1;
-    while (wpr < 8 && (pieces > 4 * wpr || (pieces > wpr && (int64_t)a.M * wpr < 4 * device_cu_count()))) wpr *= 2;
+    while (wpr < 8 && pieces > wpr) wpr *= 2;
     a.wpr = wpr;
     const int waves = wpr < 4 ? 4 : wpr, rows = waves / wpr, c = (pieces + wpr - 1) / wpr;
     if (((int64_t)a.M + rows - 1) / rows > 0xffffffffll / (64 * waves)) return -1;      // a launch has fewer than 2^32 threads
     const int grid = (int)(((int64_t)a.M + rows - 1) / rows);
-    if (c <= 1) fp8_rows_kernel<DT, PRO, 1><<<grid, 64 * waves, 0, st>>>(a);
-    else if (c <= 2) fp8_rows_kernel<DT, PRO, 2><<<grid, 64 * waves, 0, st>>>(a);
-    else if (c <= 4) fp8_rows_kernel<DT, PRO, 4><<<grid, 64 * waves, 0, st>>>(a);
-    else fp8_rows_kernel<DT, PRO, 8><<<grid, 64 * waves, 0, st>>>(a);
+    if (c <= 1) fp8_rows_kernel<DT, PRO, 1, PAST><<<grid, 64 * waves, 0, st>>>(a);
+    else if (c <= 2) fp8_rows_kernel<DT, PRO, 2, PAST><<<grid, 64 * waves, 0, st>>>(a);
+    else if (c <= 4) fp8_rows_kernel<DT, PRO, 4, PAST><<<grid, 64 * waves, 0, st>>>(a);
+    else fp8_rows_kernel<DT, PRO, 8, PAST><<<grid, 64 * waves, 0, st>>>(a);
     KCHECK();
     return 0;
+}
+template <int DT, int PRO> int launch(const Fp8Rows& a, hipStream_t st) {
+    const int64_t each = dt_size<DT>::value * (PRO == PRO_SWIGLU ? 2 : a.resid ? 3 : 1) + 1;
+    return each * a.M * a.K >= (int64_t)64 << 20 ? launch<DT, PRO, true>(a, st) : launch<DT, PRO, false>(a, st);
 }
 template <int DT> int launch_pro(int prologue, const Fp8Rows& a, hipStream_t st) {
     switch (prologue) {

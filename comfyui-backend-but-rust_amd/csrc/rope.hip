@@ -26,7 +26,7 @@ struct Rope {
 };
 
 // N consecutive elements, as one access where they lie on a multiple of their size (two of 16 bytes for eight floats).
-template <int DT, int N> __device__ __forceinline__ void load_n(const void* p, int64_t at, bool wide, float (&v)[N]) {
+template <int DT, int N, bool PAST> __device__ __forceinline__ void load_n(const void* p, int64_t at, bool wide, float (&v)[N]) {
     constexpr int WORDS = N * dt_size<DT>::value / 4;
     if (!wide) {
 #pragma unroll
@@ -39,7 +39,7 @@ template <int DT, int N> __device__ __forceinline__ void load_n(const void* p, i
     const piece* const src = reinterpret_cast<const piece*>((const char*)p + at * dt_size<DT>::value);
 #pragma unroll
     for (int i = 0; i < WORDS / PER; ++i) {
-        const piece x = src[i];
+        const piece x = PAST ? __builtin_nontemporal_load(src + i) : src[i];
 #pragma unroll
         for (int j = 0; j < PER; ++j) w[i * PER + j] = x[j];
     }
@@ -74,34 +74,47 @@ template <int DT, int N> __device__ __forceinline__ void store_n(void* p, int64_
 constexpr int kMostTokens = 4;
 
 // A lane has V pairs of a head at a time, or 2 V of the channels that stay; a head's lanes are a power of two side by side.
-template <int DT, int V, bool INTER, bool NORM>
+template <int DT, int V, bool INTER, bool NORM, bool PAST>
 __global__ __launch_bounds__(256) void rope_kernel(const Rope a) {
     __shared__ f32x2 turn[kMostTokens * 128];
     const int pairs = a.rot / 2, t0 = blockIdx.x * a.tokens, tokens = min(a.tokens, a.T - t0);
-    for (int i = threadIdx.x; i < tokens * pairs; i += 256) {
-        const int token = i / pairs;
-        const double at = (double)a.positions[t0 + token] * (a.freqs[i - token * pairs] * 0.15915494309189533577), left = at - rint(at);
+    const int turned = pairs / V, units = a.d / (2 * V), heads = a.h + a.hk;
+    const int lanes_log = units <= 1 ? 0 : 32 - __builtin_clz(units - 1), unit = threadIdx.x & ((1 << lanes_log) - 1), step = 256 >> lanes_log;
+    // The two pieces of V channels.  Halves: one in each half of what turns, or of the rest.  Neighbours, where a piece has its pairs whole: one in
+    // each half of the head, so that lanes side by side have whole lines.
+    const bool rotates = INTER ? true : unit < turned, some = unit < units;
+    const int c0 = INTER || rotates ? V * unit : a.rot + V * (unit - turned), c1 = c0 + (INTER ? a.d / 2 : rotates ? pairs : (a.d - a.rot) / 2);
+    const int end = tokens * heads;
+    const auto head_of = [&](int i, int& token, int& head) {      // -> whether it is one of q's
+        token = i / heads;
+        head = i - token * heads;
+        const bool is_q = head < a.h;
+        if (!is_q) head -= a.h;
+        return is_q;
+    };
+    float x[2][V];
+    const auto load = [&](int i) {
+        int token, head;
+        const Side& s = head_of(i, token, head) ? a.q : a.k;
+        const int64_t from = (t0 + token) * s.x_rs + head * s.x_hs;
+        if (!some) return;
+        load_n<DT, V, PAST>(s.x, from + c0, a.wide, x[0]);
+        load_n<DT, V, PAST>(s.x, from + c1, a.wide, x[1]);
+    };
+    int i = threadIdx.x >> lanes_log;
+    if (i < end) load(i);      // on its way while the sines are made
+    for (int j = threadIdx.x; j < tokens * pairs; j += 256) {
+        const int token = j / pairs;
+        const double at = (double)a.positions[t0 + token] * (a.freqs[j - token * pairs] * 0.15915494309189533577), left = at - rint(at);
         float s, c;
         sincospif(2.f * (float)left, &s, &c);
-        turn[i] = f32x2{a.factor * c, a.factor * s};
+        turn[j] = f32x2{a.factor * c, a.factor * s};
     }
     __syncthreads();
-    const int turned = pairs / V, units = turned + (a.d - a.rot) / (2 * V), heads = a.h + a.hk;
-    const int lanes_log = units <= 1 ? 0 : 32 - __builtin_clz(units - 1), unit = threadIdx.x & ((1 << lanes_log) - 1), step = 256 >> lanes_log;
-    for (int i = threadIdx.x >> lanes_log; i < tokens * heads; i += step) {
-        const int token = i / heads, h = i - token * heads;
-        const bool is_q = h < a.h;
-        const Side& s = is_q ? a.q : a.k;
-        const int head = is_q ? h : h - a.h;
-        const int64_t from = (t0 + token) * s.x_rs + head * s.x_hs, to = (t0 + token) * s.o_rs + head * s.o_hs;
-        const bool rotates = unit < turned, some = unit < units;
-        // the two pieces of V channels
-        const int c0 = rotates ? (INTER ? 2 * V * unit : V * unit) : a.rot + 2 * V * (unit - turned), c1 = rotates && !INTER ? c0 + pairs : c0 + V;
-        float x[2][V];
-        if (some) {
-            load_n<DT, V>(s.x, from + c0, a.wide, x[0]);
-            load_n<DT, V>(s.x, from + c1, a.wide, x[1]);
-        }
+    for (; i < end; i += step) {
+        int token, head;
+        const Side& s = head_of(i, token, head) ? a.q : a.k;
+        const int64_t to = (t0 + token) * s.o_rs + head * s.o_hs;
         if constexpr (NORM) {
             float sum = 0.f;
             if (some)
@@ -118,40 +131,58 @@ __global__ __launch_bounds__(256) void rope_kernel(const Rope a) {
                     for (int e = 0; e < V; ++e) x[j][e] = x[j][e] * r * s.norm[(j ? c1 : c0) + e];
             }
         }
+        float y[2][V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[0][e] = x[0][e], y[1][e] = x[1][e];
+        if (i + step < end) load(i + step);
         if (!some) continue;
         if (rotates) {
-            const f32x2* const cs = turn + token * pairs + V * unit;
+            const f32x2* const cs = turn + token * pairs;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const f32x2 t = cs[e];
-                float& p = INTER ? x[2 * e / V][2 * e % V] : x[0][e];
-                float& q = INTER ? x[(2 * e + 1) / V][(2 * e + 1) % V] : x[1][e];
+                const int half = INTER ? 2 * e / V : 0, k = INTER ? 2 * e % V : e;      // the pair's first channel
+                if (INTER && (half ? c1 : c0) >= a.rot) continue;
+                const f32x2 t = cs[INTER ? (half ? c1 : c0) / 2 + e % (V / 2) : c0 + e];
+                float& p = y[half][k];
+                float& q = INTER ? y[half][k + 1] : y[1][e];
                 const float u = fmaf(p, t[0], -(q * t[1]));
                 q = fmaf(p, t[1], q * t[0]);
                 p = u;
             }
         }
-        store_n<DT, V>(s.o, to + c0, a.wide, x[0]);
-        store_n<DT, V>(s.o, to + c1, a.wide, x[1]);
+        store_n<DT, V>(s.o, to + c0, a.wide, y[0]);
+        store_n<DT, V>(s.o, to + c1, a.wide, y[1]);
     }
 }
 
-template <int DT, int V> int launch(const Rope& a, bool interleaved, hipStream_t st) {
+template <int DT, int V, bool PAST> int launch_loads(const Rope& a, bool interleaved, hipStream_t st) {
     const int grid = (int)(((int64_t)a.T + a.tokens - 1) / a.tokens);
     const bool norm = a.q.norm || a.k.norm;
     if (interleaved) {
-        if (norm) rope_kernel<DT, V, true, true><<<grid, 256, 0, st>>>(a);
-        else rope_kernel<DT, V, true, false><<<grid, 256, 0, st>>>(a);
+        if (norm) rope_kernel<DT, V, true, true, PAST><<<grid, 256, 0, st>>>(a);
+        else rope_kernel<DT, V, true, false, PAST><<<grid, 256, 0, st>>>(a);
     } else {
-        if (norm) rope_kernel<DT, V, false, true><<<grid, 256, 0, st>>>(a);
-        else rope_kernel<DT, V, false, false><<<grid, 256, 0, st>>>(a);
+        if (norm) rope_kernel<DT, V, false, true, PAST><<<grid, 256, 0, st>>>(a);
+        else rope_kernel<DT, V, false, false, PAST><<<grid, 256, 0, st>>>(a);
     }
     KCHECK();
     return 0;
 }
+// Calls of 128 MB or more load past the caches (32768 tokens of 40 heads of 128: 131 us without, 124 with; 2048 tokens, which stay in the last-level
+// cache, 10.8 and 12.4).  A token to a workgroup, more where its heads do not fill one (16384 x 40 heads of 128: 75 us with one, 78 with four; 2048 tokens 10.7 and 12.7).
+template <int DT, int V> int launch(Rope a, bool interleaved, hipStream_t st) {
+    int lanes = 1;
+    while (lanes < a.d / (2 * V)) lanes *= 2;
+    const int fit = 256 / (lanes * (a.h + a.hk));
+    a.tokens = a.T < 4 * device_cu_count() || fit < 1 ? 1 : fit < kMostTokens ? fit : kMostTokens;
+    if (((int64_t)a.T + a.tokens - 1) / a.tokens > 0xffffffffll / 256) return -1;
+    const int64_t bytes = (int64_t)dt_size<DT>::value * 2 * a.T * (a.h + a.hk) * a.d;
+    return bytes >= (int64_t)128 << 20 ? launch_loads<DT, V, true>(a, interleaved, st) : launch_loads<DT, V, false>(a, interleaved, st);
+}
 template <int DT> int launch_width(Rope a, bool interleaved, hipStream_t st) {
     // the widest pieces that cut both parts of a head into whole ones
-    const int pairs = a.rot / 2, rest = a.d - a.rot, v = pairs % 8 == 0 && rest % 16 == 0 ? 8 : pairs % 4 == 0 && rest % 8 == 0 ? 4 : 2;
+    const auto cuts = [&](int v) { return interleaved ? a.d % (2 * v) == 0 && a.rot % v == 0 : a.rot % (2 * v) == 0 && (a.d - a.rot) % (2 * v) == 0; };
+    const int v = cuts(8) ? 8 : cuts(4) ? 4 : 2;
     const int size = dt_size<DT>::value, bytes = v * size < 16 ? v * size : 16;
     const auto on = [&](const Side& s) {
         return (uintptr_t)s.x % bytes == 0 && (uintptr_t)s.o % bytes == 0 && (s.x_rs * size) % bytes == 0 && (s.x_hs * size) % bytes == 0 && (s.o_rs * size) % bytes == 0 && (s.o_hs * size) % bytes == 0;
@@ -178,8 +209,6 @@ GPU_API int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void*
     a.k = {k, k_out, k_rs, k_hs, ko_rs, ko_hs, k_norm};
     a.positions = positions; a.freqs = freqs;
     a.T = T; a.h = h; a.hk = hk; a.d = head_dim; a.rot = rot; a.factor = factor; a.eps = eps;
-    a.tokens = T > 4 * device_cu_count() ? kMostTokens : 1;
-    if (((int64_t)T + a.tokens - 1) / a.tokens > 0xffffffffll / 256) return -1;
     const hipStream_t st = (hipStream_t)stream;
     return dtype == DT_BF16 ? launch_width<DT_BF16>(a, interleaved != 0, st) : dtype == DT_F16 ? launch_width<DT_F16>(a, interleaved != 0, st) : launch_width<DT_F32>(a, interleaved != 0, st);
 }

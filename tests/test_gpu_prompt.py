@@ -105,6 +105,14 @@ def test_quant_rows_in_place_unaligned_and_odd_values():
     q, s = ql.fp8_quant_rows(g, "swiglu")
     v = q.float() * s.t().repeat_interleave(128, 1)
     assert v[3, :128].isnan().all() and v[4, 128:].isnan().all() and abs(v[3, 130].item() - 0.7310586) < 0.05 and not v[0].any()
+    # gates at both ends
+    g = torch.zeros(1, 256, device=DEV)
+    g[0, :6], g[0, 128:] = torch.tensor([-1e5, -200.0, -88.0, 90.0, 3e38, -3e38], device=DEV), 1.0
+    q, s = ql.fp8_quant_rows(g, "swiglu")
+    assert q.float().isfinite().all() and q[0, 4].float() == 448 and s[0, 0] == torch.tensor(3e38) / 448
+    g[0, :6] = torch.tensor([-1e5, -200.0, -60.0, 20.0, -2.0, 0.5], device=DEV)
+    q, s = ql.fp8_quant_rows(g, "swiglu")
+    _rows_check(q, s, torch.nn.functional.silu(g[:, :128].double()), 70 * 2.0 ** -23, "gates")
     q, s = ql.fp8_quant_rows(torch.zeros(0, 64, device=DEV))
     assert q.shape == (0, 64) and s.shape == (1, 0)
 
