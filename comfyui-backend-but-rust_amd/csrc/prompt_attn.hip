@@ -125,6 +125,48 @@ __device__ __forceinline__ bool find(const PackedArgs& a, int group, int tile_ro
     return false;
 }
 
+// A wave's rows out, and NaN where a value that is no number counts: `found` says that some were taken out of the tiles from key first_edge on.
+template <class Src, int DP, class L_, class Stage>
+__device__ __forceinline__ void store_rows(const Common& a, const PackedArgs& sa, const Problem& pr, const L_& L, const Stage& st, int first_edge, bool found, int wr, int rows, int lane) {
+    const int g = lane >> 5;
+    // Channels of register j of block i: 32 i + key_of(j, g).
+    const int row = wr + (lane & 31), token = row / a.group, h = row - token * a.group;
+    uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + h * a.o_hs;
+    if (row < rows) {
+        const float inv = L.sum[0] == 0.f ? 0.f : 1.f / L.sum[0];
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; j += 8) {
+                if (32 * i + 2 * j >= a.d) continue;
+                uint32_t u[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = L.acc[0][i][j + 2 * e] * inv, y = L.acc[0][i][j + 2 * e + 1] * inv;
+                    u[e] = Src::DT == DT_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+                }
+                // of 16 channels a half wave has 0 .. 3 and 8 .. 11, or the others: each takes half from the other and has 8 in a row
+                const auto s0 = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
+                const u32x4 eight = {s0[0], s1[0], s0[1], s1[1]};
+                const int c = 32 * i + 2 * j + 8 * g;
+                if (c >= a.d) continue;
+                if (a.aligned & 2) *reinterpret_cast<u32x4*>(op + c) = eight;
+                else
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) op[c + e] = (uint16_t)(eight[e >> 1] >> 16 * (e & 1));
+            }
+    }
+    if (__syncthreads_or(found)) {
+        __threadfence();
+        if (row < rows)
+#pragma unroll 1
+            for (int key = first_edge; key < L.limit[0]; ++key)
+#pragma unroll 1
+                for (int c = g; c < a.d; c += 2)
+                    if (!(fabsf(elem(u32x4{st.v[key * st.v_rs + c], 0, 0, 0}, 0, Src::DT)) < INFINITY)) op[c] = 0x7fff;      // (NaN in both types)
+    }
+}
+
 // QW waves of 32 rows on the same keys, 32 NB at a time in two LDS buffers: a tile is on its way into registers while the one before goes into
 // LDS and the one before that is multiplied, SB blocks of 32 keys per step of the softmax.
 template <class Src, int DP, int QW, int NB, int SB, int OCC>
@@ -187,42 +229,239 @@ __global__ __launch_bounds__(64 * QW, OCC) void prompt_kernel(const Common a, co
     for (int t = t_mine; t < t1; ++t) next(t);      // tiles that only other waves' rows see (in a loop of its own: a branch around the products costs registers)
     L.finish(st, 0, end);
 
-    // Channels of register j of block i: 32 i + key_of(j, g).
-    const int row = wr + (lane & 31), token = row / a.group, h = row - token * a.group;
-    uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + h * a.o_hs;
-    if (row < rows) {
-        const float inv = L.sum[0] == 0.f ? 0.f : 1.f / L.sum[0];
+    store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, rows, lane);
+}
+
+// ---- head dims to 64 and to 128: products of the next tile under the softmax of this one -------------------------------------------
+
+__device__ __forceinline__ void dma16(uint32_t lds_dst, uint32_t lane_off, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_dst), "v"(lane_off), "s"(base) : "memory", "m0");
+}
+template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+template <int V> struct ic { static constexpr int value = V; };
+
+// A staged tile's rows are 2 DP bytes, one behind the other, as the DMA writes them; chunk c of 16 bytes of row r lies at slot c ^ turn(r).  K is read
+// 16 rows at one chunk at a time, V 8 rows at four chunks: both then touch every bank once.
+template <int DP> __device__ __forceinline__ int turn(int r) { return DP == 64 ? (r & 2) << 1 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3); }
+template <int DP> __device__ __forceinline__ int slot_of(int r, int c) { return r * 2 * DP + ((c ^ turn<DP>(r)) << 4); }
+
+// A workgroup's 8 waves of 32 rows, tiles of 64 keys.
+//
+// In iteration t a wave has the scores of tile t in registers.  Sixteen keys at a time it makes probabilities of them, and between those instructions run
+// the products of the sixteen keys before with V and a quarter of the next tile's scores: every slot of the matrix pipe's 8 products (256
+// cycles) has about as many cycles of vector instructions beside it.  K is a tile ahead of V.  Tiles travel by DMA into `NS` LDS stages.  That holds
+// for tiles that every row of the workgroup sees whole; the others, at the diagonal and at the prompt's end, follow in a loop that masks, with
+// their rows through registers, where values that are no numbers are taken out.
+template <class Src, int DP, int NS>
+__global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
+    constexpr int QW = 8, TK = 64, TILE = TK * 2 * DP, KS = DP / 16, DB = DP / 32, DT = Src::DT, ND = TILE / 1024 / QW;
+    static_assert(NS * TILE <= 65536, "a tensor's stages within the reach of a read's offset");
+    extern __shared__ __align__(16) uint8_t lds[];      // K's stages, then V's
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5, col = lane & 31;
+    const int slot = blockIdx.x / a.hk, head = blockIdx.x - slot * a.hk;
+    Place at;
+    if (!find(sa, a.group, 32 * QW, slot, at)) return;
+    Problem pr;
+    pr.q_at = at.first * a.q_rs + head * a.group * a.q_hs;
+    pr.o_at = at.first * a.o_rs + head * a.group * a.o_hs;
+    pr.tokens = pr.keys = at.count;
+    pr.limit0 = sa.causal ? 1 : at.count;
+    const int rows = pr.tokens * a.group, r0 = at.tile * 32 * QW, wr = r0 + 32 * wave;
+    const int end = min(pr.keys, pr.limit0 + (min(rows, r0 + 32 * QW) - 1) / a.group), t1 = (end + TK - 1) / TK;
+    const int edge = min(pr.keys, pr.limit0 + r0 / a.group) / TK;      // tiles before this one are seen whole by every row
+    const int sees = min(pr.keys, pr.limit0 + (min(rows, wr + 32) - 1) / a.group), t_mine = wr < rows ? (sees + TK - 1) / TK : 0;      // of this wave's rows
+    const int piped = DP == a.d && sa.aligned ? edge / NS * NS : 0;
+    const uint16_t *const k0 = sa.k + at.first * sa.k_rs + head * sa.k_hs, *const v0 = sa.v + at.first * sa.v_rs + head * sa.v_hs;
+    const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
+
+    // DMA: a kilobyte an instruction, rows RPI (wave + 8 j) .. of the tile
+    constexpr int CPR = DP / 8, RPI = 64 / CPR;
+    const int drow = RPI * wave + lane / CPR;
+    const uint32_t dchunk = 16 * ((lane % CPR) ^ turn<DP>(drow));      // (the same for j: 8 RPI is a multiple of 16)
+    const uint32_t k_off = 2 * drow * (int)sa.k_rs + dchunk, v_off = 2 * drow * (int)sa.v_rs + dchunk;
+    const auto fetch_k = [&](int t, auto stage) {
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
+        for (int j = 0; j < ND; ++j) dma16(lds_base + decltype(stage)::value * TILE + (wave + 8 * j) * 1024, k_off, k0 + (int64_t)(t * TK + 8 * RPI * j) * sa.k_rs);
+    };
+    const auto fetch_v = [&](int t, auto stage) {
 #pragma unroll
-            for (int j = 0; j < 16; j += 8) {
-                if (32 * i + 2 * j >= a.d) continue;
-                uint32_t u[4];
+        for (int j = 0; j < ND; ++j) dma16(lds_base + (NS + decltype(stage)::value) * TILE + (wave + 8 * j) * 1024, v_off, v0 + (int64_t)(t * TK + 8 * RPI * j) * sa.v_rs);
+    };
+    if (piped) {      // K of tiles 0 .. NS - 1, V of 0 .. NS - 2
+        fetch_k(0, ic<0>{});
+        fetch_v(0, ic<0>{});
+        if constexpr (NS > 2) {
+            fetch_k(1, ic<1>{});
+            fetch_v(1, ic<1>{});
+            fetch_k(2, ic<2>{});
+            fetch_v(2, ic<2>{});
+        }
+        fetch_k(NS - 1, ic<NS - 1>{});
+    }
+    Lanes<Src, DP, 1> L;
+    L.start(a, pr, wr, rows, lane);
+    const typename Src::Scales sc{};
+
+    // a lane's places in a stage: K row col, chunk 2 ks + g; V rows 16 h + 8 j + 4 g + r', its two chunks' half of block i
+    int at_k[KS], at_v[2][DB];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = L.acc[0][i][j + 2 * e] * inv, y = L.acc[0][i][j + 2 * e + 1] * inv;
-                    u[e] = Src::DT == DT_BF16 ? pack_bf16x2(x, y) : pack_f16x2(x, y);
+    for (int s = 0; s < KS; ++s) at_k[s] = slot_of<DP>(col, 2 * s + g);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+            at_v[j][i] = slot_of<DP>(8 * j + 4 * g + ((lane & 15) >> 2), 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+    const auto read_k = [&](int stage_at, int b, int s) { return *reinterpret_cast<const u32x4*>(lds + at_k[s] + stage_at + 32 * b * 2 * DP); };
+    const auto read_v = [&](int stage_at, int h, int i) {
+        u32x2 half[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            half[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds + at_v[j][i] + stage_at + 16 * h * 2 * DP)));
+        return u32x4{half[0][0], half[0][1], half[1][0], half[1][1]};
+    };
+    const auto meet = [] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (read: what was read from may be fetched into)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    const auto largest = [&](const f16acc& x) {
+        float m = fmaxf(x[0], x[1]);
+#pragma unroll
+        for (int i = 2; i < 16; i += 2) m = fmaxf(fmaxf(m, x[i]), x[i + 1]);
+        return m;
+    };
+    // the base moved where a row outgrew it; `top`: the row's largest score in this lane
+    const auto rebase = [&](float top) {
+        top = half_max(top) * L.c[0];
+        if (__any(top > L.base[0] + kLag)) {
+            const float nb = fmaxf(L.base[0], top);
+            const Rebase<Src> by(L.base[0], nb);
+            L.base[0] = nb;
+            L.sum[0] *= by.f;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) L.acc[0][i] *= by.f;
+        }
+    };
+    // probabilities of sixteen keys, rounded and in pairs, and their sum
+    const auto probs = [&](const f16acc (&s)[2], float from, int h, u32x4& p) {
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][8 * (h & 1) + i], L.c[0], -from));
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) p[i / 2] = pack2<DT>(e[i], e[i + 1]);
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part = add2<DT>(p[i], part);
+        L.sum[0] += part;
+    };
+
+    if (piped) {
+        wait_vmcnt<(NS - 2) * 2 * ND>();      // K and V of tile 0 at least
+        meet();
+        f16acc s[2][2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            s[0][b] = f16acc{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[0][b] = mfma<DT>(read_k(0, b, ks), L.qf[0][ks], s[0][b]);
+        }
+        rebase(fmaxf(largest(s[0][0]), largest(s[0][1])));
+        wait_vmcnt<(NS - 2) * 2 * ND>();
+        meet();
+        // tile t, whose number is `st` modulo NS: V of it and K of the next have landed
+        const auto tile = [&](int t, auto st_tag) {
+            constexpr int ST = decltype(st_tag)::value, KN = (ST + 1) % NS * TILE, VT = (NS + ST) * TILE;
+            // into the stages that were read last in the iteration before: K of tile t + NS, V of tile t + NS - 1
+            fetch_k(min(t + NS, edge - 1), ic<ST>{});
+            fetch_v(min(t + NS - 1, edge - 1), ic<(ST + NS - 1) % NS>{});
+            f16acc(&now)[2] = s[ST & 1];
+            f16acc(&next)[2] = s[(ST & 1) ^ 1];
+            const float from = L.base[0] == -INFINITY ? 0.f : L.base[0] - kShift<DT>;
+            u32x4 p[2], kf[KS / 2], vf[DB];
+            constexpr int Q = KS / 2;      // products of a quarter of the scores
+            const auto read = [&](int h) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i) vf[i] = read_v(VT, h, i);
+#pragma unroll
+                for (int i = 0; i < Q; ++i) kf[i] = read_k(KN, h >> 1, (h & 1) * Q + i);
+            };
+            probs(now, from, 0, p[0]);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                read(h);
+                if (h < 3) probs(now, from, h + 1, p[(h + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < (DB > Q ? DB : Q); ++i) {
+                    if (i < Q) next[h >> 1] = mfma<DT>(kf[i], L.qf[0][(h & 1) * Q + i], i == 0 && (h & 1) == 0 ? f16acc{} : next[h >> 1]);
+                    if (i < DB) L.acc[0][i] = mfma<DT>(vf[i], p[h & 1], L.acc[0][i]);
                 }
-                // of 16 channels a half wave has 0 .. 3 and 8 .. 11, or the others: each takes half from the other and has 8 in a row
-                const auto s0 = __builtin_amdgcn_permlane32_swap(u[0], u[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(u[1], u[3], false, false);
-                const u32x4 eight = {s0[0], s1[0], s0[1], s1[1]};
-                const int c = 32 * i + 2 * j + 8 * g;
-                if (c >= a.d) continue;
-                if (a.aligned & 2) *reinterpret_cast<u32x4*>(op + c) = eight;
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) op[c + e] = (uint16_t)(eight[e >> 1] >> 16 * (e & 1));
             }
+            rebase(fmaxf(largest(next[0]), largest(next[1])));
+            wait_vmcnt<(NS - 2) * 2 * ND>();
+            meet();
+        };
+        for (int t = 0; t < piped; t += NS) {
+            tile(t, ic<0>{});
+            tile(t + 1, ic<1>{});
+            if constexpr (NS > 2) {
+                tile(t + 2, ic<2>{});
+                tile(t + 3, ic<3>{});
+            }
+        }
+        wait_vmcnt<0>();
+        meet();
     }
-    if (__syncthreads_or(found)) {
-        __threadfence();
-        if (row < rows)
-#pragma unroll 1
-            for (int key = edge * TK; key < L.limit[0]; ++key)
-#pragma unroll 1
-                for (int c = g; c < a.d; c += 2)
-                    if (!(fabsf(elem(u32x4{st.v[key * st.v_rs + c], 0, 0, 0}, 0, Src::DT)) < INFINITY)) op[c] = 0x7fff;      // (NaN in both types)
+
+    // the other tiles, in two buffers: a tile is on its way into registers while the one before goes into LDS and the one before that is multiplied
+    bool found = false;
+    typename Src::template Stage<DP, TK, 64 * QW> st(sa, a.d, at.first, head, pr.keys, threadIdx.x);
+    if (piped < t1) {
+        int now = 0, then = TILE;
+        const auto write = [&](int to, int t) {
+            if (t >= edge) found |= st.clean();
+            constexpr int CH = decltype(st)::CH;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int i = threadIdx.x + j * 64 * QW, place = slot_of<DP>(i / CPR, i % CPR);
+                *reinterpret_cast<u32x4*>(lds + to + place) = st.kr[j];
+                *reinterpret_cast<u32x4*>(lds + NS * TILE + to + place) = st.vr[j];
+            }
+        };
+        const auto next = [&](int t) {
+            // (behind the last tile the registers hold it still, and nothing reads where it goes)
+            write(then, t + 1);
+            if (t + 2 < t1) st.load((t + 2) * TK);
+            __syncthreads();
+            const int x = now; now = then; then = x;
+        };
+        st.load(piped * TK);
+        write(now, piped);
+        if (piped + 1 < t1) st.load((piped + 1) * TK);
+        __syncthreads();
+        for (int t = piped; t < t_mine; ++t) {
+            const bool plain = (t + 1) * TK <= L.all_see;
+            f16acc s[2][1];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                s[b][0] = f16acc{};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s[b][0] = mfma<DT>(read_k(now, b, ks), L.qf[0][ks], s[b][0]);
+            }
+            float kc[1][4], from[1];
+            L.raise(s, kc, from, sc, t * TK, plain, true, g);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                u32x4 p[1];
+                L.probs(p, s, kc, from, sc, h);
+#pragma unroll
+                for (int i = 0; i < DB; ++i) L.acc[0][i] = mfma<DT>(read_v(NS * TILE + now, h, i), p[0], L.acc[0][i]);
+            }
+            next(t);
+        }
+        for (int t = max(piped, t_mine); t < t1; ++t) next(t);      // tiles that only other waves' rows see (in a loop of its own: a branch around the products costs registers)
     }
+    L.finish(st, 0, end);
+    store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, rows, lane);
 }
 
 // Rows of a workgroup.  (Row tiles of a head: all rows' and a partial one for each prompt.)
@@ -232,7 +471,14 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, int til
     const int64_t grid = tiles_of((int64_t)sa.tokens * a.group, sa.n, tile) * a.hk;
     if (grid > kMostGroups) return -1;
     if (tile == 256) {
-        if constexpr (DP == 64) prompt_kernel<Src, DP, 8, 2, 1, 4><<<(int)grid, 512, 0, st>>>(a, sa);
+        if constexpr (DP == 64 || DP == 128) {
+            constexpr int NS = 2, LDS = 2 * NS * 64 * 2 * DP;
+            const auto kern = prompt_pipe_kernel<Src, DP, NS>;
+            static PerDeviceOnce once;
+            if (const int e = allow_dynamic_lds((const void*)kern, LDS, once)) return e;
+            hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), LDS, st, a, sa);
+        }
+        else if constexpr (DP == 64) prompt_kernel<Src, DP, 8, 2, 1, 4><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 192) prompt_kernel<Src, DP, 8, 2, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 256) prompt_kernel<Src, DP, 8, 1, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else prompt_kernel<Src, DP, 8, 2, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
