@@ -239,6 +239,7 @@ __device__ __forceinline__ void dma16(uint32_t lds_dst, uint32_t lane_off, const
 }
 template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 template <int V> struct ic { static constexpr int value = V; };
+#define SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
 
 // A staged tile's rows are 2 DP bytes, one behind the other, as the DMA writes them; chunk c of 16 bytes of row r lies at slot c ^ turn(r).  K is read
 // 16 rows at one chunk at a time, V 8 rows at four chunks: both then touch every bank once.
@@ -255,6 +256,7 @@ template <int DP> __device__ __forceinline__ int slot_of(int r, int c) { return 
 template <class Src, int DP, int NS>
 __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
     constexpr int QW = 8, TK = 64, TILE = TK * 2 * DP, KS = DP / 16, DB = DP / 32, DT = Src::DT, ND = TILE / 1024 / QW;
+    constexpr int QH = KS / 4, VH = DB / 2;      // products of half a slot
     static_assert(NS * TILE <= 65536, "a tensor's stages within the reach of a read's offset");
     extern __shared__ __align__(16) uint8_t lds[];      // K's stages, then V's
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5, col = lane & 31;
@@ -342,17 +344,15 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
             for (int i = 0; i < DB; ++i) L.acc[0][i] *= by.f;
         }
     };
-    // probabilities of sixteen keys, rounded and in pairs, and their sum
-    const auto probs = [&](const f16acc (&s)[2], float from, int h, u32x4& p) {
-        float e[8];
+    // probabilities of eight of sixteen keys (four of this lane's), rounded and in pairs, and their sum
+    const auto probs = [&](const f16acc (&s)[2], float from, int h, int half, u32x4& p) {
+        float e[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][8 * (h & 1) + i], L.c[0], -from));
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) p[i / 2] = pack2<DT>(e[i], e[i + 1]);
-        float part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part = add2<DT>(p[i], part);
-        L.sum[0] += part;
+        for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][8 * (h & 1) + 4 * half + i], L.c[0], -from));
+        p[2 * half] = pack2<DT>(e[0], e[1]);
+        p[2 * half + 1] = pack2<DT>(e[2], e[3]);
+        // (as they are before the rounding: v_dot2, which adds the rounded pairs, keeps the matrix pipe from the other wave; 16384 tokens 1025 us with it, 988 so)
+        L.sum[0] += (e[0] + e[1]) + (e[2] + e[3]);
     };
 
     if (piped) {
@@ -377,26 +377,35 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
             f16acc(&now)[2] = s[ST & 1];
             f16acc(&next)[2] = s[(ST & 1) ^ 1];
             const float from = L.base[0] == -INFINITY ? 0.f : L.base[0] - kShift<DT>;
-            u32x4 p[2], kf[KS / 2], vf[DB];
-            constexpr int Q = KS / 2;      // products of a quarter of the scores
-            const auto read = [&](int h) {
+            u32x4 p[2], kf[2][QH], vf[2][VH];
+            const auto read = [&](int u) {      // the operands of half a slot: of the scores from 2 u QH products on, of V half the blocks
 #pragma unroll
-                for (int i = 0; i < DB; ++i) vf[i] = read_v(VT, h, i);
+                for (int i = 0; i < QH; ++i) kf[u & 1][i] = read_k(KN, u >> 2, (u & 3) * QH + i);
 #pragma unroll
-                for (int i = 0; i < Q; ++i) kf[i] = read_k(KN, h >> 1, (h & 1) * Q + i);
+                for (int i = 0; i < VH; ++i) vf[u & 1][i] = read_v(VT, u >> 1, (u & 1) * VH + i);
             };
-            probs(now, from, 0, p[0]);
+            read(0);
+            probs(now, from, 0, 0, p[0]);
+            probs(now, from, 0, 1, p[0]);
+            SCHED_FENCE();
+            float top = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                read(h);
-                if (h < 3) probs(now, from, h + 1, p[(h + 1) & 1]);
+            for (int u = 0; u < 8; ++u) {
+                const int h = u >> 1;
+                if (u < 7) read(u + 1);
+                if (h < 3) probs(now, from, h + 1, u & 1, p[(h + 1) & 1]);
+                if (u == 6) top = largest(next[0]);
 #pragma unroll
-                for (int i = 0; i < (DB > Q ? DB : Q); ++i) {
-                    if (i < Q) next[h >> 1] = mfma<DT>(kf[i], L.qf[0][(h & 1) * Q + i], i == 0 && (h & 1) == 0 ? f16acc{} : next[h >> 1]);
-                    if (i < DB) L.acc[0][i] = mfma<DT>(vf[i], p[h & 1], L.acc[0][i]);
-                }
+                for (int i = 0; i < QH; ++i) next[u >> 2] = mfma<DT>(kf[u & 1][i], L.qf[0][(u & 3) * QH + i], i == 0 && (u & 3) == 0 ? f16acc{} : next[u >> 2]);
+#pragma unroll
+                for (int i = 0; i < VH; ++i) L.acc[0][(u & 1) * VH + i] = mfma<DT>(vf[u & 1][i], p[h & 1], L.acc[0][(u & 1) * VH + i]);
+                // the reads, the products in a run, then the vector instructions (one by one between them: 988 us for 980)
+                __builtin_amdgcn_sched_group_barrier(0x100, QH + 2 * VH, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, QH + VH, 0);
+                __builtin_amdgcn_sched_group_barrier(0x402, 24, 0);
+                SCHED_FENCE();
             }
-            rebase(fmaxf(largest(next[0]), largest(next[1])));
+            rebase(fmaxf(top, largest(next[1])));
             wait_vmcnt<(NS - 2) * 2 * ND>();
             meet();
         };
