@@ -246,40 +246,42 @@ template <int V> struct ic { static constexpr int value = V; };
 template <int DP> __device__ __forceinline__ int turn(int r) { return DP == 64 ? (r & 2) << 1 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3); }
 template <int DP> __device__ __forceinline__ int slot_of(int r, int c) { return r * 2 * DP + ((c ^ turn<DP>(r)) << 4); }
 
-// A workgroup's 8 waves of 32 rows, tiles of 64 keys.
+// A workgroup's 8 waves: 8 / KG groups of 32 rows, which each KG waves share, every one with 64 keys of a tile of 64 KG; what they have of a row
+// meets in LDS at the end.
 //
 // In iteration t a wave has the scores of tile t in registers.  Sixteen keys at a time it makes probabilities of them, and between those instructions run
 // the products of the sixteen keys before with V and a quarter of the next tile's scores: every slot of the matrix pipe's 8 products (256
-// cycles) has about as many cycles of vector instructions beside it.  K is a tile ahead of V.  Tiles travel by DMA into `NS` LDS stages.  That holds
+// cycles) has about as many cycles of vector instructions beside it.  K is a tile ahead of V.  Tiles travel by DMA into two LDS stages.  That holds
 // for tiles that every row of the workgroup sees whole; the others, at the diagonal and at the prompt's end, follow in a loop that masks, with
 // their rows through registers, where values that are no numbers are taken out.
-template <class Src, int DP, int NS>
+template <class Src, int DP, int KG>
 __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
-    constexpr int QW = 8, TK = 64, TILE = TK * 2 * DP, KS = DP / 16, DB = DP / 32, DT = Src::DT, ND = TILE / 1024 / QW;
+    constexpr int QW = 8, RG = QW / KG, NS = 2, TK = 64 * KG, TILE = TK * 2 * DP, KS = DP / 16, DB = DP / 32, DT = Src::DT, ND = TILE / 1024 / QW;
     constexpr int QH = KS / 4, VH = DB / 2;      // products of half a slot
     static_assert(NS * TILE <= 65536, "a tensor's stages within the reach of a read's offset");
     extern __shared__ __align__(16) uint8_t lds[];      // K's stages, then V's
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rg = wave % RG, kg = wave / RG, lane = threadIdx.x & 63, g = lane >> 5, col = lane & 31;
     const int slot = blockIdx.x / a.hk, head = blockIdx.x - slot * a.hk;
     Place at;
-    if (!find(sa, a.group, 32 * QW, slot, at)) return;
+    if (!find(sa, a.group, 32 * RG, slot, at)) return;
     Problem pr;
     pr.q_at = at.first * a.q_rs + head * a.group * a.q_hs;
     pr.o_at = at.first * a.o_rs + head * a.group * a.o_hs;
     pr.tokens = pr.keys = at.count;
     pr.limit0 = sa.causal ? 1 : at.count;
-    const int rows = pr.tokens * a.group, r0 = at.tile * 32 * QW, wr = r0 + 32 * wave;
-    const int end = min(pr.keys, pr.limit0 + (min(rows, r0 + 32 * QW) - 1) / a.group), t1 = (end + TK - 1) / TK;
+    const int rows = pr.tokens * a.group, r0 = at.tile * 32 * RG, wr = r0 + 32 * rg, mine = 64 * kg;      // this wave's rows, and its keys within a tile
+    const int end = min(pr.keys, pr.limit0 + (min(rows, r0 + 32 * RG) - 1) / a.group), t1 = (end + TK - 1) / TK;
     const int edge = min(pr.keys, pr.limit0 + r0 / a.group) / TK;      // tiles before this one are seen whole by every row
-    const int sees = min(pr.keys, pr.limit0 + (min(rows, wr + 32) - 1) / a.group), t_mine = wr < rows ? (sees + TK - 1) / TK : 0;      // of this wave's rows
-    const int piped = DP == a.d && sa.aligned ? edge / NS * NS : 0;
+    const int sees = min(pr.keys, pr.limit0 + (min(rows, wr + 32) - 1) / a.group), t_mine = wr < rows ? max(0, sees - mine + TK - 1) / TK : 0;
+    const int piped = sa.aligned ? edge / NS * NS : 0;
     const uint16_t *const k0 = sa.k + at.first * sa.k_rs + head * sa.k_hs, *const v0 = sa.v + at.first * sa.v_rs + head * sa.v_hs;
     const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
 
     // DMA: a kilobyte an instruction, rows RPI (wave + 8 j) .. of the tile
     constexpr int CPR = DP / 8, RPI = 64 / CPR;
     const int drow = RPI * wave + lane / CPR;
-    const uint32_t dchunk = 16 * ((lane % CPR) ^ turn<DP>(drow));      // (the same for j: 8 RPI is a multiple of 16)
+    // (the same for j: 8 RPI is a multiple of 16.  Chunks behind the head dim are its last one again: q is 0 there, and those channels are not stored)
+    const uint32_t dchunk = 16 * min((lane % CPR) ^ turn<DP>(drow), a.d / 8 - 1);
     const uint32_t k_off = 2 * drow * (int)sa.k_rs + dchunk, v_off = 2 * drow * (int)sa.v_rs + dchunk;
     const auto fetch_k = [&](int t, auto stage) {
 #pragma unroll
@@ -292,12 +294,6 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
     if (piped) {      // K of tiles 0 .. NS - 1, V of 0 .. NS - 2
         fetch_k(0, ic<0>{});
         fetch_v(0, ic<0>{});
-        if constexpr (NS > 2) {
-            fetch_k(1, ic<1>{});
-            fetch_v(1, ic<1>{});
-            fetch_k(2, ic<2>{});
-            fetch_v(2, ic<2>{});
-        }
         fetch_k(NS - 1, ic<NS - 1>{});
     }
     Lanes<Src, DP, 1> L;
@@ -307,12 +303,12 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
     // a lane's places in a stage: K row col, chunk 2 ks + g; V rows 16 h + 8 j + 4 g + r', its two chunks' half of block i
     int at_k[KS], at_v[2][DB];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) at_k[s] = slot_of<DP>(col, 2 * s + g);
+    for (int s = 0; s < KS; ++s) at_k[s] = slot_of<DP>(mine + col, 2 * s + g);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < DB; ++i)
-            at_v[j][i] = slot_of<DP>(8 * j + 4 * g + ((lane & 15) >> 2), 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+            at_v[j][i] = slot_of<DP>(mine + 8 * j + 4 * g + ((lane & 15) >> 2), 4 * i + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
     const auto read_k = [&](int stage_at, int b, int s) { return *reinterpret_cast<const u32x4*>(lds + at_k[s] + stage_at + 32 * b * 2 * DP); };
     const auto read_v = [&](int stage_at, int h, int i) {
         u32x2 half[2];
@@ -412,10 +408,6 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
         for (int t = 0; t < piped; t += NS) {
             tile(t, ic<0>{});
             tile(t + 1, ic<1>{});
-            if constexpr (NS > 2) {
-                tile(t + 2, ic<2>{});
-                tile(t + 3, ic<3>{});
-            }
         }
         wait_vmcnt<0>();
         meet();
@@ -448,7 +440,7 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
         if (piped + 1 < t1) st.load((piped + 1) * TK);
         __syncthreads();
         for (int t = piped; t < t_mine; ++t) {
-            const bool plain = (t + 1) * TK <= L.all_see;
+            const bool plain = t * TK + mine + 64 <= L.all_see;
             f16acc s[2][1];
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
@@ -457,7 +449,7 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
                 for (int ks = 0; ks < KS; ++ks) s[b][0] = mfma<DT>(read_k(now, b, ks), L.qf[0][ks], s[b][0]);
             }
             float kc[1][4], from[1];
-            L.raise(s, kc, from, sc, t * TK, plain, true, g);
+            L.raise(s, kc, from, sc, t * TK + mine, plain, true, g);
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 u32x4 p[1];
@@ -470,27 +462,87 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
         for (int t = max(piped, t_mine); t < t1; ++t) next(t);      // tiles that only other waves' rows see (in a loop of its own: a branch around the products costs registers)
     }
     L.finish(st, 0, end);
-    store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, rows, lane);
+    if constexpr (KG > 1) {      // the waves of the same rows: the first takes the others' numerators, sums and bases, in their order
+        __syncthreads();
+        float* const out = reinterpret_cast<float*>(lds) + ((kg - 1) * RG + rg) * (DB * 16 + 2) * 64 + lane;
+        if (kg > 0) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) out[(16 * i + j) * 64] = L.acc[0][i][j];
+            out[DB * 16 * 64] = L.base[0];
+            out[(DB * 16 + 1) * 64] = L.sum[0];
+        }
+        __syncthreads();
+        if (kg == 0)
+#pragma unroll 1
+            for (int k = 1; k < KG; ++k) {
+                const float* const in = reinterpret_cast<const float*>(lds) + ((k - 1) * RG + rg) * (DB * 16 + 2) * 64 + lane;
+                const float base = in[DB * 16 * 64], nb = fmaxf(L.base[0], base);
+                const Rebase<Src> mine_by(L.base[0], nb), its(base, nb);
+                L.base[0] = nb;
+                L.sum[0] = fmaf(in[(DB * 16 + 1) * 64], its.f, L.sum[0] * mine_by.f);
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) L.acc[0][i][j] = fmaf(in[(16 * i + j) * 64], its.f, L.acc[0][i][j] * mine_by.f);
+            }
+    }
+    store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, kg == 0 ? rows : 0, lane);
 }
 
-// Rows of a workgroup.  (Row tiles of a head: all rows' and a partial one for each prompt.)
+// Row tiles of a head: all rows' and a partial one for each prompt.
 inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n; }
 
-template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, int tile, hipStream_t st) {
-    const int64_t grid = tiles_of((int64_t)sa.tokens * a.group, sa.n, tile) * a.hk;
+// How a call runs: tiles of `rows` rows, of whose keys `keys` waves each take a part (prompt_pipe_kernel), or 0: prompt_kernel.
+// Head dims to 64 and to 128.  Where tiles of 256 rows fill the CUs: the pipelined kernel, but for prompts that are short in the mean, which are
+// mostly tiles with an edge, and of which prompt_kernel has two workgroups on a CU (us, bf16: 48 prompts to 231 tokens of 20 heads of 64 40.8 and
+// 28.7; 12 to 800, mean 480, 43 and 37, 39 with 128 rows; 4 to 2500 67 and 84; of 16 heads of 128 24 to 400, mean 240, 45 and 37; 8 to 1300, mean 780, 58
+// and 58; 4 to 2500 78 and 93).  Where they do not fill them: the keys of a row over two or four waves, and tiles of 128 or 64 rows (one prompt of 2000
+// tokens, 8 over 2 heads of 128 54 us in one, 42 in two; 20 heads of 64 45 and 30; 8 over 2 heads of 64 41, 28 and in four 24; 1000
+// tokens of 20 heads of 64, 80 tiles, 27, 20 and 22).
+struct Form {
+    int rows, keys;
+};
+inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
+    const int64_t cus = device_cu_count(), rows = tokens * group;
+    Form f{0, 0};
+    const int64_t wide = tiles_of(rows, n, 256) * hk;
+    if (dp == 64 || dp == 128) {
+        const int64_t mean = tokens / n;
+        if (wide <= cus) f.keys = dp == 64 && 4 * wide <= cus ? 4 : 2;
+        else f.keys = mean >= (dp == 64 ? 800 : 500) ? 1 : 0;
+        f.rows = f.keys ? 256 / f.keys : dp == 64 && mean >= 400 ? 256 : 128;
+        return f;
+    }
+    f.rows = wide >= 2 * cus ? 256 : 128;
+    return f;
+}
+
+template <class Src, int DP, int KG> int launch_pipe(Common& a, const PackedArgs& sa, int64_t grid, hipStream_t st) {
+    constexpr int LDS = 2 * 2 * 64 * KG * 2 * DP;
+    const auto kern = prompt_pipe_kernel<Src, DP, KG>;
+    static PerDeviceOnce once;
+    if (const int e = allow_dynamic_lds((const void*)kern, LDS, once)) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), LDS, st, a, sa);
+    KCHECK();
+    return 0;
+}
+template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStream_t st) {
+    const Form f = form_of(sa.tokens, sa.n, a.group, a.hk, DP);
+    const int64_t grid = tiles_of((int64_t)sa.tokens * a.group, sa.n, f.rows) * a.hk;
     if (grid > kMostGroups) return -1;
-    if (tile == 256) {
-        if constexpr (DP == 64 || DP == 128) {
-            constexpr int NS = 2, LDS = 2 * NS * 64 * 2 * DP;
-            const auto kern = prompt_pipe_kernel<Src, DP, NS>;
-            static PerDeviceOnce once;
-            if (const int e = allow_dynamic_lds((const void*)kern, LDS, once)) return e;
-            hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), LDS, st, a, sa);
-        }
-        else if constexpr (DP == 64) prompt_kernel<Src, DP, 8, 2, 1, 4><<<(int)grid, 512, 0, st>>>(a, sa);
+    if constexpr (DP == 64 || DP == 128) {
+        if (f.keys == 1) return launch_pipe<Src, DP, 1>(a, sa, grid, st);
+        if (f.keys == 2) return launch_pipe<Src, DP, 2>(a, sa, grid, st);
+        if constexpr (DP == 64)
+            if (f.keys == 4) return launch_pipe<Src, DP, 4>(a, sa, grid, st);
+    }
+    if (f.rows == 256) {
+        if constexpr (DP == 64) prompt_kernel<Src, DP, 8, 2, 1, 4><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 192) prompt_kernel<Src, DP, 8, 2, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 256) prompt_kernel<Src, DP, 8, 1, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
-        else prompt_kernel<Src, DP, 8, 2, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
+        else if constexpr (DP == 96) prompt_kernel<Src, DP, 8, 2, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
     } else {
         if constexpr (DP == 64) prompt_kernel<Src, DP, 4, 1, 1, 4><<<(int)grid, 256, 0, st>>>(a, sa);
         else if constexpr (DP == 96) prompt_kernel<Src, DP, 4, 1, 1, 3><<<(int)grid, 256, 0, st>>>(a, sa);
@@ -502,13 +554,12 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, int til
     return 0;
 }
 template <class Src> int launch_dim(Common& a, const PackedArgs& sa, hipStream_t st) {
-    const int tile = tiles_of((int64_t)sa.tokens * a.group, sa.n, 256) * a.hk >= 2 * device_cu_count() ? 256 : 128;
     switch (padded_dim(a.d, 64)) {
-        case 64: return launch<Src, 64>(a, sa, tile, st);
-        case 96: return launch<Src, 96>(a, sa, tile, st);
-        case 128: return launch<Src, 128>(a, sa, tile, st);
-        case 192: return launch<Src, 192>(a, sa, tile, st);
-        default: return launch<Src, 256>(a, sa, tile, st);
+        case 64: return launch<Src, 64>(a, sa, st);
+        case 96: return launch<Src, 96>(a, sa, st);
+        case 128: return launch<Src, 128>(a, sa, st);
+        case 192: return launch<Src, 192>(a, sa, st);
+        default: return launch<Src, 256>(a, sa, st);
     }
 }
 
@@ -532,8 +583,16 @@ GPU_API int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs
     s.k = (const uint16_t*)k; s.v = (const uint16_t*)v;
     s.k_rs = k_rs; s.k_hs = k_hs; s.v_rs = v_rs; s.v_hs = v_hs;
     // (and rows of a tile within 32-bit offsets of its first)
-    const bool near = k_rs >= 0 && v_rs >= 0 && k_rs < (1 << 23) && v_rs < (1 << 23);
+    const bool near = k_rs >= 0 && v_rs >= 0 && k_rs < (1 << 21) && v_rs < (1 << 21);
     s.starts = starts; s.n = n; s.tokens = tokens; s.causal = causal != 0;
     s.aligned = near && sixteen(k, k_rs, k_hs) && sixteen(v, v_rs, v_hs);
     return dtype == DT_BF16 ? launch_dim<Packed<DT_BF16>>(c, s, (hipStream_t)stream) : launch_dim<Packed<DT_F16>>(c, s, (hipStream_t)stream);
+}
+
+GPU_API int gpu_internal_prompt_attn_form(int tokens, int n, int h, int hk, int head_dim, int32_t* out) {
+    if (tokens <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256 || !out) return -1;
+    const Form f = form_of(tokens, n, h / hk, hk, padded_dim(head_dim, 64));
+    out[0] = f.rows;
+    out[1] = f.keys;
+    return 0;
 }

@@ -65,6 +65,7 @@ SIGNATURES = {
     "gpu_internal_fp8_gemm_force": [_I32],
     "gpu_rope": [_I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _P, _I32, _I32, _F32, _P, _P, _F32, _I32, _I32, _P],
     "gpu_prompt_attn": [_I32] + [_P, _I64, _I64] * 4 + [_P, _I32, _I32, _I32, _I32, _I32, _F32, _I32, _P],
+    "gpu_internal_prompt_attn_form": [_I32, _I32, _I32, _I32, _I32, _P],
     "gpu_internal_act_probe": [_I32, _P, _P, _I32, _P],
     "gpu_internal_geglu_form": [_I32, _I32],
     "gpu_internal_cvt_pk_u8_probe": [_P, _P, _I32, _P],

@@ -416,6 +416,10 @@ int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const 
 int gpu_internal_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dt, int32_t* out);
 int gpu_internal_fp8_gemm_force(int form_and_slices);
 
+/* Test hook, no reference counterpart: how gpu_prompt_attn runs `tokens` tokens of n prompts.  out[0] = rows of a workgroup, out[1] = waves that share a
+ * row's keys in the pipelined kernel, 0 for the other. */
+int gpu_internal_prompt_attn_form(int tokens, int n, int h, int hk, int head_dim, int32_t* out);
+
 /* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times
  * key-value heads) of `rows` (query tokens times query heads of a key-value head, the most of any) over `keys`: out[0] = rows of a workgroup (16 and 32:
  * its waves share them, 128 and 256: a wave has 32), out[1] = workgroups that share a row's keys,

@@ -118,6 +118,7 @@ extern "C" {
         scale: f32, causal: i32, stream: PM) -> i32;
     pub fn gpu_internal_fp8_gemm_plan(m: i64, n: i64, k: i64, out_dt: i32, out: PM) -> i32;
     pub fn gpu_internal_fp8_gemm_force(form_and_slices: i32) -> i32;
+    pub fn gpu_internal_prompt_attn_form(tokens: i32, n: i32, h: i32, hk: i32, head_dim: i32, out: PM) -> i32;
     pub fn gpu_internal_states_plan(rows: i64, problems: i64, keys: i64, head_dim: i32, bytes: i32, out: PM) -> i32;
     pub fn gpu_int8_gemm_force_config(cfg: i32) -> i32;
     pub fn gpu_internal_int8_gemm_plan(m: i64, n: i64, k: i64, start: i32, aligned: i32, out: PM) -> i32;

@@ -287,13 +287,27 @@ def _attn_check(o, q, k, v, starts, scale, causal, what=""):
                 _check(o[b:e, j], want, bound, "%s prompt %d head %d" % (what, s, j))
 
 
-ATTN = [([1], 1, 1, 8), ([1, 2, 1], 4, 2, 64), ([0, 5, 0, 33, 0], 2, 2, 128), ([77, 64, 1, 200], 3, 1, 64), ([129, 31, 65], 8, 2, 128), ([300], 6, 6, 72), ([40, 513], 2, 1, 256), ([260], 7, 1, 160),
+# (rows of a workgroup, waves to a row's keys): each form that there is
+FORMS = {(64, 4): ([900, 130], 4, 1, 64), (128, 2): ([1000, 300, 1], 4, 2, 128), (256, 1): ([2100, 515, 1], 20, 20, 128), (128, 0): ([300, 5, 200, 150, 290, 70, 310, 64, 65] * 2, 16, 16, 128),
+         (256, 0): ([420, 700, 63, 640, 450, 800], 24, 24, 64)}
+
+
+def test_attn_forms_are_those_of_their_sizes():
+    import ctypes
+    ffi = pkg("ffi")
+    out = (ctypes.c_int32 * 2)()
+    for form, (lens, h, hk, d) in FORMS.items():
+        ffi.k("gpu_internal_prompt_attn_form", sum(lens), len(lens), h, hk, d, ctypes.cast(out, ctypes.c_void_p))
+        assert tuple(out) == form, (lens, tuple(out))
+
+
+ATTN = [*FORMS.values(), ([700], 20, 20, 64), ([2500, 1800], 10, 10, 64), ([1200], 3, 3, 40), ([1300, 2], 2, 1, 104), ([1111], 24, 24, 56), ([900], 33, 33, 120), ([1] * 7 + [640, 128, 256], 2, 2, 128), ([1], 1, 1, 8), ([1, 2, 1], 4, 2, 64), ([0, 5, 0, 33, 0], 2, 2, 128), ([77, 64, 1, 200], 3, 1, 64), ([129, 31, 65], 8, 2, 128), ([300], 6, 6, 72), ([40, 513], 2, 1, 256), ([260], 7, 1, 160),
         ([128, 128], 2, 2, 96), ([1111], 4, 1, 128), ([700, 3, 1300], 4, 4, 80), ([2000, 47], 12, 4, 64), ([3, 2050], 5, 5, 48), ([1500, 900], 16, 16, 192), ([1000, 700, 300], 20, 20, 256),
         ([2600], 30, 15, 88), ([1700, 300], 24, 24, 128), ([1] * 130 + [70], 2, 1, 40)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=name)
-@pytest.mark.parametrize("lens,h,hk,d", ATTN, ids=lambda v: str(v) if isinstance(v, int) else "x".join(map(str, v[:4])))
+@pytest.mark.parametrize("lens,h,hk,d", ATTN, ids=lambda v: str(v) if isinstance(v, int) else "x".join(map(str, v[-4:])))
 def test_attn(lens, h, hk, d, dtype):
     pr = pkg("prompt")
     T = sum(lens)
