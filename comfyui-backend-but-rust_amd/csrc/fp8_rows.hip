@@ -27,7 +27,7 @@ struct Fp8Rows {
     uint8_t* q;
     float* scales;
     int64_t scales_rs;
-    int M, K, wpr, wide;      // waves of a row; pieces start on whole 16 bytes: x (bit 0), resid (1), sum (2), the half at up_offset (3), norm_w (4), q on 8 (5)
+    int M, K, wpr, wide;      // waves of a row; pieces start on whole 16 bytes: x (bit 0), resid (1), sum (2), the half at up_offset (3), norm_w (4)
 };
 
 constexpr int kPiece = 8;           // columns of a lane at a time: 16 lanes to a group of 128

@@ -41,6 +41,7 @@ PyObject* fp8_quant_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (M < 1 || K < 1 || (halves && (x->size(1) % 2 || resid)) || (w != nullptr) != (pro == PRO_RMS) || !vec(w, K) || (out && !resid)) Py_RETURN_NONE;
     for (const at::Tensor* t : {resid, out})
         if (t && (t->scalar_type() != x->scalar_type() || t->dim() != 2 || t->size(0) != M || t->size(1) != K || (K > 1 && t->stride(1) != 1))) Py_RETURN_NONE;
+    if (out && M > 1 && out->stride(0) < K) Py_RETURN_NONE;
     const auto like = x->options().requires_grad(false);
     at::Tensor q = at::empty({M, K}, like.dtype(at::kFloat8_e4m3fn)), scales = at::empty({(K + 127) / 128, M}, like.dtype(at::kFloat)), total;
     if (resid) total = out ? *out : at::empty({M, K}, like);
@@ -89,7 +90,7 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::Tensor *k, *qn, *kn;
     if (n != 9 || observed() || !PyBool_Check(args[4]) || !number(args[5], &factor) || !number(args[8], &eps)) Py_RETURN_NONE;
     const at::Tensor *q = given(args[0]), *positions = given(args[2]), *freqs = given(args[3]);
-    if (!q || !positions || !freqs || !maybe(args[1], &k) || !maybe(args[6], &qn) || !maybe(args[7], &kn) || !real(*q) || q->dim() != 3) Py_RETURN_NONE;
+    if (!q || !positions || !freqs || !maybe(args[1], &k) || !maybe(args[6], &qn) || !maybe(args[7], &kn) || !real(*q) || q->dim() != 3 || (k && k->dim() != 3)) Py_RETURN_NONE;
     const int64_t T = q->size(0), h = q->size(1), d = q->size(2), hk = k ? k->size(1) : 0;
     if (T < 1 || d < 1 || !token_heads(*q, T, d, q->scalar_type()) || (k && !token_heads(*k, T, d, q->scalar_type())) || !ints(positions, 1) || positions->size(0) != T || !vec(qn, d) || !vec(kn, d) ||
         freqs->scalar_type() != at::kDouble || freqs->dim() != 1 || !freqs->is_contiguous()) Py_RETURN_NONE;

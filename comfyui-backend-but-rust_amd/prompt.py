@@ -70,10 +70,12 @@ def _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out)
     else:
         qo, ko = out
         _heads(qo, T, d, "out[0]", q)
+        qlinear._apart(qo, "out[0]")
         if qo.shape[1] != h or (ko is None) != (k is None):
             raise ValueError("out must be tensors of q's and k's shapes")
         if ko is not None:
             _heads(ko, T, d, "out[1]", q)
+            qlinear._apart(ko, "out[1]")
             if ko.shape[1] != hk:
                 raise ValueError("out must be tensors of q's and k's shapes")
     side = lambda t, heads: (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
@@ -86,7 +88,8 @@ def _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out)
 def attn(q, k, v, starts, scale, causal=True, out=None):
     """softmax(scale * q k^T) v within each prompt: rows starts[s] .. starts[s + 1] (int32 [n + 1] on the device) of q [tokens, h, d] and k, v [tokens,
     hk, d] (bf16 or f16, any strides with a dense last axis, h a multiple of hk, d a multiple of 8 up to 256).  Causal: a row sees the keys up to
-    its own.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`."""
+    its own.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`, which shares
+    no memory with q, k and v."""
     o = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.prompt_attn(q, k, v, starts, float(scale), bool(causal))
     return _attn(q, k, v, starts, scale, causal, out) if o is None else o
 
@@ -105,6 +108,7 @@ def _attn(q, k, v, starts, scale, causal, out):
     o = torch.empty((T, h, d), dtype=q.dtype, device=q.device) if out is None else out
     if out is not None:
         _heads(o, T, d, "out", q)
+        qlinear._apart(o, "out")
         if o.shape != q.shape:
             raise ValueError("out must be %s, got %s" % (tuple(q.shape), tuple(o.shape)))
     with qlinear._on(q.device) as s:

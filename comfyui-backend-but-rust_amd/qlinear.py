@@ -466,6 +466,15 @@ def fp8_quant_rows(x, prologue="plain", norm_w=None, eps=0.0, resid=None, out=No
     return _fp8_quant_rows(x, prologue, norm_w, eps, resid, out) if y is None else y
 
 
+def _apart(t, what):
+    """Rows that are written lie apart: no two share memory."""
+    reach = t.shape[-1]
+    for n, s in sorted(((n, s) for n, s in zip(t.shape[:-1], t.stride()) if n > 1), key=lambda x: x[1]):
+        if s < reach:
+            raise ValueError("%s must have rows that share no memory, got %s with strides %s" % (what, tuple(t.shape), t.stride()))
+        reach += s * (n - 1)
+
+
 def _fp8_quant_rows(x, prologue, norm_w, eps, resid, out):
     """The call in Python, here and below: what the native one leaves to it, and every refusal."""
     if x.dim() != 2 or not x.is_cuda or (x.shape[1] > 1 and x.stride(1) != 1) or x.dtype not in _TORCH_DT:
@@ -485,6 +494,8 @@ def _fp8_quant_rows(x, prologue, norm_w, eps, resid, out):
     for t, what in ((x, "x"), (resid, "resid"), (norm_w, "norm_w"), (out, "out")):
         if t is not None:
             _no_grad(t, what)
+    if out is not None:
+        _apart(out, "out")
     q = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty((-(-K // GROUP), M), dtype=torch.float32, device=x.device)
     total = None if resid is None else torch.empty((M, K), dtype=x.dtype, device=x.device) if out is None else out

@@ -385,7 +385,7 @@ int gpu_fp8_quant_rows(int dtype, int prologue, const void* x, int64_t x_stride,
  * the last block of rows of W may be parts.  bias Out[N] or null.  Out by out_dt (-4).  K a multiple of 16 (-1).  Sums in fp32, but that for 16-bit
  * outputs the matrix instruction cuts the products of each eight k off at 2^-13 of the largest one's power of two (1.5e-5 of the result on normally
  * distributed operands).  work: gpu_fp8_gemm_workspace bytes (0: null will do), 16-byte aligned (-1), in use until the work queued here has
- * run.  A call gives the same bits every time. */
+ * run.  A call gives the same bits every time.  -1 for more than 8388607 workgroups (tiles of 128 x 128 at least from 129 rows on). */
 int64_t gpu_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int out_dt);
 int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_stride, const float* ws, const void* bias, void* D, void* work,
                  int64_t M, int64_t N, int64_t K, int out_dt, void* stream);
@@ -404,7 +404,7 @@ int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, 
  * (causal) or all.  dtype DT_F16 or DT_BF16 (-4); element strides of tokens and heads, dense last axis; query head j uses key-value head
  * j / (h / hk).  Rows of no prompt are left as they are.  starts that do not grow are brought into 0 .. tokens: rows may then be left
  * out, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key makes it NaN, a value its channel NaN or
- * infinite.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
+ * infinite.  o shares no memory with q, k and v.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
  * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 128 rows or more, and n) (-1). */
 int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
                     int64_t v_rs, int64_t v_hs, void* o, int64_t o_rs, int64_t o_hs, const int32_t* starts, int n, int tokens, int h, int hk,
