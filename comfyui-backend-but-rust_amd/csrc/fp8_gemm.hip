@@ -460,16 +460,26 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
 #pragma unroll
         for (int im = 0; im < FM; ++im) f.s[im] = sx[16 * im];
     };
+    // A group's products; what the next one begins with is read a piece under each row tile (all of it under the last one: 1024 x 16384 -> 4096 84 us
+    // for 76, since the four waves then wait for LDS at once).
     const auto group = [&](First& f, First& next) {
         const uint8_t* const at = smem + get * C::STAGE;
         get = get == C::NS - 1 ? 0 : get + 1;
+        const uint8_t* const nx = smem + get * C::STAGE;
+        const float* const sx = reinterpret_cast<const float*>(smem + C::NS * C::STAGE + get * C::SCALES) + wm * (BM / 2) + frow;
         v8i fa[2];
         v8h wide[FN][4];      // (32-bit outputs)
         fa[0] = f.a;
 #pragma unroll
         for (int im = 0; im < FM; ++im) {
             if (im + 1 < FM) fa[(im + 1) & 1] = read(at, aoff + (im + 1) * 16 * kGroup);
-            else begin(next);
+            else {
+                next.a = read(nx, aoff);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) next.s[i] = sx[16 * i];
+            }
+#pragma unroll
+            for (int in = im * FN / FM; in < (im + 1) * FN / FM; ++in) next.w[in] = read(nx, woff + in * 16 * kGroup);
             SCHED_FENCE();
             const int done = im ? im - 1 : FM - 1;
             const float s = im ? f.s[im - 1] * f.ws : last;
@@ -508,11 +518,18 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
         meet();
         begin(f[0]);
         f[0].ws = scales.take();
-        for (int g = g0; g < end; g += 2) {
+        int g = g0;
+        if (n & 1) {      // (so that the loop has no way out in its middle, for which the compiler would move all sums)
+            f[1].ws = scales.take();
+            group(f[0], f[1]);
+            meet();
+            f[0] = f[1];
+            ++g;
+        }
+        for (; g < end; g += 2) {
             f[1].ws = scales.take();      // (here and not among the products: it has a branch, behind which the compiler would move the folds)
             group(f[0], f[1]);
             meet();                       // (behind the last group: the fetching waves' last)
-            if (g + 1 >= end) break;
             f[0].ws = scales.take();
             group(f[1], f[0]);
             meet();
@@ -660,7 +677,7 @@ std::atomic<int> g_force{-1};      // test hook: 100 * form + slices
 // Else the smallest sum of rounds of one workgroup a CU, in us: a fixed time, and one for every group of 128, which grows from `alone` with the share of
 // the CUs that are busy (the caches' and the memory's rates) to `full`; slices are joined for 3 us, 0.35 for each, and their planes' way out and
 // in.  Fitted to 117 sizes of 33 to 3000 rows in up to 14 forms each, weights from memory: 0.25 % slower than the best of them in the mean, 7 % at most.
-// 64 rows: 4.2 + 0.36 .. 0.45 (64 x 4096 -> 24576 29 us), 128 rows: 4.5 + 0.50 .. 0.62 (1024 x 4096 -> 4096 24 us; 35 with 64 rows), 256 x 256: 6 + 1.3 ..
+// 64 rows: 4.2 + 0.36 .. 0.45 (64 x 4096 -> 24576 29 us), 128 rows: 4.5 + 0.50 .. 0.62 (1024 x 4096 -> 4096 23 us; 35 with 64 rows), 256 x 256: 6 + 1.3 ..
 // 1.65 (2048 x 4096 -> 24576 185 us; 270 with 128 rows).  32-bit outputs take tiles of 64 rows, whose fragments leave room for the
 // weights as f16 (1111 x 2640 -> 1000 20 us, 42 in the form for any size), and that form where it has two tiles of its 128 rows a CU (2048 x 4096 ->
 // 4096 87 us, 99).
