@@ -247,6 +247,9 @@ __device__ __forceinline__ v8i tail_fragment(const uint8_t* x, int row, int limi
 }
 
 // Large sizes: tiles of 256 x 256, eight waves of 128 x 64, two LDS stages: group g + 1 travels while group g is multiplied, one barrier a group.
+// Bound by power: 8192 x 4096 -> 24576 710 us, 2.3 PFLOP/s, matrix pipes 58 % busy at 1.73 GHz (a library product with one scale, which has no folds, 2.98
+// PFLOP/s on 8192 cubed; this 2.48).  Not faster: products of 32 x 32 x 64 (730), waves that take turns at multiplying and fetching (862), the next group's
+// first fragments under the last products (727: its rows have to land earlier for that).
 constexpr int BIG = 256, BIG_STAGE = BIG * kGroup, BIG_S = 4 * BIG_STAGE, BIG_LDS = BIG_S + 2 * BIG * 4;
 
 template <int OUT_DT>
@@ -569,7 +572,7 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
 
 // Few rows: the weights' way in is what counts.  They go from memory straight into the operand of the matrix instruction, as do the rows of A (from
 // the caches): eight waves on the same 16 MT rows and 16 CT columns, each with every eighth group of K, two on their way; the waves' sums meet in
-// LDS and are added in their order.
+// LDS and are added in their order.  Bound by memory: 5 x 4096 -> 24576 20 us, 5.0 TB/s.
 template <int MT, int CT, int OUT_DT>
 __global__ void __launch_bounds__(512) fp8_gemm_few_kernel(const Fp8Gemm p) {
     constexpr int TILES = MT * CT;

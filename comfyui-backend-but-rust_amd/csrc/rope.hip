@@ -5,7 +5,7 @@
 // half a turn there, so that far positions are as exact as near ones; the sine and cosine of what is left are fp32, and everything is
 // rounded once.
 //
-// Bound by memory: 2 + 2 bytes a channel of 16 bits.  A workgroup has a few tokens: their sines and cosines go into LDS once, for all heads.
+// Bound by memory: 2 + 2 bytes a channel of 16 bits (16384 tokens of 40 heads of 128 59 us, 5.7 TB/s, a little of it from the last-level cache).  A workgroup has a few tokens: their sines and cosines go into LDS once, for all heads.
 #include "common.hpp"
 
 namespace {
