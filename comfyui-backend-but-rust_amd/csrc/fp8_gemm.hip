@@ -90,7 +90,7 @@ __device__ __forceinline__ void store_plane(const Fp8Gemm& p, int slice, int m, 
             if (n + j < p.N) to[j] = v[j];
 }
 
-// Any sizes: tiles of 128 x 128, four waves of 64 x 64, a group at a time through registers into one of two LDS stages.
+// K below 128 or from 2^23 on: tiles of 128 x 128, four waves of 64 x 64, a group at a time through registers into one of two LDS stages.
 template <int OUT_DT>
 __global__ void __launch_bounds__(256, 2) fp8_gemm_kernel(const Fp8Gemm p) {
     constexpr int STAGE = 128 * kGroup;
@@ -471,7 +471,6 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
         const uint8_t* const nx = smem + get * C::STAGE;
         const float* const sx = reinterpret_cast<const float*>(smem + C::NS * C::STAGE + get * C::SCALES) + wm * (BM / 2) + frow;
         v8i fa[2];
-        v8h wide[FN][4];      // (32-bit outputs)
         fa[0] = f.a;
 #pragma unroll
         for (int im = 0; im < FM; ++im) {
@@ -487,24 +486,6 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
             const int done = im ? im - 1 : FM - 1;
             const float s = im ? f.s[im - 1] * f.ws : last;
             // the products of this row tile, and the fold of the one before between them
-            if constexpr (OUT_DT == DT_F32) {
-                v4f d[FN];
-#pragma unroll
-                for (int in = 0; in < FN; ++in) d[in] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const v8h a = widen(fa[im & 1][2 * e], fa[im & 1][2 * e + 1]);
-#pragma unroll
-                    for (int in = 0; in < FN; ++in) {
-                        if (im == 0) wide[in][e] = widen(f.w[in][2 * e], f.w[in][2 * e + 1]);
-                        d[in] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wide[in][e], a, d[in], 0, 0, 0);
-                        if (e == 3) fold(done & 1, in, done, s);
-                    }
-                }
-#pragma unroll
-                for (int in = 0; in < FN; ++in) sums[im & 1][in] = d[in];
-                SCHED_FENCE();
-            } else
 #pragma unroll
             for (int in = 0; in < FN; ++in) {
                 const v4f d = mfma(f.w[in], fa[im & 1], v4f{0.f, 0.f, 0.f, 0.f});
@@ -558,21 +539,152 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
             }
         }
     }
-    if (p.slices > 1 || OUT_DT == DT_F32) {      // (16 bytes a lane, 64 in a row)
+    if (p.slices > 1) {      // (16 bytes a lane, 64 in a row)
 #pragma unroll
         for (int in = 0; in < FN; ++in)
 #pragma unroll
             for (int im = 0; im < FM; ++im) {
                 const int m = m0 + wm * (BM / 2) + 16 * im + frow, n = n0 + wn * 64 + 16 * in + 4 * part;
-                if (p.slices > 1) store_plane(p, slice, m, n, acc[in][im]);
-                else store_four<OUT_DT>(p, m, n, acc[in][im]);
+                store_plane(p, slice, m, n, acc[in][im]);
             }
-    } else if constexpr (OUT_DT != DT_F32) store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 64, lane);      // (the stages are idle)
+    } else store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 64, lane);      // (the stages are idle)
+}
+
+// 32-bit outputs: tiles of 64 or 128 rows by 128 columns, eight waves of BM / 2 x 32 that all fetch and multiply, so that one's conversions to f16 run
+// beside another's products, in two or three LDS stages, so that a CU has two workgroups (128 rows, 2048 x 4096 -> 4096: 76 us; 88 with four stages and one).  Bound by
+// vector issue (52 %) and the matrix pipes (38 %), which hardly overlap; 32 x 32 x 16 products are no faster (78).
+template <int BM> struct Wide {
+    static constexpr int BN = 128, STAGE = (BM + BN) * kGroup, SCALES = 128 * 4, NS = BM == 128 ? 2 : 3, LDS = NS * (STAGE + SCALES);
+    static constexpr int FM = BM / 32, FN = 2, NDMA = (BM + BN) / 64 + 1;      // of a wave and group
+};
+
+template <int BM>
+__global__ void __launch_bounds__(512, 2) fp8_gemm_wide_kernel(const Fp8Gemm p) {
+    using C = Wide<BM>;
+    constexpr int FM = C::FM, FN = C::FN;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+    const int tiles = p.tiles_m * p.tiles_n, slice = blockIdx.x / tiles;
+    int tm, tn;
+    tile_of_block((int)blockIdx.x - slice * tiles, tiles, p.tiles_m, p.tiles_n, tm, tn);
+    const int m0 = tm * BM, n0 = tn * C::BN;
+    int g0, g1;
+    slice_of(p.groups, p.slices, slice, g0, g1);
+    const bool tail = g1 == p.groups && g0 < g1 && p.K % kGroup != 0;
+    const int end = tail ? g1 - 1 : g1, n = end - g0;      // whole groups
+
+    // DMA: 8-row blocks wave + 8 j, of A and then of W; the swizzle on the memory's side.  The scales of the rows 64 (wave % 2) .., by four waves alike.
+    const uint32_t lds_base = (uint32_t)(uintptr_t)smem, lrow = (uint32_t)lane >> 3, K = (uint32_t)p.K;
+    const uint32_t chunk = ((lane & 7) ^ (((wave & 1) << 2) | (lrow >> 1))) * 16, drow = wave * 8 + lrow;
+    const uint32_t w_last = (uint32_t)min(C::BN - 1, p.N - 1 - n0), a_last = (uint32_t)min(BM - 1, p.M - 1 - m0);
+    uint32_t off[C::NDMA - 1];
+#pragma unroll
+    for (int j = 0; j < C::NDMA - 1; ++j) off[j] = (j < BM / 64 ? min(drow + 64 * j, a_last) : min(drow + 64 * (j - BM / 64), w_last)) * K + chunk;
+    const uint32_t s_off = 4u * min((uint32_t)(64 * (wave & 1) + lane), a_last);
+    const uint8_t *const a_base = p.A + (int64_t)m0 * p.K, *const w_base = p.W + (int64_t)n0 * p.K;
+    const float* const s_base = p.xs + m0;
+    int put = 0;
+    const auto fetch = [&](int g) {      // groups past the end fetch the last one again, which nothing reads
+        const int gc = g < end ? g : end - 1;
+        const uint32_t to = lds_base + put * C::STAGE + wave * 1024;
+#pragma unroll
+        for (int j = 0; j < C::NDMA - 1; ++j) dma16(to + j * 8192, off[j], (j < BM / 64 ? a_base : w_base) + (int64_t)gc * kGroup);
+        dma4(lds_base + C::NS * C::STAGE + put * C::SCALES + (wave & 1) * 256, s_off, s_base + gc * p.xs_rs);
+        put = put == C::NS - 1 ? 0 : put + 1;
+    };
+    const int frow = lane & 15, part = lane >> 4;
+    const int fsw = (part ^ ((frow >> 1) & 7)) << 4, aoff = (wm * (BM / 2) + frow) * kGroup + fsw, woff = (BM + wn * 32 + frow) * kGroup + fsw;
+    const float* const ws = p.ws + (int64_t)tn * p.groups;
+    v4f acc[FN][FM];
+#pragma unroll
+    for (int in = 0; in < FN; ++in)
+#pragma unroll
+        for (int im = 0; im < FM; ++im) acc[in][im] = v4f{0.f, 0.f, 0.f, 0.f};
+    const auto read = [&](const uint8_t* at, int o) { return two(*reinterpret_cast<const v4i*>(at + o), *reinterpret_cast<const v4i*>(at + (o ^ 64))); };
+    if (n > 0) {
+        BlockScales scales(ws, g0, end, lane);
+        asm volatile("" : "+v"(scales.now), "+v"(scales.next));      // (here, or the compiler waits for them, and so for all rows on their way, in every group)
+#pragma unroll
+        for (int i = 0; i < C::NS - 1; ++i) fetch(g0 + i);
+        int get = 0;
+        for (int g = g0; g < end; ++g) {
+            const float wg = scales.take();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // (what was read from is fetched into next)
+            wait_vmcnt<(C::NS - 2) * C::NDMA>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            fetch(g + C::NS - 1);
+            const uint8_t* const at = smem + get * C::STAGE;
+            const float* const sx = reinterpret_cast<const float*>(smem + C::NS * C::STAGE + get * C::SCALES) + wm * (BM / 2) + frow;
+            get = get == C::NS - 1 ? 0 : get + 1;
+            v8i fw[FN], fa[FM];
+            float s[FM];
+#pragma unroll
+            for (int in = 0; in < FN; ++in) fw[in] = read(at, woff + in * 16 * kGroup);
+#pragma unroll
+            for (int im = 0; im < FM; ++im) fa[im] = read(at, aoff + im * 16 * kGroup);
+#pragma unroll
+            for (int im = 0; im < FM; ++im) s[im] = sx[16 * im] * wg;
+#pragma unroll
+            for (int i2 = 0; i2 < FM; i2 += 2) {
+                v4f d[2][FN];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int in = 0; in < FN; ++in) d[i][in] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v8h w[FN];
+#pragma unroll
+                    for (int in = 0; in < FN; ++in) w[in] = widen(fw[in][2 * e], fw[in][2 * e + 1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const v8h x = widen(fa[i2 + i][2 * e], fa[i2 + i][2 * e + 1]);
+#pragma unroll
+                        for (int in = 0; in < FN; ++in) d[i][in] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[in], x, d[i][in], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int in = 0; in < FN; ++in)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) acc[in][i2 + i][c] = fmaf(d[i][in][c], s[i2 + i], acc[in][i2 + i][c]);
+            }
+        }
+        wait_vmcnt<0>();      // nothing may still be writing this workgroup's LDS when it retires
+    }
+    if (tail) {
+        const int k0 = end * kGroup;
+        v8i fw[FN];
+#pragma unroll
+        for (int in = 0; in < FN; ++in) fw[in] = tail_fragment(p.W, n0 + wn * 32 + 16 * in + frow, p.N, p.K, k0, part);
+#pragma unroll
+        for (int im = 0; im < FM; ++im) {
+            const int m = m0 + wm * (BM / 2) + 16 * im + frow;
+            const v8i fa = tail_fragment(p.A, m, p.M, p.K, k0, part);
+            const float s = p.xs[end * p.xs_rs + min(m, p.M - 1)] * ws[end];
+#pragma unroll
+            for (int in = 0; in < FN; ++in) {
+                const v4f d = product<DT_F32>(fw[in], fa);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[in][im][c] = fmaf(d[c], s, acc[in][im][c]);
+            }
+        }
+    }
+#pragma unroll
+    for (int in = 0; in < FN; ++in)
+#pragma unroll
+        for (int im = 0; im < FM; ++im) {      // (16 bytes a lane, 64 in a row)
+            const int m = m0 + wm * (BM / 2) + 16 * im + frow, c = n0 + wn * 32 + 16 * in + 4 * part;
+            if (p.slices > 1) store_plane(p, slice, m, c, acc[in][im]);
+            else store_four<DT_F32>(p, m, c, acc[in][im]);
+        }
 }
 
 // Few rows: the weights' way in is what counts.  They go from memory straight into the operand of the matrix instruction, as do the rows of A (from
 // the caches): eight waves on the same 16 MT rows and 16 CT columns, each with every eighth group of K, two on their way; the waves' sums meet in
-// LDS and are added in their order.  Bound by memory: 5 x 4096 -> 24576 20 us, 5.0 TB/s.
+// LDS and are added in their order.  Bound by memory: 5 x 4096 -> 24576 21 us, 4.8 TB/s.
 template <int MT, int CT, int OUT_DT>
 __global__ void __launch_bounds__(512) fp8_gemm_few_kernel(const Fp8Gemm p) {
     constexpr int TILES = MT * CT;
@@ -681,9 +793,9 @@ std::atomic<int> g_force{-1};      // test hook: 100 * form + slices
 // the CUs that are busy (the caches' and the memory's rates) to `full`; slices are joined for 3 us, 0.35 for each, and their planes' way out and
 // in.  Fitted to 117 sizes of 33 to 3000 rows in up to 14 forms each, weights from memory: 0.25 % slower than the best of them in the mean, 7 % at most.
 // 64 rows: 4.2 + 0.36 .. 0.45 (64 x 4096 -> 24576 29 us), 128 rows: 4.5 + 0.50 .. 0.62 (1024 x 4096 -> 4096 23 us; 35 with 64 rows), 256 x 256: 6 + 1.3 ..
-// 1.65 (2048 x 4096 -> 24576 185 us; 270 with 128 rows).  32-bit outputs take tiles of 64 rows, whose fragments leave room for the
-// weights as f16 (1111 x 2640 -> 1000 20 us, 42 in the form for any size), and that form where it has two tiles of its 128 rows a CU (2048 x 4096 ->
-// 4096 87 us, 99).
+// 1.65 (2048 x 4096 -> 24576 185 us; 270 with 128 rows).
+// 32-bit outputs: two workgroups run on a CU but no faster than one behind the other, so a fixed time of 5 us and 0.62 (64 rows) or 1.02 (128) for every group and workgroup of a CU
+// (2048 x 4096 -> 4096 72 us in 128 rows, 85 in 64; 1024 x 4096 -> 1024 26 in one slice of 64 rows, 22 in four).  Of 72 sizes of 33 to 4096 rows 1 % slower than the best in the mean.
 Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
     const int64_t cus = device_cu_count(), groups = (K + kGroup - 1) / kGroup;
     Plan p{kAny, 1, (N + 31) / 32 >= 2 * cus ? 2 : 1};
@@ -693,7 +805,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
     if (force >= 0) {
         p.form = force / 100;
         p.slices = at_most(force % 100);
-        if ((p.form == kFew && M > 32) || (p.form != kFew && !fits) || ((p.form == kBig || p.form == kMid128) && out_dt == DT_F32)) p.form = kAny;
+        if ((p.form == kFew && M > 32) || (p.form != kFew && !fits) || (p.form == kBig && out_dt == DT_F32)) p.form = kAny;
         if (p.form == kAny || p.form == kBig) p.slices = 1;
         return p;
     }
@@ -703,19 +815,22 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
         p.slices = at_most(groups / 24 < cus / tiles ? groups / 24 : cus / tiles);
         return p;
     }
-    if (!fits || (out_dt == DT_F32 && ((M + 127) / 128) * ((N + 127) / 128) >= 2 * cus)) return p;
+    if (!fits) return p;
     static const struct {
         Form form;
         int bm, bn;
         double start, alone, full;
-    } forms[] = {{kMid64, 64, 128, 4.2, 0.36, 0.45}, {kMid128, 128, 128, 4.5, 0.50, 0.62}, {kBig, 256, 256, 6.0, 1.3, 1.65}};
+    } halves[] = {{kMid64, 64, 128, 4.2, 0.36, 0.45}, {kMid128, 128, 128, 4.5, 0.50, 0.62}, {kBig, 256, 256, 6.0, 1.3, 1.65}},
+      wide[] = {{kMid64, 64, 128, 5.0, 0.62, 0.62}, {kMid128, 128, 128, 5.0, 1.02, 1.02}};
+    const bool words = out_dt == DT_F32;
     double least = 0.;
-    for (const auto& f : forms) {
-        if (f.form != kMid64 && out_dt == DT_F32) break;
+    for (int i = 0; i < (words ? 2 : 3); ++i) {
+        const auto& f = words ? wide[i] : halves[i];
         const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
         for (int s = 1; s == 1 || (f.form != kBig && s <= at_most(groups) && tiles * s <= 2 * cus); ++s) {
             const int64_t whole = tiles * s / cus, left = tiles * s % cus, steps = (groups + s - 1) / s;
-            const double us = whole * (f.start + f.full * steps) + (left ? f.start + (f.alone + (f.full - f.alone) * left / cus) * steps : 0.) +
+            const double us = (words ? f.start + (whole + (left != 0)) * f.full * steps
+                                     : whole * (f.start + f.full * steps) + (left ? f.start + (f.alone + (f.full - f.alone) * left / cus) * steps : 0.)) +
                               (s > 1 ? 3.0 + 0.35 * s + 1.44e-6 * s * M * N : 0.);
             if (p.form == kAny || us < least) {
                 least = us;
@@ -734,15 +849,20 @@ template <int OUT_DT> int launch_join(const Fp8Gemm& p, hipStream_t st) {
     KCHECK();
     return 0;
 }
+template <int BM, int OUT_DT> constexpr auto mid_kernel() {
+    if constexpr (OUT_DT == DT_F32) return fp8_gemm_wide_kernel<BM>;
+    else return fp8_gemm_mid_kernel<BM, OUT_DT>;
+}
 template <int BM, int OUT_DT> int launch_mid(Fp8Gemm p, hipStream_t st) {
-    const auto kern = fp8_gemm_mid_kernel<BM, OUT_DT>;
+    const auto kern = mid_kernel<BM, OUT_DT>();
+    constexpr int LDS = OUT_DT == DT_F32 ? Wide<BM>::LDS : Mid<BM>::LDS;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + 127) / 128;
     const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.slices;
     if (grid > 0xffffffffll / 512) return -1;
     static PerDeviceOnce once;
-    if (const int e = allow_dynamic_lds((const void*)kern, Mid<BM>::LDS, once)) return e;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), Mid<BM>::LDS, st, p);
+    if (const int e = allow_dynamic_lds((const void*)kern, LDS, once)) return e;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), LDS, st, p);
     KCHECK();
     return p.slices > 1 ? launch_join<OUT_DT>(p, st) : 0;
 }
@@ -762,10 +882,9 @@ template <int OUT_DT> int launch(Fp8Gemm p, const Plan& plan, hipStream_t st) {
         return plan.ct == 2 ? launch_few<2, 2, OUT_DT>(p, st) : launch_few<2, 1, OUT_DT>(p, st);
     }
     if (plan.form == kMid64) return launch_mid<64, OUT_DT>(p, st);
-    if constexpr (OUT_DT != DT_F32) {
+    if (plan.form == kMid128) return launch_mid<128, OUT_DT>(p, st);
+    if constexpr (OUT_DT != DT_F32)
         if (plan.form == kBig) return launch_big<OUT_DT>(p, st);
-        if (plan.form == kMid128) return launch_mid<128, OUT_DT>(p, st);
-    }
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = (p.N + 127) / 128;
     if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 256) return -1;
