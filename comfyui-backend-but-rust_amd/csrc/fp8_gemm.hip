@@ -550,15 +550,15 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
     } else store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 64, lane);      // (the stages are idle)
 }
 
-// 32-bit outputs: tiles of 64 or 128 rows by 128 columns, eight waves of BM / 2 x 32 that all fetch and multiply, so that one's conversions to f16 run
-// beside another's products, in two or three LDS stages, so that a CU has two workgroups (128 rows, 2048 x 4096 -> 4096: 76 us; 88 with four stages and one).  Bound by
-// vector issue (52 %) and the matrix pipes (38 %), which hardly overlap; 32 x 32 x 16 products are no faster (78).
+// One to two tiles a CU, and 32-bit outputs: tiles of 64 or 128 rows by 128 columns, eight waves of BM / 2 x 32 that all fetch and multiply, so that one's
+// conversions to f16 run beside another's products, in two or three LDS stages, so that a CU has two workgroups (2048 x 4096 -> 4096, 32-bit: 76 us; 88 with four stages and one).
+// With 32-bit outputs bound by vector issue (52 %) and the matrix pipes (38 %), which hardly overlap; 32 x 32 x 16 products are no faster (78).
 template <int BM> struct Wide {
     static constexpr int BN = 128, STAGE = (BM + BN) * kGroup, SCALES = 128 * 4, NS = BM == 128 ? 2 : 3, LDS = NS * (STAGE + SCALES);
     static constexpr int FM = BM / 32, FN = 2, NDMA = (BM + BN) / 64 + 1;      // of a wave and group
 };
 
-template <int BM>
+template <int BM, int OUT_DT>
 __global__ void __launch_bounds__(512, 2) fp8_gemm_wide_kernel(const Fp8Gemm p) {
     using C = Wide<BM>;
     constexpr int FM = C::FM, FN = C::FN;
@@ -631,19 +631,23 @@ __global__ void __launch_bounds__(512, 2) fp8_gemm_wide_kernel(const Fp8Gemm p) 
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int in = 0; in < FN; ++in) d[i][in] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v8h w[FN];
-#pragma unroll
-                    for (int in = 0; in < FN; ++in) w[in] = widen(fw[in][2 * e], fw[in][2 * e + 1]);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const v8h x = widen(fa[i2 + i][2 * e], fa[i2 + i][2 * e + 1]);
-#pragma unroll
-                        for (int in = 0; in < FN; ++in) d[i][in] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[in], x, d[i][in], 0, 0, 0);
+                    for (int in = 0; in < FN; ++in) {
+                        d[i][in] = v4f{0.f, 0.f, 0.f, 0.f};
+                        if constexpr (OUT_DT != DT_F32) d[i][in] = mfma(fw[in], fa[i2 + i], d[i][in]);
                     }
-                }
+                if constexpr (OUT_DT == DT_F32)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v8h w[FN];
+#pragma unroll
+                        for (int in = 0; in < FN; ++in) w[in] = widen(fw[in][2 * e], fw[in][2 * e + 1]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const v8h x = widen(fa[i2 + i][2 * e], fa[i2 + i][2 * e + 1]);
+#pragma unroll
+                            for (int in = 0; in < FN; ++in) d[i][in] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[in], x, d[i][in], 0, 0, 0);
+                        }
+                    }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -666,20 +670,24 @@ __global__ void __launch_bounds__(512, 2) fp8_gemm_wide_kernel(const Fp8Gemm p) 
             const float s = p.xs[end * p.xs_rs + min(m, p.M - 1)] * ws[end];
 #pragma unroll
             for (int in = 0; in < FN; ++in) {
-                const v4f d = product<DT_F32>(fw[in], fa);
+                const v4f d = product<OUT_DT>(fw[in], fa);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) acc[in][im][c] = fmaf(d[c], s, acc[in][im][c]);
             }
         }
     }
+    if constexpr (OUT_DT != DT_F32) {
+        __syncthreads();      // (the stages are idle)
+        store_wave_tile<OUT_DT, FM, FN>(p, smem + wave * 4096, acc, m0 + wm * (BM / 2), n0 + wn * 32, lane);
+    } else
 #pragma unroll
-    for (int in = 0; in < FN; ++in)
+        for (int in = 0; in < FN; ++in)
 #pragma unroll
-        for (int im = 0; im < FM; ++im) {      // (16 bytes a lane, 64 in a row)
-            const int m = m0 + wm * (BM / 2) + 16 * im + frow, c = n0 + wn * 32 + 16 * in + 4 * part;
-            if (p.slices > 1) store_plane(p, slice, m, c, acc[in][im]);
-            else store_four<DT_F32>(p, m, c, acc[in][im]);
-        }
+            for (int im = 0; im < FM; ++im) {      // (16 bytes a lane, 64 in a row)
+                const int m = m0 + wm * (BM / 2) + 16 * im + frow, c = n0 + wn * 32 + 16 * in + 4 * part;
+                if (p.slices > 1) store_plane(p, slice, m, c, acc[in][im]);
+                else store_four<OUT_DT>(p, m, c, acc[in][im]);
+            }
 }
 
 // Few rows: the weights' way in is what counts.  They go from memory straight into the operand of the matrix instruction, as do the rows of A (from
@@ -780,7 +788,7 @@ template <int OUT_DT> __global__ void __launch_bounds__(256) fp8_gemm_join_kerne
 }
 
 // How a call runs.
-enum Form { kAny, kBig, kMid128, kMid64, kFew };
+enum Form { kAny, kBig, kMid128, kMid64, kFew, kWide };
 struct Plan {
     int form, slices, ct;
 };
@@ -793,7 +801,8 @@ std::atomic<int> g_force{-1};      // test hook: 100 * form + slices
 // the CUs that are busy (the caches' and the memory's rates) to `full`; slices are joined for 3 us, 0.35 for each, and their planes' way out and
 // in.  Fitted to 117 sizes of 33 to 3000 rows in up to 14 forms each, weights from memory: 0.25 % slower than the best of them in the mean, 7 % at most.
 // 64 rows: 4.2 + 0.36 .. 0.45 (64 x 4096 -> 24576 29 us), 128 rows: 4.5 + 0.50 .. 0.62 (1024 x 4096 -> 4096 23 us; 35 with 64 rows), 256 x 256: 6 + 1.3 ..
-// 1.65 (2048 x 4096 -> 24576 185 us; 270 with 128 rows).
+// 1.65 (2048 x 4096 -> 24576 185 us; 270 with 128 rows).  128 rows with two workgroups on a CU where there are so many, for which the fixed time comes once: 5.5 + 0.48
+// .. 1.19 for both's groups (2048 x 4096 -> 4096 43 us; 46 with one at a time, 52 in tiles of 256 x 256; 700 x 1024 -> 6144 13, 16 and 16).
 // 32-bit outputs: two workgroups run on a CU but no faster than one behind the other, so a fixed time of 5 us and 0.62 (64 rows) or 1.02 (128) for every group and workgroup of a CU
 // (2048 x 4096 -> 4096 72 us in 128 rows, 85 in 64; 1024 x 4096 -> 1024 26 in one slice of 64 rows, 22 in four).  Of 72 sizes of 33 to 4096 rows 1 % slower than the best in the mean.
 Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
@@ -805,8 +814,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
     if (force >= 0) {
         p.form = force / 100;
         p.slices = at_most(force % 100);
-        if ((p.form == kFew && M > 32) || (p.form != kFew && !fits) || (p.form == kBig && out_dt == DT_F32)) p.form = kAny;
-        if (p.form == kAny || p.form == kBig) p.slices = 1;
+        if ((p.form == kFew && M > 32) || (p.form != kFew && !fits) || ((p.form == kBig || p.form == kWide) && out_dt == DT_F32)) p.form = kAny;
+        if (p.form == kAny || p.form == kBig || p.form == kWide) p.slices = 1;
         return p;
     }
     if (M <= 32) {
@@ -820,17 +829,19 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
         Form form;
         int bm, bn;
         double start, alone, full;
-    } halves[] = {{kMid64, 64, 128, 4.2, 0.36, 0.45}, {kMid128, 128, 128, 4.5, 0.50, 0.62}, {kBig, 256, 256, 6.0, 1.3, 1.65}},
+    } halves[] = {{kMid64, 64, 128, 4.2, 0.36, 0.45}, {kMid128, 128, 128, 4.5, 0.50, 0.62}, {kBig, 256, 256, 6.0, 1.3, 1.65}, {kWide, 128, 128, 5.5, 0.48, 1.19}},
       wide[] = {{kMid64, 64, 128, 5.0, 0.62, 0.62}, {kMid128, 128, 128, 5.0, 1.02, 1.02}};
     const bool words = out_dt == DT_F32;
     double least = 0.;
-    for (int i = 0; i < (words ? 2 : 3); ++i) {
+    for (int i = 0; i < (words ? 2 : 4); ++i) {
         const auto& f = words ? wide[i] : halves[i];
         const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
-        for (int s = 1; s == 1 || (f.form != kBig && s <= at_most(groups) && tiles * s <= 2 * cus); ++s) {
-            const int64_t whole = tiles * s / cus, left = tiles * s % cus, steps = (groups + s - 1) / s;
-            const double us = (words ? f.start + (whole + (left != 0)) * f.full * steps
-                                     : whole * (f.start + f.full * steps) + (left ? f.start + (f.alone + (f.full - f.alone) * left / cus) * steps : 0.)) +
+        for (int s = 1; s == 1 || (f.form != kBig && f.form != kWide && s <= at_most(groups) && tiles * s <= 2 * cus); ++s) {
+            const int64_t slots = f.form == kWide ? 2 * cus : cus, whole = tiles * s / slots, left = tiles * s % slots, steps = (groups + s - 1) / s;
+            const double part = left ? f.alone + (f.full - f.alone) * left / slots : 0.;      // of the last round's groups
+            const double us = (f.form == kWide ? f.start + (whole * f.full + part) * steps
+                               : words         ? f.start + (whole + (left != 0)) * f.full * steps
+                                               : whole * (f.start + f.full * steps) + (left ? f.start + part * steps : 0.)) +
                               (s > 1 ? 3.0 + 0.35 * s + 1.44e-6 * s * M * N : 0.);
             if (p.form == kAny || us < least) {
                 least = us;
@@ -849,13 +860,13 @@ template <int OUT_DT> int launch_join(const Fp8Gemm& p, hipStream_t st) {
     KCHECK();
     return 0;
 }
-template <int BM, int OUT_DT> constexpr auto mid_kernel() {
-    if constexpr (OUT_DT == DT_F32) return fp8_gemm_wide_kernel<BM>;
+template <int BM, int OUT_DT, bool WIDE> constexpr auto mid_kernel() {
+    if constexpr (WIDE) return fp8_gemm_wide_kernel<BM, OUT_DT>;
     else return fp8_gemm_mid_kernel<BM, OUT_DT>;
 }
-template <int BM, int OUT_DT> int launch_mid(Fp8Gemm p, hipStream_t st) {
-    const auto kern = mid_kernel<BM, OUT_DT>();
-    constexpr int LDS = OUT_DT == DT_F32 ? Wide<BM>::LDS : Mid<BM>::LDS;
+template <int BM, int OUT_DT, bool WIDE = OUT_DT == DT_F32> int launch_mid(Fp8Gemm p, hipStream_t st) {
+    const auto kern = mid_kernel<BM, OUT_DT, WIDE>();
+    constexpr int LDS = WIDE ? Wide<BM>::LDS : Mid<BM>::LDS;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + 127) / 128;
     const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.slices;
@@ -883,8 +894,10 @@ template <int OUT_DT> int launch(Fp8Gemm p, const Plan& plan, hipStream_t st) {
     }
     if (plan.form == kMid64) return launch_mid<64, OUT_DT>(p, st);
     if (plan.form == kMid128) return launch_mid<128, OUT_DT>(p, st);
-    if constexpr (OUT_DT != DT_F32)
+    if constexpr (OUT_DT != DT_F32) {
         if (plan.form == kBig) return launch_big<OUT_DT>(p, st);
+        if (plan.form == kWide) return launch_mid<128, OUT_DT, true>(p, st);
+    }
     p.tiles_m = (p.M + 127) / 128;
     p.tiles_n = (p.N + 127) / 128;
     if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 256) return -1;

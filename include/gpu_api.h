@@ -411,7 +411,7 @@ int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const 
                     int head_dim, float scale, int causal, void* stream);
 
 /* Test hooks, no reference counterpart: how gpu_fp8_gemm runs a size, out[0] = form (0 any size, 1 tiles of 256 x 256, 2 of 128 x 128 and 3 of
- * 64 x 128 with K in slices, 4 up to 32 rows), out[1] = slices of K; and a form forced on the calls of the process, 100 * form + slices
+ * 64 x 128 with K in slices, 4 up to 32 rows, 5 of 128 x 128 two to a CU, for 16-bit outputs), out[1] = slices of K; and a form forced on the calls of the process, 100 * form + slices
  * (-1: by the sizes; 0 where the form does not take the size).  The workspace follows. */
 int gpu_internal_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dt, int32_t* out);
 int gpu_internal_fp8_gemm_force(int form_and_slices);

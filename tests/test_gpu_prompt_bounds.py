@@ -2,11 +2,13 @@
 
 Bounds as in test_gpu_prompt.
 """
+import ctypes
+
 import pytest
 import torch
 
 from conftest import pkg
-from test_gpu_prompt import DEV, _attn_check, _codes, _product, _randn
+from test_gpu_prompt import DEV, _attn_check, _codes, _operands, _product, _randn
 from test_gpu_states import _check
 
 pytestmark = pytest.mark.gpu
@@ -54,6 +56,35 @@ def test_products_past_32_bits(M, N, K):
     cut = sum(7 * 2.0 ** -13 * (A[:, None, k:k + 8].abs() * W[None, :, k:k + 8].abs()).amax(-1) for k in range(0, K, 8))
     _check(d[-last_m:, -last_n:], want, (2.0 ** -8 * want.abs()).clamp(min=1e-38) + (128 + G + 4) * 2.0 ** -23 * mass + cut, "the last rows and columns")
     assert not d[:M - last_m:499].any() and not d[:, :N - last_n:499].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("M,N,K", [(1, 8, 128), (130, 260, 640), (300, 129, 1296), (257, 1000, 272), (128, 128, 8400)])
+def test_products_two_workgroups_to_a_cu(M, N, K, dtype):
+    ql, ffi = pkg("qlinear"), pkg("ffi")
+    a, w, xs, ws, bias = _operands(M, N, K, dtype, seed=60)
+    ffi.k("gpu_internal_fp8_gemm_force", 501)
+    try:
+        got = [ql.fp8_gemm(a, w, xs, ws, b, dtype) for b in (bias, None, None)]
+        room = torch.zeros(M * N + 1, dtype=dtype, device=DEV)[1:].view(M, N)      # (an address that is no multiple of 16)
+        ql.fp8_gemm(a, w, xs, ws, None, dtype, room)
+    finally:
+        ffi.k("gpu_internal_fp8_gemm_force", -1)
+    for b, d in ((bias, got[0]), (None, got[1])):
+        want, bound = _product(a, w, xs, ws, b, dtype)
+        _check(d, want, bound, "bias" if b is not None else "no bias")
+    assert torch.equal(got[1], got[2]) and torch.equal(room, got[1])
+
+
+@pytest.mark.parametrize("M,N,K,dtype,form", [(2048, 4096, 256, torch.bfloat16, 5), (2048, 4096, 256, torch.float32, 2), (33, 256, 4096, torch.float32, 3), (200, 128, 64, torch.float32, 0)])
+def test_sizes_take_the_forms_that_are_made_for_them(M, N, K, dtype, form):
+    ql, ffi = pkg("qlinear"), pkg("ffi")
+    out = (ctypes.c_int32 * 2)()
+    ffi.k("gpu_internal_fp8_gemm_plan", M, N, K, ffi.DT_BF16 if dtype == torch.bfloat16 else ffi.DT_F32, ctypes.cast(out, ctypes.c_void_p))
+    assert out[0] == form
+    a, w, xs, ws, bias = _operands(M, N, K, dtype, seed=70)
+    want, bound = _product(a[-40:], w, xs[:, -40:], ws, bias, dtype)
+    _check(ql.fp8_gemm(a, w, xs, ws, bias, dtype)[-40:], want, bound, "the last rows")
 
 
 def test_rope_past_32_bits():
