@@ -499,7 +499,8 @@ inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n;
 // Head dims to 64 and to 128.  Where tiles of 256 rows fill the CUs: the pipelined kernel, but for prompts that are short in the mean, which are
 // mostly tiles with an edge, and of which prompt_kernel has two workgroups on a CU (us, bf16: 48 prompts to 231 tokens of 20 heads of 64 40.8 and
 // 28.7; 12 to 800, mean 480, 43 and 37, 39 with 128 rows; 4 to 2500 67 and 84; of 16 heads of 128 24 to 400, mean 240, 45 and 37; 8 to 1300, mean 780, 58
-// and 58; 4 to 2500 78 and 93).  Where they do not fill them: the keys of a row over two or four waves, and tiles of 128 or 64 rows (one prompt of 2000
+// and 58; 4 to 2500 78 and 93).  Very short ones of 64 channels in tiles of 64 rows (64
+// prompts of 20 heads to 77 tokens, mean 46, 14.8 us, 16.6 in 128; to 20 8.6 and 10.3; to 100, mean 60, 18.8 and 18.0).  Where they do not fill them: the keys of a row over two or four waves, and tiles of 128 or 64 rows (one prompt of 2000
 // tokens, 8 over 2 heads of 128 54 us in one, 42 in two; 20 heads of 64 45 and 30; 8 over 2 heads of 64 41, 28 and in four 24; 1000
 // tokens of 20 heads of 64, 80 tiles, 27, 20 and 22).
 struct Form {
@@ -513,7 +514,7 @@ inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
         const int64_t mean = tokens / n;
         if (wide <= cus) f.keys = dp == 64 && 4 * wide <= cus ? 4 : 2;
         else f.keys = mean >= (dp == 64 ? 800 : 500) ? 1 : 0;
-        f.rows = f.keys ? 256 / f.keys : dp == 64 && mean >= 400 ? 256 : 128;
+        f.rows = f.keys ? 256 / f.keys : dp == 64 && mean >= 400 ? 256 : dp == 64 && mean < 50 ? 64 : 128;
         return f;
     }
     f.rows = wide >= 2 * cus ? 256 : 128;
@@ -545,8 +546,10 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStre
         else if constexpr (DP == 256) prompt_kernel<Src, DP, 8, 1, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 96) prompt_kernel<Src, DP, 8, 2, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
     } else {
-        if constexpr (DP == 64) prompt_kernel<Src, DP, 4, 1, 1, 4><<<(int)grid, 256, 0, st>>>(a, sa);
-        else if constexpr (DP == 96) prompt_kernel<Src, DP, 4, 1, 1, 3><<<(int)grid, 256, 0, st>>>(a, sa);
+        if constexpr (DP == 64) {
+            if (f.rows == 64) prompt_kernel<Src, DP, 2, 1, 1, 4><<<(int)grid, 128, 0, st>>>(a, sa);
+            else prompt_kernel<Src, DP, 4, 1, 1, 4><<<(int)grid, 256, 0, st>>>(a, sa);
+        } else if constexpr (DP == 96) prompt_kernel<Src, DP, 4, 1, 1, 3><<<(int)grid, 256, 0, st>>>(a, sa);
         else if constexpr (DP == 128) prompt_kernel<Src, DP, 4, 2, 2, 2><<<(int)grid, 256, 0, st>>>(a, sa);
         else if constexpr (DP == 192) prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
         else prompt_kernel<Src, DP, 4, 1, 1, 1><<<(int)grid, 256, 0, st>>>(a, sa);

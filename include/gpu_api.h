@@ -405,7 +405,7 @@ int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, 
  * j / (h / hk).  Rows of no prompt are left as they are.  starts that do not grow are brought into 0 .. tokens: rows may then be left
  * out, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key makes it NaN, a value its channel NaN or
  * infinite.  o shares no memory with q, k and v.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
- * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 128 rows or more, and n) (-1). */
+ * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 64 rows or more, and n) (-1). */
 int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
                     int64_t v_rs, int64_t v_hs, void* o, int64_t o_rs, int64_t o_hs, const int32_t* starts, int n, int tokens, int h, int hk,
                     int head_dim, float scale, int causal, void* stream);

@@ -3,6 +3,7 @@
 Bounds as in test_gpu_prompt.
 """
 import ctypes
+import math
 
 import pytest
 import torch
@@ -108,6 +109,30 @@ def test_attention_past_32_bits():
     heads = slice(h - 2, h)
     _attn_check(o[-each:, heads], q[-each:, heads], k[-each:, heads], v[-each:, heads], [0, each], d ** -0.5, True, "the last prompt")
     assert not o[:T - each:997].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("d", [64, 40])
+def test_attention_of_very_short_prompts(d, dtype):
+    """Tiles of 64 rows: prompts of a token, of a whole tile, of one more, and of none."""
+    pr, ffi = pkg("prompt"), pkg("ffi")
+    lens, h, hk = [20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 8
+    T, out = sum(lens), (ctypes.c_int32 * 2)()
+    ffi.k("gpu_internal_prompt_attn_form", T, len(lens), h, hk, d, ctypes.cast(out, ctypes.c_void_p))
+    assert tuple(out) == (64, 0)
+    starts = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    qkv = _randn(80, T, h + 2 * hk, d, size=1.3).to(dtype)
+    q, k, v = qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]
+    at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    for causal in (True, False):
+        o = pr.attn(q, k, v, at, d ** -0.5, causal)
+        _attn_check(o, q, k, v, starts[:9], d ** -0.5, causal, "causal" if causal else "all keys")
+        assert torch.equal(o, pr.attn(q, k, v, at, d ** -0.5, causal))
+    # a NaN behind a row's keys does not reach it, one among them does
+    v = v.clone()
+    v[30, :, 3] = math.nan
+    o = pr.attn(q, k, v, at, d ** -0.5)
+    assert o[30:84, :, 3].isnan().all() and not o[:30].isnan().any() and not o[84:].isnan().any() and not o[..., 4:].isnan().any()
 
 
 def test_outputs_with_rows_that_share_memory_and_other_ranks_are_refused():
