@@ -495,29 +495,35 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
 // Row tiles of a head: all rows' and a partial one for each prompt.
 inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n; }
 
-// How a call runs: tiles of `rows` rows, of whose keys `keys` waves each take a part (prompt_pipe_kernel), or 0: prompt_kernel.
+// How a call runs: tiles of `rows` rows, of whose keys `keys` waves each take a part (prompt_pipe_kernel), or 0: prompt_kernel, 32 `blocks` keys at a
+// time where there is a choice.
 // Head dims to 64 and to 128.  Where tiles of 256 rows fill the CUs: the pipelined kernel, but for prompts that are short in the mean, which are
 // mostly tiles with an edge, and of which prompt_kernel has two workgroups on a CU (us, bf16: 48 prompts to 231 tokens of 20 heads of 64 40.8 and
 // 28.7; 12 to 800, mean 480, 43 and 37, 39 with 128 rows; 4 to 2500 67 and 84; of 16 heads of 128 24 to 400, mean 240, 45 and 37; 8 to 1300, mean 780, 58
-// and 58; 4 to 2500 78 and 93).  Very short ones of 64 channels in tiles of 64 rows (64
-// prompts of 20 heads to 77 tokens, mean 46, 14.8 us, 16.6 in 128; to 20 8.6 and 10.3; to 100, mean 60, 18.8 and 18.0).  Where they do not fill them: the keys of a row over two or four waves, and tiles of 128 or 64 rows (one prompt of 2000
-// tokens, 8 over 2 heads of 128 54 us in one, 42 in two; 20 heads of 64 45 and 30; 8 over 2 heads of 64 41, 28 and in four 24; 1000
+// and 58; 4 to 2500 78 and 93).  Of 128 channels below 160 tokens 32 keys at a time and not 64, which have three workgroups on a CU (64 prompts to 77 tokens, 16 over 4
+// heads 15.1 and 16.8; 48 to 160 29.3 and 30.8; 32 to 320, mean 192, 38.4 and 37.1).  Where they do not fill them: the keys of a row over two or four waves, and tiles of 128 or
+// 64 rows (one prompt of 2000 tokens, 8 over 2 heads of 128 54 us in one, 42 in two; 20 heads of 64 45 and 30; 8 over 2 heads of 64 41, 28 and in four 24; 1000
 // tokens of 20 heads of 64, 80 tiles, 27, 20 and 22).
+// Prompts of fewer rows than half such a tile in tiles of 64 (64 prompts to 20 tokens of 16 heads: of 64 channels 9.1 for 10.6, of 96 10.9 for 13.7, of 128 10.7 for 14.4, of 256
+// 28.4 for 37.7; to 77 tokens, 46 rows, of 64 13.4 for 13.0, and of 20 heads 14.8 for 16.6; of 96 22.8 for 21.0; of 192 never: 34 for 21).
+// The other head dims, 256 rows or 128: of 96 48 prompts to 160 tokens 33.7 and 26.1, 8 to 2500 142 and 131, 6 to 2500 of 16 over 4 heads 108 and 116; of 192 24 to 600, mean 360, 119
+// and 111, 12 to 1200 145 and 157; of 256 24 to 600 174 and 177, 8 to 2500 416 and 522.
 struct Form {
-    int rows, keys;
+    int rows, keys, blocks;
 };
 inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
-    const int64_t cus = device_cu_count(), rows = tokens * group;
-    Form f{0, 0};
+    const int64_t cus = device_cu_count(), rows = tokens * group, mean = tokens / n, each = rows / n;      // of a prompt, in the mean
+    Form f{0, 0, 0};
     const int64_t wide = tiles_of(rows, n, 256) * hk;
     if (dp == 64 || dp == 128) {
-        const int64_t mean = tokens / n;
         if (wide <= cus) f.keys = dp == 64 && 4 * wide <= cus ? 4 : 2;
         else f.keys = mean >= (dp == 64 ? 800 : 500) ? 1 : 0;
-        f.rows = f.keys ? 256 / f.keys : dp == 64 && mean >= 400 ? 256 : dp == 64 && mean < 50 ? 64 : 128;
+        f.rows = f.keys ? 256 / f.keys : each < (dp == 64 ? 48 : 32) ? 64 : dp == 64 && mean >= 400 ? 256 : 128;
+        if (dp == 128 && f.rows == 128) f.blocks = mean >= 160 ? 2 : 1;
         return f;
     }
-    f.rows = wide >= 2 * cus ? 256 : 128;
+    const bool long_enough = dp == 96 ? each >= 4000 : dp == 192 ? mean >= 500 : each >= 32;
+    f.rows = wide >= 2 * cus && long_enough ? 256 : dp != 192 && each < 32 ? 64 : 128;
     return f;
 }
 
@@ -545,13 +551,15 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStre
         else if constexpr (DP == 192) prompt_kernel<Src, DP, 8, 2, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 256) prompt_kernel<Src, DP, 8, 1, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 96) prompt_kernel<Src, DP, 8, 2, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
+    } else if (f.rows == 64) {
+        if constexpr (DP != 192) prompt_kernel<Src, DP, 2, 1, 1, DP == 64 ? 4 : DP == 256 ? 1 : 2><<<(int)grid, 128, 0, st>>>(a, sa);
     } else {
-        if constexpr (DP == 64) {
-            if (f.rows == 64) prompt_kernel<Src, DP, 2, 1, 1, 4><<<(int)grid, 128, 0, st>>>(a, sa);
-            else prompt_kernel<Src, DP, 4, 1, 1, 4><<<(int)grid, 256, 0, st>>>(a, sa);
-        } else if constexpr (DP == 96) prompt_kernel<Src, DP, 4, 1, 1, 3><<<(int)grid, 256, 0, st>>>(a, sa);
-        else if constexpr (DP == 128) prompt_kernel<Src, DP, 4, 2, 2, 2><<<(int)grid, 256, 0, st>>>(a, sa);
-        else if constexpr (DP == 192) prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
+        if constexpr (DP == 64) prompt_kernel<Src, DP, 4, 1, 1, 4><<<(int)grid, 256, 0, st>>>(a, sa);
+        else if constexpr (DP == 96) prompt_kernel<Src, DP, 4, 1, 1, 3><<<(int)grid, 256, 0, st>>>(a, sa);
+        else if constexpr (DP == 128) {
+            if (f.blocks == 1) prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
+            else prompt_kernel<Src, DP, 4, 2, 2, 2><<<(int)grid, 256, 0, st>>>(a, sa);
+        } else if constexpr (DP == 192) prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
         else prompt_kernel<Src, DP, 4, 1, 1, 1><<<(int)grid, 256, 0, st>>>(a, sa);
     }
     KCHECK();

@@ -112,27 +112,31 @@ def test_attention_past_32_bits():
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda t: str(t)[6:])
-@pytest.mark.parametrize("d", [64, 40])
-def test_attention_of_very_short_prompts(d, dtype):
-    """Tiles of 64 rows: prompts of a token, of a whole tile, of one more, and of none."""
+@pytest.mark.parametrize("lens,h,hk,d,rows", [([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 64, 64), ([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 40, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 80, 64),
+                                              ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 128, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 256, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 192, 128),
+                                              ([150, 129, 1, 65, 0, 77] * 9, 16, 8, 104, 128), ([150, 129, 1, 65, 0, 77] * 18, 16, 16, 88, 128), ([520] * 12, 24, 24, 160, 256), ([2050], 66, 33, 96, 256)])
+def test_attention_forms_by_the_prompts_lengths(lens, h, hk, d, rows, dtype):
+    """Prompts of a token, of a whole tile, of one more, and of none."""
     pr, ffi = pkg("prompt"), pkg("ffi")
-    lens, h, hk = [20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 8
     T, out = sum(lens), (ctypes.c_int32 * 2)()
     ffi.k("gpu_internal_prompt_attn_form", T, len(lens), h, hk, d, ctypes.cast(out, ctypes.c_void_p))
-    assert tuple(out) == (64, 0)
+    assert tuple(out) == (rows, 0)
     starts = [sum(lens[:i]) for i in range(len(lens) + 1)]
     qkv = _randn(80, T, h + 2 * hk, d, size=1.3).to(dtype)
     q, k, v = qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]
     at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    heads = slice(h - 2 * h // hk, h), slice(hk - 2, hk)
     for causal in (True, False):
         o = pr.attn(q, k, v, at, d ** -0.5, causal)
-        _attn_check(o, q, k, v, starts[:9], d ** -0.5, causal, "causal" if causal else "all keys")
+        _attn_check(o[:, heads[0]], q[:, heads[0]], k[:, heads[1]], v[:, heads[1]], starts[:7], d ** -0.5, causal, "causal" if causal else "all keys")
         assert torch.equal(o, pr.attn(q, k, v, at, d ** -0.5, causal))
     # a NaN behind a row's keys does not reach it, one among them does
+    n = next(i for i, l in enumerate(lens) if l > 4)
+    hole, end = starts[n] + 3, starts[n + 1]
     v = v.clone()
-    v[30, :, 3] = math.nan
+    v[hole, :, 3] = math.nan
     o = pr.attn(q, k, v, at, d ** -0.5)
-    assert o[30:84, :, 3].isnan().all() and not o[:30].isnan().any() and not o[84:].isnan().any() and not o[..., 4:].isnan().any()
+    assert o[hole:end, :, 3].isnan().all() and not o[:hole].isnan().any() and not o[end:].isnan().any() and not o[..., 4:].isnan().any()
 
 
 def test_outputs_with_rows_that_share_memory_and_other_ranks_are_refused():
