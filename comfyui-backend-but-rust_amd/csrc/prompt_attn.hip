@@ -503,8 +503,9 @@ inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n;
 // and 58; 4 to 2500 78 and 93).  Of 128 channels below 160 tokens 32 keys at a time and not 64, which have three workgroups on a CU (64 prompts to 77 tokens, 16 over 4
 // heads 15.1 and 16.8; 48 to 160 29.3 and 30.8; 32 to 320, mean 192, 38.4 and 37.1).  Where they do not fill them: the keys of a row over two or four waves, and tiles of 128 or
 // 64 rows (one prompt of 2000 tokens, 8 over 2 heads of 128 54 us in one, 42 in two; 20 heads of 64 45 and 30; 8 over 2 heads of 64 41, 28 and in four 24; 1000
-// tokens of 20 heads of 64, 80 tiles, 27, 20 and 22).
-// Prompts of fewer rows than half such a tile in tiles of 64 (64 prompts to 20 tokens of 16 heads: of 64 channels 9.1 for 10.6, of 96 10.9 for 13.7, of 128 10.7 for 14.4, of 256
+// tokens of 20 heads of 64, 80 tiles, 27, 20 and 22), but for prompts of less than 128 tokens (one of 77 of 16 heads of 64 9.1 in tiles of 128 rows, 11.0 so, of 128 11.5 and 12.7;
+// one of 231 13.3 and 12.1, 16.1 and 15.6).
+// Many prompts of fewer rows than half such a tile in tiles of 64 (64 prompts to 20 tokens of 16 heads: of 64 channels 9.1 for 10.6, of 96 10.9 for 13.7, of 128 10.7 for 14.4, of 256
 // 28.4 for 37.7; to 77 tokens, 46 rows, of 64 13.4 for 13.0, and of 20 heads 14.8 for 16.6; of 96 22.8 for 21.0; of 192 never: 34 for 21).
 // The other head dims, 256 rows or 128: of 96 48 prompts to 160 tokens 33.7 and 26.1, 8 to 2500 142 and 131, 6 to 2500 of 16 over 4 heads 108 and 116; of 192 24 to 600, mean 360, 119
 // and 111, 12 to 1200 145 and 157; of 256 24 to 600 174 and 177, 8 to 2500 416 and 522.
@@ -516,9 +517,9 @@ inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
     Form f{0, 0, 0};
     const int64_t wide = tiles_of(rows, n, 256) * hk;
     if (dp == 64 || dp == 128) {
-        if (wide <= cus) f.keys = dp == 64 && 4 * wide <= cus ? 4 : 2;
+        if (wide <= cus) f.keys = mean < 128 ? 0 : dp == 64 && 4 * wide <= cus ? 4 : 2;
         else f.keys = mean >= (dp == 64 ? 800 : 500) ? 1 : 0;
-        f.rows = f.keys ? 256 / f.keys : each < (dp == 64 ? 48 : 32) ? 64 : dp == 64 && mean >= 400 ? 256 : 128;
+        f.rows = f.keys ? 256 / f.keys : wide > cus && each < (dp == 64 ? 48 : 32) ? 64 : dp == 64 && mean >= 400 ? 256 : 128;
         if (dp == 128 && f.rows == 128) f.blocks = mean >= 160 ? 2 : 1;
         return f;
     }

@@ -114,7 +114,8 @@ def test_attention_past_32_bits():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda t: str(t)[6:])
 @pytest.mark.parametrize("lens,h,hk,d,rows", [([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 64, 64), ([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 40, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 80, 64),
                                               ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 128, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 256, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 192, 128),
-                                              ([150, 129, 1, 65, 0, 77] * 9, 16, 8, 104, 128), ([150, 129, 1, 65, 0, 77] * 18, 16, 16, 88, 128), ([520] * 12, 24, 24, 160, 256), ([2050], 66, 33, 96, 256)])
+                                              ([150, 129, 1, 65, 0, 77] * 9, 16, 8, 104, 128), ([150, 129, 1, 65, 0, 77] * 18, 16, 16, 88, 128), ([520] * 12, 24, 24, 160, 256), ([2050], 66, 33, 96, 256),
+                                              ([77, 127, 64, 1], 12, 4, 64, 128), ([77, 127, 128, 1], 4, 1, 128, 128)])
 def test_attention_forms_by_the_prompts_lengths(lens, h, hk, d, rows, dtype):
     """Prompts of a token, of a whole tile, of one more, and of none."""
     pr, ffi = pkg("prompt"), pkg("ffi")
