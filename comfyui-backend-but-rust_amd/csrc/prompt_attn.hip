@@ -507,7 +507,7 @@ inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n;
 // one of 231 13.3 and 12.1, 16.1 and 15.6).
 // Many prompts of fewer rows than half such a tile in tiles of 64 (64 prompts to 20 tokens of 16 heads: of 64 channels 9.1 for 10.6, of 96 10.9 for 13.7, of 128 10.7 for 14.4, of 256
 // 28.4 for 37.7; to 77 tokens, 46 rows, of 64 13.4 for 13.0, and of 20 heads 14.8 for 16.6; of 96 22.8 for 21.0; of 192 never: 34 for 21).
-// The other head dims, 256 rows or 128: of 96 48 prompts to 160 tokens 33.7 and 26.1, 8 to 2500 142 and 131, 6 to 2500 of 16 over 4 heads 108 and 116; of 192 24 to 600, mean 360, 119
+// The other head dims, 256 rows or 128 (of 96 128: 48 prompts to 160 tokens 33.7 and 26.1, 8 to 2500 142 and 131): of 192 24 to 600, mean 360, 119
 // and 111, 12 to 1200 145 and 157; of 256 24 to 600 174 and 177, 8 to 2500 416 and 522.
 struct Form {
     int rows, keys, blocks;
@@ -523,9 +523,17 @@ inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
         if (dp == 128 && f.rows == 128) f.blocks = mean >= 160 ? 2 : 1;
         return f;
     }
-    const bool long_enough = dp == 96 ? each >= 4000 : dp == 192 ? mean >= 500 : each >= 32;
-    f.rows = wide >= 2 * cus && long_enough ? 256 : dp != 192 && each < 32 ? 64 : 128;
+    const bool long_enough = dp == 192 ? mean >= 500 : each >= 32;
+    f.rows = dp != 96 && wide >= 2 * cus && long_enough ? 256 : dp != 192 && each < 32 ? 64 : 128;
     return f;
+}
+
+// The channels that a call is padded to.  Of 72 to 96 there are 128 in the pipelined kernel, where few tiles leave CUs idle (one prompt of 2500 tokens of 16 heads of 96 51 us, 113 in
+// 96; three to 700 of 16 over 4 heads 23 and 31), and for long prompts (10 to 2500, mean 1500, 160 and 184; 16 to 1200, mean 720, 76 and 68).
+inline int dim_of(int head_dim, int64_t tokens, int n, int group, int hk) {
+    const int dp = padded_dim(head_dim, 64);
+    if (dp != 96) return dp;
+    return tokens / n >= (tiles_of(tokens * group, n, 256) * hk <= device_cu_count() ? 128 : 1000) ? 128 : 96;
 }
 
 template <class Src, int DP, int KG> int launch_pipe(Common& a, const PackedArgs& sa, int64_t grid, hipStream_t st) {
@@ -551,7 +559,6 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStre
         if constexpr (DP == 64) prompt_kernel<Src, DP, 8, 2, 1, 4><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 192) prompt_kernel<Src, DP, 8, 2, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 256) prompt_kernel<Src, DP, 8, 1, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
-        else if constexpr (DP == 96) prompt_kernel<Src, DP, 8, 2, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
     } else if (f.rows == 64) {
         if constexpr (DP != 192) prompt_kernel<Src, DP, 2, 1, 1, DP == 64 ? 4 : DP == 256 ? 1 : 2><<<(int)grid, 128, 0, st>>>(a, sa);
     } else {
@@ -567,7 +574,7 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStre
     return 0;
 }
 template <class Src> int launch_dim(Common& a, const PackedArgs& sa, hipStream_t st) {
-    switch (padded_dim(a.d, 64)) {
+    switch (dim_of(a.d, sa.tokens, sa.n, a.group, a.hk)) {
         case 64: return launch<Src, 64>(a, sa, st);
         case 96: return launch<Src, 96>(a, sa, st);
         case 128: return launch<Src, 128>(a, sa, st);
@@ -604,7 +611,7 @@ GPU_API int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs
 
 GPU_API int gpu_internal_prompt_attn_form(int tokens, int n, int h, int hk, int head_dim, int32_t* out) {
     if (tokens <= 0 || n <= 0 || h <= 0 || hk <= 0 || h % hk != 0 || head_dim <= 0 || head_dim > 256 || !out) return -1;
-    const Form f = form_of(tokens, n, h / hk, hk, padded_dim(head_dim, 64));
+    const Form f = form_of(tokens, n, h / hk, hk, dim_of(head_dim, tokens, n, h / hk, hk));
     out[0] = f.rows;
     out[1] = f.keys;
     return 0;

@@ -114,7 +114,7 @@ def test_attention_past_32_bits():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda t: str(t)[6:])
 @pytest.mark.parametrize("lens,h,hk,d,rows", [([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 64, 64), ([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 40, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 80, 64),
                                               ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 128, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 256, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 192, 128),
-                                              ([150, 129, 1, 65, 0, 77] * 9, 16, 8, 104, 128), ([150, 129, 1, 65, 0, 77] * 18, 16, 16, 88, 128), ([520] * 12, 24, 24, 160, 256), ([2050], 66, 33, 96, 256),
+                                              ([150, 129, 1, 65, 0, 77] * 9, 16, 8, 104, 128), ([150, 129, 1, 65, 0, 77] * 18, 16, 16, 88, 128), ([520] * 12, 24, 24, 160, 256), ([520] * 12, 24, 24, 96, 128), ([77, 127, 64, 1], 12, 4, 80, 128),
                                               ([77, 127, 64, 1], 12, 4, 64, 128), ([77, 127, 128, 1], 4, 1, 128, 128)])
 def test_attention_forms_by_the_prompts_lengths(lens, h, hk, d, rows, dtype):
     """Prompts of a token, of a whole tile, of one more, and of none."""
@@ -138,6 +138,32 @@ def test_attention_forms_by_the_prompts_lengths(lens, h, hk, d, rows, dtype):
     v[hole, :, 3] = math.nan
     o = pr.attn(q, k, v, at, d ** -0.5)
     assert o[hole:end, :, 3].isnan().all() and not o[:hole].isnan().any() and not o[end:].isnan().any() and not o[..., 4:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize("lens,h,hk,d,form", [([2050], 66, 33, 96, (256, 1)), ([1300, 3, 900, 1], 6, 3, 72, (128, 2)), ([200], 5, 5, 80, (128, 2)), ([129, 150], 4, 1, 88, (128, 2))])
+def test_attention_of_72_to_96_channels_as_128(lens, h, hk, d, form, dtype):
+    """Rows at other addresses than whole 16 bytes too, and numbers behind the channels that there are: not read as channels."""
+    pr, ffi = pkg("prompt"), pkg("ffi")
+    T, out = sum(lens), (ctypes.c_int32 * 2)()
+    ffi.k("gpu_internal_prompt_attn_form", T, len(lens), h, hk, d, ctypes.cast(out, ctypes.c_void_p))
+    assert tuple(out) == form
+    starts = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    wide = torch.full((T, h + 2 * hk, 128), math.nan, dtype=dtype, device=DEV)
+    wide[..., :d] = _randn(90, T, h + 2 * hk, d, size=1.3).to(dtype)
+    qkv = wide[..., :d]
+    q, k, v = qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]
+    at = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    out = torch.full((T, h, 128), 7.0, dtype=dtype, device=DEV)
+    o = pr.attn(q, k, v, at, d ** -0.5, out=out[..., :d])
+    heads = slice(h - 2 * h // hk, h), slice(hk - 2, hk)
+    if hk == 1:
+        heads = slice(0, h), slice(0, 1)
+    _attn_check(o[:, heads[0]], q[:, heads[0]], k[:, heads[1]], v[:, heads[1]], starts, d ** -0.5, True, "causal")
+    assert (out[..., d:] == 7).all()
+    room = [torch.zeros(t.numel() + 1, dtype=dtype, device=DEV)[1:].view(t.shape).copy_(t) for t in (q, k, v)]
+    far = pr.attn(*room, at, d ** -0.5)
+    _attn_check(far[:, heads[0]], q[:, heads[0]], k[:, heads[1]], v[:, heads[1]], starts, d ** -0.5, True, "odd addresses")
 
 
 def test_outputs_with_rows_that_share_memory_and_other_ranks_are_refused():
