@@ -167,32 +167,62 @@ __device__ __forceinline__ void store_rows(const Common& a, const PackedArgs& sa
     }
 }
 
-// QW waves of 32 rows on the same keys, 32 NB at a time in two LDS buffers: a tile is on its way into registers while the one before goes into
+// The waves of the same rows: the first takes the others' numerators, sums and bases, in their order, through LDS that is idle.
+template <int DB, int KG, int RG> constexpr int kJoinBytes = (KG - 1) * RG * (DB * 16 + 2) * 256;
+template <class Src, int DB, int KG, int RG, class L_> __device__ __forceinline__ void join_waves(L_& L, uint8_t* lds, int kg, int rg, int lane) {
+    __syncthreads();
+    float* const out = reinterpret_cast<float*>(lds) + ((kg - 1) * RG + rg) * (DB * 16 + 2) * 64 + lane;
+    if (kg > 0) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) out[(16 * i + j) * 64] = L.acc[0][i][j];
+        out[DB * 16 * 64] = L.base[0];
+        out[(DB * 16 + 1) * 64] = L.sum[0];
+    }
+    __syncthreads();
+    if (kg == 0)
+#pragma unroll 1
+        for (int k = 1; k < KG; ++k) {
+            const float* const in = reinterpret_cast<const float*>(lds) + ((k - 1) * RG + rg) * (DB * 16 + 2) * 64 + lane;
+            const float base = in[DB * 16 * 64], nb = fmaxf(L.base[0], base);
+            const Rebase<Src> mine_by(L.base[0], nb), its(base, nb);
+            L.base[0] = nb;
+            L.sum[0] = fmaf(in[(DB * 16 + 1) * 64], its.f, L.sum[0] * mine_by.f);
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) L.acc[0][i][j] = fmaf(in[(16 * i + j) * 64], its.f, L.acc[0][i][j] * mine_by.f);
+        }
+}
+
+// QW waves of 32 rows on the same keys, or QW / KG of which KG waves each share the keys, 32 NB at a time in two LDS buffers: a tile is on its way into registers while the one before goes into
 // LDS and the one before that is multiplied, SB blocks of 32 keys per step of the softmax.
-template <class Src, int DP, int QW, int NB, int SB, int OCC>
+template <class Src, int DP, int QW, int NB, int SB, int OCC, int KG = 1>
 __global__ __launch_bounds__(64 * QW, OCC) void prompt_kernel(const Common a, const PackedArgs sa) {
-    constexpr int TK = 32 * NB, TILE_K = TK * kRowK<DP>, TILE_V = TK * kRowV<DP>;
+    constexpr int TK = 32 * NB, TILE_K = TK * kRowK<DP>, TILE_V = TK * kRowV<DP>, RG = QW / KG, MB = NB / KG;      // (MB: blocks of a wave)
+    static_assert(MB % SB == 0 && (KG == 1 || kJoinBytes<DP / 32, KG, RG> <= 2 * (TILE_K + TILE_V)), "whole steps, and room to join in");
     __shared__ __align__(16) uint8_t lds[2 * (TILE_K + TILE_V)];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 5, rg = KG == 1 ? wave : wave % RG, kg = KG == 1 ? 0 : wave / RG, mine = 32 * MB * kg;
     // workgroups are dealt to the XCDs in turn: each has its own heads where their number allows, and as many long tiles as the others
     const int slot = blockIdx.x / a.hk, head = blockIdx.x - slot * a.hk;
     Place at;
-    if (!find(sa, a.group, 32 * QW, slot, at)) return;
+    if (!find(sa, a.group, 32 * RG, slot, at)) return;
     Problem pr;
     pr.q_at = at.first * a.q_rs + head * a.group * a.q_hs;
     pr.o_at = at.first * a.o_rs + head * a.group * a.o_hs;
     pr.tokens = pr.keys = at.count;
     pr.limit0 = sa.causal ? 1 : at.count;
-    const int rows = pr.tokens * a.group, r0 = at.tile * 32 * QW, wr = r0 + 32 * wave;
-    const int end = min(pr.keys, pr.limit0 + (min(rows, r0 + 32 * QW) - 1) / a.group), t1 = (end + TK - 1) / TK;
-    const int sees = min(pr.keys, pr.limit0 + (min(rows, wr + 32) - 1) / a.group), t_mine = wr < rows ? (sees + TK - 1) / TK : 0;      // of this wave's rows
+    const int rows = pr.tokens * a.group, r0 = at.tile * 32 * RG, wr = r0 + 32 * rg;
+    const int end = min(pr.keys, pr.limit0 + (min(rows, r0 + 32 * RG) - 1) / a.group), t1 = (end + TK - 1) / TK;
+    const int sees = min(pr.keys, pr.limit0 + (min(rows, wr + 32) - 1) / a.group), t_mine = wr < rows ? max(0, sees - mine + TK - 1) / TK : 0;      // of this wave's rows and keys
     typename Src::template Stage<DP, TK, 64 * QW> st(sa, a.d, at.first, head, pr.keys, threadIdx.x);
     st.load(0);
     Lanes<Src, DP, 1> L;
     L.start(a, pr, wr, rows, lane);
     uint8_t *kb = lds, *vb = lds + 2 * TILE_K;                       // the tile that is multiplied
     uint8_t *kn = lds + TILE_K, *vn = lds + 2 * TILE_K + TILE_V;     // and the one behind it
-    const int at_k = lane_k<DP>(lane), at_v = lane_v<DP>(lane);
+    const int at_k = lane_k<DP>(lane) + mine * kRowK<DP>, at_v = lane_v<DP>(lane) + mine * kRowV<DP>;
     const int edge = min(pr.keys, pr.limit0 + r0 / a.group) / TK;      // tiles before this one are seen whole by every row
     bool found = false;
     if (edge == 0) found |= st.clean();
@@ -210,13 +240,13 @@ __global__ __launch_bounds__(64 * QW, OCC) void prompt_kernel(const Common a, co
         uint8_t* const v = vb; vb = vn; vn = v;
     };
     for (int t = 0; t < t_mine; ++t) {
-        const bool plain = (t + 1) * TK <= L.all_see;
+        const bool plain = t * TK + mine + 32 * MB <= L.all_see;
 #pragma unroll
-        for (int b = 0; b < NB; b += SB) {
+        for (int b = 0; b < MB; b += SB) {
             f16acc s[SB][1];
             float kc[1][2 * SB], from[1];
             L.scores(s, kb + at_k + 32 * b * kRowK<DP>, (const float*)nullptr, g);
-            L.raise(s, kc, from, sc, t * TK + 32 * b, plain, true, g);
+            L.raise(s, kc, from, sc, t * TK + mine + 32 * b, plain, true, g);
 #pragma unroll
             for (int h = 0; h < 2 * SB; ++h) {
                 u32x4 p[1];
@@ -228,8 +258,8 @@ __global__ __launch_bounds__(64 * QW, OCC) void prompt_kernel(const Common a, co
     }
     for (int t = t_mine; t < t1; ++t) next(t);      // tiles that only other waves' rows see (in a loop of its own: a branch around the products costs registers)
     L.finish(st, 0, end);
-
-    store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, rows, lane);
+    if constexpr (KG > 1) join_waves<Src, DP / 32, KG, RG>(L, lds, kg, rg, lane);
+    store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, kg == 0 ? rows : 0, lane);
 }
 
 // ---- head dims to 64 and to 128: products of the next tile under the softmax of this one -------------------------------------------
@@ -463,40 +493,15 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
         for (int t = max(piped, t_mine); t < t1; ++t) next(t);      // tiles that only other waves' rows see (in a loop of its own: a branch around the products costs registers)
     }
     L.finish(st, 0, end);
-    if constexpr (KG > 1) {      // the waves of the same rows: the first takes the others' numerators, sums and bases, in their order
-        __syncthreads();
-        float* const out = reinterpret_cast<float*>(lds) + ((kg - 1) * RG + rg) * (DB * 16 + 2) * 64 + lane;
-        if (kg > 0) {
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) out[(16 * i + j) * 64] = L.acc[0][i][j];
-            out[DB * 16 * 64] = L.base[0];
-            out[(DB * 16 + 1) * 64] = L.sum[0];
-        }
-        __syncthreads();
-        if (kg == 0)
-#pragma unroll 1
-            for (int k = 1; k < KG; ++k) {
-                const float* const in = reinterpret_cast<const float*>(lds) + ((k - 1) * RG + rg) * (DB * 16 + 2) * 64 + lane;
-                const float base = in[DB * 16 * 64], nb = fmaxf(L.base[0], base);
-                const Rebase<Src> mine_by(L.base[0], nb), its(base, nb);
-                L.base[0] = nb;
-                L.sum[0] = fmaf(in[(DB * 16 + 1) * 64], its.f, L.sum[0] * mine_by.f);
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) L.acc[0][i][j] = fmaf(in[(16 * i + j) * 64], its.f, L.acc[0][i][j] * mine_by.f);
-            }
-    }
+    if constexpr (KG > 1) join_waves<Src, DB, KG, RG>(L, lds, kg, rg, lane);
     store_rows<Src, DP>(a, sa, pr, L, st, edge * TK, found, wr, kg == 0 ? rows : 0, lane);
 }
 
 // Row tiles of a head: all rows' and a partial one for each prompt.
 inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n; }
 
-// How a call runs: tiles of `rows` rows, of whose keys `keys` waves each take a part (prompt_pipe_kernel), or 0: prompt_kernel, 32 `blocks` keys at a
-// time where there is a choice.
+// How a call runs: tiles of `rows` rows, of whose keys `keys` waves each take a part, or 0: one wave has them all, in
+// prompt_kernel.  Head dims to 64 and to 128 run in prompt_pipe_kernel where `keys` is not 0, the others always in prompt_kernel, 32 `blocks` keys at a time where there is a choice.
 // Head dims to 64 and to 128.  Where tiles of 256 rows fill the CUs: the pipelined kernel, but for prompts that are short in the mean, which are
 // mostly tiles with an edge, and of which prompt_kernel has two workgroups on a CU (us, bf16: 48 prompts to 231 tokens of 20 heads of 64 40.8 and
 // 28.7; 12 to 800, mean 480, 43 and 37, 39 with 128 rows; 4 to 2500 67 and 84; of 16 heads of 128 24 to 400, mean 240, 45 and 37; 8 to 1300, mean 780, 58
@@ -509,6 +514,9 @@ inline int64_t tiles_of(int64_t rows, int n, int tile) { return rows / tile + n;
 // 28.4 for 37.7; to 77 tokens, 46 rows, of 64 13.4 for 13.0, and of 20 heads 14.8 for 16.6; of 96 22.8 for 21.0; of 192 never: 34 for 21).
 // The other head dims, 256 rows or 128 (of 96 128: 48 prompts to 160 tokens 33.7 and 26.1, 8 to 2500 142 and 131): of 192 24 to 600, mean 360, 119
 // and 111, 12 to 1200 145 and 157; of 256 24 to 600 174 and 177, 8 to 2500 416 and 522.
+// And where there are few tiles a row's keys over two waves: of 192 in tiles of 128 rows (one prompt of 300 tokens of 16 heads 21 us, 26 with one wave to a row, of 700 36 and 56, of 8000 of
+// 8 over 4 heads 315 and 577; 16 to 300 24 and 33; one of 77 15.3 and 14.9; 24 to 600 of 16 over 4 heads, 820 tiles, 93 and 75), of 256 in tiles of 64, since eight waves' registers do not
+// hold it (16 heads 300 27 and 29, 700 45 and 58, 2500, 640 tiles, 178 and 176; of 8 over 4 heads 2500 116 and 175, 16 to 300, mean 165, 41 and 35).
 struct Form {
     int rows, keys, blocks;
 };
@@ -525,6 +533,8 @@ inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
     }
     const bool long_enough = dp == 192 ? mean >= 500 : each >= 32;
     f.rows = dp != 96 && wide >= 2 * cus && long_enough ? 256 : dp != 192 && each < 32 ? 64 : 128;
+    if (f.rows == 128 && dp == 192 && mean >= 128 && tiles_of(rows, n, 128) * hk <= 2 * cus) f.keys = 2;
+    if (f.rows == 128 && dp == 256 && mean >= 200 && tiles_of(rows, n, 64) * hk <= 2 * cus) f.keys = 2, f.rows = 64;
     return f;
 }
 
@@ -560,14 +570,20 @@ template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStre
         else if constexpr (DP == 192) prompt_kernel<Src, DP, 8, 2, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
         else if constexpr (DP == 256) prompt_kernel<Src, DP, 8, 1, 1, 2><<<(int)grid, 512, 0, st>>>(a, sa);
     } else if (f.rows == 64) {
-        if constexpr (DP != 192) prompt_kernel<Src, DP, 2, 1, 1, DP == 64 ? 4 : DP == 256 ? 1 : 2><<<(int)grid, 128, 0, st>>>(a, sa);
+        if constexpr (DP == 256) {
+            if (f.keys == 2) prompt_kernel<Src, DP, 4, 2, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
+            else prompt_kernel<Src, DP, 2, 1, 1, 1><<<(int)grid, 128, 0, st>>>(a, sa);
+        } else if constexpr (DP != 192) prompt_kernel<Src, DP, 2, 1, 1, DP == 64 ? 4 : 2><<<(int)grid, 128, 0, st>>>(a, sa);
     } else {
         if constexpr (DP == 64) prompt_kernel<Src, DP, 4, 1, 1, 4><<<(int)grid, 256, 0, st>>>(a, sa);
         else if constexpr (DP == 96) prompt_kernel<Src, DP, 4, 1, 1, 3><<<(int)grid, 256, 0, st>>>(a, sa);
         else if constexpr (DP == 128) {
             if (f.blocks == 1) prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
             else prompt_kernel<Src, DP, 4, 2, 2, 2><<<(int)grid, 256, 0, st>>>(a, sa);
-        } else if constexpr (DP == 192) prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
+        } else if constexpr (DP == 192) {
+            if (f.keys == 2) prompt_kernel<Src, DP, 8, 2, 1, 2, 2><<<(int)grid, 512, 0, st>>>(a, sa);
+            else prompt_kernel<Src, DP, 4, 1, 1, 2><<<(int)grid, 256, 0, st>>>(a, sa);
+        }
         else prompt_kernel<Src, DP, 4, 1, 1, 1><<<(int)grid, 256, 0, st>>>(a, sa);
     }
     KCHECK();

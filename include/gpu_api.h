@@ -417,7 +417,7 @@ int gpu_internal_fp8_gemm_plan(int64_t M, int64_t N, int64_t K, int out_dt, int3
 int gpu_internal_fp8_gemm_force(int form_and_slices);
 
 /* Test hook, no reference counterpart: how gpu_prompt_attn runs `tokens` tokens of n prompts.  out[0] = rows of a workgroup, out[1] = waves that share a
- * row's keys in the pipelined kernel, 0 for the other. */
+ * row's keys (of head dims to 128 in the pipelined kernel, where that may be 1), 0: none. */
 int gpu_internal_prompt_attn_form(int tokens, int n, int h, int hk, int head_dim, int32_t* out);
 
 /* Test hook, no reference counterpart: how gpu_cross_attn (bytes 2) and gpu_kv8_attn (bytes 1) run `problems` (batch items or sequences times

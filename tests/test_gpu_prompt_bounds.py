@@ -115,13 +115,15 @@ def test_attention_past_32_bits():
 @pytest.mark.parametrize("lens,h,hk,d,rows", [([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 64, 64), ([20, 64, 1, 65, 0, 33, 77, 2] * 9, 16, 16, 40, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 80, 64),
                                               ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 128, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 256, 64), ([20, 64, 1, 65, 0, 5] * 9, 12, 12, 192, 128),
                                               ([150, 129, 1, 65, 0, 77] * 9, 16, 8, 104, 128), ([150, 129, 1, 65, 0, 77] * 18, 16, 16, 88, 128), ([520] * 12, 24, 24, 160, 256), ([520] * 12, 24, 24, 96, 128), ([77, 127, 64, 1], 12, 4, 80, 128),
-                                              ([77, 127, 64, 1], 12, 4, 64, 128), ([77, 127, 128, 1], 4, 1, 128, 128)])
+                                              ([77, 127, 64, 1], 12, 4, 64, 128), ([77, 127, 128, 1], 4, 1, 128, 128),
+                                              ([900, 130, 1], 4, 2, 160, (128, 2)), ([129, 127, 0, 300, 104], 6, 6, 192, (128, 2)), ([900, 130, 1], 4, 2, 256, (64, 2)), ([33, 500, 64, 1, 600], 6, 3, 200, (64, 2)),
+                                              ([100, 33], 4, 2, 160, 128), ([199], 4, 2, 256, 128)])
 def test_attention_forms_by_the_prompts_lengths(lens, h, hk, d, rows, dtype):
     """Prompts of a token, of a whole tile, of one more, and of none."""
     pr, ffi = pkg("prompt"), pkg("ffi")
     T, out = sum(lens), (ctypes.c_int32 * 2)()
     ffi.k("gpu_internal_prompt_attn_form", T, len(lens), h, hk, d, ctypes.cast(out, ctypes.c_void_p))
-    assert tuple(out) == (rows, 0)
+    assert tuple(out) == (rows if isinstance(rows, tuple) else (rows, 0))
     starts = [sum(lens[:i]) for i in range(len(lens) + 1)]
     qkv = _randn(80, T, h + 2 * hk, d, size=1.3).to(dtype)
     q, k, v = qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]
