@@ -375,7 +375,7 @@ int gpu_kv8_copy_pages(int8_t* ck, int8_t* cv, float* k_scale, float* v_scale, i
  *   A = max(largest |n| of the group, 2^-100), scales[g * scales_stride + m] = A / 448, q[m, k] = e4m3(n * (448 / A)), nearest even
  * x, resid, sum: T[M, stride], dtype bf16, f16 or f32 (else -4), dense rows at any stride; sum may be x or resid, with its stride.
  * norm_w f32 [K].  q [M, K], 8-byte aligned; scales f32 [ceil(K / 128), scales_stride], scales_stride >= M; the last group may be part of one.
- * A group that holds a NaN or an infinity stands for NaN throughout.  K a multiple of 16 (-1) up to 32768 (-2); -3 prologue. */
+ * A group that holds a NaN or an infinity stands for NaN throughout.  K a multiple of 16 (-1) up to 32768 (-2); M up to 8388607 at least (-1); -3 prologue. */
 int gpu_fp8_quant_rows(int dtype, int prologue, const void* x, int64_t x_stride, const void* resid, int64_t resid_stride, void* sum,
                        int64_t sum_stride, int64_t up_offset, const float* norm_w, float eps, void* q, float* scales,
                        int64_t scales_stride, int M, int K, void* stream);
@@ -394,7 +394,8 @@ int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_strid
  * last axis) the first `rot` channels are pairs, (j, j + rot / 2) or, interleaved, (2j, 2j + 1); pair j of token t turns by the angle
  * positions[t] * freqs[j] (radians; 64 bits), (a, b) -> factor * (a cos - b sin, a sin + b cos); the other channels stay.  With q_norm or k_norm
  * (f32 [d]) the heads of that side are first divided by sqrt(mean(x^2) + eps) over d and multiplied by it.  fp32 throughout, rounded
- * once.  Outputs may be the inputs, with their strides.  d and rot multiples of 4, d up to 256, up to 65536 heads (-1); either side may have 0 heads. */
+ * once.  Outputs may be the inputs, with their strides.  d and rot multiples of 4, d up to 256, up to 65536 heads, T up to
+ * 16777215 at least (-1); either side may have 0 heads. */
 int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, int64_t qo_rs, int64_t qo_hs, int h, const void* k,
              int64_t k_rs, int64_t k_hs, void* k_out, int64_t ko_rs, int64_t ko_hs, int hk, const int32_t* positions, const double* freqs,
              int rot, int interleaved, float factor, const float* q_norm, const float* k_norm, float eps, int T, int head_dim, void* stream);
