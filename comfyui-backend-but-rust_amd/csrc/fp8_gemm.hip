@@ -451,7 +451,6 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
         v8i w[FN], a;
         float s[FM], ws;
     };
-    BlockScales scales(ws, g0, n > 0 ? end : g0 + 1, lane);
     int get = 0;
     const auto read = [&](const uint8_t* at, int o) { return two(*reinterpret_cast<const v4i*>(at + o), *reinterpret_cast<const v4i*>(at + (o ^ 64))); };
     const auto begin = [&](First& f) {      // of the stage `get`
@@ -498,6 +497,7 @@ __global__ void __launch_bounds__(512, 1) fp8_gemm_mid_kernel(const Fp8Gemm p) {
     };
     static_assert(FM % 2 == 0, "row tiles alternate between two sets of sums");
     if (n > 0) {
+        BlockScales scales(ws, g0, end, lane);
         First f[2];
         meet();
         begin(f[0]);
@@ -809,7 +809,12 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
     const int64_t cus = device_cu_count(), groups = (K + kGroup - 1) / kGroup;
     Plan p{kAny, 1, (N + 31) / 32 >= 2 * cus ? 2 : 1};
     const bool fits = K >= kGroup && K < (1 << 23);
-    const auto at_most = [&](int64_t s) { return (int)(s < 1 ? 1 : s > groups ? groups : s > 32 ? 32 : s); };
+    // (as many as have groups: slices of ceil(groups / s) may use them up before the last, which would begin behind the scales)
+    const auto at_most = [&](int64_t s) {
+        s = s < 1 ? 1 : s > groups ? groups : s > 32 ? 32 : s;
+        const int64_t share = (groups + s - 1) / s;
+        return (int)((groups + share - 1) / share);
+    };
     const int force = g_force.load(std::memory_order_relaxed);
     if (force >= 0) {
         p.form = force / 100;
@@ -832,12 +837,14 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
     } halves[] = {{kMid64, 64, 128, 4.2, 0.36, 0.45}, {kMid128, 128, 128, 4.5, 0.50, 0.62}, {kBig, 256, 256, 6.0, 1.3, 1.65}, {kWide, 128, 128, 5.5, 0.48, 1.19}},
       wide[] = {{kMid64, 64, 128, 5.0, 0.62, 0.62}, {kMid128, 128, 128, 5.0, 1.02, 1.02}};
     const bool words = out_dt == DT_F32;
+    const int most = at_most(groups);
     double least = 0.;
     for (int i = 0; i < (words ? 2 : 4); ++i) {
         const auto& f = words ? wide[i] : halves[i];
         const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
-        for (int s = 1; s == 1 || (f.form != kBig && f.form != kWide && s <= at_most(groups) && tiles * s <= 2 * cus); ++s) {
+        for (int s = 1; s == 1 || (f.form != kBig && f.form != kWide && s <= most && tiles * s <= 2 * cus); ++s) {
             const int64_t slots = f.form == kWide ? 2 * cus : cus, whole = tiles * s / slots, left = tiles * s % slots, steps = (groups + s - 1) / s;
+            if ((s - 1) * steps >= groups) continue;
             const double part = left ? f.alone + (f.full - f.alone) * left / slots : 0.;      // of the last round's groups
             const double us = (f.form == kWide ? f.start + (whole * f.full + part) * steps
                                : words         ? f.start + (whole + (left != 0)) * f.full * steps
