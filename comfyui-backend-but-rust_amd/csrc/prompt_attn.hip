@@ -92,19 +92,29 @@ template <int DTYPE> struct Packed {
 };
 
 // Which prompt the tile `slot` of a key-value head's row tiles lies in: a wave counts the tiles of 64 prompts at a time.  `starts` is device data
-// that the host has not seen: everything from it is brought into 0 .. tokens.
+// that the host has not seen: everything from it is brought into 0 .. tokens, and one that is below an earlier one counts as that one, so that no
+// row belongs to two prompts, whose workgroups would both write it, and the tiles are no more than the launch has.
 struct Place {
     int first, count, tile;      // the prompt's tokens; its row tile, the last one first: those have the most keys
 };
 __device__ __forceinline__ bool find(const PackedArgs& a, int group, int tile_rows, int slot, Place& p) {
     const int lane = threadIdx.x & 63;
+    int high = 0;      // the largest of the starts before
     for (int s0 = 0; s0 < a.n; s0 += 64) {
         const int s = s0 + lane;
-        int first = 0, count = 0;
+        int first = 0, end = 0;
         if (s < a.n) {
             first = min(max(a.starts[s], 0), a.tokens);
-            count = min(max(a.starts[s + 1], first), a.tokens) - first;
+            end = min(max(a.starts[s + 1], 0), a.tokens);
         }
+        if (__any(s < a.n && (first < high || end < first))) {
+            first = max(first, high);
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) first = max(first, __shfl_up(first, d));      // (a lane below d gets its own)
+            end = max(end, first);
+        }
+        high = __builtin_amdgcn_readlane(end, 63);      // (read where another 64 follow)
+        const int count = end - first;
         const int tiles = (count * group + tile_rows - 1) / tile_rows;
         int upto = tiles;
 #pragma unroll

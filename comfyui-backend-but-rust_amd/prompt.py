@@ -88,7 +88,7 @@ def _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out)
 def attn(q, k, v, starts, scale, causal=True, out=None):
     """softmax(scale * q k^T) v within each prompt: rows starts[s] .. starts[s + 1] (int32 [n + 1] on the device) of q [tokens, h, d] and k, v [tokens,
     hk, d] (bf16 or f16, any strides with a dense last axis, h a multiple of hk, d a multiple of 8 up to 256).  Causal: a row sees the keys up to
-    its own.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`, which shares
+    its own.  A start below an earlier one counts as that one.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`, which shares
     no memory with q, k and v."""
     o = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.prompt_attn(q, k, v, starts, float(scale), bool(causal))
     return _attn(q, k, v, starts, scale, causal, out) if o is None else o

@@ -403,8 +403,8 @@ int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, 
 /* Attention over whole prompts that lie one behind the other: rows starts[s] .. starts[s + 1] of q [tokens, h, d], k and v [tokens, hk, d] and o
  * [tokens, h, d] are prompt s (int32 [n + 1] on the device); o = softmax(scale * q k^T) v within it, over the keys up to the row's own
  * (causal) or all.  dtype DT_F16 or DT_BF16 (-4); element strides of tokens and heads, dense last axis; query head j uses key-value head
- * j / (h / hk).  Rows of no prompt are left as they are.  starts that do not grow are brought into 0 .. tokens: rows may then be left
- * out, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key makes it NaN, a value its channel NaN or
+ * j / (h / hk).  Rows of no prompt are left as they are.  starts outside 0 .. tokens are brought there, and one below an earlier one
+ * counts as that one: no row belongs to two prompts, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key makes it NaN, a value its channel NaN or
  * infinite.  o shares no memory with q, k and v.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
  * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 64 rows or more, and n) (-1). */
 int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
