@@ -286,6 +286,22 @@ template <int V> struct ic { static constexpr int value = V; };
 template <int DP> __device__ __forceinline__ int turn(int r) { return DP == 64 ? (r & 2) << 1 | (r >> 2 & 3) : (r & 3) << 2 | (r >> 2 & 3); }
 template <int DP> __device__ __forceinline__ int slot_of(int r, int c) { return r * 2 * DP + ((c ^ turn<DP>(r)) << 4); }
 
+// A row's sum takes the probabilities as they are rounded, as in Lanes::probs, which says why.  Here that is bf16 by v_dot2, and f16, which
+// v_fma_mix reads as fp32, as lo + hi: the other way 16384 tokens take 1009 us for 998 (bf16; 967 with the sum of what is not rounded yet) and 1077 for 1036 (f16; 1083).
+template <int DT> __device__ __forceinline__ float add_two(uint32_t a, uint32_t b, float sum) {
+    if constexpr (DT == DT_BF16) return add2<DT>(a, add2<DT>(b, sum));
+    else {
+        float one = 1.f;
+        asm("" : "+s"(one));      // (a factor that the compiler does not see, or it would convert both and add)
+        const auto pair = [&](uint32_t two) {
+            float lo, hi;
+            unpack_f16x2(two, lo, hi);
+            return fmaf(lo, one, hi);
+        };
+        return sum + (pair(a) + pair(b));
+    }
+}
+
 // A workgroup's 8 waves: 8 / KG groups of 32 rows, which each KG waves share, every one with 64 keys of a tile of 64 KG; what they have of a row
 // meets in LDS at the end.
 //
@@ -293,7 +309,7 @@ template <int DP> __device__ __forceinline__ int slot_of(int r, int c) { return 
 // the products of the sixteen keys before with V and a quarter of the next tile's scores: every slot of the matrix pipe's 8 products (256
 // cycles) has about as many cycles of vector instructions beside it.  K is a tile ahead of V.  Tiles travel by DMA into two LDS stages.  That holds
 // for tiles that every row of the workgroup sees whole; the others, at the diagonal and at the prompt's end, follow in a loop that masks, with
-// their rows through registers, where values that are no numbers are taken out.  16384 tokens of 16 over 4 heads of 128, causal: 951 us, 1.15 PFLOP/s, where
+// their rows through registers, where values that are no numbers are taken out.  16384 tokens of 16 over 4 heads of 128, causal: 1000 us, 1.10 PFLOP/s, where
 // a library's large product reaches 1.35; matrix pipes 59 %, vector issue 50 % busy.
 template <class Src, int DP, int KG>
 __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
@@ -381,15 +397,13 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
             for (int i = 0; i < DB; ++i) L.acc[0][i] *= by.f;
         }
     };
-    // probabilities of eight of sixteen keys (four of this lane's), rounded and in pairs, and their sum
+    // probabilities of eight of sixteen keys (four of this lane's), rounded and in pairs
     const auto probs = [&](const f16acc (&s)[2], float from, int h, int half, u32x4& p) {
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[h >> 1][8 * (h & 1) + 4 * half + i], L.c[0], -from));
         p[2 * half] = pack2<DT>(e[0], e[1]);
         p[2 * half + 1] = pack2<DT>(e[2], e[3]);
-        // (as they are before the rounding: v_dot2, which adds the rounded pairs, keeps the matrix pipe from the other wave; 16384 tokens 1025 us with it, 988 so)
-        L.sum[0] += (e[0] + e[1]) + (e[2] + e[3]);
     };
 
     if (piped) {
@@ -431,6 +445,7 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
                 const int h = u >> 1;
                 if (u < 7) read(u + 1);
                 if (h < 3) probs(now, from, h + 1, u & 1, p[(h + 1) & 1]);
+                L.sum[0] = add_two<DT>(p[h & 1][2 * (u & 1)], p[h & 1][2 * (u & 1) + 1], L.sum[0]);      // (of the keys that are multiplied: nothing waits for it)
                 if (u == 6) top = largest(next[0]);
 #pragma unroll
                 for (int i = 0; i < QH; ++i) next[u >> 2] = mfma<DT>(kf[u & 1][i], L.qf[0][(u & 3) * QH + i], i == 0 && (u & 3) == 0 ? f16acc{} : next[u >> 2]);
