@@ -143,7 +143,7 @@ __device__ __forceinline__ void store_rows(const Common& a, const PackedArgs& sa
     const int row = wr + (lane & 31), token = row / a.group, h = row - token * a.group;
     uint16_t* const op = (uint16_t*)a.o + pr.o_at + token * a.o_rs + h * a.o_hs;
     if (row < rows) {
-        const float inv = L.sum[0] == 0.f ? 0.f : 1.f / L.sum[0];
+        const float inv = 1.f / L.sum[0];      // (a row sees its own key at least: 0 is the sum of scores of -inf alone, and makes it NaN)
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i)
 #pragma unroll

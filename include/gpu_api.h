@@ -404,8 +404,8 @@ int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, 
  * [tokens, h, d] are prompt s (int32 [n + 1] on the device); o = softmax(scale * q k^T) v within it, over the keys up to the row's own
  * (causal) or all.  dtype DT_F16 or DT_BF16 (-4); element strides of tokens and heads, dense last axis; query head j uses key-value head
  * j / (h / hk).  Rows of no prompt are left as they are.  starts outside 0 .. tokens are brought there, and one below an earlier one
- * counts as that one: no row belongs to two prompts, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key makes it NaN, a value its channel NaN or
- * infinite.  o shares no memory with q, k and v.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
+ * counts as that one: no row belongs to two prompts, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key that holds NaN makes it NaN, and so does an
+ * infinite score, but that -inf beside numbers weighs nothing; a value makes its channel NaN or infinite.  o shares no memory with q, k and v.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
  * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 64 rows or more, and n) (-1). */
 int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
                     int64_t v_rs, int64_t v_hs, void* o, int64_t o_rs, int64_t o_hs, const int32_t* starts, int n, int tokens, int h, int hk,
