@@ -21,6 +21,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 #define SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
 
 constexpr int kGroup = 128;
+constexpr int64_t kMostGroups = 0xffffffff / 512;      // a launch has fewer than 2^32 threads
 
 struct Fp8Gemm {
     const uint8_t *A, *W;
@@ -365,7 +366,7 @@ template <int OUT_DT> int launch_big(Fp8Gemm p, hipStream_t st) {
     const auto kern = fp8_gemm_big_kernel<OUT_DT>;
     p.tiles_m = (p.M + BIG - 1) / BIG;
     p.tiles_n = (p.N + BIG - 1) / BIG;
-    if ((int64_t)p.tiles_m * p.tiles_n > 0xffffffffll / 512) return -1;
+    if ((int64_t)p.tiles_m * p.tiles_n > kMostGroups) return -1;
     static PerDeviceOnce once;
     if (const int e = allow_dynamic_lds((const void*)kern, BIG_LDS, once)) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(512), BIG_LDS, st, p);
@@ -823,8 +824,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
         if (p.form == kAny || p.form == kBig || p.form == kWide) p.slices = 1;
         return p;
     }
-    if (M <= 32) {
-        const int64_t tiles = (N + 16 * p.ct - 1) / (16 * p.ct);
+    const int64_t tiles = (N + 16 * p.ct - 1) / (16 * p.ct);
+    if (M <= 32 && tiles <= kMostGroups) {
         p.form = kFew;
         p.slices = at_most(groups / 24 < cus / tiles ? groups / 24 : cus / tiles);
         return p;
@@ -844,7 +845,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int out_dt) {
         const int64_t tiles = ((M + f.bm - 1) / f.bm) * ((N + f.bn - 1) / f.bn);
         for (int s = 1; s == 1 || (f.form != kBig && f.form != kWide && s <= most && tiles * s <= 2 * cus); ++s) {
             const int64_t slots = f.form == kWide ? 2 * cus : cus, whole = tiles * s / slots, left = tiles * s % slots, steps = (groups + s - 1) / s;
-            if ((s - 1) * steps >= groups) continue;
+            if ((s - 1) * steps >= groups || tiles * s > kMostGroups) continue;      // (larger tiles where a launch does not hold so many; where it holds none of them, the form for any size)
             const double part = left ? f.alone + (f.full - f.alone) * left / slots : 0.;      // of the last round's groups
             const double us = (f.form == kWide ? f.start + (whole * f.full + part) * steps
                                : words         ? f.start + (whole + (left != 0)) * f.full * steps
@@ -877,7 +878,7 @@ template <int BM, int OUT_DT, bool WIDE = OUT_DT == DT_F32> int launch_mid(Fp8Ge
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + 127) / 128;
     const int64_t grid = (int64_t)p.tiles_m * p.tiles_n * p.slices;
-    if (grid > 0xffffffffll / 512) return -1;
+    if (grid > kMostGroups) return -1;
     static PerDeviceOnce once;
     if (const int e = allow_dynamic_lds((const void*)kern, LDS, once)) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), LDS, st, p);
@@ -887,7 +888,7 @@ template <int BM, int OUT_DT, bool WIDE = OUT_DT == DT_F32> int launch_mid(Fp8Ge
 template <int MT, int CT, int OUT_DT> int launch_few(Fp8Gemm p, hipStream_t st) {
     p.tiles_n = (p.N + 16 * CT - 1) / (16 * CT);
     const int64_t grid = (int64_t)p.tiles_n * p.slices;
-    if (grid > 0xffffffffll / 512) return -1;
+    if (grid > kMostGroups) return -1;
     fp8_gemm_few_kernel<MT, CT, OUT_DT><<<(int)grid, 512, 0, st>>>(p);
     KCHECK();
     return p.slices > 1 ? launch_join<OUT_DT>(p, st) : 0;

@@ -385,7 +385,7 @@ int gpu_fp8_quant_rows(int dtype, int prologue, const void* x, int64_t x_stride,
  * the last block of rows of W may be parts.  bias Out[N] or null.  Out by out_dt (-4).  K a multiple of 16 (-1).  Sums in fp32, but that for 16-bit
  * outputs the matrix instruction cuts the products of each eight k off at 2^-13 of the largest one's power of two (1.5e-5 of the result on normally
  * distributed operands).  work: gpu_fp8_gemm_workspace bytes (0: null will do), 16-byte aligned (-1), in use until the work queued here has
- * run.  A call gives the same bits every time.  -1 for more than 8388607 workgroups (tiles of 128 x 128 at least from 129 rows on). */
+ * run.  A call gives the same bits every time.  Sizes of 8388607 tiles of 128 x 128 at least (-1). */
 int64_t gpu_fp8_gemm_workspace(int64_t M, int64_t N, int64_t K, int out_dt);
 int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_stride, const float* ws, const void* bias, void* D, void* work,
                  int64_t M, int64_t N, int64_t K, int out_dt, void* stream);
