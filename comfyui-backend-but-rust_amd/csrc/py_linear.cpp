@@ -17,6 +17,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <numeric>
 
 #include "../../include/gpu_api.h"
 

@@ -39,10 +39,10 @@ def _heads(t, tokens, dim, what, like):
 
 def rope(q, k, positions, freqs, interleaved=False, factor=1.0, q_norm=None, k_norm=None, eps=1e-6, out=None):
     """q [tokens, h, d] and k [tokens, hk, d] (bf16, f16 or f32, or k None) with their positions (int32 [tokens]) turned into them, as new tensors
-    or into out = (q_out, k_out), which may be q and k.  The first 2 * len(freqs) channels of each head turn, in pairs of both halves or,
+    or into out = (q_out, k_out), which may be q and k, with their strides, and share no memory else.  The first 2 * len(freqs) channels of each head turn, in pairs of both halves or,
     interleaved, of neighbours; freqs float64: radians a token (rope_freqs).  factor scales what turns.  q_norm, k_norm (float32 [d]): each head
     is RMS-normed with that weight and eps first.  Returns (q_out, k_out)."""
-    y = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.rope(q, k, positions, freqs, bool(interleaved), float(factor), q_norm, k_norm, float(eps))
+    y = None if qlinear._pycalls is None else qlinear._pycalls.rope(q, k, positions, freqs, bool(interleaved), float(factor), q_norm, k_norm, float(eps), out)
     return _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out) if y is None else y
 
 
@@ -78,6 +78,8 @@ def _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out)
             qlinear._apart(ko, "out[1]")
             if ko.shape[1] != hk:
                 raise ValueError("out must be tensors of q's and k's shapes")
+            qlinear._separate(ko, "out[1]", (qo, q, positions, freqs, q_norm, k_norm), (k,))
+        qlinear._separate(qo, "out[0]", (k, positions, freqs, q_norm, k_norm), (q,))
     side = lambda t, heads: (0, 0, 0) if t is None else (t.data_ptr(), t.stride(0), t.stride(1))
     with qlinear._on(q.device) as s:
         ffi.k("gpu_rope", qlinear._TORCH_DT[q.dtype], *side(q, h), *side(qo, h), h, *side(k, hk), *side(ko, hk), hk, positions.data_ptr(), freqs.data_ptr(), 2 * freqs.shape[0],
@@ -88,9 +90,9 @@ def _rope(q, k, positions, freqs, interleaved, factor, q_norm, k_norm, eps, out)
 def attn(q, k, v, starts, scale, causal=True, out=None):
     """softmax(scale * q k^T) v within each prompt: rows starts[s] .. starts[s + 1] (int32 [n + 1] on the device) of q [tokens, h, d] and k, v [tokens,
     hk, d] (bf16 or f16, any strides with a dense last axis, h a multiple of hk, d a multiple of 8 up to 256).  Causal: a row sees the keys up to
-    its own.  A start below an earlier one counts as that one.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`, which shares
-    no memory with q, k and v."""
-    o = None if out is not None or qlinear._pycalls is None else qlinear._pycalls.prompt_attn(q, k, v, starts, float(scale), bool(causal))
+    its own.  A start below an earlier one counts as that one.  Returns o [tokens, h, d]; rows of no prompt are left as they are in `out`, which may be q,
+    with its strides, and shares no memory with q, k and v else."""
+    o = None if qlinear._pycalls is None else qlinear._pycalls.prompt_attn(q, k, v, starts, float(scale), bool(causal), out)
     return _attn(q, k, v, starts, scale, causal, out) if o is None else o
 
 
@@ -111,6 +113,7 @@ def _attn(q, k, v, starts, scale, causal, out):
         qlinear._apart(o, "out")
         if o.shape != q.shape:
             raise ValueError("out must be %s, got %s" % (tuple(q.shape), tuple(o.shape)))
+        qlinear._separate(o, "out", (k, v, starts), (q,))
     with qlinear._on(q.device) as s:
         ffi.k("gpu_prompt_attn", _DT[q.dtype], q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), o.data_ptr(),
               o.stride(0), o.stride(1), starts.data_ptr(), starts.shape[0] - 1, T, h, hk, d, float(scale), 1 if causal else 0, s)

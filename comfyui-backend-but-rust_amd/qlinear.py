@@ -5,6 +5,7 @@ the stream; all arithmetic happens in libgpu_kernels.so.
 import contextlib
 import importlib.machinery
 import importlib.util
+import math
 import os
 
 import torch
@@ -461,7 +462,7 @@ def fp8_quant_rows(x, prologue="plain", norm_w=None, eps=0.0, resid=None, out=No
     """Rows as e4m3 codes with a scale for each group of 128 columns: (q [M, K] float8_e4m3fn, scales float32 [ceil(K / 128), M]), and with a
     residual also the sum x + resid in x's type, (q, scales, sum).  x and resid: [M, K] bf16, f16 or f32, any row stride.  "rms": the rows are
     normed, with weight norm_w (float32 [K]) and eps; "swiglu": x is [M, 2K], silu of its first half times the second.  out: where the sum goes
-    instead of a new tensor; it may be x or resid."""
+    instead of a new tensor; it may be x or resid, with its strides, and shares no memory with them else."""
     y = None if _pycalls is None else _pycalls.fp8_quant_rows(x, _FP8_ROWS.get(prologue, -1), norm_w, float(eps), resid, out)
     return _fp8_quant_rows(x, prologue, norm_w, eps, resid, out) if y is None else y
 
@@ -473,6 +474,66 @@ def _apart(t, what):
         if s < reach:
             raise ValueError("%s must have rows that share no memory, got %s with strides %s" % (what, tuple(t.shape), t.stride()))
         reach += s * (n - 1)
+
+
+def _runs(t):
+    """(address, bytes, [(count, bytes apart), ...]) of the runs of bytes that a tensor has, the widest step last; None where it has none."""
+    if t.numel() == 0:
+        return None
+    width, axes = t.element_size(), []
+    for step, n in sorted((s * t.element_size(), n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if not axes and step <= width:
+            width += (n - 1) * step
+        elif axes and step == axes[-1][0] * axes[-1][1]:
+            axes[-1] = axes[-1][0] * n, axes[-1][1]
+        else:
+            axes.append((n, step))
+    return t.data_ptr(), width, axes
+
+
+def _meet(a, b):
+    """Whether two tensors share a byte."""
+    p, q = a.data_ptr(), b.data_ptr()
+    if p + a.untyped_storage().nbytes() <= q or q + b.untyped_storage().nbytes() <= p:      # (mostly)
+        return False
+    a, b = _runs(a), _runs(b)
+    if a is None or b is None:
+        return False
+    (p, w, x), (q, v, y) = a, b
+    reach = lambda width, axes: width + sum((n - 1) * step for n, step in axes)
+    if p + reach(w, x) <= q or q + reach(v, y) <= p:
+        return False
+    if not x and not y:
+        return True
+
+    def apart(step, first, second):      # columns of the same rows: what each has of every `step` bytes
+        r = (q - p) % step
+        return first <= r and r + second <= step
+
+    if apart(math.gcd(*(step for _, step in x + y)), w, v) or (x and y and x[-1][1] == y[-1][1] and apart(x[-1][1], reach(w, x[:-1]), reach(v, y[:-1]))):
+        return False
+    # else run by run (a second for ten million of them)
+    mine, other = torch.tensor([p], device="cpu"), torch.tensor([q], device="cpu")
+    for n, step in x:
+        mine = (mine[:, None] + torch.arange(n, device="cpu") * step).flatten()
+    for n, step in y:
+        other = (other[:, None] + torch.arange(n, device="cpu") * step).flatten()
+    mine = mine.sort().values
+    i = torch.searchsorted(mine, other - w, right=True)      # the first of mine that ends behind its start
+    return bool(((i < len(mine)) & (mine[i.clamp(max=len(mine) - 1)] < other + v)).any())
+
+
+def _separate(out, what, reads, places=()):
+    """An output shares no memory with the tensors that a call reads while it writes, but may be one of `places` itself, in whose place it goes."""
+    for t in places:
+        if t is not None and out.data_ptr() == t.data_ptr() and out.shape == t.shape and out.dtype == t.dtype and all(n == 1 or s == r for n, s, r in zip(out.shape, out.stride(), t.stride())):
+            continue
+        reads = (*reads, t)
+    for t in reads:
+        if t is not None and _meet(out, t):
+            raise ValueError("%s must share no memory with the call's other tensors%s: %s %s with strides %s at %#x and %s %s with strides %s at %#x do"
+                             % (what, " unless it goes in the place of one, with its strides" if places else "", out.dtype, tuple(out.shape), out.stride(), out.data_ptr(), t.dtype, tuple(t.shape),
+                                t.stride(), t.data_ptr()))
 
 
 def _fp8_quant_rows(x, prologue, norm_w, eps, resid, out):
@@ -496,6 +557,7 @@ def _fp8_quant_rows(x, prologue, norm_w, eps, resid, out):
             _no_grad(t, what)
     if out is not None:
         _apart(out, "out")
+        _separate(out, "out", (norm_w,), (x, resid))
     q = torch.empty((M, K), dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty((-(-K // GROUP), M), dtype=torch.float32, device=x.device)
     total = None if resid is None else torch.empty((M, K), dtype=x.dtype, device=x.device) if out is None else out
@@ -507,7 +569,8 @@ def _fp8_quant_rows(x, prologue, norm_w, eps, resid, out):
 
 def fp8_gemm(A, W, xs, ws, bias=None, out_dtype=torch.bfloat16, D=None):
     """A . W^T of e4m3 operands with block scales: A [M, K] and xs float32 [ceil(K / 128), M] as fp8_quant_rows gives them, W [N, K] with ws
-    float32 [ceil(N / 128), ceil(K / 128)], a scale for each block of 128 x 128; bias [N] in out_dtype."""
+    float32 [ceil(N / 128), ceil(K / 128)], a scale for each block of 128 x 128; bias [N] in out_dtype.  D: where the result goes
+    instead of a new tensor, apart from the operands."""
     y = None if _pycalls is None else _pycalls.fp8_gemm(A, W, xs, ws, bias, out_dtype, D)
     return _fp8_gemm(A, W, xs, ws, bias, out_dtype, D) if y is None else y
 
@@ -518,7 +581,8 @@ def _fp8_gemm(A, W, xs, ws, bias, out_dtype, D):
     M, K = A.shape
     N = W.shape[0]
     G = -(-K // GROUP)
-    D = torch.empty((M, N), dtype=out_dtype, device=A.device) if D is None else D
+    given = D is not None
+    D = D if given else torch.empty((M, N), dtype=out_dtype, device=A.device)
     _dense(A, W, ws, bias, D)
     _want(A, torch.float8_e4m3fn, "A"); _want(W, torch.float8_e4m3fn, "W"); _want(xs, torch.float32, "xs"); _want(ws, torch.float32, "ws"); _want(bias, out_dtype, "bias"); _want(D, out_dtype, "D")
     if out_dtype not in _TORCH_DT:
@@ -532,6 +596,8 @@ def _fp8_gemm(A, W, xs, ws, bias, out_dtype, D):
             if t.device != A.device:
                 raise ValueError("%s must be on A's device, got %s and %s" % (what, t.device, A.device))
             _no_grad(t, what)
+    if given:
+        _separate(D, "D", (A, W, xs, ws, bias))
     with _on(A.device) as s:
         need = ffi.lib.gpu_fp8_gemm_workspace(M, N, K, _TORCH_DT[out_dtype])
         work = torch.empty((need,), dtype=torch.uint8, device=A.device) if need else None

@@ -394,7 +394,7 @@ int gpu_fp8_gemm(const void* A, const void* W, const float* xs, int64_t xs_strid
  * last axis) the first `rot` channels are pairs, (j, j + rot / 2) or, interleaved, (2j, 2j + 1); pair j of token t turns by the angle
  * positions[t] * freqs[j] (radians; 64 bits), (a, b) -> factor * (a cos - b sin, a sin + b cos); the other channels stay.  With q_norm or k_norm
  * (f32 [d]) the heads of that side are first divided by sqrt(mean(x^2) + eps) over d and multiplied by it.  fp32 throughout, rounded
- * once.  Outputs may be the inputs, with their strides.  d and rot multiples of 4, d up to 256, up to 65536 heads, T up to
+ * once.  Outputs may be the inputs, with their strides, and share no memory else.  d and rot multiples of 4, d up to 256, up to 65536 heads, T up to
  * 16777215 at least (-1); either side may have 0 heads. */
 int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, int64_t qo_rs, int64_t qo_hs, int h, const void* k,
              int64_t k_rs, int64_t k_hs, void* k_out, int64_t ko_rs, int64_t ko_hs, int hk, const int32_t* positions, const double* freqs,
@@ -405,7 +405,7 @@ int gpu_rope(int dtype, const void* q, int64_t q_rs, int64_t q_hs, void* q_out, 
  * (causal) or all.  dtype DT_F16 or DT_BF16 (-4); element strides of tokens and heads, dense last axis; query head j uses key-value head
  * j / (h / hk).  Rows of no prompt are left as they are.  starts outside 0 .. tokens are brought there, and one below an earlier one
  * counts as that one: no row belongs to two prompts, nothing outside is touched.  What a row does not see may be no number; of what it sees, a key that holds NaN makes it NaN, and so does an
- * infinite score, but that -inf beside numbers weighs nothing; a value makes its channel NaN or infinite.  o shares no memory with q, k and v.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
+ * infinite score, but that -inf beside numbers weighs nothing; a value makes its channel NaN or infinite.  o may be q, with its strides, and shares no memory with q, k and v else.  Scores, sums and outputs in fp32, probabilities rounded to the row type for the product with v.
  * head_dim a multiple of 8 up to 256, up to 2^30 tokens, and 8388607 workgroups: hk times (tokens * h / hk in tiles of 64 rows or more, and n) (-1). */
 int gpu_prompt_attn(int dtype, const void* q, int64_t q_rs, int64_t q_hs, const void* k, int64_t k_rs, int64_t k_hs, const void* v,
                     int64_t v_rs, int64_t v_hs, void* o, int64_t o_rs, int64_t o_hs, const int32_t* starts, int n, int tokens, int h, int hk,
