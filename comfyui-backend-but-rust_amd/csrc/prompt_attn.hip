@@ -302,7 +302,7 @@ template <int DT> __device__ __forceinline__ float add_two(uint32_t a, uint32_t 
     }
 }
 
-// A workgroup's 8 waves: 8 / KG groups of 32 rows, which each KG waves share, every one with 64 keys of a tile of 64 KG; what they have of a row
+// A workgroup's 8 waves (WHOLE: the head dim is DP): 8 / KG groups of 32 rows, which each KG waves share, every one with 64 keys of a tile of 64 KG; what they have of a row
 // meets in LDS at the end.
 //
 // In iteration t a wave has the scores of tile t in registers.  Sixteen keys at a time it makes probabilities of them, and between those instructions run
@@ -311,7 +311,7 @@ template <int DT> __device__ __forceinline__ float add_two(uint32_t a, uint32_t 
 // for tiles that every row of the workgroup sees whole; the others, at the diagonal and at the prompt's end, follow in a loop that masks, with
 // their rows through registers, where values that are no numbers are taken out.  16384 tokens of 16 over 4 heads of 128, causal: 1000 us, 1.10 PFLOP/s, where
 // a library's large product reaches 1.35; matrix pipes 59 %, vector issue 50 % busy.
-template <class Src, int DP, int KG>
+template <class Src, int DP, int KG, bool WHOLE>
 __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
     constexpr int QW = 8, RG = QW / KG, NS = 2, TK = 64 * KG, TILE = TK * 2 * DP, KS = DP / 16, DB = DP / 32, DT = Src::DT, ND = TILE / 1024 / QW;
     constexpr int QH = KS / 4, VH = DB / 2;      // products of half a slot
@@ -337,17 +337,24 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
     // DMA: a kilobyte an instruction, rows RPI (wave + 8 j) .. of the tile
     constexpr int CPR = DP / 8, RPI = 64 / CPR;
     const int drow = RPI * wave + lane / CPR;
-    // (the same for j: 8 RPI is a multiple of 16.  Chunks behind the head dim are its last one again: q is 0 there, and those channels are not stored)
-    const uint32_t dchunk = 16 * min((lane % CPR) ^ turn<DP>(drow), a.d / 8 - 1);
+    // (the same for j: 8 RPI is a multiple of 16.  Behind the head dim V has its last chunk again, since those channels are not stored; K has zeros, which
+    // no DMA writes over, since q is 0 there and 0 times an infinite key would be none)
+    const int chunk = (lane % CPR) ^ turn<DP>(drow);
+    const uint32_t dchunk = 16 * min(chunk, a.d / 8 - 1);
+    const bool channels = chunk < a.d / 8;
     const uint32_t k_off = 2 * drow * (int)sa.k_rs + dchunk, v_off = 2 * drow * (int)sa.v_rs + dchunk;
     const auto fetch_k = [&](int t, auto stage) {
+        if (WHOLE || channels)
 #pragma unroll
-        for (int j = 0; j < ND; ++j) dma16(lds_base + decltype(stage)::value * TILE + (wave + 8 * j) * 1024, k_off, k0 + (int64_t)(t * TK + 8 * RPI * j) * sa.k_rs);
+            for (int j = 0; j < ND; ++j) dma16(lds_base + decltype(stage)::value * TILE + (wave + 8 * j) * 1024, k_off, k0 + (int64_t)(t * TK + 8 * RPI * j) * sa.k_rs);
     };
     const auto fetch_v = [&](int t, auto stage) {
 #pragma unroll
         for (int j = 0; j < ND; ++j) dma16(lds_base + (NS + decltype(stage)::value) * TILE + (wave + 8 * j) * 1024, v_off, v0 + (int64_t)(t * TK + 8 * RPI * j) * sa.v_rs);
     };
+    if (!WHOLE && piped && !channels)
+#pragma unroll
+        for (int j = 0; j < NS * ND; ++j) *reinterpret_cast<u32x4*>(lds + (wave + 8 * j) * 1024 + 16 * lane) = u32x4{0, 0, 0, 0};
     if (piped) {      // K of tiles 0 .. NS - 1, V of 0 .. NS - 2
         fetch_k(0, ic<0>{});
         fetch_v(0, ic<0>{});
@@ -571,14 +578,19 @@ inline int dim_of(int head_dim, int64_t tokens, int n, int group, int hk) {
     return tokens / n >= (tiles_of(tokens * group, n, 256) * hk <= device_cu_count() ? 128 : 1000) ? 128 : 96;
 }
 
-template <class Src, int DP, int KG> int launch_pipe(Common& a, const PackedArgs& sa, int64_t grid, hipStream_t st) {
+template <class Src, int DP, int KG, bool WHOLE> int launch_pipe_as(Common& a, const PackedArgs& sa, int64_t grid, hipStream_t st) {
     constexpr int LDS = 2 * 2 * 64 * KG * 2 * DP;
-    const auto kern = prompt_pipe_kernel<Src, DP, KG>;
+    const auto kern = prompt_pipe_kernel<Src, DP, KG, WHOLE>;
     static PerDeviceOnce once;
     if (const int e = allow_dynamic_lds((const void*)kern, LDS, once)) return e;
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(512), LDS, st, a, sa);
     KCHECK();
     return 0;
+}
+// (a kernel of its own where no channels are padded: the condition at K's loads costs 16384 tokens 996 us for 987, in f16 1045 for 1019, five prompts of 32 heads 329 for 323; where it is
+// needed, ten prompts to 2500 of 16 heads of 96 take 167 for 164)
+template <class Src, int DP, int KG> int launch_pipe(Common& a, const PackedArgs& sa, int64_t grid, hipStream_t st) {
+    return a.d == DP ? launch_pipe_as<Src, DP, KG, true>(a, sa, grid, st) : launch_pipe_as<Src, DP, KG, false>(a, sa, grid, st);
 }
 template <class Src, int DP> int launch(Common& a, const PackedArgs& sa, hipStream_t st) {
     const Form f = form_of(sa.tokens, sa.n, a.group, a.hk, DP);

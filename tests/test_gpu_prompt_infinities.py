@@ -44,6 +44,29 @@ def test_the_first_keys_of_prompts(lens, h, hk, d, dtype, sign):
                 _check(got[~nan], want[~nan], bound[~nan], "prompt at %d, head %d" % (b, j))
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=name)
+@pytest.mark.parametrize("lens,h,hk,d", [([1000] * 4, 16, 16, 56), ([900, 130], 4, 1, 40), ([1000, 900], 10, 10, 24), ([1000] * 4, 16, 16, 96), ([1000, 300, 1], 4, 2, 120), ([1000] * 4, 16, 16, 120),
+                                         ([290, 70, 310, 1], 16, 16, 104), ([1000, 300], 2, 2, 160), ([1000, 300], 2, 2, 248)], ids=str)
+def test_the_last_channel_of_head_dims_that_are_padded(lens, h, hk, d, dtype, sign):
+    """A key that is infinite in a head's last channel: the padding behind it is none of its channels."""
+    pr = pkg("prompt")
+    T, at = sum(lens), [sum(lens[:i]) for i in range(len(lens) + 1)]
+    qkv = _randn(13, T, h + 2 * hk, d, size=1.3).to(dtype)
+    q, k, v = qkv[:, :h].clone(), qkv[:, h:h + hk].clone(), qkv[:, h + hk:]
+    q[..., -1] = torch.where(q[..., -1] == 0, torch.ones_like(q[..., -1]), q[..., -1])
+    starts = torch.tensor(at, dtype=torch.int32, device=DEV)
+    holes = [b + n for b, e in zip(at[:-1], at[1:]) for n in (5, 70) if b + n < e]
+    k[holes, :, -1] = sign * math.inf
+    out = pr.attn(q, k, v, starts, d ** -0.5)
+    for b, e in zip(at[:-1], at[1:]):
+        row = torch.arange(e - b, device=DEV)
+        seen = (row >= 5) if e - b > 5 else torch.zeros(e - b, dtype=torch.bool, device=DEV)
+        for j in sorted({0, h - 1}):
+            up = seen & (sign * q[b:e, j, -1] > 0)
+            assert out[b:e, j][up].isnan().all() and not out[b:e, j][~up].isnan().any(), (b, j)
+
+
 @pytest.mark.parametrize("T,h,d", [(300, 2, 128), (1000, 16, 128), (77, 2, 64), (300, 2, 192)])
 def test_every_key_of_a_row_at_minus_infinity(T, h, d):
     """All keys infinite against the queries' sign, and finite ones whose products leave fp32 downwards."""
