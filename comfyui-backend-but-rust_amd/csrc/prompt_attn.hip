@@ -309,7 +309,7 @@ template <int DT> __device__ __forceinline__ float add_two(uint32_t a, uint32_t 
 // the products of the sixteen keys before with V and a quarter of the next tile's scores: every slot of the matrix pipe's 8 products (256
 // cycles) has about as many cycles of vector instructions beside it.  K is a tile ahead of V.  Tiles travel by DMA into two LDS stages.  That holds
 // for tiles that every row of the workgroup sees whole; the others, at the diagonal and at the prompt's end, follow in a loop that masks, with
-// their rows through registers, where values that are no numbers are taken out.  16384 tokens of 16 over 4 heads of 128, causal: 1000 us, 1.10 PFLOP/s, where
+// their rows through registers, where values that are no numbers are taken out.  16384 tokens of 16 over 4 heads of 128, causal: 990 to 1040 us, 1.06 to 1.11 PFLOP/s, where
 // a library's large product reaches 1.35; matrix pipes 59 %, vector issue 50 % busy.
 template <class Src, int DP, int KG, bool WHOLE>
 __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
@@ -412,6 +412,10 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
         p[2 * half] = pack2<DT>(e[0], e[1]);
         p[2 * half + 1] = pack2<DT>(e[2], e[3]);
     };
+    // their sum, while they are multiplied, so that nothing waits for it: behind the other instructions of half a slot for bf16 of 128 channels (16384 tokens 989 us, among
+    // them 996), among them else (16384 of f16 1018 and 1034, 8192 of 20 heads of 64 224 and 228)
+    constexpr bool kSumLast = DT == DT_BF16 && DP == 128;
+    const auto sum = [&](const u32x4& p, int half) { L.sum[0] = add_two<DT>(p[2 * half], p[2 * half + 1], L.sum[0]); };
 
     if (piped) {
         wait_vmcnt<(NS - 2) * 2 * ND>();      // K and V of tile 0 at least
@@ -452,7 +456,7 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
                 const int h = u >> 1;
                 if (u < 7) read(u + 1);
                 if (h < 3) probs(now, from, h + 1, u & 1, p[(h + 1) & 1]);
-                L.sum[0] = add_two<DT>(p[h & 1][2 * (u & 1)], p[h & 1][2 * (u & 1) + 1], L.sum[0]);      // (of the keys that are multiplied: nothing waits for it)
+                if (!kSumLast) sum(p[h & 1], u & 1);
                 if (u == 6) top = largest(next[0]);
 #pragma unroll
                 for (int i = 0; i < QH; ++i) next[u >> 2] = mfma<DT>(kf[u & 1][i], L.qf[0][(u & 3) * QH + i], i == 0 && (u & 3) == 0 ? f16acc{} : next[u >> 2]);
@@ -463,6 +467,10 @@ __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, con
                 __builtin_amdgcn_sched_group_barrier(0x008, QH + VH, 0);
                 __builtin_amdgcn_sched_group_barrier(0x402, 24, 0);
                 SCHED_FENCE();
+                if (kSumLast) {
+                    sum(p[h & 1], u & 1);
+                    SCHED_FENCE();
+                }
             }
             rebase(fmaxf(top, largest(next[1])));
             wait_vmcnt<(NS - 2) * 2 * ND>();
@@ -570,8 +578,8 @@ inline Form form_of(int64_t tokens, int n, int group, int hk, int dp) {
     return f;
 }
 
-// The channels that a call is padded to.  Of 72 to 96 there are 128 in the pipelined kernel, where few tiles leave CUs idle (one prompt of 2500 tokens of 16 heads of 96 51 us, 113 in
-// 96; three to 700 of 16 over 4 heads 23 and 31), and for long prompts (10 to 2500, mean 1500, 160 and 184; 16 to 1200, mean 720, 76 and 68).
+// The channels that a call is padded to.  Of 72 to 96 there are 128 in the pipelined kernel, where few tiles leave CUs idle (one prompt of 2500 tokens of 16 heads of 96 52 us, 114 in
+// 96; three to 700 of 16 over 4 heads 23 and 35), and for long prompts (10 to 2500, mean 1500, 169 and 187; 16 to 1200 of 16 over 4 heads, mean 680, 69 and 65).
 inline int dim_of(int head_dim, int64_t tokens, int n, int group, int hk) {
     const int dp = padded_dim(head_dim, 64);
     if (dp != 96) return dp;
