@@ -248,7 +248,7 @@ __device__ __forceinline__ v8i tail_fragment(const uint8_t* x, int row, int limi
 }
 
 // Large sizes: tiles of 256 x 256, eight waves of 128 x 64, two LDS stages: group g + 1 travels while group g is multiplied, one barrier a group.
-// Bound by power: 8192 x 4096 -> 24576 710 us, 2.3 PFLOP/s, matrix pipes 58 % busy at 1.73 GHz (a library product with one scale, which has no folds, 2.98
+// Bound by power: 8192 x 4096 -> 24576 710 to 745 us by the box, 2.2 to 2.3 PFLOP/s, matrix pipes 58 % busy at 1.73 GHz (a library product with one scale, which has no folds, 2.98
 // PFLOP/s on 8192 cubed; this 2.48).  Not faster: products of 32 x 32 x 64 (730), waves that take turns at multiplying and fetching (862), the next group's
 // first fragments under the last products (727: its rows have to land earlier for that).
 constexpr int BIG = 256, BIG_STAGE = BIG * kGroup, BIG_S = 4 * BIG_STAGE, BIG_LDS = BIG_S + 2 * BIG * 4;

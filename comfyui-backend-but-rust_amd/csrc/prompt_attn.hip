@@ -310,7 +310,7 @@ template <int DT> __device__ __forceinline__ float add_two(uint32_t a, uint32_t 
 // cycles) has about as many cycles of vector instructions beside it.  K is a tile ahead of V.  Tiles travel by DMA into two LDS stages.  That holds
 // for tiles that every row of the workgroup sees whole; the others, at the diagonal and at the prompt's end, follow in a loop that masks, with
 // their rows through registers, where values that are no numbers are taken out.  16384 tokens of 16 over 4 heads of 128, causal: 990 to 1040 us, 1.06 to 1.11 PFLOP/s, where
-// a library's large product reaches 1.35; matrix pipes 59 %, vector issue 50 % busy.
+// a library's large product reaches 1.35; matrix pipes 54 %, vector issue 42 % busy.
 template <class Src, int DP, int KG, bool WHOLE>
 __global__ __launch_bounds__(512, 2) void prompt_pipe_kernel(const Common a, const PackedArgs sa) {
     constexpr int QW = 8, RG = QW / KG, NS = 2, TK = 64 * KG, TILE = TK * 2 * DP, KS = DP / 16, DB = DP / 32, DT = Src::DT, ND = TILE / 1024 / QW;

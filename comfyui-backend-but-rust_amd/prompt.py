@@ -15,7 +15,8 @@ _DT = {torch.float16: ffi.DT_F16, torch.bfloat16: ffi.DT_BF16}
 def rope_freqs(rot, base=10000.0, stretch=1.0, parts=None, device="cuda:0"):
     """Radians that each of the rot / 2 pairs of channels turns per token, float64: base ** (-2 j / rot).  For contexts longer than a model was
     trained on: `stretch` divides all of them (positions interpolated); `parts` = (factor, trained length, slow, fast) divides by `factor` those
-    that turn fewer than `slow` times over the trained length, leaves those that turn more than `fast` times, and blends in between."""
+    that turn fewer than `slow` times over the trained length, leaves those that turn more than `fast` times, and blends in
+    between, linearly in the turns.  (Models that blend linearly in the pair's number instead have other tables: the calls take any.)"""
     if rot <= 0 or rot % 4:
         raise ValueError("a multiple of four channels turns, not %d" % rot)
     f = torch.tensor([base ** (-2.0 * j / rot) for j in range(rot // 2)], dtype=torch.float64) / stretch
